@@ -71,14 +71,15 @@ def _activations(tokens, k, g):
 
 
 def _weight(n, k, g):
-    """A frozen projection as block-FP8 checkpoints hold it: codes [n, k], scales [ceil(n / 128), ceil(k / 128)]."""
+    """A frozen projection as block-FP8 checkpoints hold it: codes [n, k], scales [ceil(n / 128), ceil(k / 128)]. Rows of codes start on
+    16 bytes, as a program lays them out once for bulk tensor copies."""
     nb, kb = -(-n // BLOCK), -(-k // BLOCK)
     w = torch.zeros(nb * BLOCK, kb * BLOCK, device=DEV)
     w[:n, :k] = torch.randn(n, k, device=DEV, generator=g) * k ** -0.5
     blocks = w.view(nb, BLOCK, kb, BLOCK)
     scale = blocks.abs().amax((1, 3)) / 448
-    codes = (blocks / scale[:, None, :, None]).view(nb * BLOCK, kb * BLOCK)[:n, :k].to(torch.float8_e4m3fn)
-    return codes.contiguous(), scale
+    codes = (blocks / scale[:, None, :, None]).view(nb * BLOCK, kb * BLOCK)[:n, :-(-k // 16) * 16].to(torch.float8_e4m3fn).contiguous()
+    return codes[:, :k], scale
 
 
 def prepare(case, seed):
