@@ -1,0 +1,383 @@
+// C[M, N] = A B^T (+ A2 B2^T) with A and B in E4M3 and scales for blocks of 128 along K:
+//
+//   C[m, n] = sum_b sA[b][m] sB[n / 128, b] (sum_{k in b} a[m, k] b[n, k]) + sum_r a2[m, r] b2[n, r]
+//
+// A: codes [M, K] with a scale per row and block (csrc/fp8_rows.cu); B: codes of a frozen weight with one fp32 scale per 128 x 128
+// block, [N, K] (forward) or stored [K, N] (b_mn: the input gradient reads the same codes as an MN-major operand, no second copy).
+// A2 / B2: bf16 K-extension, the low-rank update of an adapter, accumulated as further blocks of scale 1.
+//
+// The scales change every 128 columns of K, so an accumulator cannot stay in TMEM: the four MMAs of a block start a new one, and
+// eight epilogue warps add it, times its scale, to fp32 sums in registers (packed fused multiply-adds) while the tensor cores work
+// on the next. A thread owns a row: one scale for all its columns. Tiles: 256 x 256 by a CTA pair (two accumulators of 256 columns,
+// 128 sums a thread) and 128 x 128 by one CTA (four accumulators of 128 columns).
+#include "axb_common.cuh"
+
+namespace {
+
+constexpr int G_THREADS = 320;                 // TMA, MMA, eight epilogue warps
+constexpr int G_BK = 128;                      // bytes of a K block: 128 codes, or 64 bf16 of the extension
+constexpr int G_OP = 128 * G_BK;               // an operand tile of a CTA
+constexpr int G_STAGE = 2 * G_OP;
+constexpr int G_STAGES = 6;
+constexpr int G_EPI = 8 * 4096;                // per epilogue warp: 32 rows x 64 bf16
+constexpr int G_SMEM = G_STAGES * G_STAGE + G_EPI + 1024 + 256;
+
+struct Fp8GemmParams {
+  const float* sa;
+  const float* sb;
+  long long ldsa, sb_n, sb_k;                  // scale of block b: sa[b * ldsa + m], sb[(n / 128) * sb_n + b * sb_k]
+  __nv_bfloat16* C;
+  long long ldc;
+  int M, N, K, K2;
+  int group_m, tma_store;
+  int* status;
+};
+
+AXB_DEVICE void umma_f8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
+      "}\n"
+      :
+      : "r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+AXB_DEVICE void umma_f8_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
+      "}\n"
+      :
+      : "r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Instruction descriptor, kind::f8f6f4: E4M3 operands (format 0), fp32 accumulator.
+AXB_DEVICE constexpr uint32_t make_idesc_e4m3(int m, int n, int b_mn_major) {
+  return (1u << 4) | (uint32_t(b_mn_major) << 16) | (uint32_t(n >> 3) << 17) | (uint32_t(m >> 4) << 24);
+}
+
+// tiles in bands of group_m tile rows that sweep over N together (their A rows stay in L2)
+AXB_DEVICE void fp8_tile(int tile, int num_m, int num_n, int group_m, int& m_blk, int& n_blk) {
+  const int per = group_m * num_n, group = tile / per, first = group * group_m;
+  const int rows = min(num_m - first, group_m), in = tile - group * per;
+  m_blk = first + in % rows;
+  n_blk = in / rows;
+}
+
+template <bool PAIR, bool B_MN>
+__global__ void __launch_bounds__(G_THREADS, 1)
+    fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                    const __grid_constant__ CUtensorMap tmA2, const __grid_constant__ CUtensorMap tmB2,
+                    const __grid_constant__ CUtensorMap tmC, const Fp8GemmParams p) {
+  constexpr int CTAS = PAIR ? 2 : 1;
+  constexpr int TILE = 128 * CTAS;             // rows and columns of a tile
+  constexpr int COLS = TILE / 2;               // columns of an epilogue warp
+  constexpr int ACCS = 512 / TILE;             // accumulators in TMEM
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* sEpi = smem + G_STAGES * G_STAGE;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sEpi + G_EPI);   // leader's: both CTAs' loads of the stage
+  uint64_t* empty = full + G_STAGES;                            // one per CTA
+  uint64_t* tfull = empty + G_STAGES;                           // one per CTA
+  uint64_t* tempty = tfull + ACCS;                              // leader's: eight warps of every CTA
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + ACCS);
+  const int warp = uniform_warp(), lane = threadIdx.x & 31;
+  const int rank = PAIR ? (int)cluster_ctarank() : 0;
+  const int worker = blockIdx.x / CTAS, workers = gridDim.x / CTAS;
+  const int num_m = (p.M + TILE - 1) / TILE, num_n = (p.N + TILE - 1) / TILE, tiles = num_m * num_n;
+  const int nk_main = (p.K + 127) / 128, nk = nk_main + (p.K2 + 63) / 64;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < G_STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < ACCS; ++s) {
+      mbar_init(&tfull[s], 1);
+      mbar_init(&tempty[s], 8 * CTAS);
+    }
+    mbar_fence_init();
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+  }
+  if (warp == 1) {
+    if constexpr (PAIR) {
+      tmem_alloc_pair(tmem_slot, 512);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(tmem_slot, 512);
+      tmem_relinquish();
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (PAIR) cluster_sync();          // the barriers of both CTAs are ready before anything arrives on them
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int tile = worker; tile < tiles && ok; tile += workers) {
+      int m_blk, n_blk;
+      fp8_tile(tile, num_m, num_n, p.group_m, m_blk, n_blk);
+      const int m0 = m_blk * TILE + rank * 128, n0 = n_blk * TILE + rank * 128;
+      for (int kb = 0; kb < nk; ++kb) {
+        if (!warp_all(mbar_wait_spin(&empty[stage], phase ^ 1, p.status, AXB_TIMEOUT_EMPTY))) {
+          ok = false;
+          break;
+        }
+        const bool ext = kb >= nk_main;
+        uint8_t* a = smem + stage * G_STAGE;
+        uint8_t* b = a + G_OP;
+        if (elect_one()) {
+          auto load = [&](uint8_t* dst, const CUtensorMap* m, int c0, int c1) {
+            if constexpr (PAIR) tma_load_2d_pair(dst, m, mapa_u32(smem_u32(&full[stage]), 0), c0, c1);
+            else tma_load_2d(dst, m, &full[stage], c0, c1);
+          };
+          if (rank == 0) mbar_expect_tx(&full[stage], CTAS * G_STAGE);
+          if (!ext) {
+            load(a, &tmA, kb * 128, m0);
+            if (B_MN) load(b, &tmB, n0, kb * 128);
+            else load(b, &tmB, kb * 128, n0);
+          } else {
+            const int k0 = (kb - nk_main) * 64;
+            load(a, &tmA2, k0, m0);
+            if (B_MN) {
+              load(b, &tmB2, n0, k0);
+              load(b + G_OP / 2, &tmB2, n0 + 64, k0);
+            } else {
+              load(b, &tmB2, k0, n0);
+            }
+          }
+        }
+        __syncwarp();
+        if (++stage == G_STAGES) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (rank == 0) {
+      constexpr uint32_t id8 = make_idesc_e4m3(TILE, TILE, B_MN ? 1 : 0);
+      constexpr uint32_t id16 = make_idesc_bf16(TILE, TILE, 0, B_MN ? 1 : 0);
+      const uint64_t base_a = make_smem_desc_sw128(smem_u32(smem), 16, 1024);
+      // MN-major: 128 codes (one 1024-byte atom per 8 k) or two chunks of 64 bf16, G_OP / 2 apart
+      const uint64_t base_b = make_smem_desc_sw128(smem_u32(smem + G_OP), B_MN ? G_OP / 2 : 16, 1024);
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int tile = worker; tile < tiles && ok; tile += workers) {
+        for (int kb = 0; kb < nk; ++kb) {
+          ok = warp_all(mbar_wait_spin(&tempty[acc], acc_phase ^ 1, p.status, AXB_TIMEOUT_TMEM_EMPTY) &&
+                        mbar_wait_spin(&full[stage], phase, p.status, AXB_TIMEOUT_FULL));
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t a = base_a + (uint32_t)(stage * (G_STAGE / 16)), b = base_b + (uint32_t)(stage * (G_STAGE / 16));
+          const uint32_t d = tmem + acc * TILE;
+          if (elect_one()) {
+            if (kb < nk_main) {
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk) {  // 32 codes each
+                const uint64_t bk = b + kk * (B_MN ? 4096 / 16 : 2);
+                if constexpr (PAIR) umma_f8_pair(d, a + kk * 2, bk, id8, kk > 0 ? 1u : 0u);
+                else umma_f8(d, a + kk * 2, bk, id8, kk > 0 ? 1u : 0u);
+              }
+            } else {
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk) {  // 16 bf16 each
+                const uint64_t bk = b + kk * (B_MN ? 2048 / 16 : 2);
+                if constexpr (PAIR) umma_f16_pair(d, a + kk * 2, bk, id16, kk > 0 ? 1u : 0u);
+                else umma_f16(d, a + kk * 2, bk, id16, kk > 0 ? 1u : 0u);
+              }
+            }
+            if constexpr (PAIR) {
+              umma_commit_pair_mc(&empty[stage]);
+              umma_commit_pair_mc(&tfull[acc]);
+            } else {
+              umma_commit(&empty[stage]);
+              umma_commit(&tfull[acc]);
+            }
+          }
+          __syncwarp();
+          if (++stage == G_STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+          if (++acc == ACCS) {
+            acc = 0;
+            acc_phase ^= 1;
+          }
+        }
+      }
+    }
+  } else {
+    const int quad = warp & 3, half = (warp - 2) >> 2;
+    uint8_t* stg = sEpi + (warp - 2) * 4096;
+    const uint32_t t_base = tmem + (uint32_t(quad * 32) << 16) + half * COLS;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    bool ok = true;
+    for (int tile = worker; tile < tiles && ok; tile += workers) {
+      int m_blk, n_blk;
+      fp8_tile(tile, num_m, num_n, p.group_m, m_blk, n_blk);
+      const int row0 = m_blk * TILE + rank * 128 + quad * 32, row = row0 + lane;
+      const int col0 = n_blk * TILE + half * COLS;
+      const bool live = row < p.M;
+      const float* sa = p.sa + (live ? row : 0);
+      const float* sb = p.sb + (long long)(min(col0, p.N - 1) >> 7) * p.sb_n;
+      uint64_t sum[COLS / 2];
+#pragma unroll
+      for (int j = 0; j < COLS / 2; ++j) sum[j] = 0ull;
+      float next = __ldg(sa) * __ldg(sb);
+      for (int kb = 0; kb < nk; ++kb) {
+        const float sc = next;
+        next = kb + 1 < nk_main ? __ldg(sa + (long long)(kb + 1) * p.ldsa) * __ldg(sb + (long long)(kb + 1) * p.sb_k) : 1.f;
+        ok = warp_all(mbar_wait_spin(&tfull[acc], acc_phase, p.status, AXB_TIMEOUT_TMEM_FULL));
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t sc2 = pack_f32x2(sc, sc);
+#pragma unroll
+        for (int c = 0; c < COLS / 32; ++c) {
+          uint32_t r[32];
+          tmem_ld_32x32(t_base + acc * TILE + c * 32, r);
+          tmem_ld_wait();
+          if (c == COLS / 32 - 1) {            // the accumulator has been read
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+              if constexpr (PAIR) mbar_arrive_cluster(mapa_u32(smem_u32(&tempty[acc]), 0));
+              else mbar_arrive(&tempty[acc]);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 16; ++j) sum[c * 16 + j] = fma_f32x2(pack_b32x2(r[2 * j], r[2 * j + 1]), sc2, sum[c * 16 + j]);
+        }
+        if (++acc == ACCS) {
+          acc = 0;
+          acc_phase ^= 1;
+        }
+      }
+      if (!ok) break;
+#pragma unroll
+      for (int c = 0; c < COLS / 64; ++c) {
+        const int cc = col0 + c * 64;
+        uint4 w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          uint32_t o[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 f = unpack_f32x2(sum[c * 32 + j * 4 + e]);
+            o[e] = pack_bf16x2(f.x, f.y);
+          }
+          w[j] = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+        if (p.tma_store) {
+          if (row0 < p.M && cc < p.N) {        // the same for the whole warp
+            if (lane == 0) bulk_wait_group_read<0>();
+            __syncwarp();
+            stage_row128(stg, lane, w);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_2d(&tmC, stg, cc, row0);
+              bulk_commit_group();
+            }
+          }
+        } else if (live) {
+          __nv_bfloat16* o = p.C + (long long)row * p.ldc + cc;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const uint32_t q[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (cc + j * 8 + e < p.N) o[j * 8 + e] = __ushort_as_bfloat16((unsigned short)(q[e >> 1] >> (16 * (e & 1))));
+          }
+        }
+      }
+    }
+    if (lane == 0) bulk_wait_group<0>();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (PAIR) cluster_sync();          // neither CTA leaves while its partner still signals it
+  if (warp == 1) {
+    tc_fence_after();
+    if constexpr (PAIR) tmem_dealloc_pair(tmem, 512);
+    else tmem_dealloc(tmem, 512);
+  }
+}
+
+int fp8_sm_count() {
+  int dev = 0, n = 0;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  return n > 1 ? n : 148;
+}
+
+template <bool PAIR, bool B_MN>
+int launch_fp8(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& a2, const CUtensorMap& b2, const CUtensorMap& c,
+               const Fp8GemmParams& p, cudaStream_t st) {
+  constexpr int CTAS = PAIR ? 2 : 1, TILE = 128 * CTAS;
+  auto kern = fp8_gemm_kernel<PAIR, B_MN>;
+  static std::atomic<unsigned long long> allowed{0};
+  if (const int rc = axb_allow_smem((const void*)kern, G_SMEM, allowed)) return rc;
+  const long long tiles = (long long)((p.M + TILE - 1) / TILE) * ((p.N + TILE - 1) / TILE);
+  const long long workers = tiles < fp8_sm_count() / CTAS ? tiles : fp8_sm_count() / CTAS;
+  AxbLaunch l(dim3((unsigned)(workers * CTAS)), G_THREADS, G_SMEM, st, PAIR ? 2 : 0, false);
+  const cudaError_t e = cudaLaunchKernelEx(&l.cfg, kern, a, b, a2, b2, c, p);
+  return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
+}
+
+}  // namespace
+
+// See the head of this file. A: codes [M, K], rows of lda bytes; sa: fp32 [ceil(K / 128)][ldsa]; B: codes [N, K] (b_mn: [K, N]), rows of
+// ldb bytes; sb: fp32, the scale of columns n and block b at sb[(n / 128) * sb_n + b * sb_k]; C: bf16 [M, N]; A2 [M, K2] and B2 [N, K2]
+// (b_mn: [K2, N]) bf16, K2 = 0: none. Operands start on 16 bytes and have row strides of whole 16 bytes.
+extern "C" int axb_fp8_gemm(const void* A, long long lda, const float* sa, long long ldsa, const void* B, long long ldb, const float* sb,
+                            long long sb_n, long long sb_k, int b_mn, void* C, long long ldc, int M, int N, int K, const void* A2,
+                            long long lda2, const void* B2, long long ldb2, int K2, int tile, int* status, void* stream) {
+  if (M <= 0 || N <= 0) return 0;
+  auto bad = [](const void* q, long long bytes) { return (reinterpret_cast<uintptr_t>(q) & 15) != 0 || (bytes & 15) != 0; };
+  if (K <= 0 || bad(A, lda) || bad(B, ldb) || ldsa < M) return -2;
+  if (K2 > 0 && (bad(A2, 2 * lda2) || bad(B2, 2 * ldb2))) return -2;
+  const bool pair = tile == 256;
+  CUtensorMap tA, tB, tA2, tB2, tC;
+  int rc = axb_make_tmap_2d(&tA, A, M, K, lda, 128, 128, 1);
+  if (!rc) rc = b_mn ? axb_make_tmap_2d(&tB, B, K, N, ldb, 128, 128, 1) : axb_make_tmap_2d(&tB, B, N, K, ldb, 128, 128, 1);
+  tA2 = tC = tA;
+  tB2 = tB;
+  if (!rc && K2 > 0) {
+    rc = axb_make_tmap_2d(&tA2, A2, M, K2, lda2, 128, 64);
+    if (!rc) rc = b_mn ? axb_make_tmap_2d(&tB2, B2, K2, N, ldb2, 64, 64) : axb_make_tmap_2d(&tB2, B2, N, K2, ldb2, 128, 64);
+  }
+  const int tma_store = !bad(C, 2 * ldc);
+  if (!rc && tma_store) rc = axb_make_tmap_2d(&tC, C, M, N, ldc, 32, 64);
+  if (rc) return -100 - rc;
+  Fp8GemmParams p = {};
+  p.sa = sa;
+  p.sb = sb;
+  p.ldsa = ldsa;
+  p.sb_n = sb_n;
+  p.sb_k = sb_k;
+  p.C = reinterpret_cast<__nv_bfloat16*>(C);
+  p.ldc = ldc;
+  p.M = M;
+  p.N = N;
+  p.K = K;
+  p.K2 = K2 > 0 ? K2 : 0;
+  p.tma_store = tma_store;
+  p.status = status;
+  const long long band = (20ll << 20) / ((pair ? 256ll : 128ll) * K);   // A rows of a band: about 20 MB of the L2
+  p.group_m = (int)(band < 2 ? 2 : (band > 16 ? 16 : band));
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (pair) return b_mn ? launch_fp8<true, true>(tA, tB, tA2, tB2, tC, p, st) : launch_fp8<true, false>(tA, tB, tA2, tB2, tC, p, st);
+  return b_mn ? launch_fp8<false, true>(tA, tB, tA2, tB2, tC, p, st) : launch_fp8<false, false>(tA, tB, tA2, tB2, tC, p, st);
+}

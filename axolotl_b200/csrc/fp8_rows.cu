@@ -1,0 +1,225 @@
+// Activations in 8 bits: E4M3 codes with one power-of-two scale for each row and 128 columns.
+//
+//   s[b][t] = 2^ceil(log2(max |x[t, 128 b ..]| / 448))   (1 for a block of zeros, never below 2^-126),   q = rn_e4m3(x / s)
+//
+// A power of two makes x / s exact, so that a code is the nearest E4M3 number whatever the precision it is computed in, and q s exact
+// in bf16 (four significant bits): what comes back is what every product of the codes has seen. NaN and infinities become NaN codes
+// and take no part in the maximum, so their neighbours keep their values. A finite value stays finite: where the nearest code would
+// stand for 2^128 it is the one below.
+// Scales are stored [block][row]: a GEMM's thread owns a row of the accumulator and reads its scale beside its neighbours'.
+//
+// Bound: HBM, 2 bytes read and 1 written per value (and the other way round); a warp takes 1024 columns of a row with all its
+// 16-byte loads in flight, eight neighbouring rows share a block so that their 4-byte scales fill whole sectors.
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "axb_common.cuh"
+
+namespace {
+
+constexpr int Q_ROWS = 8;          // rows (warps) of a block
+constexpr int Q_COLS = 1024;       // columns of a warp: four vectors of eight values for every lane
+
+template <typename T>
+AXB_DEVICE float to_f32(T v);
+template <>
+AXB_DEVICE float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <>
+AXB_DEVICE float to_f32(__half v) { return __half2float(v); }
+template <>
+AXB_DEVICE float to_f32(float v) { return v; }
+template <typename T>
+AXB_DEVICE T from_f32(float v);
+template <>
+AXB_DEVICE __nv_bfloat16 from_f32(float v) { return __float2bfloat16(v); }
+template <>
+AXB_DEVICE __half from_f32(float v) { return __float2half(v); }
+template <>
+AXB_DEVICE float from_f32(float v) { return v; }
+
+// biased exponent of the block's scale
+AXB_DEVICE int scale_exponent(float top) {
+  const uint32_t b = __float_as_uint(top);
+  const int e = (int)(b >> 23) - 8 + ((b & 0x7FFFFFu) > 0x600000u ? 1 : 0);   // 448 = 1.75 * 2^8
+  return top == 0.f ? 127 : max(e, 1);
+}
+
+AXB_DEVICE float group_max(float m) {     // over the 16 lanes that hold a block of 128 columns
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  return m;
+}
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(Q_ROWS * 32)
+    fp8_quantize_rows_kernel(const T* __restrict__ x, long long ldx, uint8_t* __restrict__ q, long long ldq, float* __restrict__ s,
+                             long long lds, long long rows, int K) {
+  const int lane = threadIdx.x & 31;
+  const long long row = (long long)blockIdx.x * Q_ROWS + (threadIdx.x >> 5);
+  const int c0 = blockIdx.y * Q_COLS;
+  if (row >= rows) return;                       // whole warps
+  const T* xr = x + row * ldx;
+  float v[4][8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int c = c0 + i * 256 + lane * 8;
+    if (VEC && c + 8 <= K) {
+      constexpr int N16 = sizeof(T) * 8 / 16;
+      uint4 raw[N16];
+#pragma unroll
+      for (int h = 0; h < N16; ++h) raw[h] = __ldg(reinterpret_cast<const uint4*>(xr + c) + h);
+      const T* e = reinterpret_cast<const T*>(raw);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i][j] = to_f32<T>(e[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i][j] = c + j < K ? to_f32<T>(xr[c + j]) : 0.f;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int c = c0 + i * 256 + lane * 8;
+    if (c0 + i * 256 >= K) break;                // the whole warp
+    float top = 0.f;
+    bool odd = false;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float a = fabsf(v[i][j]);
+      odd |= !(a <= 3.402823466e38f);
+      top = fmaxf(top, a);                       // NaN takes no part
+    }
+    if (__any_sync(0xffffffffu, odd)) {
+      top = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float a = fabsf(v[i][j]);
+        if (a <= 3.402823466e38f) top = fmaxf(top, a);
+        else v[i][j] = __uint_as_float(0x7FC00000u);
+      }
+    }
+    const int e = scale_exponent(group_max(top));
+    const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
+    if (e >= 247) {                              // scale 2^120: the code 256 would stand for 2^128
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (fabsf(v[i][j]) > 240.f * 0x1p120f) v[i][j] = copysignf(240.f * 0x1p120f, v[i][j]);
+    }
+    uint32_t w[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[i][4 * h] * inv, v[i][4 * h + 1] * inv), __NV_SATFINITE, __NV_E4M3);
+      const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[i][4 * h + 2] * inv, v[i][4 * h + 3] * inv), __NV_SATFINITE, __NV_E4M3);
+      w[h] = lo | (hi << 16);
+    }
+    // rows of codes start on 16 bytes and are padded to them, so a vector that begins inside a row ends inside its padding
+    if (c < K) *reinterpret_cast<uint2*>(q + row * ldq + c) = make_uint2(w[0], w[1]);
+    if ((lane & 15) == 0 && c < K) s[(long long)(c >> 7) * lds + row] = __uint_as_float((uint32_t)e << 23);
+  }
+}
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(Q_ROWS * 32)
+    fp8_dequantize_rows_kernel(const uint8_t* __restrict__ q, long long ldq, const float* __restrict__ s, long long lds,
+                               T* __restrict__ x, long long ldx, long long rows, int K) {
+  const int lane = threadIdx.x & 31;
+  const long long row = (long long)blockIdx.x * Q_ROWS + (threadIdx.x >> 5);
+  const int c0 = blockIdx.y * Q_COLS;
+  if (row >= rows) return;
+  uint2 raw[4];
+  float sc[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int c = c0 + i * 256 + lane * 8;
+    raw[i] = make_uint2(0u, 0u);
+    sc[i] = 0.f;
+    if (c < K) {
+      if (c + 8 <= K) {
+        raw[i] = __ldg(reinterpret_cast<const uint2*>(q + row * ldq + c));
+      } else {
+        for (int j = 0; c + j < K; ++j) (j < 4 ? raw[i].x : raw[i].y) |= (uint32_t)q[row * ldq + c + j] << (8 * (j & 3));
+      }
+      sc[i] = __ldg(s + (long long)(c >> 7) * lds + row);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int c = c0 + i * 256 + lane * 8;
+    if (c >= K) break;
+    T o[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const __nv_fp8x2_storage_t two = (__nv_fp8x2_storage_t)((j < 2 ? raw[i].x : raw[i].y) >> (16 * (j & 1)));
+      const float2 f = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(two, __NV_E4M3)));
+      o[2 * j] = from_f32<T>(f.x * sc[i]);
+      o[2 * j + 1] = from_f32<T>(f.y * sc[i]);
+    }
+    T* xr = x + row * ldx + c;
+    if (VEC && c + 8 <= K) {
+#pragma unroll
+      for (int h = 0; h < (int)(sizeof(T) * 8 / 16); ++h) reinterpret_cast<uint4*>(xr)[h] = reinterpret_cast<const uint4*>(o)[h];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c + j < K) xr[j] = o[j];
+    }
+  }
+}
+
+bool rows_aligned(const void* p, long long ld, int size) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * size) % 16 == 0;
+}
+
+template <typename T>
+int launch_quantize(const void* x, long long ldx, void* q, long long ldq, float* s, long long lds, long long rows, int K, cudaStream_t st) {
+  const dim3 grid((unsigned)((rows + Q_ROWS - 1) / Q_ROWS), (unsigned)((K + Q_COLS - 1) / Q_COLS));
+  if (rows_aligned(x, ldx, sizeof(T)))
+    fp8_quantize_rows_kernel<T, true><<<grid, Q_ROWS * 32, 0, st>>>((const T*)x, ldx, (uint8_t*)q, ldq, s, lds, rows, K);
+  else
+    fp8_quantize_rows_kernel<T, false><<<grid, Q_ROWS * 32, 0, st>>>((const T*)x, ldx, (uint8_t*)q, ldq, s, lds, rows, K);
+  return (int)cudaGetLastError();
+}
+
+template <typename T>
+int launch_dequantize(const void* q, long long ldq, const float* s, long long lds, void* x, long long ldx, long long rows, int K,
+                      cudaStream_t st) {
+  const dim3 grid((unsigned)((rows + Q_ROWS - 1) / Q_ROWS), (unsigned)((K + Q_COLS - 1) / Q_COLS));
+  if (rows_aligned(x, ldx, sizeof(T)))
+    fp8_dequantize_rows_kernel<T, true><<<grid, Q_ROWS * 32, 0, st>>>((const uint8_t*)q, ldq, s, lds, (T*)x, ldx, rows, K);
+  else
+    fp8_dequantize_rows_kernel<T, false><<<grid, Q_ROWS * 32, 0, st>>>((const uint8_t*)q, ldq, s, lds, (T*)x, ldx, rows, K);
+  return (int)cudaGetLastError();
+}
+
+bool bad_rows(const void* q, long long ldq, long long lds, long long rows, int K) {
+  return rows > (1ll << 33) || K > (1 << 26) || (reinterpret_cast<uintptr_t>(q) & 15) || (ldq & 15) || ldq < K || lds < rows;
+}
+
+}  // namespace
+
+// x [rows, K] with row stride ldx (elements); dtype 0: bf16, 1: fp16, 2: fp32. q: codes, rows of ldq bytes (a multiple of 16, on 16
+// bytes); s: fp32 [ceil(K / 128)][lds], lds >= rows.
+extern "C" int axb_fp8_quantize_rows(const void* x, long long ldx, int dtype, void* q, long long ldq, float* s, long long lds,
+                                     long long rows, int K, void* stream) {
+  if (rows <= 0 || K <= 0) return 0;
+  if (bad_rows(q, ldq, lds, rows, K)) return -2;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  switch (dtype) {
+    case 0: return launch_quantize<__nv_bfloat16>(x, ldx, q, ldq, s, lds, rows, K, st);
+    case 1: return launch_quantize<__half>(x, ldx, q, ldq, s, lds, rows, K, st);
+    case 2: return launch_quantize<float>(x, ldx, q, ldq, s, lds, rows, K, st);
+    default: return -2;
+  }
+}
+
+extern "C" int axb_fp8_dequantize_rows(const void* q, long long ldq, const float* s, long long lds, void* x, long long ldx, int dtype,
+                                       long long rows, int K, void* stream) {
+  if (rows <= 0 || K <= 0) return 0;
+  if (bad_rows(q, ldq, lds, rows, K)) return -2;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  switch (dtype) {
+    case 0: return launch_dequantize<__nv_bfloat16>(q, ldq, s, lds, x, ldx, rows, K, st);
+    case 1: return launch_dequantize<__half>(q, ldq, s, lds, x, ldx, rows, K, st);
+    case 2: return launch_dequantize<float>(q, ldq, s, lds, x, ldx, rows, K, st);
+    default: return -2;
+  }
+}

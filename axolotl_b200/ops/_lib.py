@@ -42,6 +42,11 @@ _CUDA_SIGS = {
     "axb_moe_combine_dw": [vp, vp, vp, vp, i64, i32, i32, vp],
     "axb_nf4_dequant": [vp, vp, vp, i64, i32, vp],
     "axb_fp8_block_dequant": [vp, vp, vp, i64, i64, i32, vp],
+    # x, ldx, dtype, codes, ldq, scales, lds, rows, K, stream; back: codes, ldq, scales, lds, x, ldx, dtype, rows, K, stream
+    "axb_fp8_quantize_rows": [vp, i64, i32, vp, i64, vp, i64, i64, i32, vp],
+    "axb_fp8_dequantize_rows": [vp, i64, vp, i64, vp, i64, i32, i64, i32, vp],
+    # A, lda, sa, ldsa, B, ldb, sb, sb_n, sb_k, b_mn, C, ldc, M, N, K, A2, lda2, B2, ldb2, K2, tile, status, stream
+    "axb_fp8_gemm": [vp, i64, vp, i64, vp, i64, vp, i64, i64, i32, vp, i64, i32, i32, i32, vp, i64, vp, i64, i32, i32, vp, vp],
     "axb_nvfp4_dequant_batched": [vp, vp, vp, vp, i64, i64, i64, vp, vp],
     # A, lda, W, A2, lda2, W2, C, ldc, E, N, K, K2, trans_w, alpha, out_mode, bn, blk_expert, n_blocks, max_blocks, status, stream
     "axb_grouped_gemm": [vp, i64, vp, vp, i64, vp, vp, i64, i32, i32, i32, i32, i32, f32, i32, i32, vp, vp, i32, vp, vp],

@@ -1,0 +1,324 @@
+"""8-bit blocks: E4M3 activations with a power-of-two scale for each row and 128 columns, frozen E4M3 weights with an fp32 scale for
+each 128 x 128 block (the layout of block-FP8 checkpoints), and the linear layers on them.
+
+A row's block is held as ``q s`` with ``s = 2^ceil(log2(max |x| / 448))`` (1 for a block of zeros, never below 2^-126) and ``q`` the
+nearest E4M3 number to ``x / s``, ties to even. A power of two divides exactly, so that ``q`` does not depend on the precision it is
+computed in and ``q s`` is a bf16 number. NaN and infinities become NaN codes; the other values of their block keep their scale. A
+finite value stays finite: where the nearest code would stand for 2^128, ``q`` is the one below.
+
+``fp8_linear`` and ``fp8_lora_linear`` quantise their input once: the codes are the operand of the forward product and all that is
+kept of the input for the backward pass, half of what bf16 takes. The backward pass quantises the output gradient the same way and
+reads the same weight codes as the other operand order. The quantisers pass gradients straight through.
+
+The reference keeps such weights in FP8 only under adapters (src/axolotl/integrations/kernels/libs/dsv4/lora_fp8.py:1-147: a library
+product in the forward pass, the weight expanded to bf16 in the backward pass) and expands them elsewhere
+(src/axolotl/kernels/quantize.py:109-135).
+"""
+from __future__ import annotations
+
+import contextlib
+from dataclasses import dataclass
+
+import torch
+
+from . import _lib
+
+BLOCK = 128
+E4M3_MAX = 448.0
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def _device_of(t):
+    """Launches go to the current device: makes it the tensor's where it is another one."""
+    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def _blocks(n: int) -> int:
+    return -(-n // BLOCK)
+
+
+def _padded(rows: int, cols: int, device):
+    """Codes [rows, cols] whose rows start on 16 bytes (bulk tensor copies)."""
+    ld = -(-cols // 16) * 16
+    return torch.empty((rows, ld), dtype=torch.float8_e4m3fn, device=device)[:, :cols]
+
+
+def _check_codes(codes, what):
+    if codes.dtype != torch.float8_e4m3fn:
+        raise TypeError(f"{what}: codes are float8_e4m3fn, got {codes.dtype}")
+    if codes.dim() != 2 or 0 in codes.shape[1:]:
+        raise ValueError(f"{what}: codes are a matrix [rows, columns] with a column at least, got {tuple(codes.shape)}")
+
+
+def _check_scale(scale, shape, device, what):
+    if scale.dtype != torch.float32 or tuple(scale.shape) != shape or scale.device != device:
+        raise ValueError(f"{what}: scales are float32 {shape} on {device}, got {scale.dtype} {tuple(scale.shape)} on {scale.device}")
+
+
+def _rows16(codes):
+    """``codes`` with rows of whole 16 bytes: as they are, or laid out again."""
+    if codes.stride(1) == 1 and codes.stride(0) % 16 == 0 and codes.stride(0) >= codes.shape[1] and codes.data_ptr() % 16 == 0:
+        return codes
+    out = _padded(*codes.shape, codes.device)
+    out.view(torch.uint8).copy_(codes.view(torch.uint8))
+    return out
+
+
+def _row_scales(scale, rows):
+    """(tensor, row stride) of the scales [blocks, rows] as the kernels read them."""
+    if scale.stride(1) != 1 or (scale.shape[0] > 1 and scale.stride(0) < rows):
+        scale = scale.contiguous()
+    return scale, max(scale.stride(0), rows)
+
+
+# ------------------------------------------------------------------ rows
+def quantize_fp8_rows(x: torch.Tensor):
+    """x [rows, columns] (bf16, fp16 or fp32) -> (codes float8_e4m3fn [rows, columns], scales fp32 [ceil(columns / 128), rows]). Rows of
+    codes start on 16 bytes, so that they are operands of the tensor-core kernels as they are."""
+    if x.dim() != 2 or x.shape[1] == 0:
+        raise ValueError(f"quantize_fp8_rows takes a matrix [rows, columns] with a column at least, got {tuple(x.shape)}")
+    if x.dtype not in _DTYPES:
+        raise TypeError(f"quantize_fp8_rows takes bfloat16, float16 or float32, got {x.dtype}")
+    x = x.detach()
+    T, K = x.shape
+    if not x.is_cuda:
+        return _quantize_rows_plain(x)
+    if x.stride(1) != 1 and K > 1:
+        x = x.contiguous()
+    with _device_of(x):
+        codes = _padded(T, K, x.device)
+        scale = torch.empty((_blocks(K), T), dtype=torch.float32, device=x.device)
+        _lib.check_rc(_lib.cuda_lib().axb_fp8_quantize_rows(x.data_ptr(), x.stride(0), _DTYPES[x.dtype], codes.data_ptr(), codes.stride(0),
+                                                            scale.data_ptr(), T, T, K, _lib.stream_ptr()), "fp8_quantize_rows")
+    return codes, scale
+
+
+def _quantize_rows_plain(x):
+    T, K = x.shape
+    kb = _blocks(K)
+    v = torch.nn.functional.pad(x.float(), (0, kb * BLOCK - K)).view(T, kb, BLOCK)
+    v = v.masked_fill(v.isinf(), float("nan"))
+    top = v.nan_to_num(nan=0.0).abs().amax(-1)
+    m, e = torch.frexp(top)                                # top = m 2^e with m in [0.5, 1); 448 = 0.875 * 2^9
+    e = (e - 9 + (m > 0.875).to(e.dtype)).clamp(min=-126)
+    scale = torch.where(top > 0, torch.ldexp(torch.ones_like(top), e), torch.ones_like(top))
+    codes = _padded(T, K, x.device)
+    v = v.clamp(-240 * 2.0 ** 120, 240 * 2.0 ** 120)
+    codes.copy_((v / scale[..., None]).to(torch.float8_e4m3fn).view(T, kb * BLOCK)[:, :K])
+    return codes, scale.t().contiguous()
+
+
+def dequantize_fp8_rows(codes: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = torch.bfloat16):
+    """The values that the codes of ``quantize_fp8_rows`` stand for (exact in bf16 and fp32), [rows, columns]."""
+    _check_codes(codes, "dequantize_fp8_rows")
+    T, K = codes.shape
+    _check_scale(scale, (_blocks(K), T), codes.device, "dequantize_fp8_rows")
+    if dtype not in _DTYPES:
+        raise TypeError(f"dequantize_fp8_rows gives bfloat16, float16 or float32, not {dtype}")
+    if not codes.is_cuda:
+        return (codes.float() * scale.t().repeat_interleave(BLOCK, 1)[:, :K]).to(dtype)
+    with _device_of(codes):
+        codes = _rows16(codes)
+        scale, lds = _row_scales(scale, T)
+        out = torch.empty((T, K), dtype=dtype, device=codes.device)
+        _lib.check_rc(_lib.cuda_lib().axb_fp8_dequantize_rows(codes.data_ptr(), codes.stride(0), scale.data_ptr(), lds, out.data_ptr(), K,
+                                                              _DTYPES[dtype], T, K, _lib.stream_ptr()), "fp8_dequantize_rows")
+    return out
+
+
+# ------------------------------------------------------------------ weights
+@dataclass
+class Fp8State:
+    """Scales of a frozen weight held as codes [N, K]: fp32 [ceil(N / 128), ceil(K / 128)]."""
+    shape: tuple
+    scale: torch.Tensor
+
+    def to(self, device):
+        return Fp8State(self.shape, self.scale.to(device))
+
+    def nbytes(self):
+        return self.scale.numel() * self.scale.element_size()
+
+
+@torch.no_grad()
+def quantize_fp8_weight(w: torch.Tensor):
+    """w [N, K] -> (codes float8_e4m3fn [N, K] in rows of whole 16 bytes, scales fp32 [ceil(N / 128), ceil(K / 128)]): the block's largest
+    magnitude becomes 448. Done once, when a weight is loaded."""
+    if w.dim() != 2 or 0 in w.shape:
+        raise ValueError(f"quantize_fp8_weight takes a matrix that is not empty, got {tuple(w.shape)}")
+    N, K = w.shape
+    codes = _padded(N, K, w.device)
+    scale = torch.empty((_blocks(N), _blocks(K)), dtype=torch.float32, device=w.device)
+    for i in range(scale.shape[0]):                       # 128 rows at a time: no fp32 copy of the whole weight
+        rows = w[i * BLOCK:(i + 1) * BLOCK].float()
+        pad = torch.nn.functional.pad(rows, (0, scale.shape[1] * BLOCK - K)).view(rows.shape[0], -1, BLOCK)
+        s = pad.abs().amax((0, 2)) / E4M3_MAX
+        s = torch.where(s > 0, s, torch.ones_like(s))
+        scale[i] = s
+        q = (pad / s[:, None]).clamp(-E4M3_MAX, E4M3_MAX).to(torch.float8_e4m3fn)
+        codes[i * BLOCK:(i + 1) * BLOCK].copy_(q.view(rows.shape[0], -1)[:, :K])
+    return codes, scale
+
+
+def dequantize_fp8_weight(codes: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = torch.bfloat16):
+    """codes [N, K] times their block's scale."""
+    _check_weight(codes, scale, "dequantize_fp8_weight")
+    from .nf4 import dequantize_fp8_block
+
+    return dequantize_fp8_block(codes, scale, BLOCK, dtype)
+
+
+def _check_weight(codes, scale, what):
+    _check_codes(codes, what)
+    _check_scale(scale, (_blocks(codes.shape[0]), _blocks(codes.shape[1])), codes.device, what)
+
+
+# ------------------------------------------------------------------ products
+def fp8_gemm(codes, row_scale, w_codes, w_scale, *, trans_w=False, a2=None, b2=None):
+    """bf16 ``x8 W8^T`` (``trans_w``: ``x8 W8``) of quantised rows and a frozen weight, plus ``a2 b2^T`` (``a2 b2``) of a bf16
+    K-extension: the low-rank update of an adapter, in the same accumulation."""
+    _check_codes(codes, "fp8_gemm")
+    _check_weight(w_codes, w_scale, "fp8_gemm")
+    M, K = codes.shape
+    Kw, N = w_codes.shape if trans_w else w_codes.shape[::-1]
+    if K != Kw or w_codes.device != codes.device:
+        raise ValueError(f"fp8_gemm: rows of {K} columns on {codes.device} against a weight of {Kw} on {w_codes.device}")
+    _check_scale(row_scale, (_blocks(K), M), codes.device, "fp8_gemm")
+    K2 = 0
+    if a2 is not None:
+        K2 = a2.shape[1]
+        if a2.shape[0] != M or tuple(b2.shape) != ((K2, N) if trans_w else (N, K2)):
+            raise ValueError(f"fp8_gemm: extension {tuple(a2.shape)} x {tuple(b2.shape)} for a result [{M}, {N}]")
+    if not codes.is_cuda:
+        w = w_codes.float() * w_scale.repeat_interleave(BLOCK, 0)[:w_codes.shape[0]].repeat_interleave(BLOCK, 1)[:, :w_codes.shape[1]]
+        y = dequantize_fp8_rows(codes, row_scale, torch.float32) @ (w if trans_w else w.t())
+        if K2:
+            y = y + a2.float() @ (b2 if trans_w else b2.t()).float()
+        return y.to(torch.bfloat16)
+    with _device_of(codes):
+        codes, w_codes = _rows16(codes), _rows16(w_codes)
+        row_scale, lds = _row_scales(row_scale, M)
+        if K2:
+            from .gemm import _row_major_2d
+
+            if a2.dtype != torch.bfloat16 or b2.dtype != torch.bfloat16:
+                raise TypeError("fp8_gemm: the K-extension is bf16")
+            a2, b2 = _row_major_2d(a2), _row_major_2d(b2)
+        out = torch.empty((M, N), dtype=torch.bfloat16, device=codes.device)
+        sn, sk = (w_scale.stride(1), w_scale.stride(0)) if trans_w else w_scale.stride()
+        _lib.check_rc(_lib.cuda_lib().axb_fp8_gemm(
+            codes.data_ptr(), codes.stride(0), row_scale.data_ptr(), lds, w_codes.data_ptr(), w_codes.stride(0), w_scale.data_ptr(), sn, sk,
+            int(trans_w), out.data_ptr(), N, M, N, K, _lib.ptr(a2), a2.stride(0) if K2 else 0, _lib.ptr(b2), b2.stride(0) if K2 else 0, K2,
+            _tile(M, N), _lib.status_word(codes.device).data_ptr(), _lib.stream_ptr()), "fp8_gemm")
+    return out
+
+
+def _tile(M, N) -> int:
+    """256 x 256 tiles of a CTA pair, or 128 x 128."""
+    return 256 if M > 128 and N > 128 and -(-M // 256) * -(-N // 256) >= 74 else 128
+
+
+class _Fp8LinearFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, codes, scale, bias):
+        y = fp8_gemm(*quantize_fp8_rows(x), codes, scale)
+        if bias is not None:
+            y = y + bias
+        ctx.save_for_backward(codes, scale)               # the weight is frozen: nothing of x is needed again
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        codes, scale = ctx.saved_tensors
+        dx = fp8_gemm(*quantize_fp8_rows(dy), codes, scale, trans_w=True) if ctx.needs_input_grad[0] else None
+        dbias = dy.float().sum(0).to(ctx.bias_dtype) if ctx.needs_input_grad[3] else None
+        return dx, None, None, dbias
+
+
+class _Fp8LoRALinearFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, codes, scale, A, B, A16, B16, scaling, blocks, bias):
+        from .lora import skinny_gemm
+
+        q, s = quantize_fp8_rows(x)
+        xa = skinny_gemm(x, A16, alpha=scaling)            # [T, R], of the bf16 input
+        y = fp8_gemm(q, s, codes, scale, a2=xa, b2=B16)
+        if bias is not None:
+            y = y + bias
+        ctx.save_for_backward(q, s, codes, scale, A, B, A16, B16, xa)
+        ctx.scaling, ctx.blocks, ctx.bias_dtype = scaling, blocks, None if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        from .lora import _adapter_grads, _t_and_dB
+
+        q, s, codes, scale, A, B, A16, B16, xa = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dy = dy.contiguous()
+        t, dB_fused, dB_done = _t_and_dB(dy, B, B16, xa, ctx.blocks, ctx.scaling, need[4])
+        dx = fp8_gemm(*quantize_fp8_rows(dy), codes, scale, trans_w=True, a2=t, b2=A16) if need[0] else None
+        dA = None
+        if need[3]:
+            tgt = getattr(A, "_axb_grad", None)
+            buf = fp8_adapter_grad(t, q, s, out=tgt)
+            dA = None if tgt is not None else buf.to(A.dtype)
+        _, dB = _adapter_grads(None, B if need[4] else None, t, q, dy, xa, ctx.blocks, dB_done, dB_fused)
+        dbias = dy.float().sum(0).to(ctx.bias_dtype) if need[9] else None
+        return dx, None, None, dA, dB, None, None, None, None, dbias
+
+
+def fp8_adapter_grad(t, codes, row_scale, out=None):
+    """``t^T x8`` [R, K] in fp32 for ``t`` [T, R] bf16 and the quantised rows [T, K] that a forward pass kept: the gradient of an adapter's
+    A. ``out``: added to it in place."""
+    _check_codes(codes, "fp8_adapter_grad")
+    T, K = codes.shape
+    _check_scale(row_scale, (_blocks(K), T), codes.device, "fp8_adapter_grad")
+    if t.dim() != 2 or t.shape[0] != T or t.device != codes.device:
+        raise ValueError(f"fp8_adapter_grad: {tuple(t.shape)} on {t.device} for {T} rows on {codes.device}")
+    R = t.shape[1]
+    if out is not None and (tuple(out.shape) != (R, K) or out.dtype != torch.float32 or out.device != codes.device):
+        raise ValueError(f"fp8_adapter_grad: the result is float32 [{R}, {K}] on {codes.device}")
+    x = dequantize_fp8_rows(codes, row_scale, torch.bfloat16 if codes.is_cuda else torch.float32)
+    if out is None:
+        out = torch.zeros((R, K), dtype=torch.float32, device=codes.device)
+    if not codes.is_cuda:
+        return out.add_(t.float().t() @ x)
+    from .gemm import gemm, pick_splits
+
+    with _device_of(codes):
+        return gemm(t, x, trans_a=True, trans_b=True, out=out, accumulate=True, splits=pick_splits((K + 255) // 256, (T + 63) // 64))
+
+
+def _check_linear(x, codes, scale, what):
+    _check_weight(codes, scale, what)
+    if x.dim() < 1 or x.shape[-1] != codes.shape[1]:
+        raise ValueError(f"{what}: input {tuple(x.shape)} for a weight [{codes.shape[0]}, {codes.shape[1]}]")
+    if x.is_cuda and x.dtype != torch.bfloat16:
+        raise TypeError(f"{what} takes bf16 on the device, got {x.dtype}")
+    if x.device != codes.device:
+        raise ValueError(f"{what}: input on {x.device}, weight on {codes.device}")
+
+
+def fp8_linear(x, codes, scale, bias=None):
+    """``x8 W8^T (+ bias)`` of a frozen block-FP8 weight (codes [N, K], scales [ceil(N / 128), ceil(K / 128)]); ``x`` [..., K] in bf16. The
+    input gradient is ``dy8 W8``; nothing of ``x`` is kept for it."""
+    _check_linear(x, codes, scale, "fp8_linear")
+    shp = x.shape
+    y = _Fp8LinearFn.apply(x.reshape(-1, shp[-1]), codes, scale, bias)
+    return y.view(*shp[:-1], y.shape[-1]).to(x.dtype)
+
+
+def fp8_lora_linear(x, codes, scale, A, B, A16, B16, scaling, blocks, bias=None):
+    """``x8 W8^T + scaling (x A^T) B^T (+ bias)``: ``fp8_linear`` with the adapter of ``ops.lora.lora_linear`` (same arguments). The 8-bit
+    rows of ``x`` are kept for ``dA = (scaling dy B)^T x8``."""
+    _check_linear(x, codes, scale, "fp8_lora_linear")
+    shp = x.shape
+    x2 = x.reshape(-1, shp[-1])
+    if not x.is_cuda:
+        y = _Fp8LinearFn.apply(x2, codes, scale, bias).to(x.dtype)
+        y = y + scaling * ((x2 @ A.to(x2.dtype).t()) @ B.to(x2.dtype).t())
+        return y.view(*shp[:-1], y.shape[-1])
+    y = _Fp8LoRALinearFn.apply(x2.contiguous(), codes, scale, A, B, A16, B16, float(scaling), blocks, bias)
+    return y.view(*shp[:-1], y.shape[-1])

@@ -147,8 +147,47 @@ class DiskStore(HostStore):
         super()._request(h)
 
 
+class Fp8Store:
+    """Checkpointed layer inputs stay on the device in 8 bits (E4M3 with a power-of-two scale for each row and 128 columns, half of what
+    bf16 takes): one kernel each way, no copy engine and no host memory. ``get`` returns the values that the codes stand for, so the
+    recomputation sees a rounded layer input; the layer's own forward pass has seen the exact one."""
+
+    def __init__(self, device):
+        self.device = torch.device(device)
+        self.bytes_out = 0
+
+    def put(self, t: torch.Tensor) -> _Handle:
+        from ..ops.fp8 import quantize_fp8_rows
+
+        h = _Handle()
+        h.shape, h.dtype, h.device = t.shape, t.dtype, t.device
+        if t.dtype not in (torch.bfloat16, torch.float16, torch.float32) or t.numel() == 0 or t.dim() == 0:
+            h.gpu = t.detach()                             # kept as it is
+            h.nbytes = t.numel() * t.element_size()
+        else:
+            h.gpu = quantize_fp8_rows(t.detach().reshape(-1, t.shape[-1]))
+            h.nbytes = sum(p.untyped_storage().nbytes() for p in h.gpu)
+        self.bytes_out += h.nbytes
+        return h
+
+    def get(self, h: _Handle) -> torch.Tensor:
+        from ..ops.fp8 import dequantize_fp8_rows
+
+        kept, h.gpu = h.gpu, None
+        if kept is None:
+            raise RuntimeError("this checkpoint has been given back already")
+        if torch.is_tensor(kept):
+            return kept
+        return dequantize_fp8_rows(*kept, dtype=h.dtype).view(h.shape)
+
+    def reset(self):
+        pass
+
+
 def make_store(mode, device, directory=None):
-    """``mode``: True / "legacy" / "hidden_states" -> pinned host memory, "disk" -> files."""
+    """``mode``: True / "legacy" / "hidden_states" -> pinned host memory, "disk" -> files, "fp8" -> on the device in 8 bits."""
+    if mode == "fp8":
+        return Fp8Store(device)
     if mode == "disk":
         return DiskStore(device, directory)
     return HostStore(device)

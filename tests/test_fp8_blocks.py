@@ -1,0 +1,391 @@
+"""8-bit blocks (``ops/fp8.py``): rows and weights in E4M3 with scales for blocks of 128, the products on them, the layers and the
+checkpoint store. Expected values come from the definitions in 64 bits.
+
+Tolerances. Codes and what they stand for are compared exactly: a power-of-two scale leaves one nearest E4M3 number. A product of M x K
+by K x N is rounded to bf16 once (2^-8 relative) after sums in fp32: each of the K products of a row enters one addition in the tensor
+core and each of the K / 128 blocks one scaled addition, every one off by at most 2^-23 of the sum of magnitudes (the tensor core may
+drop bits instead of rounding), so |y - exact| <= 2^-8 |exact| + (K + 2 K / 128 + 4) 2^-23 sum |x8| |w8| (1 + 2^-8)."""
+import math
+
+import pytest
+import torch
+
+from axolotl_b200.ops.fp8 import (dequantize_fp8_rows, dequantize_fp8_weight, fp8_adapter_grad, fp8_gemm, fp8_linear, fp8_lora_linear,
+                                  quantize_fp8_rows, quantize_fp8_weight)
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+BF16, EPS32 = 2.0 ** -8, 2.0 ** -23
+
+
+def _table():
+    """The finite numbers of E4M3 by their definition: sign, four exponent bits with bias 7, three of mantissa."""
+    vals = {}
+    for c in range(127):
+        e, m = c >> 3, c & 7
+        vals[c] = (m / 8) * 2.0 ** -6 if e == 0 else (1 + m / 8) * 2.0 ** (e - 7)
+    return torch.tensor([vals[c] for c in range(127)], dtype=torch.float64)
+
+
+def _codes_by_search(x):
+    """(values q s, scales) of rows, by search in the table in 64 bits; x finite."""
+    T, K = x.shape
+    table = _table()
+    nb = -(-K // 128)
+    out, scales = torch.zeros(T, K, dtype=torch.float64), torch.ones(nb, T, dtype=torch.float64)
+    for b in range(nb):
+        v = x[:, b * 128:(b + 1) * 128].double()
+        for t in range(T):
+            top = v[t].abs().max().item()
+            s = 1.0
+            if top > 0:
+                e = math.frexp(top / 448)[1]              # 64 bits: exact to far below a bf16 or fp32 step
+                s = 2.0 ** (e - 1) if top == 448 * 2.0 ** (e - 1) else 2.0 ** e
+                s = max(s, 2.0 ** -126)
+            u = v[t].abs() / s
+            i = torch.searchsorted(table, u).clamp(max=126)
+            lo = (i - 1).clamp(min=0)
+            dl, dh = u - table[lo], table[i] - u
+            pick = torch.where((dl < dh) | ((dl == dh) & (lo % 2 == 0)), lo, i)
+            pick = torch.where(table[pick] * s < 2.0 ** 128, pick, lo)      # a finite value stays finite
+            out[t, b * 128:(b + 1) * 128] = table[pick] * s * v[t].sign()
+            scales[b, t] = s
+    return out, scales
+
+
+def _weight8(codes, scale):
+    n, k = codes.shape
+    return codes.cpu().double() * scale.cpu().double().repeat_interleave(128, 0)[:n].repeat_interleave(128, 1)[:, :k]
+
+
+def _make(shape, seed, dtype=torch.bfloat16, spread=2.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * torch.exp(spread * torch.randn(shape[0], 1, generator=g))).to(dtype)
+
+
+def _assert_product(y, a, b, extra=None, terms=0):
+    """y [M, N] bf16 against a [M, K] b [K, N] (+ a2 b2) in 64 bits."""
+    want, size = a @ b, a.abs() @ b.abs()
+    K = a.shape[1]
+    if extra is not None:
+        want, size = want + extra[0] @ extra[1], size + extra[0].abs() @ extra[1].abs()
+        K += extra[0].shape[1]
+    tol = BF16 * want.abs() + (K + 2 * (K // 128 + 1) + 4 + terms) * EPS32 * size * (1 + BF16) + 1e-38
+    diff = (y.cpu().double() - want).abs()
+    assert y.dtype == torch.bfloat16 and (diff <= tol).all(), f"worst excess {(diff - tol).max().item()}"
+
+
+# ------------------------------------------------------------------ rows
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("T,K", [(1, 1), (1, 128), (3, 127), (2, 129), (9, 200), (5, 1032), (17, 2056)])
+def test_rows_are_the_nearest_codes(T, K, dtype, dev):
+    x = _make((T, K), T * 1000 + K, dtype)
+    x[0, : min(K, 3)] = 0
+    codes, scale = quantize_fp8_rows(x.to(dev))
+    want, scales = _codes_by_search(x)
+    assert codes.shape == (T, K) and codes.dtype == torch.float8_e4m3fn and codes.stride(0) % 16 == 0
+    assert torch.equal(scale.cpu().double(), scales)
+    # in fp32 every value of the codes is exact; bf16 holds them too
+    assert torch.equal(dequantize_fp8_rows(codes, scale, torch.float32).cpu().double(), want)
+    assert torch.equal(dequantize_fp8_rows(codes, scale).cpu().double(), want)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_rows_ties_borders_and_extremes(dev):
+    """Ties to even, a maximum of exactly 448 2^j and just above, zeros, the smallest and largest numbers, subnormal ones."""
+    x = torch.zeros(8, 256)
+    x[0, :6] = torch.tensor([448.0, 1.0625, 1.1875, 17.0, 19.0, -17.0])           # scale 1, ties between codes
+    x[1, :2] = torch.tensor([450.0, 3.0])                                         # just above 448: scale 2
+    x[2, 0] = torch.finfo(torch.bfloat16).max
+    x[3, :2] = torch.tensor([2.0 ** -133, -(2.0 ** -130)])                        # bf16 subnormals: scale 2^-126
+    x[4, 130] = 3.5
+    x[5, :3] = torch.tensor([448.0 * 2 ** -20, 2.0 ** -30, 2.0 ** -31])
+    x[6, :3] = torch.tensor([256.0, 2.0 ** -9, 2.0 ** -10])                       # smallest code, half of it (a tie with zero)
+    x = x.bfloat16()
+    codes, scale = quantize_fp8_rows(x.to(dev))
+    want, scales = _codes_by_search(x)
+    assert torch.equal(scale.cpu().double(), scales) and scale[0, 7] == 1 and scale[0, 0] == 1 and scale[0, 1] == 2
+    assert torch.equal(dequantize_fp8_rows(codes, scale, torch.float32).cpu().double(), want)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_rows_nan_and_infinity_leave_their_neighbours_alone(dev):
+    x = _make((4, 300), 3)
+    y = x.clone()
+    y[0, 5], y[1, 130], y[2, 299], y[3, :128] = float("nan"), float("inf"), float("-inf"), float("nan")
+    x[0, 5] = x[1, 130] = x[2, 299] = 0                   # what the others' maximum is taken over
+    x[3, :128] = 0
+    want, got = (dequantize_fp8_rows(*quantize_fp8_rows(t.to(dev))).cpu() for t in (x, y))
+    odd = ~torch.isfinite(y)
+    assert torch.equal(torch.isnan(got), odd) and torch.equal(got[~odd], want[~odd])
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_rows_of_other_strides(dev):
+    base = _make((12, 700), 5).to(dev)
+    for x in (base[:, 1:650], base[::2, 8:520], base.t()[:300], base[3:4].expand(5, 700), base[:, :1].expand(12, 256)):
+        codes, scale = quantize_fp8_rows(x)
+        want, scales = quantize_fp8_rows(x.clone().contiguous())
+        assert torch.equal(scale, scales) and torch.equal(codes.view(torch.uint8), want.view(torch.uint8))
+        # codes and scales of other strides back
+        odd = torch.empty(codes.shape[0], codes.shape[1] + 3, dtype=torch.uint8, device=dev)[:, 3:].view(torch.float8_e4m3fn)
+        odd.view(torch.uint8).copy_(codes.view(torch.uint8))
+        assert torch.equal(dequantize_fp8_rows(odd, scale.t().contiguous().t()), dequantize_fp8_rows(codes, scale))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_rows_none(dev):
+    codes, scale = quantize_fp8_rows(torch.empty(0, 256, dtype=torch.bfloat16, device=dev))
+    assert codes.shape == (0, 256) and scale.shape == (2, 0) and dequantize_fp8_rows(codes, scale).shape == (0, 256)
+
+
+def test_refusals():
+    x = torch.randn(4, 256).bfloat16()
+    codes, scale = quantize_fp8_rows(x)
+    w, ws = quantize_fp8_weight(torch.randn(130, 256))
+    for bad, kind in ((x[0], ValueError), (torch.zeros(3, 0), ValueError), (x.double(), TypeError), (x.int(), TypeError)):
+        with pytest.raises(kind):
+            quantize_fp8_rows(bad)
+    for args, kind in (((codes.view(torch.uint8), scale), TypeError), ((codes, scale.t()), ValueError), ((codes, scale.double()), ValueError),
+                       ((codes, scale[:1]), ValueError), ((codes[0], scale), ValueError), ((codes, scale, torch.float64), TypeError)):
+        with pytest.raises(kind):
+            dequantize_fp8_rows(*args)
+    for bad in (torch.zeros(0, 5), torch.zeros(3)):
+        with pytest.raises(ValueError):
+            quantize_fp8_weight(bad)
+    for args, kind in (((codes[:, :128], scale[:1], w, ws), ValueError), ((codes, scale, w, ws[:1]), ValueError),
+                       ((codes, scale, w.view(torch.uint8), ws), TypeError), ((codes, scale[:, :3], w, ws), ValueError)):
+        with pytest.raises(kind):
+            fp8_gemm(*args)
+    with pytest.raises(ValueError):
+        fp8_gemm(codes, scale, w, ws, a2=torch.zeros(4, 8).bfloat16(), b2=torch.zeros(8, 130).bfloat16())
+    for args in ((x[:, :200], w, ws), (x, w, ws[:, :1]), (x.to("meta"), w, ws)):
+        with pytest.raises(ValueError):
+            fp8_linear(*args)
+    for args, kw in (((torch.zeros(5, 8).bfloat16(), codes, scale), {}), ((torch.zeros(4).bfloat16(), codes, scale), {}),
+                     ((torch.zeros(4, 8).bfloat16(), codes, scale), dict(out=torch.zeros(8, 255))),
+                     ((torch.zeros(4, 8).bfloat16(), codes, scale), dict(out=torch.zeros(8, 256).bfloat16()))):
+        with pytest.raises(ValueError):
+            fp8_adapter_grad(*args, **kw)
+
+
+# ------------------------------------------------------------------ weights and products
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("N,K", [(1, 1), (128, 128), (130, 200), (300, 129)])
+def test_weight_codes_are_half_a_step_off(N, K, dev):
+    w = _make((N, K), N + K, torch.float32, 1.0)
+    w[0, : K // 2] = 0
+    codes, scale = quantize_fp8_weight(w.to(dev))
+    assert codes.shape == (N, K) and codes.stride(0) % 16 == 0 and scale.shape == (-(-N // 128), -(-K // 128))
+    back = _weight8(codes, scale)
+    s = scale.cpu().double().repeat_interleave(128, 0)[:N].repeat_interleave(128, 1)[:, :K]
+    # half a step of E4M3, 2^-4 relative or 2^-10 of the scale below its normal range, and the fp32 division's rounding
+    assert ((back - w.double()).abs() <= torch.maximum(w.double().abs() * 2.0 ** -4, s * 2.0 ** -10) * (1 + 2.0 ** -20)).all()
+    got = dequantize_fp8_weight(codes, scale).cpu().double()
+    assert ((got - back).abs() <= BF16 * back.abs()).all()
+
+
+PRODUCTS = [(1, 1, 1), (1, 16, 128), (5, 130, 300), (33, 128, 256), (128, 128, 128), (129, 257, 384), (200, 520, 1032), (300, 1000, 136)]
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("trans", [False, True])
+@pytest.mark.parametrize("M,N,K", PRODUCTS)
+def test_product(M, N, K, trans, dev):
+    x = _make((M, K), M + N + K, spread=1.0)
+    codes, scale = quantize_fp8_rows(x.to(dev))
+    w, ws = quantize_fp8_weight(_make((K, N) if trans else (N, K), 7 * M + K, torch.float32, 1.0).to(dev))
+    y = fp8_gemm(codes, scale, w, ws, trans_w=trans)
+    x8, w8 = dequantize_fp8_rows(codes, scale, torch.float32).cpu().double(), _weight8(w, ws)
+    _assert_product(y, x8, w8 if trans else w8.t())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tile", [128, 256])
+@pytest.mark.parametrize("trans", [False, True])
+@pytest.mark.parametrize("rank", [0, 8, 16, 72])
+def test_product_tiles_and_extension(tile, trans, rank, monkeypatch):
+    """Both tile sizes whatever the rule picks, with and without the bf16 K-extension, more tiles than workers."""
+    from axolotl_b200.ops import fp8
+
+    monkeypatch.setattr(fp8, "_tile", lambda M, N, *a: tile)
+    for M, N, K in ((130, 264, 200), (2100, 2600, 256)):
+        x = _make((M, K), M, spread=1.0).cuda()
+        codes, scale = quantize_fp8_rows(x)
+        w, ws = quantize_fp8_weight(_make((K, N) if trans else (N, K), K, torch.float32, 1.0).cuda())
+        a2 = _make((M, rank), 3, spread=0.0).cuda() if rank else None
+        b2 = _make((rank, N) if trans else (N, rank), 4, spread=0.0).cuda() if rank else None
+        y = fp8_gemm(codes, scale, w, ws, trans_w=trans, a2=a2, b2=b2)
+        x8, w8 = dequantize_fp8_rows(codes, scale, torch.float32).cpu().double(), _weight8(w, ws)
+        ext = (a2.cpu().double(), (b2 if trans else b2.t()).cpu().double()) if rank else None
+        _assert_product(y, x8, w8 if trans else w8.t(), ext)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_product_of_nan_rows(dev):
+    """A NaN in one row of the input is that row's alone; a NaN code of the weight is its output column's."""
+    x = _make((140, 256), 1, spread=0.0)
+    w, ws = quantize_fp8_weight(_make((136, 256), 2, torch.float32, 0.0).to(dev))
+    clean = fp8_linear(x.to(dev), w, ws)
+    x[3, 17], x[139, 200] = float("nan"), float("inf")
+    got = fp8_linear(x.to(dev), w, ws)
+    rows = torch.tensor([i not in (3, 139) for i in range(140)])
+    assert torch.isnan(got[~rows]).all() and torch.equal(got[rows], clean[rows])
+    wn = w.clone()
+    wn[100, 9] = float("nan")
+    col = fp8_linear(_make((140, 256), 1, spread=0.0).to(dev), wn, ws)
+    cols = torch.arange(136) != 100
+    assert torch.isnan(col[:, 100]).all() and torch.equal(col[:, cols], clean[:, cols])
+
+
+# ------------------------------------------------------------------ layers
+def _rows8(x):
+    return dequantize_fp8_rows(*quantize_fp8_rows(x.cpu()), dtype=torch.float32).double()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("shape,N", [((3, 7, 200), 136), ((1, 128), 16), ((260, 264), 520)])
+def test_linear_and_its_input_gradient(shape, N, dev):
+    K = shape[-1]
+    x = _make((math.prod(shape[:-1]), K), K, spread=0.5).view(shape)
+    dy = _make((math.prod(shape[:-1]), N), N, spread=0.5).view(*shape[:-1], N) * 1e-3
+    dy[..., :1, :] = 0
+    w, ws = quantize_fp8_weight(_make((N, K), 5, torch.float32, 0.0).to(dev))
+    xl = x.to(dev).requires_grad_(True)
+    y = fp8_linear(xl, w, ws)
+    (dx,) = torch.autograd.grad(y, [xl], dy.to(dev))
+    w8 = _weight8(w, ws)
+    assert y.shape == (*shape[:-1], N) and dx.shape == shape
+    _assert_product(y.reshape(-1, N), _rows8(x.reshape(-1, K)), w8.t())
+    _assert_product(dx.reshape(-1, K), _rows8(dy.reshape(-1, N)), w8)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_linear_bias_and_its_gradient(dev):
+    x, w32 = _make((40, 256), 1, spread=0.0), _make((64, 256), 2, torch.float32, 0.0)
+    w, ws = quantize_fp8_weight(w32.to(dev))
+    bias = _make((1, 64), 3, spread=0.0)[0].to(dev).requires_grad_(True)
+    y = fp8_linear(x.to(dev), w, ws, bias)
+    assert torch.equal(y, fp8_linear(x.to(dev), w, ws) + bias)
+    dy = _make((40, 64), 4, spread=0.0)
+    (db,) = torch.autograd.grad(y, [bias], dy.to(dev))
+    want = dy.double().sum(0)
+    assert ((db.cpu().double() - want).abs() <= BF16 * want.abs() + 40 * EPS32 * dy.double().abs().sum(0)).all()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_linear_gradient_by_differences(dev):
+    """Where every value is its own code (small integers; weights that are powers of two) the layer is linear without rounding: the
+    gradient is what differences give, exactly."""
+    g = torch.Generator().manual_seed(0)
+    x = torch.randint(-2, 3, (6, 128), generator=g).bfloat16()
+    x[:, 0] = 2                                            # the block's maximum stays where it is
+    w = torch.where(torch.rand(16, 128, generator=g) < 0.1, 0.5, 0.0)
+    w[0, 0] = 0.5
+    codes, scale = quantize_fp8_weight(w.to(dev))
+    dy = torch.randint(-2, 3, (6, 16), generator=g).bfloat16()
+    xl = x.to(dev).requires_grad_(True)
+    (dx,) = torch.autograd.grad(fp8_linear(xl, codes, scale), [xl], dy.to(dev))
+    for t, k in ((0, 1), (3, 77), (5, 127)):
+        step = torch.zeros(6, 128).bfloat16()
+        step[t, k] = 1
+        up, down = (fp8_linear((x + d * step).to(dev), codes, scale).cpu().double() for d in (1, -1))
+        assert ((up - down) * dy.double()).sum() / 2 == dx[t, k].cpu().double()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,K,N,blocks", [(1, 256, 128, ((0, 128, 0, 8),)), (70, 520, 264, ((0, 200, 0, 8), (200, 64, 8, 8))),
+                                          (600, 1024, 640, ((0, 640, 0, 16),)), (700, 264, 1032, ((128, 904, 0, 32),))])
+def test_lora_linear_and_its_gradients(T, K, N, blocks):
+    R = sum(b[3] for b in blocks)
+    x, dy = _make((T, K), 1, spread=0.5), _make((T, N), 2, spread=0.5) * 1e-2
+    dy[: T // 3] = 0
+    w, ws = quantize_fp8_weight(_make((N, K), 3, torch.float32, 0.0).cuda())
+    A = _make((R, K), 4, torch.float32, 0.0) * K ** -0.5
+    B = torch.zeros(N, R)
+    for r0, rows, c0, r in blocks:
+        B[r0:r0 + rows, c0:c0 + r] = _make((rows, r), 5, torch.float32, 0.0) * 0.1
+    A16, B16 = A.bfloat16(), B.bfloat16()
+    xl, Al, Bl = x.cuda().requires_grad_(True), A.cuda().requires_grad_(True), B.cuda().requires_grad_(True)
+    y = fp8_lora_linear(xl, w, ws, Al, Bl, A16.cuda(), B16.cuda(), 2.0, blocks)
+    dx, dA, dB = torch.autograd.grad(y, [xl, Al, Bl], dy.cuda())
+    a, b, w8, x64, dy64 = A16.double(), B16.double(), _weight8(w, ws), x.double(), dy.double()
+    x8 = _rows8(x)
+    low, tall = 2 * x64 @ a.t(), 2 * dy64 @ b
+    # the two low-rank products are rounded to bf16 after sums of K or N terms: each is off by 2^-8 of itself and that
+    low_e = BF16 * low.abs() + (K + 2) * EPS32 * 2 * x64.abs() @ a.abs().t()
+    tall_e = BF16 * tall.abs() + (N + 2) * EPS32 * 2 * dy64.abs() @ b.abs()
+
+    def near(got, want, off, terms):
+        tol = off + terms * EPS32 * (want.abs() + off)
+        assert ((got.cpu().double() - want).abs() <= tol + 1e-30).all()
+
+    want = x8 @ w8.t() + low @ b.t()
+    size = x8.abs() @ w8.abs().t() + low.abs() @ b.abs().t()
+    near(y, want, BF16 * want.abs() + (low_e @ b.abs().t() + (K + R + 40) * EPS32 * size) * (1 + BF16), 4)
+    dy8 = _rows8(dy)
+    want = dy8 @ w8 + tall @ a
+    size = dy8.abs() @ w8.abs() + tall.abs() @ a.abs()
+    near(dx, want, BF16 * want.abs() + (tall_e @ a.abs() + (N + R + 40) * EPS32 * size) * (1 + BF16), 4)
+    near(dA, tall.t() @ x8, tall_e.t() @ x8.abs() + (T + 8) * EPS32 * tall.abs().t() @ x8.abs(), 4)
+    wantB, offB = dy64.t() @ low, dy64.abs().t() @ low_e + (T + 8) * EPS32 * dy64.abs().t() @ low.abs()
+    for r0, rows, c0, r in blocks:
+        near(dB[r0:r0 + rows, c0:c0 + r], wantB[r0:r0 + rows, c0:c0 + r], offB[r0:r0 + rows, c0:c0 + r], 4)
+    assert (dB.cpu()[B == 0] == 0).all() or len(blocks) == 1
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("T,K,R", [(1, 128, 8), (77, 200, 16), (300, 1000, 40), (1030, 264, 64)])
+def test_adapter_gradient_from_saved_rows(T, K, R, dev):
+    x, t = _make((T, K), T + K, spread=0.5), _make((T, R), R, spread=0.5)
+    codes, scale = quantize_fp8_rows(x.to(dev))
+    want, size = t.double().t() @ _rows8(x), t.double().abs().t() @ _rows8(x).abs()
+    tol = (T + 16) * EPS32 * size + 1e-30                   # T products in fp32 sums
+    got = fp8_adapter_grad(t.to(dev), codes, scale)
+    assert got.dtype == torch.float32 and ((got.cpu().double() - want).abs() <= tol).all()
+    base = _make((R, K), 9, torch.float32, 0.0)
+    into = base.clone().to(dev)
+    assert fp8_adapter_grad(t.to(dev), codes, scale, out=into) is into
+    assert ((into.cpu().double() - base.double() - want).abs() <= tol + (T + 16) * EPS32 * base.double().abs()).all()
+
+
+# ------------------------------------------------------------------ checkpoints
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_store_gives_back_the_coded_values(dtype, dev):
+    from axolotl_b200.train.activation_memory import make_store
+
+    store = make_store("fp8", dev)
+    for shape in ((5, 300), (2, 3, 128), (7,), (0, 64), ()):
+        x = torch.randn(shape).to(dtype).to(dev)
+        got = store.get(store.put(x))
+        assert got.shape == x.shape and got.dtype == dtype and got.device == x.device
+        if x.dim() and x.numel():
+            want = _codes_by_search(x.cpu().reshape(-1, shape[-1]))[0].to(dtype).view(shape)
+            assert torch.equal(got.cpu(), want)
+        else:
+            assert torch.equal(got, x)
+    ids = torch.arange(6, device=dev)
+    h = store.put(ids)
+    assert torch.equal(store.get(h), ids)
+    with pytest.raises(RuntimeError):
+        store.get(h)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_checkpoint_recomputes_from_the_coded_input(dev):
+    """The forward pass sees the exact layer input, the recomputation the coded one: gradients are those of the layer at ``x8``."""
+    from axolotl_b200.train.activation_memory import make_store, offloaded_checkpoint
+
+    g = torch.Generator().manual_seed(2)
+    W = torch.randn(128, 128, generator=g).to(dev).requires_grad_(True)
+    x = torch.randn(64, 128, generator=g).to(dev).requires_grad_(True)
+    dy = torch.randn(64, 128, generator=g).to(dev)
+    layer = lambda h, r: (torch.tanh(h @ W), h if r is None else r)
+    y, _ = offloaded_checkpoint(layer, make_store("fp8", dev), (x, None))
+    assert torch.equal(y, torch.tanh(x @ W))
+    y.backward(dy)
+    x8 = dequantize_fp8_rows(*quantize_fp8_rows(x.detach()), dtype=torch.float32).requires_grad_(True)
+    W2 = W.detach().clone().requires_grad_(True)
+    torch.tanh(x8 @ W2).backward(dy)
+    assert torch.equal(x.grad, x8.grad) and torch.equal(W.grad, W2.grad)
