@@ -646,8 +646,8 @@ def check_gradient_checkpointing_w_offload(c):
 @rule
 def check_activation_offloading_wo_gc(c):
     ao = c.get("activation_offloading")
-    if ao and ao not in (True, "legacy", "disk", "hidden_states"):
-        raise ValueError(f"unknown activation_offloading mode '{ao}' (true, legacy, disk or hidden_states)")
+    if ao and ao not in (True, "legacy", "disk", "hidden_states", "fp8"):
+        raise ValueError(f"unknown activation_offloading mode '{ao}' (true, legacy, disk, hidden_states or fp8)")
     if ao and not c.get("gradient_checkpointing"):
         raise ValueError("activation_offloading requires gradient_checkpointing")
 

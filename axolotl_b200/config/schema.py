@@ -540,6 +540,7 @@ class AxolotlConfig(_Base):
     # ---- MoE
     experts_implementation: str | None = None
     router_aux_loss_coef: float | None = None
+    base_weights_fp8: bool | None = None  # extension: frozen projections in E4M3 with 128 x 128 block scales, products in 8 bits
     expert_weights_nvfp4: bool | None = None  # extension: quantise frozen expert weights to NVFP4 at load
     # ---- misc
     plugins: list[str] | None = None

@@ -282,6 +282,18 @@ AXB_DEVICE void umma_f16(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint
       : "r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// the same with 8-bit floating-point operands, 32 columns of K an instruction
+AXB_DEVICE void umma_f8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
+      "}\n"
+      :
+      : "r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
 // the same with A in tensor memory (K-major: column c of a lane holds elements 2c and 2c + 1 of its row)
 AXB_DEVICE void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -554,6 +566,13 @@ AXB_DEVICE uint64_t mul_f32x2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
+}
+
+// 8-bit rows (fp8_rows.cu): biased exponent of the scale of a block whose largest magnitude is `top`
+AXB_DEVICE int fp8_scale_exponent(float top) {
+  const uint32_t b = __float_as_uint(top);
+  const int e = (int)(b >> 23) - 8 + ((b & 0x7FFFFFu) > 0x600000u ? 1 : 0);   // 448 = 1.75 * 2^8
+  return top == 0.f ? 127 : max(e, 1);
 }
 
 // Row `lane` of a 32-row staging tile with 128-byte rows (64 bf16) and the 128-byte swizzle the

@@ -7,10 +7,18 @@
 // A2 / B2: bf16 K-extension, the low-rank update of an adapter, accumulated as further blocks of scale 1.
 //
 // The scales change every 128 columns of K, so an accumulator cannot stay in TMEM: the four MMAs of a block start a new one, and
-// eight epilogue warps add it, times its scale, to fp32 sums in registers (packed fused multiply-adds) while the tensor cores work
-// on the next. A thread owns a row: one scale for all its columns. Tiles: 256 x 256 by a CTA pair (two accumulators of 256 columns,
-// 128 sums a thread) and 128 x 128 by one CTA (four accumulators of 128 columns).
+// eight epilogue warps add it, times its scale, to fp32 sums in registers while the tensor cores work on the next. A thread owns a
+// row: one scale for all its columns of a weight block.
+// Tiles: 256 x 256 by a CTA pair, 128 x 128 by one CTA. In the pair a block is two products of 128 columns with two accumulators each
+// (columns of both CTAs' B rows: 64 h .. of either), one for each half of the epilogue warps, so that one half drains its
+// accumulator while the other's is computed.
 #include "axb_common.cuh"
+
+extern "C" int axb_fp8_quantize_rows(const void* x, long long ldx, int dtype, void* q, long long ldq, float* s, long long lds,
+                                     long long rows, int K, void* stream);
+extern "C" int axb_fp8_skinny(const void* x, long long ldx, const void* W, long long ldw, const float* sw, long long sw_n, long long sw_k,
+                              void* y, long long ldy, int T, int N, int K, const void* X2, long long ldx2, const void* B2, long long ldb2,
+                              int K2, int* status, void* stream);
 
 namespace {
 
@@ -33,17 +41,6 @@ struct Fp8GemmParams {
   int* status;
 };
 
-AXB_DEVICE void umma_f8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t"
-      ".reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
-      "}\n"
-      :
-      : "r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
 AXB_DEVICE void umma_f8_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t"
@@ -54,6 +51,10 @@ AXB_DEVICE void umma_f8_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, 
       :
       : "r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
       : "memory");
+}
+// MN-major tile in chunks of 64 codes: 64-byte rows, one k each, 64-byte swizzle (8-row atoms of 512 bytes); lbo = bytes between chunks.
+AXB_DEVICE uint64_t make_smem_desc_sw64(uint32_t saddr, uint32_t lbo_bytes) {
+  return (make_smem_desc_sw128(saddr, lbo_bytes, 512) & ~(7ull << 61)) | (4ull << 61);
 }
 // Instruction descriptor, kind::f8f6f4: E4M3 operands (format 0), fp32 accumulator.
 AXB_DEVICE constexpr uint32_t make_idesc_e4m3(int m, int n, int b_mn_major) {
@@ -75,16 +76,17 @@ __global__ void __launch_bounds__(G_THREADS, 1)
                     const __grid_constant__ CUtensorMap tmC, const Fp8GemmParams p) {
   constexpr int CTAS = PAIR ? 2 : 1;
   constexpr int TILE = 128 * CTAS;             // rows and columns of a tile
-  constexpr int COLS = TILE / 2;               // columns of an epilogue warp
-  constexpr int ACCS = 512 / TILE;             // accumulators in TMEM
+  constexpr int SETS = CTAS;                   // products of 128 columns a block
+  constexpr int BUFS = 4 / SETS;               // accumulators of each
+  constexpr int GROUPS = SETS;                 // groups of 64 columns that an epilogue warp owns
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* sEpi = smem + G_STAGES * G_STAGE;
   uint64_t* full = reinterpret_cast<uint64_t*>(sEpi + G_EPI);   // leader's: both CTAs' loads of the stage
   uint64_t* empty = full + G_STAGES;                            // one per CTA
-  uint64_t* tfull = empty + G_STAGES;                           // one per CTA
-  uint64_t* tempty = tfull + ACCS;                              // leader's: eight warps of every CTA
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + ACCS);
+  uint64_t* tfull = empty + G_STAGES;                           // [set][buffer], one per CTA
+  uint64_t* tempty = tfull + 4;                                 // leader's: the epilogue warps that read the accumulator
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 4);
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
   const int rank = PAIR ? (int)cluster_ctarank() : 0;
   const int worker = blockIdx.x / CTAS, workers = gridDim.x / CTAS;
@@ -96,9 +98,9 @@ __global__ void __launch_bounds__(G_THREADS, 1)
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    for (int s = 0; s < ACCS; ++s) {
+    for (int s = 0; s < 4; ++s) {
       mbar_init(&tfull[s], 1);
-      mbar_init(&tempty[s], 8 * CTAS);
+      mbar_init(&tempty[s], 8);
     }
     mbar_fence_init();
     tma_prefetch_desc(&tmA);
@@ -141,19 +143,14 @@ __global__ void __launch_bounds__(G_THREADS, 1)
             else tma_load_2d(dst, m, &full[stage], c0, c1);
           };
           if (rank == 0) mbar_expect_tx(&full[stage], CTAS * G_STAGE);
-          if (!ext) {
-            load(a, &tmA, kb * 128, m0);
-            if (B_MN) load(b, &tmB, n0, kb * 128);
-            else load(b, &tmB, kb * 128, n0);
+          const CUtensorMap* mb = ext ? &tmB2 : &tmB;
+          const int ka = ext ? (kb - nk_main) * 64 : kb * 128;
+          load(a, ext ? &tmA2 : &tmA, ka, m0);
+          if (B_MN) {
+            load(b, mb, n0, ka);
+            load(b + G_OP / 2, mb, n0 + 64, ka);
           } else {
-            const int k0 = (kb - nk_main) * 64;
-            load(a, &tmA2, k0, m0);
-            if (B_MN) {
-              load(b, &tmB2, n0, k0);
-              load(b + G_OP / 2, &tmB2, n0 + 64, k0);
-            } else {
-              load(b, &tmB2, k0, n0);
-            }
+            load(b, mb, ka, n0);
           }
         }
         __syncwarp();
@@ -165,54 +162,66 @@ __global__ void __launch_bounds__(G_THREADS, 1)
     }
   } else if (warp == 1) {
     if (rank == 0) {
-      constexpr uint32_t id8 = make_idesc_e4m3(TILE, TILE, B_MN ? 1 : 0);
-      constexpr uint32_t id16 = make_idesc_bf16(TILE, TILE, 0, B_MN ? 1 : 0);
+      constexpr uint32_t id8 = make_idesc_e4m3(TILE, 128, B_MN ? 1 : 0);
+      constexpr uint32_t id16 = make_idesc_bf16(TILE, 128, 0, B_MN ? 1 : 0);
       const uint64_t base_a = make_smem_desc_sw128(smem_u32(smem), 16, 1024);
-      // MN-major: 128 codes (one 1024-byte atom per 8 k) or two chunks of 64 bf16, G_OP / 2 apart
-      const uint64_t base_b = make_smem_desc_sw128(smem_u32(smem + G_OP), B_MN ? G_OP / 2 : 16, 1024);
-      int stage = 0, acc = 0;
-      uint32_t phase = 0, acc_phase = 0;
+      // MN-major: two chunks of 64 columns (64-byte rows of codes, 128-byte rows of bf16), G_OP / 2 apart
+      const uint64_t base_b8 = B_MN ? make_smem_desc_sw64(smem_u32(smem + G_OP), G_OP / 2) : base_a + G_OP / 16;
+      const uint64_t base_b16 = B_MN ? make_smem_desc_sw128(smem_u32(smem + G_OP), G_OP / 2, 1024) : base_a + G_OP / 16;
+      int stage = 0, buf = 0;
+      uint32_t phase = 0, buf_phase = 0;
       bool ok = true;
       for (int tile = worker; tile < tiles && ok; tile += workers) {
-        for (int kb = 0; kb < nk; ++kb) {
-          ok = warp_all(mbar_wait_spin(&tempty[acc], acc_phase ^ 1, p.status, AXB_TIMEOUT_TMEM_EMPTY) &&
-                        mbar_wait_spin(&full[stage], phase, p.status, AXB_TIMEOUT_FULL));
+        for (int kb = 0; kb < nk && ok; ++kb) {
+          ok = warp_all(mbar_wait_spin(&full[stage], phase, p.status, AXB_TIMEOUT_FULL));
           if (!ok) break;
-          tc_fence_after();
-          const uint64_t a = base_a + (uint32_t)(stage * (G_STAGE / 16)), b = base_b + (uint32_t)(stage * (G_STAGE / 16));
-          const uint32_t d = tmem + acc * TILE;
-          if (elect_one()) {
-            if (kb < nk_main) {
+          const uint32_t at = (uint32_t)(stage * (G_STAGE / 16));
+          const uint64_t a = base_a + at;
 #pragma unroll
-              for (int kk = 0; kk < 4; ++kk) {  // 32 codes each
-                const uint64_t bk = b + kk * (B_MN ? 4096 / 16 : 2);
-                if constexpr (PAIR) umma_f8_pair(d, a + kk * 2, bk, id8, kk > 0 ? 1u : 0u);
-                else umma_f8(d, a + kk * 2, bk, id8, kk > 0 ? 1u : 0u);
+          for (int h = 0; h < SETS; ++h) {
+            // the arrivals order no memory but the reads of TMEM: a release of every access in flight would wait for the scales that
+            // were requested for the next block (4096 x 8192 by 4096: 257 us with it, 131 without)
+            uint64_t* free = &tempty[h * BUFS + buf];
+            ok = warp_all(PAIR ? mbar_wait_partner(free, buf_phase ^ 1, p.status, AXB_TIMEOUT_TMEM_EMPTY)
+                               : mbar_wait_spin(free, buf_phase ^ 1, p.status, AXB_TIMEOUT_TMEM_EMPTY));
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t d = tmem + (h * BUFS + buf) * 128;
+            if (elect_one()) {
+              if (kb < nk_main) {
+                const uint64_t b = base_b8 + at + h * (G_OP / 2 / 16);
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk) {  // 32 codes each
+                  const uint64_t bk = b + kk * (B_MN ? 2048 / 16 : 2);
+                  if constexpr (PAIR) umma_f8_pair(d, a + kk * 2, bk, id8, kk > 0 ? 1u : 0u);
+                  else umma_f8(d, a + kk * 2, bk, id8, kk > 0 ? 1u : 0u);
+                }
+              } else {
+                const uint64_t b = base_b16 + at + h * (G_OP / 2 / 16);
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk) {  // 16 bf16 each
+                  const uint64_t bk = b + kk * (B_MN ? 2048 / 16 : 2);
+                  if constexpr (PAIR) umma_f16_pair(d, a + kk * 2, bk, id16, kk > 0 ? 1u : 0u);
+                  else umma_f16(d, a + kk * 2, bk, id16, kk > 0 ? 1u : 0u);
+                }
               }
-            } else {
-#pragma unroll
-              for (int kk = 0; kk < 4; ++kk) {  // 16 bf16 each
-                const uint64_t bk = b + kk * (B_MN ? 2048 / 16 : 2);
-                if constexpr (PAIR) umma_f16_pair(d, a + kk * 2, bk, id16, kk > 0 ? 1u : 0u);
-                else umma_f16(d, a + kk * 2, bk, id16, kk > 0 ? 1u : 0u);
+              if constexpr (PAIR) {
+                umma_commit_pair_mc(&tfull[h * BUFS + buf]);
+                if (h == SETS - 1) umma_commit_pair_mc(&empty[stage]);
+              } else {
+                umma_commit(&tfull[h * BUFS + buf]);
+                if (h == SETS - 1) umma_commit(&empty[stage]);
               }
             }
-            if constexpr (PAIR) {
-              umma_commit_pair_mc(&empty[stage]);
-              umma_commit_pair_mc(&tfull[acc]);
-            } else {
-              umma_commit(&empty[stage]);
-              umma_commit(&tfull[acc]);
-            }
+            __syncwarp();
           }
-          __syncwarp();
           if (++stage == G_STAGES) {
             stage = 0;
             phase ^= 1;
           }
-          if (++acc == ACCS) {
-            acc = 0;
-            acc_phase ^= 1;
+          if (++buf == BUFS) {
+            buf = 0;
+            buf_phase ^= 1;
           }
         }
       }
@@ -220,61 +229,70 @@ __global__ void __launch_bounds__(G_THREADS, 1)
   } else {
     const int quad = warp & 3, half = (warp - 2) >> 2;
     uint8_t* stg = sEpi + (warp - 2) * 4096;
-    const uint32_t t_base = tmem + (uint32_t(quad * 32) << 16) + half * COLS;
-    int acc = 0;
-    uint32_t acc_phase = 0;
+    const int set = PAIR ? half : 0;
+    const uint32_t t_base = tmem + (uint32_t(quad * 32) << 16) + (PAIR ? set * BUFS * 128 : half * 64);
+    int buf = 0;
+    uint32_t buf_phase = 0;
     bool ok = true;
     for (int tile = worker; tile < tiles && ok; tile += workers) {
       int m_blk, n_blk;
       fp8_tile(tile, num_m, num_n, p.group_m, m_blk, n_blk);
       const int row0 = m_blk * TILE + rank * 128 + quad * 32, row = row0 + lane;
-      const int col0 = n_blk * TILE + half * COLS;
+      const int col0 = n_blk * TILE + half * 64;                // group g: col0 + 128 g ..
       const bool live = row < p.M;
       const float* sa = p.sa + (live ? row : 0);
-      const float* sb = p.sb + (long long)(min(col0, p.N - 1) >> 7) * p.sb_n;
-      uint64_t sum[COLS / 2];
+      const float* sb = p.sb + (long long)(col0 >> 7) * p.sb_n;
+      const long long sb1 = col0 + 128 < p.N ? p.sb_n : 0;      // of group 1
+      uint64_t sum[GROUPS * 32];
 #pragma unroll
-      for (int j = 0; j < COLS / 2; ++j) sum[j] = 0ull;
-      float next = __ldg(sa) * __ldg(sb);
+      for (int j = 0; j < GROUPS * 32; ++j) sum[j] = 0ull;
+      float na = __ldg(sa), nb0 = __ldg(sb), nb1 = GROUPS > 1 ? __ldg(sb + sb1) : 0.f;   // the next block's, requested a block ahead
       for (int kb = 0; kb < nk; ++kb) {
-        const float sc = next;
-        next = kb + 1 < nk_main ? __ldg(sa + (long long)(kb + 1) * p.ldsa) * __ldg(sb + (long long)(kb + 1) * p.sb_k) : 1.f;
-        ok = warp_all(mbar_wait_spin(&tfull[acc], acc_phase, p.status, AXB_TIMEOUT_TMEM_FULL));
+        const float s0 = na * nb0, s1 = na * nb1;
+        na = nb0 = nb1 = 1.f;
+        if (kb + 1 < nk_main) {
+          sa += p.ldsa;
+          sb += p.sb_k;
+          na = __ldg(sa);
+          nb0 = __ldg(sb);
+          if (GROUPS > 1) nb1 = __ldg(sb + sb1);
+        }
+        ok = warp_all(mbar_wait_spin(&tfull[set * BUFS + buf], buf_phase, p.status, AXB_TIMEOUT_TMEM_FULL));
         if (!ok) break;
         tc_fence_after();
-        const uint64_t sc2 = pack_f32x2(sc, sc);
 #pragma unroll
-        for (int c = 0; c < COLS / 32; ++c) {
-          uint32_t r[32];
-          tmem_ld_32x32(t_base + acc * TILE + c * 32, r);
+        for (int c = 0; c < GROUPS * 4; ++c) {
+          uint32_t r[16];
+          tmem_ld_32x16(t_base + buf * 128 + c * 16, r);
           tmem_ld_wait();
-          if (c == COLS / 32 - 1) {            // the accumulator has been read
+          if (c == GROUPS * 4 - 1) {           // the accumulator has been read
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
-              if constexpr (PAIR) mbar_arrive_cluster(mapa_u32(smem_u32(&tempty[acc]), 0));
-              else mbar_arrive(&tempty[acc]);
+              if constexpr (PAIR) mbar_arrive_partner(mapa_u32(smem_u32(&tempty[set * BUFS + buf]), 0));
+              else mbar_arrive(&tempty[buf]);
             }
           }
+          const uint64_t sc = c < 4 ? pack_f32x2(s0, s0) : pack_f32x2(s1, s1);
 #pragma unroll
-          for (int j = 0; j < 16; ++j) sum[c * 16 + j] = fma_f32x2(pack_b32x2(r[2 * j], r[2 * j + 1]), sc2, sum[c * 16 + j]);
+          for (int j = 0; j < 8; ++j) sum[c * 8 + j] = fma_f32x2(pack_b32x2(r[2 * j], r[2 * j + 1]), sc, sum[c * 8 + j]);
         }
-        if (++acc == ACCS) {
-          acc = 0;
-          acc_phase ^= 1;
+        if (++buf == BUFS) {
+          buf = 0;
+          buf_phase ^= 1;
         }
       }
       if (!ok) break;
 #pragma unroll
-      for (int c = 0; c < COLS / 64; ++c) {
-        const int cc = col0 + c * 64;
+      for (int g = 0; g < GROUPS; ++g) {
+        const int cc = col0 + g * 128;
         uint4 w[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           uint32_t o[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float2 f = unpack_f32x2(sum[c * 32 + j * 4 + e]);
+            const float2 f = unpack_f32x2(sum[g * 32 + j * 4 + e]);
             o[e] = pack_bf16x2(f.x, f.y);
           }
           w[j] = make_uint4(o[0], o[1], o[2], o[3]);
@@ -351,7 +369,7 @@ extern "C" int axb_fp8_gemm(const void* A, long long lda, const float* sa, long 
   const bool pair = tile == 256;
   CUtensorMap tA, tB, tA2, tB2, tC;
   int rc = axb_make_tmap_2d(&tA, A, M, K, lda, 128, 128, 1);
-  if (!rc) rc = b_mn ? axb_make_tmap_2d(&tB, B, K, N, ldb, 128, 128, 1) : axb_make_tmap_2d(&tB, B, N, K, ldb, 128, 128, 1);
+  if (!rc) rc = b_mn ? axb_make_tmap_2d(&tB, B, K, N, ldb, 128, 64, 1, false, true) : axb_make_tmap_2d(&tB, B, N, K, ldb, 128, 128, 1);
   tA2 = tC = tA;
   tB2 = tB;
   if (!rc && K2 > 0) {
@@ -380,4 +398,20 @@ extern "C" int axb_fp8_gemm(const void* A, long long lda, const float* sa, long 
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (pair) return b_mn ? launch_fp8<true, true>(tA, tB, tA2, tB2, tC, p, st) : launch_fp8<true, false>(tA, tB, tA2, tB2, tC, p, st);
   return b_mn ? launch_fp8<false, true>(tA, tB, tA2, tB2, tC, p, st) : launch_fp8<false, false>(tA, tB, tA2, tB2, tC, p, st);
+}
+
+// y = x8 W8^T (b_mn: x8 W8) (+ X2 B2) of bf16 rows x [T, K] in one call. q: where the 8-bit rows go, T rows of K rounded up to 16 bytes and
+// behind them the scales, fp32 [ceil(K / 128)][T]; null: they are not kept (at most 64 rows, forward). The other arguments are those of
+// axb_fp8_gemm.
+extern "C" int axb_fp8_linear(const void* x, long long ldx, void* q, const void* W, long long ldw, const float* sw, long long sw_n,
+                              long long sw_k, int b_mn, void* y, int T, int N, int K, const void* X2, long long ldx2, const void* B2,
+                              long long ldb2, int K2, int tile, int* status, void* stream) {
+  if (!q) {
+    if (b_mn) return -2;
+    return axb_fp8_skinny(x, ldx, W, ldw, sw, sw_n, sw_k, y, N, T, N, K, X2, ldx2, B2, ldb2, K2, status, stream);
+  }
+  const long long ldq = (K + 15ll) & ~15ll;
+  float* s = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(q) + ldq * T);
+  const int rc = axb_fp8_quantize_rows(x, ldx, 0, q, ldq, s, T, T, K, stream);
+  return rc ? rc : axb_fp8_gemm(q, ldq, s, T, W, ldw, sw, sw_n, sw_k, b_mn, y, N, T, N, K, X2, ldx2, B2, ldb2, K2, tile, status, stream);
 }

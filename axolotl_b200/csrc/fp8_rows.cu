@@ -37,13 +37,6 @@ AXB_DEVICE __half from_f32(float v) { return __float2half(v); }
 template <>
 AXB_DEVICE float from_f32(float v) { return v; }
 
-// biased exponent of the block's scale
-AXB_DEVICE int scale_exponent(float top) {
-  const uint32_t b = __float_as_uint(top);
-  const int e = (int)(b >> 23) - 8 + ((b & 0x7FFFFFu) > 0x600000u ? 1 : 0);   // 448 = 1.75 * 2^8
-  return top == 0.f ? 127 : max(e, 1);
-}
-
 AXB_DEVICE float group_max(float m) {     // over the 16 lanes that hold a block of 128 columns
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -97,7 +90,7 @@ __global__ void __launch_bounds__(Q_ROWS * 32)
         else v[i][j] = __uint_as_float(0x7FC00000u);
       }
     }
-    const int e = scale_exponent(group_max(top));
+    const int e = fp8_scale_exponent(group_max(top));
     const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
     if (e >= 247) {                              // scale 2^120: the code 256 would stand for 2^128
 #pragma unroll

@@ -224,9 +224,9 @@ class FusedLinear(nn.Module):
     def _dense_weight(self):
         st = getattr(self.weight, "_axb_quant", None)
         if st is not None:
-            from ..ops.nf4 import dequantize_nf4
+            from ..ops.nf4 import expand_weight
 
-            return dequantize_nf4(self.weight.data, st, dtype=torch.bfloat16 if self.weight.is_cuda else torch.float32)
+            return expand_weight(self.weight.data, st, dtype=torch.bfloat16 if self.weight.is_cuda else torch.float32)
         return self.weight.detach()
 
     @torch.no_grad()
@@ -306,12 +306,26 @@ class FusedLinear(nn.Module):
         self.weight = w
 
     @torch.no_grad()
+    def quantize_fp8_(self):
+        """Replaces the frozen weight by E4M3 codes [N, K] with one fp32 scale for each 128 x 128 block: the products read the codes
+        (``ops.fp8.fp8_linear``), and the input is quantised by row and 128 columns. The codes are held as bytes, which a change of the
+        module's dtype leaves alone."""
+        from ..ops.fp8 import Fp8State, quantize_fp8_weight
+
+        if getattr(self.weight, "_axb_quant", None) is not None:
+            return
+        codes, scale = quantize_fp8_weight(self.weight.detach())
+        w = nn.Parameter(codes.view(torch.uint8), requires_grad=False)
+        w._axb_quant = Fp8State(tuple(self.weight.shape), scale)
+        self.weight = w
+
+    @torch.no_grad()
     def dequantize_(self, dtype=torch.bfloat16):
         st = getattr(self.weight, "_axb_quant", None)
         if st is not None:
-            from ..ops.nf4 import dequantize_nf4
+            from ..ops.nf4 import expand_weight
 
-            self.weight = nn.Parameter(dequantize_nf4(self.weight.data, st, dtype=dtype).clone(), requires_grad=False)
+            self.weight = nn.Parameter(expand_weight(self.weight.data, st, dtype=dtype).clone(), requires_grad=False)
 
     @torch.no_grad()
     def merge_lora_(self):

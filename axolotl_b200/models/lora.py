@@ -263,12 +263,23 @@ def inject_lora(model, spec: LoraSpec, freeze_base: bool = True, adapter_dtype=t
 def quantize_base_nf4_(model, double_quant=True):
     """QLoRA: every projection of the decoder layers is stored as NF4 (embeddings, norms, router
     and lm_head stay in bf16, as with bitsandbytes' ``load_in_4bit``). Returns bytes saved."""
+    return _quantize_base_(model, lambda m: m.quantize_nf4_(double_quant))
+
+
+@torch.no_grad()
+def quantize_base_fp8_(model):
+    """Every projection of the decoder layers in 8-bit blocks (``FusedLinear.quantize_fp8_``); embeddings, norms, router and lm_head stay
+    as they are. Returns bytes saved."""
+    return _quantize_base_(model, lambda m: m.quantize_fp8_())
+
+
+def _quantize_base_(model, quantize):
     saved = 0
     for name, m in model.fused_linears():
         if not isinstance(m, FusedLinear) or not name.startswith("layers."):
             continue
         before = m.weight.numel() * m.weight.element_size()
-        m.quantize_nf4_(double_quant)
+        quantize(m)
         saved += before - m.weight.numel() - m.weight._axb_quant.nbytes()
     return saved
 

@@ -721,7 +721,8 @@ class CausalLM(nn.Module):
 
     def enable_gradient_checkpointing(self, flag=True, offload=None, selective=False, offload_dir=None):
         """``offload``: None keeps checkpointed layer inputs on the device; True / "legacy" /
-        "hidden_states" park them in pinned host memory, "disk" in files under ``offload_dir``.
+        "hidden_states" park them in pinned host memory, "disk" in files under ``offload_dir``, "fp8" keeps them on
+        the device in 8 bits.
         ``selective`` keeps the attention result and recomputes only the rest of each layer."""
         self.gradient_checkpointing = flag
         self.ckpt_selective = bool(selective) and flag

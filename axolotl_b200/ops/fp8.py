@@ -79,21 +79,53 @@ def quantize_fp8_rows(x: torch.Tensor):
         raise ValueError(f"quantize_fp8_rows takes a matrix [rows, columns] with a column at least, got {tuple(x.shape)}")
     if x.dtype not in _DTYPES:
         raise TypeError(f"quantize_fp8_rows takes bfloat16, float16 or float32, got {x.dtype}")
-    x = x.detach()
+    return _unpacked(_pack(x.detach()), *x.shape)
+
+
+def _pack(x):
+    """The 8-bit rows of x [T, K] as one block of bytes: T rows of codes, K rounded up to 16 bytes, and behind them the scales, fp32
+    [ceil(K / 128)][T]. What the layers and the checkpoint store keep."""
     T, K = x.shape
+    ld = (K + 15) & ~15
     if not x.is_cuda:
-        return _quantize_rows_plain(x)
+        return _pack_plain(x, ld)
+    if x.device.index != torch.cuda.current_device():
+        with torch.cuda.device(x.device):
+            return _pack(x)
     if x.stride(1) != 1 and K > 1:
         x = x.contiguous()
-    with _device_of(x):
-        codes = _padded(T, K, x.device)
-        scale = torch.empty((_blocks(K), T), dtype=torch.float32, device=x.device)
-        _lib.check_rc(_lib.cuda_lib().axb_fp8_quantize_rows(x.data_ptr(), x.stride(0), _DTYPES[x.dtype], codes.data_ptr(), codes.stride(0),
-                                                            scale.data_ptr(), T, T, K, _lib.stream_ptr()), "fp8_quantize_rows")
-    return codes, scale
+    q = torch.empty(T * (ld + 4 * _blocks(K)), dtype=torch.uint8, device=x.device)
+    at = q.data_ptr()
+    _lib.check_rc(_lib.cuda_lib().axb_fp8_quantize_rows(x.data_ptr(), x.stride(0), _DTYPES[x.dtype], at, ld, at + T * ld, T, T, K,
+                                                        _lib.stream_ptr()), "fp8_quantize_rows")
+    return q
 
 
-def _quantize_rows_plain(x):
+def _unpacked(q, T, K):
+    """(codes [T, K], scales [ceil(K / 128), T]): views of a block of ``_pack``."""
+    ld = (K + 15) & ~15
+    if T == 0:
+        return q.new_empty((0, K)).view(torch.float8_e4m3fn), torch.empty((_blocks(K), 0), device=q.device)
+    codes = q[:T * ld].view(T, ld).view(torch.float8_e4m3fn)
+    return (codes if ld == K else codes[:, :K]), q[T * ld:].view(torch.float32).view(_blocks(K), T)
+
+
+def _unpack(q, T, K, dtype):
+    """The values of a block of ``_pack``, [T, K]."""
+    if not q.is_cuda:
+        return dequantize_fp8_rows(*_unpacked(q, T, K), dtype)
+    if q.device.index != torch.cuda.current_device():
+        with torch.cuda.device(q.device):
+            return _unpack(q, T, K, dtype)
+    ld = (K + 15) & ~15
+    at = q.data_ptr()
+    out = torch.empty((T, K), dtype=dtype, device=q.device)
+    _lib.check_rc(_lib.cuda_lib().axb_fp8_dequantize_rows(at, ld, at + T * ld, T, out.data_ptr(), K, _DTYPES[dtype], T, K,
+                                                          _lib.stream_ptr()), "fp8_dequantize_rows")
+    return out
+
+
+def _pack_plain(x, ld):
     T, K = x.shape
     kb = _blocks(K)
     v = torch.nn.functional.pad(x.float(), (0, kb * BLOCK - K)).view(T, kb, BLOCK)
@@ -102,10 +134,9 @@ def _quantize_rows_plain(x):
     m, e = torch.frexp(top)                                # top = m 2^e with m in [0.5, 1); 448 = 0.875 * 2^9
     e = (e - 9 + (m > 0.875).to(e.dtype)).clamp(min=-126)
     scale = torch.where(top > 0, torch.ldexp(torch.ones_like(top), e), torch.ones_like(top))
-    codes = _padded(T, K, x.device)
     v = v.clamp(-240 * 2.0 ** 120, 240 * 2.0 ** 120)
-    codes.copy_((v / scale[..., None]).to(torch.float8_e4m3fn).view(T, kb * BLOCK)[:, :K])
-    return codes, scale.t().contiguous()
+    codes = (v / scale[..., None]).to(torch.float8_e4m3fn).view(T, kb * BLOCK)[:, :ld]
+    return torch.cat([codes.reshape(-1).view(torch.uint8), scale.t().reshape(-1).view(torch.uint8)])
 
 
 def dequantize_fp8_rows(codes: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = torch.bfloat16):
@@ -218,10 +249,48 @@ def _tile(M, N) -> int:
     return 256 if M > 128 and N > 128 and -(-M // 256) * -(-N // 256) >= 74 else 128
 
 
+_FEW = 64      # rows up to which a product that keeps no codes is one launch (csrc/fp8_skinny.cu)
+
+
+def _product(x, codes, scale, trans=False, a2=None, b2=None, keep=False):
+    """(x8 W8^T or x8 W8 (+ a2 b2) in bf16, block of ``_pack`` of x or None) of bf16 rows x [T, K]. One call: with at most 64 rows whose
+    codes nobody keeps, one launch."""
+    if not x.is_cuda:
+        q = _pack(x)
+        y = fp8_gemm(*_unpacked(q, *x.shape), codes, scale, trans_w=trans, a2=a2, b2=b2)
+        return y, q
+    if x.device.index != torch.cuda.current_device():
+        with torch.cuda.device(x.device):
+            return _product(x, codes, scale, trans, a2, b2, keep)
+    T, K = x.shape
+    N = codes.shape[1] if trans else codes.shape[0]
+    if x.stride(1) != 1 and K > 1:
+        x = x.contiguous()
+    codes = _rows16(codes)
+    sn, sk = scale.stride()
+    if trans:
+        sn, sk = sk, sn
+    K2 = 0
+    if a2 is not None:
+        from .gemm import _row_major_2d
+
+        a2, b2, K2 = _row_major_2d(a2), _row_major_2d(b2), a2.shape[1]
+    y = torch.empty((T, N), dtype=torch.bfloat16, device=x.device)
+    q = None
+    if keep or trans or T > _FEW or K2 % 8:
+        q = torch.empty(T * (((K + 15) & ~15) + 4 * _blocks(K)), dtype=torch.uint8, device=x.device)
+    _lib.check_rc(_lib.cuda_lib().axb_fp8_linear(
+        x.data_ptr(), x.stride(0), None if q is None else q.data_ptr(), codes.data_ptr(), codes.stride(0), scale.data_ptr(), sn, sk,
+        trans, y.data_ptr(), T, N, K, None if K2 == 0 else a2.data_ptr(), 0 if K2 == 0 else a2.stride(0),
+        None if K2 == 0 else b2.data_ptr(), 0 if K2 == 0 else b2.stride(0), K2, _tile(T, N), _lib.status_word(x.device).data_ptr(),
+        _lib.stream_ptr()), "fp8_linear")
+    return y, q
+
+
 class _Fp8LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, codes, scale, bias):
-        y = fp8_gemm(*quantize_fp8_rows(x), codes, scale)
+        y, _ = _product(x, codes, scale)
         if bias is not None:
             y = y + bias
         ctx.save_for_backward(codes, scale)               # the weight is frozen: nothing of x is needed again
@@ -231,7 +300,7 @@ class _Fp8LinearFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         codes, scale = ctx.saved_tensors
-        dx = fp8_gemm(*quantize_fp8_rows(dy), codes, scale, trans_w=True) if ctx.needs_input_grad[0] else None
+        dx = _product(dy, codes, scale, trans=True)[0] if ctx.needs_input_grad[0] else None
         dbias = dy.float().sum(0).to(ctx.bias_dtype) if ctx.needs_input_grad[3] else None
         return dx, None, None, dbias
 
@@ -241,12 +310,11 @@ class _Fp8LoRALinearFn(torch.autograd.Function):
     def forward(ctx, x, codes, scale, A, B, A16, B16, scaling, blocks, bias):
         from .lora import skinny_gemm
 
-        q, s = quantize_fp8_rows(x)
         xa = skinny_gemm(x, A16, alpha=scaling)            # [T, R], of the bf16 input
-        y = fp8_gemm(q, s, codes, scale, a2=xa, b2=B16)
+        y, q = _product(x, codes, scale, a2=xa, b2=B16, keep=ctx.needs_input_grad[3])
         if bias is not None:
             y = y + bias
-        ctx.save_for_backward(q, s, codes, scale, A, B, A16, B16, xa)
+        ctx.save_for_backward(q if ctx.needs_input_grad[3] else None, codes, scale, A, B, A16, B16, xa)
         ctx.scaling, ctx.blocks, ctx.bias_dtype = scaling, blocks, None if bias is None else bias.dtype
         return y
 
@@ -254,17 +322,17 @@ class _Fp8LoRALinearFn(torch.autograd.Function):
     def backward(ctx, dy):
         from .lora import _adapter_grads, _t_and_dB
 
-        q, s, codes, scale, A, B, A16, B16, xa = ctx.saved_tensors
+        q, codes, scale, A, B, A16, B16, xa = ctx.saved_tensors
         need = ctx.needs_input_grad
         dy = dy.contiguous()
         t, dB_fused, dB_done = _t_and_dB(dy, B, B16, xa, ctx.blocks, ctx.scaling, need[4])
-        dx = fp8_gemm(*quantize_fp8_rows(dy), codes, scale, trans_w=True, a2=t, b2=A16) if need[0] else None
+        dx = _product(dy, codes, scale, trans=True, a2=t, b2=A16)[0] if need[0] else None
         dA = None
         if need[3]:
             tgt = getattr(A, "_axb_grad", None)
-            buf = fp8_adapter_grad(t, q, s, out=tgt)
+            buf = fp8_adapter_grad(t, *_unpacked(q, dy.shape[0], codes.shape[1]), out=tgt)
             dA = None if tgt is not None else buf.to(A.dtype)
-        _, dB = _adapter_grads(None, B if need[4] else None, t, q, dy, xa, ctx.blocks, dB_done, dB_fused)
+        _, dB = _adapter_grads(None, B if need[4] else None, t, codes, dy, xa, ctx.blocks, dB_done, dB_fused)
         dbias = dy.float().sum(0).to(ctx.bias_dtype) if need[9] else None
         return dx, None, None, dA, dB, None, None, None, None, dbias
 
@@ -292,33 +360,44 @@ def fp8_adapter_grad(t, codes, row_scale, out=None):
 
 
 def _check_linear(x, codes, scale, what):
+    cs, ss = codes.shape, scale.shape
+    if (len(cs) == 2 and len(ss) == 2 and cs[0] and cs[1] and x.dim() and x.shape[-1] == cs[1] and codes.dtype == torch.float8_e4m3fn
+            and scale.dtype == torch.float32 and ss[0] == _blocks(cs[0]) and ss[1] == _blocks(cs[1]) and x.device == codes.device
+            and x.device == scale.device and (x.dtype == torch.bfloat16 or not x.is_cuda)):
+        return
     _check_weight(codes, scale, what)
-    if x.dim() < 1 or x.shape[-1] != codes.shape[1]:
-        raise ValueError(f"{what}: input {tuple(x.shape)} for a weight [{codes.shape[0]}, {codes.shape[1]}]")
-    if x.is_cuda and x.dtype != torch.bfloat16:
-        raise TypeError(f"{what} takes bf16 on the device, got {x.dtype}")
+    if 0 in cs or x.dim() < 1 or x.shape[-1] != cs[1]:
+        raise ValueError(f"{what}: input {tuple(x.shape)} for a weight {tuple(cs)}")
     if x.device != codes.device:
         raise ValueError(f"{what}: input on {x.device}, weight on {codes.device}")
+    raise TypeError(f"{what} takes bf16 on the device, got {x.dtype}")
+
+
+def _rows_of(x):
+    return x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+
+
+def _shaped(y, x):
+    y = y if y.dtype == x.dtype else y.to(x.dtype)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], y.shape[-1])
 
 
 def fp8_linear(x, codes, scale, bias=None):
     """``x8 W8^T (+ bias)`` of a frozen block-FP8 weight (codes [N, K], scales [ceil(N / 128), ceil(K / 128)]); ``x`` [..., K] in bf16. The
     input gradient is ``dy8 W8``; nothing of ``x`` is kept for it."""
     _check_linear(x, codes, scale, "fp8_linear")
-    shp = x.shape
-    y = _Fp8LinearFn.apply(x.reshape(-1, shp[-1]), codes, scale, bias)
-    return y.view(*shp[:-1], y.shape[-1]).to(x.dtype)
+    if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
+        return _shaped(_Fp8LinearFn.apply(_rows_of(x), codes, scale, bias), x)
+    y, _ = _product(_rows_of(x), codes, scale)
+    return _shaped(y if bias is None else y + bias, x)
 
 
 def fp8_lora_linear(x, codes, scale, A, B, A16, B16, scaling, blocks, bias=None):
     """``x8 W8^T + scaling (x A^T) B^T (+ bias)``: ``fp8_linear`` with the adapter of ``ops.lora.lora_linear`` (same arguments). The 8-bit
     rows of ``x`` are kept for ``dA = (scaling dy B)^T x8``."""
     _check_linear(x, codes, scale, "fp8_lora_linear")
-    shp = x.shape
-    x2 = x.reshape(-1, shp[-1])
+    x2 = _rows_of(x)
     if not x.is_cuda:
         y = _Fp8LinearFn.apply(x2, codes, scale, bias).to(x.dtype)
-        y = y + scaling * ((x2 @ A.to(x2.dtype).t()) @ B.to(x2.dtype).t())
-        return y.view(*shp[:-1], y.shape[-1])
-    y = _Fp8LoRALinearFn.apply(x2.contiguous(), codes, scale, A, B, A16, B16, float(scaling), blocks, bias)
-    return y.view(*shp[:-1], y.shape[-1])
+        return _shaped(y + scaling * ((x2 @ A.to(x2.dtype).t()) @ B.to(x2.dtype).t()), x)
+    return _shaped(_Fp8LoRALinearFn.apply(x2.contiguous(), codes, scale, A, B, A16, B16, float(scaling), blocks, bias), x)

@@ -79,11 +79,12 @@ def gemm(
     dh [M, I] and ``out`` [M, 2I] receives d_gate | d_up (``out`` may be ``gate_up`` itself)."""
     quant = getattr(b, "_axb_quant", None)
     if quant is not None:
-        # frozen 4-bit weight: expand into the shared bf16 scratch right before the GEMM reads it
-        from .nf4 import dequantize_nf4, scratch_weight
+        # frozen 4-bit weight: expand into the shared bf16 scratch right before the GEMM reads it (8-bit blocks have a product of their
+        # own, ops/fp8.py; what asks for the bf16 one gets it of the expanded weight)
+        from .nf4 import NF4State, expand_weight, scratch_weight
 
-        b = dequantize_nf4(b, quant, out=scratch_weight(quant.shape, b.device) if b.is_cuda else None,
-                           dtype=torch.bfloat16 if b.is_cuda else a.dtype)
+        b = expand_weight(b, quant, out=scratch_weight(quant.shape, b.device) if b.is_cuda and isinstance(quant, NF4State) else None,
+                          dtype=torch.bfloat16 if b.is_cuda else a.dtype)
     shard = getattr(b, "_axb_shard", None)
     if shard is not None:
         return _gemm_allgather(a, b, shard, trans_a=trans_a, trans_b=trans_b, a2=a2, b2=b2, alpha=alpha,

@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import torch
 
+from .fp8 import Fp8State, fp8_linear, fp8_lora_linear
 from .gemm import gemm, glu_fusable, pick_splits
 
 
@@ -242,7 +243,7 @@ class _GLUMLPFn(torch.autograd.Function):
 
 def _plain_fused(m) -> bool:
     """A FusedLinear the fused MLP can drive directly: dense or LoRA, nothing else attached."""
-    return (m.bias is None and m.dora_magnitude is None and m.mora_M is None and m.qat is None
+    return (m.bias is None and fp8_state(m.weight) is None and m.dora_magnitude is None and m.mora_M is None and m.qat is None
             and not (m.lora_A is not None and m.lora_dropout > 0.0 and m.training))
 
 
@@ -283,14 +284,23 @@ def _cpu_weight(W, dtype):
     """Dense view of a (possibly 4-bit) weight for the CPU reference path."""
     st = getattr(W, "_axb_quant", None)
     if st is not None:
-        from .nf4 import dequantize_nf4
+        from .nf4 import expand_weight
 
-        return dequantize_nf4(W.data, st, dtype=dtype)
+        return expand_weight(W.data, st, dtype=dtype)
     return W.to(dtype)
 
 
+def fp8_state(W):
+    """The scales of a frozen weight held in 8-bit blocks, None for any other weight."""
+    st = getattr(W, "_axb_quant", None)
+    return st if isinstance(st, Fp8State) else None
+
+
 def linear(x, W, bias=None):
-    """``x @ W^T (+ bias)``; 2-D or N-D ``x``. CPU tensors use torch ops directly."""
+    """``x @ W^T (+ bias)``; 2-D or N-D ``x``. CPU tensors use torch ops directly; a weight in 8-bit blocks takes ``fp8_linear``."""
+    st = fp8_state(W)
+    if st is not None:
+        return fp8_linear(x, W.data.view(torch.float8_e4m3fn), st.scale, bias)
     if not x.is_cuda:
         return torch.nn.functional.linear(x, _cpu_weight(W, x.dtype), None if bias is None else bias.to(x.dtype))
     shp = x.shape
@@ -303,15 +313,18 @@ def lora_linear(x, W, A, B, A16, B16, scaling, blocks, bias=None, dropout_p=0.0,
     fp32 masters on CUDA and may be None on CPU."""
     shp = x.shape
     x2 = x.reshape(-1, shp[-1])
+    st = fp8_state(W)
+    if st is not None and not (dropout_p > 0.0 and training):
+        return fp8_lora_linear(x, W.data.view(torch.float8_e4m3fn), st.scale, A, B, A16, B16, scaling, blocks, bias)
     if not x.is_cuda or (dropout_p > 0.0 and training):
         xd = torch.nn.functional.dropout(x2, dropout_p, training) if dropout_p > 0.0 else x2
         if x.is_cuda:
-            base = _LinearFn.apply(x2.contiguous(), W, bias)
+            base = linear(x2, W, bias)
             lo = _LinearFn.apply(_LinearFn.apply(xd.contiguous(), A.to(x.dtype), None),
                                  B.to(x.dtype), None)
             y = base + scaling * lo
         else:
-            y = torch.nn.functional.linear(x2, _cpu_weight(W, x2.dtype), None if bias is None else bias.to(x2.dtype))
+            y = linear(x2, W, bias)
             y = y + scaling * ((xd @ A.to(x2.dtype).t()) @ B.to(x2.dtype).t())
         return y.view(*shp[:-1], y.shape[-1])
     y = _LoRALinearFn.apply(x2.contiguous(), W, A, B, A16, B16, float(scaling), blocks, bias)

@@ -126,6 +126,15 @@ def dequantize_nf4(qdata: torch.Tensor, st: NF4State, out: torch.Tensor | None =
     return res
 
 
+def expand_weight(w: torch.Tensor, st, out: torch.Tensor | None = None, dtype=torch.bfloat16):
+    """The dense form of a frozen quantised weight by its state: NF4 codes, or 8-bit blocks (``ops.fp8.Fp8State``)."""
+    if isinstance(st, NF4State):
+        return dequantize_nf4(w, st, out=out, dtype=dtype)
+    from .fp8 import dequantize_fp8_weight
+
+    return dequantize_fp8_weight(w.view(torch.float8_e4m3fn), st.scale, dtype)
+
+
 _SCRATCH: dict = {}
 
 

@@ -19,9 +19,11 @@ from concurrent.futures import ThreadPoolExecutor
 
 import torch
 
+from ..ops import fp8
+
 
 class _Handle:
-    __slots__ = ("shape", "dtype", "device", "host", "event", "gpu", "gpu_event", "prev", "path", "future", "nbytes")
+    __slots__ = ("shape", "dtype", "device", "host", "event", "gpu", "gpu_event", "prev", "path", "future", "coded", "nbytes")
 
     def __init__(self):
         self.host = self.event = self.gpu = self.gpu_event = self.prev = self.path = self.future = None
@@ -157,28 +159,26 @@ class Fp8Store:
         self.bytes_out = 0
 
     def put(self, t: torch.Tensor) -> _Handle:
-        from ..ops.fp8 import quantize_fp8_rows
-
         h = _Handle()
         h.shape, h.dtype, h.device = t.shape, t.dtype, t.device
         if t.dtype not in (torch.bfloat16, torch.float16, torch.float32) or t.numel() == 0 or t.dim() == 0:
-            h.gpu = t.detach()                             # kept as it is
-            h.nbytes = t.numel() * t.element_size()
+            h.gpu, h.coded = t.detach(), False            # kept as it is
         else:
-            h.gpu = quantize_fp8_rows(t.detach().reshape(-1, t.shape[-1]))
-            h.nbytes = sum(p.untyped_storage().nbytes() for p in h.gpu)
+            t = t.detach()
+            h.gpu, h.coded = fp8._pack(t if t.dim() == 2 else t.reshape(-1, t.shape[-1])), True
+        h.nbytes = h.gpu.numel() * h.gpu.element_size()
         self.bytes_out += h.nbytes
         return h
 
     def get(self, h: _Handle) -> torch.Tensor:
-        from ..ops.fp8 import dequantize_fp8_rows
-
         kept, h.gpu = h.gpu, None
         if kept is None:
             raise RuntimeError("this checkpoint has been given back already")
-        if torch.is_tensor(kept):
+        if not h.coded:
             return kept
-        return dequantize_fp8_rows(*kept, dtype=h.dtype).view(h.shape)
+        K = h.shape[-1]
+        x = fp8._unpack(kept, h.shape.numel() // K, K, h.dtype)
+        return x if len(h.shape) == 2 else x.view(h.shape)
 
     def reset(self):
         pass

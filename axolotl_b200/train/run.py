@@ -122,6 +122,11 @@ def setup_adapter(cfg, model):
         qcfg = cfg.get("bnb_config_kwargs") or {}
         saved = quantize_base_nf4_(model, double_quant=qcfg.get("bnb_4bit_use_double_quant", True) is not False)
         LOG.info("base projections stored as NF4: %.2f GiB saved", saved / 1024 ** 3)
+    if cfg.get("base_weights_fp8"):
+        from ..models.lora import quantize_base_fp8_
+
+        saved = quantize_base_fp8_(model)
+        LOG.info("base projections stored in 8-bit blocks: %.2f GiB saved", saved / 1024 ** 3)
     adapter_dtype = torch.float32 if cfg.get("peft_autocast_adapter_dtype", True) is not False else model.dtype
     if cfg.get("lora_target_linear") and isinstance(spec.target_modules, (list, tuple)):
         from ..models.lora import discover_linear_names
