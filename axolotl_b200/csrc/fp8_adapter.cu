@@ -1,0 +1,273 @@
+// dA[r, k] (+)= sum_t g[t, r] x8[t, k]: the gradient of an adapter's A from the 8-bit rows that the forward pass kept (codes q [T, K] and
+// scales s[k / 128][t], csrc/fp8_rows.cu) and g [T, R] = s dy B in bf16.
+//
+// Bound: one pass over the codes (HBM), half of what the bf16 rows would take. The scales lie along the contracted axis, so the codes
+// are widened first: eight warps turn a tile of 64 rows x 128 columns into bf16 (exact: four significant bits and a power of two) as the
+// MN-major 128-row operand of tcgen05.mma, g is the other one, 64 of its columns at a time. About 110 instructions a thread and tile,
+// 230 cycles, against the 350 that an SM's share of HBM takes for the codes. The rows are split over a cluster whose partial sums meet in
+// distributed shared memory in a fixed order: no atomics, the same bits every time.
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "axb_common.cuh"
+
+namespace {
+
+constexpr int FA_T = 320;                 // TMA, MMA, eight widening warps
+constexpr int FA_ROWS = 64;               // rows of a step
+constexpr int FA_Q = FA_ROWS * 128;       // codes of a step
+constexpr int FA_G = FA_ROWS * 128;       // g of a step: 64 columns in bf16
+constexpr int FA_STAGES = 4;
+constexpr int FA_X = FA_ROWS * 256;       // widened tile: two chunks of 64 columns
+constexpr int FA_XBUFS = 2;
+constexpr int FA_SMEM = FA_STAGES * (FA_Q + FA_G) + FA_XBUFS * FA_X + 1024 + 256;
+static_assert(64 * 128 * 4 <= FA_STAGES * (FA_Q + FA_G), "the partial tile reuses the ring");
+
+struct Fp8AdapterParams {
+  const float* s;
+  float* out;
+  long long lds, ldo;
+  int T, K, R, accumulate, vec;
+  int* status;
+};
+
+template <int NR>
+__global__ void __launch_bounds__(FA_T, 2)
+    fp8_adapter_grad_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmG, const Fp8AdapterParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* sX = smem + FA_STAGES * (FA_Q + FA_G);
+  uint64_t* full = reinterpret_cast<uint64_t*>(sX + FA_XBUFS * FA_X);   // codes and g have arrived
+  uint64_t* empty = full + FA_STAGES;                                   // the product that read g has ended
+  uint64_t* xfull = empty + FA_STAGES;                                  // widened by eight warps
+  uint64_t* xempty = xfull + FA_XBUFS;
+  uint64_t* done = xempty + FA_XBUFS;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  const int tid = threadIdx.x, warp = uniform_warp(), lane = tid & 31;
+  const int rank = (int)cluster_ctarank(), cs = (int)cluster_nctarank();
+  const int tile = blockIdx.x / cs, r0 = blockIdx.y * 64;
+  const int steps = (p.T + FA_ROWS - 1) / FA_ROWS;
+  const int t0 = (int)((long long)steps * rank / cs), t1 = (int)((long long)steps * (rank + 1) / cs);
+
+  if (tid == 0) {
+    for (int s = 0; s < FA_STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < FA_XBUFS; ++s) {
+      mbar_init(&xfull[s], 8);
+      mbar_init(&xempty[s], 1);
+    }
+    mbar_init(done, 1);
+    mbar_fence_init();
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmG);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, NR < 32 ? 32 : NR);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    int s = 0;
+    uint32_t phase = 0;
+    for (int t = t0; t < t1; ++t) {
+      if (!warp_all(mbar_wait(&empty[s], phase ^ 1, p.status, AXB_TIMEOUT_EMPTY))) break;
+      if (elect_one()) {
+        uint8_t* dst = smem + s * (FA_Q + FA_G);
+        mbar_expect_tx(&full[s], FA_Q + FA_G);
+        tma_load_2d(dst, &tmQ, &full[s], tile * 128, t * FA_ROWS);
+        tma_load_2d(dst + FA_Q, &tmG, &full[s], r0, t * FA_ROWS);
+      }
+      __syncwarp();
+      if (++s == FA_STAGES) {
+        s = 0;
+        phase ^= 1;
+      }
+    }
+  } else if (warp == 1) {
+    constexpr uint32_t idesc = make_idesc_bf16(128, NR, 1, 1);
+    const uint64_t base_x = make_smem_desc_sw128(smem_u32(sX), FA_X / 2, 1024);
+    const uint64_t base_g = make_smem_desc_sw128(smem_u32(smem + FA_Q), 16, 1024);
+    int s = 0, b = 0;
+    uint32_t phase = 0;
+    for (int t = t0; t < t1; ++t) {
+      // the widening warps have waited for the stage's copies; this warp's own wait makes g visible to its product
+      if (!warp_all(mbar_wait(&xfull[b], phase, p.status, AXB_TIMEOUT_GENERIC) &&
+                    mbar_wait(&full[s], (uint32_t)((t - t0) / FA_STAGES) & 1, p.status, AXB_TIMEOUT_FULL)))
+        break;
+      tc_fence_after();
+      const uint64_t x = base_x + (uint32_t)(b * (FA_X / 16)), g = base_g + (uint32_t)(s * ((FA_Q + FA_G) / 16));
+      if (elect_one()) {
+#pragma unroll
+        for (int kk = 0; kk < FA_ROWS / 16; ++kk)
+          umma_f16(tmem, x + kk * (2048 / 16), g + kk * (2048 / 16), idesc, t > t0 || kk > 0 ? 1u : 0u);
+        umma_commit(&empty[s]);
+        umma_commit(&xempty[b]);
+        if (t == t1 - 1) umma_commit(done);
+      }
+      __syncwarp();
+      if (++s == FA_STAGES) s = 0;
+      if (++b == FA_XBUFS) {
+        b = 0;
+        phase ^= 1;
+      }
+    }
+  } else {
+    // 16 codes of a row at a time: this thread's rows are r and 32 + r of a step
+    const int w = tid - 64, r = w >> 3, c16 = w & 7;
+    const float* sc = p.s + (long long)tile * p.lds;
+    float next[2];
+    auto fetch = [&](int t) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = t * FA_ROWS + i * 32 + r;
+        next[i] = row < p.T ? __ldg(sc + row) : 0.f;
+      }
+    };
+    fetch(t0);
+    int s = 0, b = 0;
+    uint32_t phase = 0, xphase = 0;
+    for (int t = t0; t < t1; ++t) {
+      const float scale[2] = {next[0], next[1]};
+      if (t + 1 < t1) fetch(t + 1);
+      if (!warp_all(mbar_wait(&full[s], phase, p.status, AXB_TIMEOUT_FULL) &&
+                    mbar_wait(&xempty[b], xphase ^ 1, p.status, AXB_TIMEOUT_EMPTY)))
+        break;
+      const uint8_t* src = smem + s * (FA_Q + FA_G);
+      uint8_t* dst = sX + b * FA_X + (c16 >> 2) * (FA_X / 2);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int row = i * 32 + r;
+        const uint4 q = *reinterpret_cast<const uint4*>(src + row * 128 + c16 * 16);
+        const uint32_t in[4] = {q.x, q.y, q.z, q.w};
+        uint32_t o[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const __nv_fp8x2_storage_t two = (__nv_fp8x2_storage_t)(in[j >> 1] >> (16 * (j & 1)));
+          const float2 f = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(two, __NV_E4M3)));
+          o[j] = pack_bf16x2(f.x * scale[i], f.y * scale[i]);
+        }
+        uint8_t* to = dst + row * 128;
+        const int j0 = (c16 & 3) * 2;
+        *reinterpret_cast<uint4*>(to + ((j0 ^ (row & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+        *reinterpret_cast<uint4*>(to + (((j0 + 1) ^ (row & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&xfull[b]);
+      if (++s == FA_STAGES) {
+        s = 0;
+        phase ^= 1;
+      }
+      if (++b == FA_XBUFS) {
+        b = 0;
+        xphase ^= 1;
+      }
+    }
+  }
+  __syncwarp();
+  warp_all(mbar_wait(done, 0, p.status, AXB_TIMEOUT_TMEM_FULL));
+  tc_fence_after();
+  __syncthreads();                        // every warp has left the ring
+  float* part = reinterpret_cast<float*>(smem);          // partial tile, [r][128 columns]
+  if (warp >= 2 && warp < 6) {
+#pragma unroll
+    for (int c = 0; c < NR / 16; ++c) {
+      uint32_t v[16];
+      tmem_ld_32x16(tmem + (uint32_t((warp & 3) * 32) << 16) + c * 16, v);
+      tmem_ld_wait();
+#pragma unroll
+      for (int j = 0; j < 16; ++j) part[(c * 16 + j) * 128 + (warp & 3) * 32 + lane] = __uint_as_float(v[j]);
+    }
+  }
+  tc_fence_before();
+  if (cs > 1) cluster_sync();
+  else __syncthreads();
+  const uint32_t pbase = smem_u32(part);
+  const int rows = min(p.R - r0, 64);
+  for (int i = rank * FA_T + tid; i < rows * 32; i += cs * FA_T) {
+    const int rr = i >> 5, c = (i & 31) * 4, k = tile * 128 + c;
+    if (k >= p.K) continue;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int q = 0; q < cs; ++q) {
+      const float4 u = cs == 1 ? *reinterpret_cast<const float4*>(part + rr * 128 + c) : ld_cluster_f32x4(mapa_u32(pbase + (rr * 128 + c) * 4, q));
+      a.x += u.x;
+      a.y += u.y;
+      a.z += u.z;
+      a.w += u.w;
+    }
+    float* o = p.out + (long long)(r0 + rr) * p.ldo + k;
+    if (p.vec && k + 4 <= p.K) {
+      if (p.accumulate) {
+        const float4 u = *reinterpret_cast<const float4*>(o);
+        a.x += u.x;
+        a.y += u.y;
+        a.z += u.z;
+        a.w += u.w;
+      }
+      *reinterpret_cast<float4*>(o) = a;
+    } else {
+      const float v[4] = {a.x, a.y, a.z, a.w};
+      for (int j = 0; j < 4 && k + j < p.K; ++j) o[j] = v[j] + (p.accumulate ? o[j] : 0.f);
+    }
+  }
+  if (cs > 1) cluster_sync();             // peers may still read this CTA's partial tile
+  else __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, NR < 32 ? 32 : NR);
+  }
+}
+
+template <int NR>
+int launch_adapter_grad(const CUtensorMap& q, const CUtensorMap& g, const Fp8AdapterParams& p, int tiles, int chunks, int splits,
+                        cudaStream_t st) {
+  auto kern = fp8_adapter_grad_kernel<NR>;
+  static std::atomic<unsigned long long> allowed{0};
+  if (const int rc = axb_allow_smem((const void*)kern, FA_SMEM, allowed)) return rc;
+  AxbLaunch l(dim3((unsigned)(tiles * splits), (unsigned)chunks), FA_T, FA_SMEM, st, splits, false);
+  const cudaError_t e = cudaLaunchKernelEx(&l.cfg, kern, q, g, p);
+  return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
+}
+
+}  // namespace
+
+// q: codes [T, K], rows of ldq bytes; s: fp32 [ceil(K / 128)][lds]; g: bf16 [T, R], row stride ldg; out: fp32 [R, K], row stride ldo, added
+// to (accumulate) or written. q and g start on 16 bytes and have row strides of whole 16 bytes.
+extern "C" int axb_fp8_adapter_grad(const void* q, long long ldq, const float* s, long long lds, const void* g, long long ldg, float* out,
+                                    long long ldo, int T, int K, int R, int accumulate, int* status, void* stream) {
+  if (K <= 0 || R <= 0) return 0;
+  auto bad = [](const void* v, long long bytes) { return (reinterpret_cast<uintptr_t>(v) & 15) != 0 || (bytes & 15) != 0; };
+  if (T <= 0 || bad(q, ldq) || bad(g, 2 * ldg) || lds < T || ldo < K) return -2;
+  CUtensorMap tQ, tG;
+  int rc = axb_make_tmap_2d(&tQ, q, T, K, ldq, FA_ROWS, 128, 1, false);
+  if (!rc) rc = axb_make_tmap_2d(&tG, g, T, R, ldg, FA_ROWS, 64);
+  if (rc) return -100 - rc;
+  const int tiles = (K + 127) / 128, chunks = (R + 63) / 64, steps = (T + FA_ROWS - 1) / FA_ROWS;
+  if (chunks > 65535) return -2;
+  // rows of a tile over the largest cluster of which the chip holds one per tile at once (33 of eight, 70 of four, 148 of two)
+  const int sizes[][2] = {{8, 33}, {4, 70}, {2, 148}};
+  int splits = 1;
+  for (const auto& z : sizes)
+    if (splits == 1 && (long long)tiles * chunks <= z[1] && steps >= 2 * z[0]) splits = z[0];
+  Fp8AdapterParams p = {};
+  p.s = s;
+  p.out = out;
+  p.lds = lds;
+  p.ldo = ldo;
+  p.T = T;
+  p.K = K;
+  p.R = R;
+  p.accumulate = accumulate;
+  p.vec = (ldo & 3) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+  p.status = status;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (R <= 16) return launch_adapter_grad<16>(tQ, tG, p, tiles, chunks, splits, st);
+  if (R <= 32) return launch_adapter_grad<32>(tQ, tG, p, tiles, chunks, splits, st);
+  return launch_adapter_grad<64>(tQ, tG, p, tiles, chunks, splits, st);
+}

@@ -218,28 +218,30 @@ __global__ void __launch_bounds__(FS_T, 2)
         uint4 o;
         float scale = 1.f;
         if (kb < nk_main) {
-          float f[16], top = 0.f;
-          bool odd = false;
+          // the largest magnitude of a block, two values an instruction; NaN takes no part
+          const bool live = t < p.T;
+          __nv_bfloat162 m2 = __habs2(*reinterpret_cast<__nv_bfloat162*>(&v[q][0]));
+#pragma unroll
+          for (int j = 1; j < 8; ++j) m2 = __hmax2(m2, __habs2(*reinterpret_cast<__nv_bfloat162*>(&v[q][j])));
+          float top = live ? __bfloat162float(__hmax(m2.x, m2.y)) : 0.f, f[16];
+#pragma unroll
+          for (int m = 4; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             const float2 u = unpack_bf16x2(v[q][j]);
-            f[2 * j] = t < p.T ? u.x : 0.f;
-            f[2 * j + 1] = t < p.T ? u.y : 0.f;
+            f[2 * j] = live ? u.x : 0.f;
+            f[2 * j + 1] = live ? u.y : 0.f;
           }
-#pragma unroll
-          for (int j = 0; j < 16; ++j) odd |= !(fabsf(f[j]) <= 3.402823466e38f);
-          if (__any_sync(0xffffffffu, odd)) {
+          if (__any_sync(0xffffffffu, !(top <= 3.402823466e38f))) {
+            top = 0.f;
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
               if (fabsf(f[j]) <= 3.402823466e38f) top = fmaxf(top, fabsf(f[j]));
               else f[j] = __uint_as_float(0x7FC00000u);
             }
-          } else {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) top = fmaxf(top, fabsf(f[j]));
+            for (int m = 4; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
           }
-#pragma unroll
-          for (int m = 4; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
           const int e = fp8_scale_exponent(top);
           const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
           scale = __uint_as_float((uint32_t)e << 23);

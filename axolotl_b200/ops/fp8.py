@@ -330,7 +330,9 @@ class _Fp8LoRALinearFn(torch.autograd.Function):
         dA = None
         if need[3]:
             tgt = getattr(A, "_axb_grad", None)
-            buf = fp8_adapter_grad(t, *_unpacked(q, dy.shape[0], codes.shape[1]), out=tgt)
+            T, K = dy.shape[0], codes.shape[1]
+            ld, at = (K + 15) & ~15, q.data_ptr()
+            buf = _adapter_grad(t, at, ld, at + T * ld, T, K, tgt)
             dA = None if tgt is not None else buf.to(A.dtype)
         _, dB = _adapter_grads(None, B if need[4] else None, t, codes, dy, xa, ctx.blocks, dB_done, dB_fused)
         dbias = dy.float().sum(0).to(ctx.bias_dtype) if need[9] else None
@@ -348,15 +350,32 @@ def fp8_adapter_grad(t, codes, row_scale, out=None):
     R = t.shape[1]
     if out is not None and (tuple(out.shape) != (R, K) or out.dtype != torch.float32 or out.device != codes.device):
         raise ValueError(f"fp8_adapter_grad: the result is float32 [{R}, {K}] on {codes.device}")
-    x = dequantize_fp8_rows(codes, row_scale, torch.bfloat16 if codes.is_cuda else torch.float32)
-    if out is None:
-        out = torch.zeros((R, K), dtype=torch.float32, device=codes.device)
     if not codes.is_cuda:
-        return out.add_(t.float().t() @ x)
-    from .gemm import gemm, pick_splits
-
+        x = t.float().t() @ dequantize_fp8_rows(codes, row_scale, torch.float32)
+        return x if out is None else out.add_(x)
+    if t.dtype != torch.bfloat16:
+        raise TypeError(f"fp8_adapter_grad takes bf16 on the device, got {t.dtype}")
     with _device_of(codes):
-        return gemm(t, x, trans_a=True, trans_b=True, out=out, accumulate=True, splits=pick_splits((K + 255) // 256, (T + 63) // 64))
+        codes = _rows16(codes)
+        row_scale, lds = _row_scales(row_scale, T)
+        return _adapter_grad(t, codes.data_ptr(), codes.stride(0), row_scale.data_ptr(), lds, K, out)
+
+
+def _adapter_grad(t, q, ldq, s, lds, K, out):
+    """The launch of ``fp8_adapter_grad`` on codes at ``q`` and scales at ``s``."""
+    T, R = t.shape
+    if T == 0 or R == 0:
+        return torch.zeros((R, K), dtype=torch.float32, device=t.device) if out is None else out
+    if out is not None and out.stride(1) != 1:
+        return out.add_(_adapter_grad(t, q, ldq, s, lds, K, None))
+    if t.stride(1) != 1 or t.stride(0) % 8 or t.data_ptr() % 16:
+        t = torch.nn.functional.pad(t, (0, -R % 8))[:, :R] if R % 8 else t.contiguous()
+    add = out is not None
+    if not add:
+        out = torch.empty((R, K), dtype=torch.float32, device=t.device)
+    _lib.check_rc(_lib.cuda_lib().axb_fp8_adapter_grad(q, ldq, s, lds, t.data_ptr(), t.stride(0), out.data_ptr(), out.stride(0) if R > 1 else K, T, K, R,
+                                                       add, _lib.status_word(t.device).data_ptr(), _lib.stream_ptr()), "fp8_adapter_grad")
+    return out
 
 
 def _check_linear(x, codes, scale, what):

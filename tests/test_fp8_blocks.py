@@ -335,7 +335,7 @@ def test_lora_linear_and_its_gradients(T, K, N, blocks):
 
 
 @pytest.mark.parametrize("dev", DEVICES)
-@pytest.mark.parametrize("T,K,R", [(1, 128, 8), (77, 200, 16), (300, 1000, 40), (1030, 264, 64)])
+@pytest.mark.parametrize("T,K,R", [(1, 128, 8), (77, 200, 16), (300, 1000, 40), (1030, 264, 64), (2100, 136, 5), (129, 4360, 1), (700, 520, 200)])
 def test_adapter_gradient_from_saved_rows(T, K, R, dev):
     x, t = _make((T, K), T + K, spread=0.5), _make((T, R), R, spread=0.5)
     codes, scale = quantize_fp8_rows(x.to(dev))
@@ -347,6 +347,11 @@ def test_adapter_gradient_from_saved_rows(T, K, R, dev):
     into = base.clone().to(dev)
     assert fp8_adapter_grad(t.to(dev), codes, scale, out=into) is into
     assert ((into.cpu().double() - base.double() - want).abs() <= tol + (T + 16) * EPS32 * base.double().abs()).all()
+    # a result and codes of other strides, the same sums
+    wide = torch.zeros(K, R, device=dev).t()
+    assert torch.equal(fp8_adapter_grad(t.to(dev), codes, scale, out=wide), got)
+    turned = scale.t().contiguous().t()
+    assert torch.equal(fp8_adapter_grad(t.t().contiguous().t().to(dev), codes, turned), got)
 
 
 # ------------------------------------------------------------------ checkpoints
@@ -582,3 +587,23 @@ def test_few_tokens_with_nan_and_infinity():
     x[0, 3], x[1, 5] = torch.finfo(torch.bfloat16).max, 2.0 ** -133
     w, ws = quantize_fp8_weight((torch.eye(256) * 2.0 ** -6).cuda())
     _assert_product(fp8._product(x, w, ws)[0], _rows8(x), _weight8(w, ws).t())
+
+
+def test_adapter_gradient_of_no_rows():
+    codes, scale = quantize_fp8_rows(torch.empty(0, 256, dtype=torch.bfloat16))
+    assert torch.equal(fp8_adapter_grad(torch.empty(0, 8).bfloat16(), codes, scale), torch.zeros(8, 256))
+
+
+@pytest.mark.gpu
+def test_adapter_gradient_with_nan():
+    """NaN codes reach the columns they stand in and no others."""
+    x = _make((300, 384), 1, spread=0.0)
+    t = _make((300, 16), 2, spread=0.0).cuda()
+    clean = fp8_adapter_grad(t, *quantize_fp8_rows(x.cuda()))
+    x[299, 5], x[0, 130] = float("inf"), float("nan")
+    got = fp8_adapter_grad(t, *quantize_fp8_rows(x.cuda()))
+    nan = torch.isnan(got).all(0).cpu()
+    assert nan.nonzero().flatten().tolist() == [5, 130] and torch.isfinite(got[:, ~nan]).all()
+    same = torch.ones(384, dtype=torch.bool)
+    same[:256] = False                                     # blocks whose maximum may have been the value that is gone
+    assert torch.equal(got[:, same], clean[:, same])
