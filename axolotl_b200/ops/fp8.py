@@ -17,6 +17,7 @@ product in the forward pass, the weight expanded to bf16 in the backward pass) a
 from __future__ import annotations
 
 import contextlib
+import ctypes as C
 from dataclasses import dataclass
 
 import torch
@@ -305,37 +306,102 @@ class _Fp8LinearFn(torch.autograd.Function):
         return dx, None, None, dbias
 
 
-class _Fp8LoRALinearFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, codes, scale, A, B, A16, B16, scaling, blocks, bias):
+class _Lora(C.Structure):
+    """AxbFp8Lora of csrc/fp8_lora.cu."""
+    _fields_ = ([(n, C.c_void_p) for n in ("x", "q", "W", "sw", "A", "B", "xa", "y", "qx", "t32", "t", "dA", "dB", "blocks", "status")]
+                + [(n, C.c_longlong) for n in ("ldx", "ldw", "sw_n", "sw_k", "lda", "ldb", "ldda", "lddb")]
+                + [(n, C.c_int) for n in ("T", "N", "K", "R", "tile", "n_blocks", "add_dA", "add_dB")] + [("scaling", C.c_float)])
+
+
+def _lora_args(x, codes, scale, A16, B16, scaling, T, N, K, R, tile):
+    l = _Lora()
+    l.x, l.ldx, l.W, l.ldw, l.sw = x.data_ptr(), x.stride(0), codes.data_ptr(), codes.stride(0), scale.data_ptr()
+    l.sw_n, l.sw_k = scale.stride()
+    l.A, l.lda, l.B, l.ldb = A16.data_ptr(), A16.stride(0), B16.data_ptr(), B16.stride(0)
+    l.T, l.N, l.K, l.R, l.tile, l.scaling = T, N, K, R, tile, scaling
+    l.status = _lib.status_word(x.device).data_ptr()
+    return l
+
+
+def _operand16(t):
+    return t.dtype == torch.bfloat16 and t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0
+
+
+def _lora_forward(x, codes, scale, A16, B16, scaling, keep):
+    """(y, scaling x A^T, block of ``_pack`` of x or None): one call where the operands are what the kernels read as they are."""
+    T, K = x.shape
+    R, N = A16.shape[0], codes.shape[0]
+    if not (T and R <= 128 and R % 8 == 0 and _operand16(x) and _operand16(A16) and _operand16(B16)
+            and x.device.index == torch.cuda.current_device()):
         from .lora import skinny_gemm
 
         xa = skinny_gemm(x, A16, alpha=scaling)            # [T, R], of the bf16 input
-        y, q = _product(x, codes, scale, a2=xa, b2=B16, keep=ctx.needs_input_grad[3])
+        y, q = _product(x, codes, scale, a2=xa, b2=B16, keep=keep)
+        return y, xa, q
+    codes = _rows16(codes)
+    l = _lora_args(x, codes, scale, A16, B16, scaling, T, N, K, R, _tile(T, N))
+    y = torch.empty((T, N), dtype=torch.bfloat16, device=x.device)
+    xa = torch.empty((T, R), dtype=torch.bfloat16, device=x.device)
+    l.y, l.xa, q = y.data_ptr(), xa.data_ptr(), None
+    if keep or T > _FEW:
+        q = torch.empty(T * (((K + 15) & ~15) + 4 * _blocks(K)), dtype=torch.uint8, device=x.device)
+        l.q = q.data_ptr()
+    _lib.check_rc(_lib.cuda_lib().axb_fp8_lora_fwd(C.byref(l), _lib.stream_ptr()), "fp8_lora_fwd")
+    return y, xa, q
+
+
+class _Fp8LoRALinearFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, codes, scale, A, B, A16, B16, scaling, blocks, bias):
+        y, xa, q = _lora_forward(x, codes, scale, A16, B16, scaling, ctx.needs_input_grad[3])
         if bias is not None:
             y = y + bias
-        ctx.save_for_backward(q if ctx.needs_input_grad[3] else None, codes, scale, A, B, A16, B16, xa)
+        ctx.save_for_backward(q, codes, scale, A, B, A16, B16, xa)
         ctx.scaling, ctx.blocks, ctx.bias_dtype = scaling, blocks, None if bias is None else bias.dtype
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        from .lora import _adapter_grads, _t_and_dB
+        from .lora import _adapter_grads, _t_and_dB, fused_dy_ok
 
         q, codes, scale, A, B, A16, B16, xa = ctx.saved_tensors
         need = ctx.needs_input_grad
         dy = dy.contiguous()
+        (T, N), K, R = dy.shape, codes.shape[1], A16.shape[0]
+        dbias = dy.float().sum(0).to(ctx.bias_dtype) if need[9] else None
+        dx = dA = dB = None
+        if need[4] and fused_dy_ok(dy, B16, xa) and R % 8 == 0 and all(map(_operand16, (dy, A16, B16, xa))) and len(ctx.blocks) <= 8:
+            # one pass over dy for t and dB, the product and dA behind it: one call
+            codes = _rows16(codes)
+            l = _lora_args(dy, codes, scale, A16, B16, ctx.scaling, T, N, K, R, _tile(T, K))
+            n = T * R
+            work = torch.empty(6 * n + (T * (((N + 15) & ~15) + 4 * _blocks(N)) if need[0] else 0), dtype=torch.uint8, device=dy.device)
+            l.t32, l.t, l.xa = work.data_ptr(), work.data_ptr() + 4 * n, xa.data_ptr()
+            if need[0]:
+                dx = torch.empty((T, K), dtype=torch.bfloat16, device=dy.device)
+                l.q, l.y = work.data_ptr() + 6 * n, dx.data_ptr()
+            tB = getattr(B, "_axb_grad", None)
+            dB = tB if tB is not None else torch.empty((N, R), dtype=torch.float32, device=dy.device)
+            l.dB, l.lddb, l.add_dB = dB.data_ptr(), dB.stride(0), tB is not None
+            tA = None
+            if need[3]:
+                tA = getattr(A, "_axb_grad", None)
+                dA = tA if tA is not None else torch.empty((R, K), dtype=torch.float32, device=dy.device)
+                l.qx, l.dA, l.ldda, l.add_dA = q.data_ptr(), dA.data_ptr(), dA.stride(0), tA is not None
+            flat = (C.c_int * (4 * len(ctx.blocks)))(*[int(v) for b in ctx.blocks for v in b])
+            l.blocks, l.n_blocks = C.addressof(flat), len(ctx.blocks)
+            _lib.check_rc(_lib.cuda_lib().axb_fp8_lora_bwd(C.byref(l), _lib.stream_ptr()), "fp8_lora_bwd")
+            dA = None if dA is None or tA is not None else dA.to(A.dtype)
+            dB = None if tB is not None else dB.to(B.dtype)
+            return dx, None, None, dA, dB, None, None, None, None, dbias
         t, dB_fused, dB_done = _t_and_dB(dy, B, B16, xa, ctx.blocks, ctx.scaling, need[4])
         dx = _product(dy, codes, scale, trans=True, a2=t, b2=A16)[0] if need[0] else None
-        dA = None
         if need[3]:
             tgt = getattr(A, "_axb_grad", None)
-            T, K = dy.shape[0], codes.shape[1]
             ld, at = (K + 15) & ~15, q.data_ptr()
             buf = _adapter_grad(t, at, ld, at + T * ld, T, K, tgt)
             dA = None if tgt is not None else buf.to(A.dtype)
         _, dB = _adapter_grads(None, B if need[4] else None, t, codes, dy, xa, ctx.blocks, dB_done, dB_fused)
-        dbias = dy.float().sum(0).to(ctx.bias_dtype) if need[9] else None
         return dx, None, None, dA, dB, None, None, None, None, dbias
 
 
@@ -419,4 +485,8 @@ def fp8_lora_linear(x, codes, scale, A, B, A16, B16, scaling, blocks, bias=None)
     if not x.is_cuda:
         y = _Fp8LinearFn.apply(x2, codes, scale, bias).to(x.dtype)
         return _shaped(y + scaling * ((x2 @ A.to(x2.dtype).t()) @ B.to(x2.dtype).t()), x)
-    return _shaped(_Fp8LoRALinearFn.apply(x2.contiguous(), codes, scale, A, B, A16, B16, float(scaling), blocks, bias), x)
+    x2 = x2.contiguous()
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, A, B, bias)):
+        return _shaped(_Fp8LoRALinearFn.apply(x2, codes, scale, A, B, A16, B16, float(scaling), blocks, bias), x)
+    y = _lora_forward(x2, codes, scale, A16, B16, float(scaling), False)[0]
+    return _shaped(y if bias is None else y + bias, x)

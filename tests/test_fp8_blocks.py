@@ -607,3 +607,42 @@ def test_adapter_gradient_with_nan():
     same = torch.ones(384, dtype=torch.bool)
     same[:256] = False                                     # blocks whose maximum may have been the value that is gone
     assert torch.equal(got[:, same], clean[:, same])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,R", [(70, 8), (600, 16), (600, 72)])
+def test_lora_gradients_into_flat_buffers(T, R):
+    """Parameters whose gradient has a place of its own get the same gradients there, added to what it holds."""
+    K, N = 520, 264
+    x, dy = _make((T, K), 1, spread=0.5).cuda(), (_make((T, N), 2, spread=0.5) * 1e-2).cuda()
+    w, ws = quantize_fp8_weight(_make((N, K), 3, torch.float32, 0.0).cuda())
+    A, B = (_make((R, K), 4, torch.float32, 0.0) * K ** -0.5).cuda(), (_make((N, R), 5, torch.float32, 0.0) * 0.1).cuda()
+    grads = []
+    for flat in (False, True):
+        Al, Bl, xl = A.clone().requires_grad_(True), B.clone().requires_grad_(True), x.clone().requires_grad_(True)
+        if flat:
+            Al._axb_grad, Bl._axb_grad = torch.ones_like(A), torch.full_like(B, 2.0)
+        y = fp8_lora_linear(xl, w, ws, Al, Bl, A.bfloat16(), B.bfloat16(), 0.5, ((0, N, 0, R),))
+        y.backward(dy)
+        assert (Al.grad is None) == flat and (Bl.grad is None) == flat
+        grads.append((y, xl.grad, Al._axb_grad - 1 if flat else Al.grad, Bl._axb_grad - 2 if flat else Bl.grad))
+    assert torch.equal(grads[0][0], grads[1][0])
+    for a, b in zip(grads[0][1:], grads[1][1:]):
+        # t and dB are summed by fp32 atomics in any order; adding to 1 or 2 rounds to 2^-23
+        assert ((a.double() - b.double()).abs() <= 1e-2 * a.double().abs().max() * 2.0 ** -4 + 2.0 ** -21).all()
+
+
+@pytest.mark.gpu
+def test_lora_without_gradients_keeps_nothing():
+    """Under no_grad, or with a frozen adapter, the layer gives the same result; without an adapter gradient no codes are kept."""
+    x = _make((40, 256), 1, spread=0.5).cuda()
+    w, ws = quantize_fp8_weight(_make((128, 256), 3, torch.float32, 0.0).cuda())
+    A, B = _make((8, 256), 4, spread=0.0).cuda() * 0.06, _make((128, 8), 5, spread=0.0).cuda() * 0.1
+    args = (w, ws, A, B, A, B, 2.0, ((0, 128, 0, 8),))
+    with torch.no_grad():
+        want = fp8_lora_linear(x, *args)
+    xl = x.clone().requires_grad_(True)
+    y = fp8_lora_linear(xl, *args)
+    assert torch.equal(y, want) and y.grad_fn.saved_tensors[0] is None
+    (dx,) = torch.autograd.grad(y, [xl], torch.ones_like(y))
+    assert torch.isfinite(dx).all()
