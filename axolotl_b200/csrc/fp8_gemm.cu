@@ -16,9 +16,9 @@
 
 extern "C" int axb_fp8_quantize_rows(const void* x, long long ldx, int dtype, void* q, long long ldq, float* s, long long lds,
                                      long long rows, int K, void* stream);
-extern "C" int axb_fp8_skinny(const void* x, long long ldx, const void* W, long long ldw, const float* sw, long long sw_n, long long sw_k,
-                              void* y, long long ldy, int T, int N, int K, const void* X2, long long ldx2, const void* B2, long long ldb2,
-                              int K2, int* status, void* stream);
+extern "C" int axb_fp8_skinny(const void* x, long long ldx, const void* q, long long ldq, const float* sx, const void* W, long long ldw,
+                              const float* sw, long long sw_n, long long sw_k, void* y, long long ldy, int T, int N, int K, const void* X2,
+                              long long ldx2, const void* B2, long long ldb2, int K2, int* status, void* stream);
 
 namespace {
 
@@ -408,10 +408,13 @@ extern "C" int axb_fp8_linear(const void* x, long long ldx, void* q, const void*
                               long long ldb2, int K2, int tile, int* status, void* stream) {
   if (!q) {
     if (b_mn) return -2;
-    return axb_fp8_skinny(x, ldx, W, ldw, sw, sw_n, sw_k, y, N, T, N, K, X2, ldx2, B2, ldb2, K2, status, stream);
+    return axb_fp8_skinny(x, ldx, nullptr, 0, nullptr, W, ldw, sw, sw_n, sw_k, y, N, T, N, K, X2, ldx2, B2, ldb2, K2, status, stream);
   }
   const long long ldq = (K + 15ll) & ~15ll;
   float* s = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(q) + ldq * T);
-  const int rc = axb_fp8_quantize_rows(x, ldx, 0, q, ldq, s, T, T, K, stream);
-  return rc ? rc : axb_fp8_gemm(q, ldq, s, T, W, ldw, sw, sw_n, sw_k, b_mn, y, N, T, N, K, X2, ldx2, B2, ldb2, K2, tile, status, stream);
+  int rc = axb_fp8_quantize_rows(x, ldx, 0, q, ldq, s, T, T, K, stream);
+  if (rc) return rc;
+  if (!b_mn && tile == 0)
+    return axb_fp8_skinny(x, ldx, q, ldq, s, W, ldw, sw, sw_n, sw_k, y, N, T, N, K, X2, ldx2, B2, ldb2, K2, status, stream);
+  return axb_fp8_gemm(q, ldq, s, T, W, ldw, sw, sw_n, sw_k, b_mn, y, N, T, N, K, X2, ldx2, B2, ldb2, K2, tile, status, stream);
 }

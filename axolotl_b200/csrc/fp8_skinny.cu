@@ -1,12 +1,12 @@
 // y[t, n] = sum_b sx[t, b] sw[n / 128, b] (sum_{k in b} q[t, k] w[n, k]) (+ sum_r a2[t, r] b2[n, r]) for at most 64 tokens: a generation
-// step through a frozen weight in 8-bit blocks (codes [N, K], csrc/fp8_gemm.cu), from the bf16 rows x in one launch.
+// step through a frozen weight in 8-bit blocks (codes [N, K], csrc/fp8_gemm.cu).
 //
 // Bound: one pass over the codes (HBM). The weight is the 128-row operand of tcgen05.mma (kind::f8f6f4), so no tensor-core row is
 // padding, and the tokens are its N = 16 .. 64 columns. The K range of a tile is split over a cluster of up to 8 CTAs and two CTAs share
 // an SM, so that some 160 KB of codes per SM are in flight; the partial tiles meet in distributed shared memory in a fixed order.
-// Four warps quantise the rows of x into the operand tile while the weight's bulk copies arrive: the codes and their scales never reach
-// memory. Every block of 128 columns starts an accumulator of its own; four warps (a thread owns a weight row) add it to sums in
-// registers, times the weight's scale and the token's.
+// Every block of 128 columns starts an accumulator of its own; four warps (a thread owns a weight row) add it to sums in registers,
+// times the weight's scale and the token's. The rows come as codes (csrc/fp8_rows.cu), or (FUSED) in bf16: then four warps quantise them
+// into the operand tile while the weight's bulk copies arrive, and the codes and their scales never reach memory. ops/fp8.py says when.
 #include <cuda_fp8.h>
 
 #include "axb_common.cuh"
@@ -20,6 +20,7 @@ constexpr int FS_RING = 16;               // blocks whose row scales are held (s
 struct Fp8SkinnyParams {
   const __nv_bfloat16* x;
   const __nv_bfloat16* x2;                // bf16 extension of the tokens
+  const float* sx;                        // scales of quantised rows [block][T] (FUSED: not there)
   const float* sw;
   __nv_bfloat16* y;
   long long ldx, ldx2, sw_n, sw_k, ldy;
@@ -56,9 +57,10 @@ AXB_DEVICE void load16(const Fp8SkinnyParams& p, const __nv_bfloat16* row, int c
   }
 }
 
-template <int NT>
+template <int NT, bool FUSED>
 __global__ void __launch_bounds__(FS_T, 2)
-    fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmB2, const Fp8SkinnyParams p) {
+    fp8_skinny_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmB2, const __grid_constant__ CUtensorMap tmX,
+                      const __grid_constant__ CUtensorMap tmX2, const Fp8SkinnyParams p) {
   using C = FsCfg<NT>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -68,7 +70,8 @@ __global__ void __launch_bounds__(FS_T, 2)
   uint64_t* tfull = empty + C::STAGES;
   uint64_t* tempty = tfull + C::BUFS;
   uint64_t* ready = tempty + C::BUFS;                                          // row scales of a block are in the ring
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ready + FS_RING);
+  uint64_t* freed = ready + FS_RING;                                           // and have been used (where the rows come quantised)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(freed + FS_RING);
   const int tid = threadIdx.x, warp = uniform_warp(), lane = tid & 31;
   const int rank = (int)cluster_ctarank(), cs = (int)cluster_nctarank();
   const int tile = blockIdx.x / cs;
@@ -77,14 +80,17 @@ __global__ void __launch_bounds__(FS_T, 2)
 
   if (tid == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
-      mbar_init(&full[s], 5);
+      mbar_init(&full[s], FUSED ? 5 : 1);
       mbar_init(&empty[s], 1);
     }
     for (int s = 0; s < C::BUFS; ++s) {
       mbar_init(&tfull[s], 1);
       mbar_init(&tempty[s], 4);
     }
-    for (int s = 0; s < FS_RING; ++s) mbar_init(&ready[s], 4);
+    for (int s = 0; s < FS_RING; ++s) {
+      mbar_init(&ready[s], 4);
+      mbar_init(&freed[s], 4);
+    }
     mbar_fence_init();
     tma_prefetch_desc(&tmW);
   }
@@ -105,8 +111,10 @@ __global__ void __launch_bounds__(FS_T, 2)
       if (!warp_all(mbar_wait(&empty[s], phase ^ 1, p.status, AXB_TIMEOUT_EMPTY))) break;
       if (elect_one()) {
         const bool ext = kb >= nk_main;
-        mbar_expect_tx(&full[s], FS_P);
-        tma_load_2d(smem + s * C::STAGE, ext ? &tmB2 : &tmW, &full[s], ext ? (kb - nk_main) * 64 : kb * 128, tile * 128);
+        const int k0 = ext ? (kb - nk_main) * 64 : kb * 128;
+        mbar_expect_tx(&full[s], FUSED ? FS_P : C::STAGE);
+        tma_load_2d(smem + s * C::STAGE, ext ? &tmB2 : &tmW, &full[s], k0, tile * 128);
+        if (!FUSED) tma_load_2d(smem + s * C::STAGE + FS_P, ext ? &tmX2 : &tmX, &full[s], k0, 0);
       }
       __syncwarp();
       if (++s == C::STAGES) {
@@ -182,7 +190,10 @@ __global__ void __launch_bounds__(FS_T, 2)
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&tempty[buf]);
+      if (lane == 0) {
+        mbar_arrive(&tempty[buf]);
+        if (!FUSED) mbar_arrive(&freed[i % FS_RING]);
+      }
       if (++buf == C::BUFS) {
         buf = 0;
         buf_phase ^= 1;
@@ -192,6 +203,22 @@ __global__ void __launch_bounds__(FS_T, 2)
 #pragma unroll
     for (int j = 0; j < NT; ++j)
       if (j < p.T) part[j * 128 + (warp & 3) * 32 + lane] = sum[j];
+  } else if (!FUSED) {
+    // the rows' scales into the ring, a quarter of the tokens a warp, as far ahead as the ring goes. (Not by the operands' `empty`: nothing
+    // keeps these warps within one phase of it.)
+    const int t = (warp - 6) * (NT / 4) + lane;
+    const bool mine = lane < NT / 4;
+    auto fetch = [&](int kb) { return mine && kb < nk_main && t < p.T ? __ldg(p.sx + (long long)kb * p.T + t) : 1.f; };
+    float next = fetch(kb0);
+    for (int kb = kb0; kb < kb1; ++kb) {
+      const int i = kb - kb0, slot = i % FS_RING;
+      const float v = next;
+      next = fetch(kb + 1);
+      if (!warp_all(mbar_wait(&freed[slot], ((uint32_t)(i / FS_RING) & 1) ^ 1, p.status, AXB_TIMEOUT_EMPTY))) break;
+      if (mine) scales[slot * NT + t] = v;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ready[slot]);
+    }
   } else {
     // eight lanes hold the block of a row (16 values each), four rows a pass; tokens past T leave their columns as they are
     const int sub = lane >> 3, at = lane & 7;
@@ -311,13 +338,13 @@ __global__ void __launch_bounds__(FS_T, 2)
   }
 }
 
-template <int NT>
-int launch_fp8_skinny(const CUtensorMap& w, const CUtensorMap& b2, const Fp8SkinnyParams& p, int tiles, int splits, cudaStream_t st) {
-  auto kern = fp8_skinny_kernel<NT>;
+template <int NT, bool FUSED>
+int launch_fp8_skinny(const CUtensorMap (&m)[4], const Fp8SkinnyParams& p, int tiles, int splits, cudaStream_t st) {
+  auto kern = fp8_skinny_kernel<NT, FUSED>;
   static std::atomic<unsigned long long> allowed{0};
   if (const int rc = axb_allow_smem((const void*)kern, FsCfg<NT>::SMEM, allowed)) return rc;
   AxbLaunch l(dim3((unsigned)(tiles * splits)), FS_T, FsCfg<NT>::SMEM, st, splits, false);
-  const cudaError_t e = cudaLaunchKernelEx(&l.cfg, kern, w, b2, p);
+  const cudaError_t e = cudaLaunchKernelEx(&l.cfg, kern, m[0], m[1], m[2], m[3], p);
   return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }
 
@@ -332,23 +359,28 @@ int fp8_skinny_splits(int tiles, int nk) {
 
 }  // namespace
 
-// See the head of this file. x: bf16 [T, K], T <= 64; W: codes [N, K], rows of ldw bytes, and their scales sw[(n / 128) * sw_n + b * sw_k];
-// y: bf16 [T, N]; X2 [T, K2] and B2 [N, K2] bf16, K2 = 0: none. W, X2 and B2 start on 16 bytes and have row strides of whole 16 bytes.
-extern "C" int axb_fp8_skinny(const void* x, long long ldx, const void* W, long long ldw, const float* sw, long long sw_n, long long sw_k,
-                              void* y, long long ldy, int T, int N, int K, const void* X2, long long ldx2, const void* B2, long long ldb2,
-                              int K2, int* status, void* stream) {
+// See the head of this file. x: bf16 [T, K], T <= 64; q (null: the rows are quantised by the kernel): their codes, rows of ldq bytes, and
+// sx: their scales [ceil(K / 128)][T]; W: codes [N, K], rows of ldw bytes, and their scales sw[(n / 128) * sw_n + b * sw_k]; y: bf16
+// [T, N]; X2 [T, K2] and B2 [N, K2] bf16, K2 = 0: none. q, W, X2 and B2 start on 16 bytes and have row strides of whole 16 bytes.
+extern "C" int axb_fp8_skinny(const void* x, long long ldx, const void* q, long long ldq, const float* sx, const void* W, long long ldw,
+                              const float* sw, long long sw_n, long long sw_k, void* y, long long ldy, int T, int N, int K, const void* X2,
+                              long long ldx2, const void* B2, long long ldb2, int K2, int* status, void* stream) {
   if (T <= 0 || N <= 0) return 0;
-  auto bad = [](const void* q, long long bytes) { return (reinterpret_cast<uintptr_t>(q) & 15) != 0 || (bytes & 15) != 0; };
-  if (T > 64 || K <= 0 || bad(W, ldw)) return -2;
+  auto bad = [](const void* a, long long bytes) { return (reinterpret_cast<uintptr_t>(a) & 15) != 0 || (bytes & 15) != 0; };
+  if (T > 64 || K <= 0 || bad(W, ldw) || (q && bad(q, ldq))) return -2;
   if (K2 > 0 && (bad(X2, 2 * ldx2) || bad(B2, 2 * ldb2) || (K2 & 7))) return -2;
-  CUtensorMap tW, tB2;
-  int rc = axb_make_tmap_2d(&tW, W, N, K, ldw, 128, 128, 1);
-  tB2 = tW;
-  if (!rc && K2 > 0) rc = axb_make_tmap_2d(&tB2, B2, N, K2, ldb2, 128, 64);
+  const int NT = T <= 16 ? 16 : (T <= 32 ? 32 : 64);
+  CUtensorMap m[4];
+  int rc = axb_make_tmap_2d(&m[0], W, N, K, ldw, 128, 128, 1);
+  m[1] = m[2] = m[3] = m[0];
+  if (!rc && K2 > 0) rc = axb_make_tmap_2d(&m[1], B2, N, K2, ldb2, 128, 64);
+  if (!rc && q) rc = axb_make_tmap_2d(&m[2], q, T, K, ldq, NT, 128, 1);
+  if (!rc && q && K2 > 0) rc = axb_make_tmap_2d(&m[3], X2, T, K2, ldx2, NT, 64);
   if (rc) return -100 - rc;
   Fp8SkinnyParams p = {};
   p.x = (const __nv_bfloat16*)x;
   p.x2 = (const __nv_bfloat16*)X2;
+  p.sx = sx;
   p.sw = sw;
   p.y = (__nv_bfloat16*)y;
   p.ldx = ldx;
@@ -364,7 +396,12 @@ extern "C" int axb_fp8_skinny(const void* x, long long ldx, const void* W, long 
   p.status = status;
   const int tiles = (N + 127) / 128, nk = (K + 127) / 128 + (p.K2 + 63) / 64, splits = fp8_skinny_splits(tiles, nk);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (T <= 16) return launch_fp8_skinny<16>(tW, tB2, p, tiles, splits, st);
-  if (T <= 32) return launch_fp8_skinny<32>(tW, tB2, p, tiles, splits, st);
-  return launch_fp8_skinny<64>(tW, tB2, p, tiles, splits, st);
+  if (q) {
+    if (NT == 16) return launch_fp8_skinny<16, false>(m, p, tiles, splits, st);
+    if (NT == 32) return launch_fp8_skinny<32, false>(m, p, tiles, splits, st);
+    return launch_fp8_skinny<64, false>(m, p, tiles, splits, st);
+  }
+  if (NT == 16) return launch_fp8_skinny<16, true>(m, p, tiles, splits, st);
+  if (NT == 32) return launch_fp8_skinny<32, true>(m, p, tiles, splits, st);
+  return launch_fp8_skinny<64, true>(m, p, tiles, splits, st);
 }

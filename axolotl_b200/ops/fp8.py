@@ -250,7 +250,21 @@ def _tile(M, N) -> int:
     return 256 if M > 128 and N > 128 and -(-M // 256) * -(-N // 256) >= 74 else 128
 
 
-_FEW = 64      # rows up to which a product that keeps no codes is one launch (csrc/fp8_skinny.cu)
+def _few(T, N, K):
+    """How the product of a few tokens runs: 2 in one launch, quantising inside (csrc/fp8_skinny.cu), 1 by the same kernel on rows that a
+    launch before it has quantised, 0 by tiles. Inside, every CTA quantises the blocks of its part of K, 16 tokens at a time: some
+    0.5 us each, against 3 us for the launch that does it once. Microseconds, inside / before / tiles: 24 x 4096 by 4096 (4 blocks a
+    CTA, two passes) 16.5 / 20.2 / 21.5; 16 x 4096 by 6144 (8, one) 15.9 / 19.0 / 21.5, 64 (four) 27.0 / 21.4 / 22.8; 1 x 4096 by 28672
+    (32, one) 32.6 / 29.7 / 47.6; 64 x 14336 by 4096 (14, four) 37.8 / 29.4 / 46.4; 64 x 4096 by 28672, where the tiles fill the chip
+    by themselves, 66.1 / 39.5 / 34.8."""
+    if T > 64:
+        return 0
+    tiles, nk = (N + 127) >> 7, (K + 127) >> 7
+    # CTAs of a tile: fp8_skinny_splits
+    splits = 8 if tiles <= 33 and nk >= 16 else 4 if tiles <= 70 and nk >= 8 else 2 if tiles <= 148 and nk >= 4 else 1
+    if -(-nk // splits) * (1 if T <= 16 else 2 if T <= 32 else 4) <= 16:
+        return 2
+    return 0 if T > 32 and tiles > 70 else 1
 
 
 def _product(x, codes, scale, trans=False, a2=None, b2=None, keep=False):
@@ -278,13 +292,14 @@ def _product(x, codes, scale, trans=False, a2=None, b2=None, keep=False):
         a2, b2, K2 = _row_major_2d(a2), _row_major_2d(b2), a2.shape[1]
     y = torch.empty((T, N), dtype=torch.bfloat16, device=x.device)
     q = None
-    if keep or trans or T > _FEW or K2 % 8:
+    few = 0 if trans or K2 % 8 else _few(T, N, K)
+    if keep or few < 2:
         q = torch.empty(T * (((K + 15) & ~15) + 4 * _blocks(K)), dtype=torch.uint8, device=x.device)
     _lib.check_rc(_lib.cuda_lib().axb_fp8_linear(
         x.data_ptr(), x.stride(0), None if q is None else q.data_ptr(), codes.data_ptr(), codes.stride(0), scale.data_ptr(), sn, sk,
         trans, y.data_ptr(), T, N, K, None if K2 == 0 else a2.data_ptr(), 0 if K2 == 0 else a2.stride(0),
-        None if K2 == 0 else b2.data_ptr(), 0 if K2 == 0 else b2.stride(0), K2, _tile(T, N), _lib.status_word(x.device).data_ptr(),
-        _lib.stream_ptr()), "fp8_linear")
+        None if K2 == 0 else b2.data_ptr(), 0 if K2 == 0 else b2.stride(0), K2, 0 if few else _tile(T, N),
+        _lib.status_word(x.device).data_ptr(), _lib.stream_ptr()), "fp8_linear")
     return y, q
 
 
@@ -339,11 +354,12 @@ def _lora_forward(x, codes, scale, A16, B16, scaling, keep):
         y, q = _product(x, codes, scale, a2=xa, b2=B16, keep=keep)
         return y, xa, q
     codes = _rows16(codes)
-    l = _lora_args(x, codes, scale, A16, B16, scaling, T, N, K, R, _tile(T, N))
+    few = _few(T, N, K)
+    l = _lora_args(x, codes, scale, A16, B16, scaling, T, N, K, R, 0 if few else _tile(T, N))
     y = torch.empty((T, N), dtype=torch.bfloat16, device=x.device)
     xa = torch.empty((T, R), dtype=torch.bfloat16, device=x.device)
     l.y, l.xa, q = y.data_ptr(), xa.data_ptr(), None
-    if keep or T > _FEW:
+    if keep or few < 2:
         q = torch.empty(T * (((K + 15) & ~15) + 4 * _blocks(K)), dtype=torch.uint8, device=x.device)
         l.q = q.data_ptr()
     _lib.check_rc(_lib.cuda_lib().axb_fp8_lora_fwd(C.byref(l), _lib.stream_ptr()), "fp8_lora_fwd")
