@@ -61,6 +61,8 @@ AXB_DEVICE constexpr uint32_t make_idesc_e4m3(int m, int n, int b_mn_major) {
   return (1u << 4) | (uint32_t(b_mn_major) << 16) | (uint32_t(n >> 3) << 17) | (uint32_t(m >> 4) << 24);
 }
 
+AXB_DEVICE const float* at_bytes(const float* p, long long n) { return reinterpret_cast<const float*>(reinterpret_cast<const char*>(p) + n); }
+
 // tiles in bands of group_m tile rows that sweep over N together (their A rows stay in L2)
 AXB_DEVICE void fp8_tile(int tile, int num_m, int num_n, int group_m, int& m_blk, int& n_blk) {
   const int per = group_m * num_n, group = tile / per, first = group * group_m;
@@ -120,6 +122,7 @@ __global__ void __launch_bounds__(G_THREADS, 1)
   if constexpr (PAIR) cluster_sync();          // the barriers of both CTAs are ready before anything arrives on them
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  pdl_wait();                                  // in a dependent launch: the rows have been quantised
 
   if (warp == 0) {
     int stage = 0;
@@ -130,7 +133,7 @@ __global__ void __launch_bounds__(G_THREADS, 1)
       fp8_tile(tile, num_m, num_n, p.group_m, m_blk, n_blk);
       const int m0 = m_blk * TILE + rank * 128, n0 = n_blk * TILE + rank * 128;
       for (int kb = 0; kb < nk; ++kb) {
-        if (!warp_all(mbar_wait_spin(&empty[stage], phase ^ 1, p.status, AXB_TIMEOUT_EMPTY))) {
+        if (!warp_all(mbar_wait(&empty[stage], phase ^ 1, p.status, AXB_TIMEOUT_EMPTY))) {
           ok = false;
           break;
         }
@@ -231,6 +234,7 @@ __global__ void __launch_bounds__(G_THREADS, 1)
     uint8_t* stg = sEpi + (warp - 2) * 4096;
     const int set = PAIR ? half : 0;
     const uint32_t t_base = tmem + (uint32_t(quad * 32) << 16) + (PAIR ? set * BUFS * 128 : half * 64);
+    const long long step_a = p.ldsa * 4, step_b = p.sb_k * 4;   // bytes: the address arithmetic stays off the multipliers
     int buf = 0;
     uint32_t buf_phase = 0;
     bool ok = true;
@@ -242,22 +246,22 @@ __global__ void __launch_bounds__(G_THREADS, 1)
       const bool live = row < p.M;
       const float* sa = p.sa + (live ? row : 0);
       const float* sb = p.sb + (long long)(col0 >> 7) * p.sb_n;
-      const long long sb1 = col0 + 128 < p.N ? p.sb_n : 0;      // of group 1
+      const float* sb2 = sb + (col0 + 128 < p.N ? p.sb_n : 0);  // of group 1
       uint64_t sum[GROUPS * 32];
 #pragma unroll
       for (int j = 0; j < GROUPS * 32; ++j) sum[j] = 0ull;
-      float na = __ldg(sa), nb0 = __ldg(sb), nb1 = GROUPS > 1 ? __ldg(sb + sb1) : 0.f;   // the next block's, requested a block ahead
+      float na = __ldg(sa), nb0 = __ldg(sb), nb1 = GROUPS > 1 ? __ldg(sb2) : 0.f;   // the next block's, requested a block ahead
       for (int kb = 0; kb < nk; ++kb) {
         const float s0 = na * nb0, s1 = na * nb1;
         na = nb0 = nb1 = 1.f;
         if (kb + 1 < nk_main) {
-          sa += p.ldsa;
-          sb += p.sb_k;
+          sa = at_bytes(sa, step_a);
+          sb = at_bytes(sb, step_b);
           na = __ldg(sa);
           nb0 = __ldg(sb);
-          if (GROUPS > 1) nb1 = __ldg(sb + sb1);
+          if (GROUPS > 1) nb1 = __ldg(sb2 = at_bytes(sb2, step_b));
         }
-        ok = warp_all(mbar_wait_spin(&tfull[set * BUFS + buf], buf_phase, p.status, AXB_TIMEOUT_TMEM_FULL));
+        ok = warp_all(mbar_wait(&tfull[set * BUFS + buf], buf_phase, p.status, AXB_TIMEOUT_TMEM_FULL));
         if (!ok) break;
         tc_fence_after();
 #pragma unroll
@@ -342,14 +346,14 @@ int fp8_sm_count() {
 
 template <bool PAIR, bool B_MN>
 int launch_fp8(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& a2, const CUtensorMap& b2, const CUtensorMap& c,
-               const Fp8GemmParams& p, cudaStream_t st) {
+               const Fp8GemmParams& p, bool pdl, cudaStream_t st) {
   constexpr int CTAS = PAIR ? 2 : 1, TILE = 128 * CTAS;
   auto kern = fp8_gemm_kernel<PAIR, B_MN>;
   static std::atomic<unsigned long long> allowed{0};
   if (const int rc = axb_allow_smem((const void*)kern, G_SMEM, allowed)) return rc;
   const long long tiles = (long long)((p.M + TILE - 1) / TILE) * ((p.N + TILE - 1) / TILE);
   const long long workers = tiles < fp8_sm_count() / CTAS ? tiles : fp8_sm_count() / CTAS;
-  AxbLaunch l(dim3((unsigned)(workers * CTAS)), G_THREADS, G_SMEM, st, PAIR ? 2 : 0, false);
+  AxbLaunch l(dim3((unsigned)(workers * CTAS)), G_THREADS, G_SMEM, st, PAIR ? 2 : 0, pdl);
   const cudaError_t e = cudaLaunchKernelEx(&l.cfg, kern, a, b, a2, b2, c, p);
   return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }
@@ -358,10 +362,11 @@ int launch_fp8(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& a2
 
 // See the head of this file. A: codes [M, K], rows of lda bytes; sa: fp32 [ceil(K / 128)][ldsa]; B: codes [N, K] (b_mn: [K, N]), rows of
 // ldb bytes; sb: fp32, the scale of columns n and block b at sb[(n / 128) * sb_n + b * sb_k]; C: bf16 [M, N]; A2 [M, K2] and B2 [N, K2]
-// (b_mn: [K2, N]) bf16, K2 = 0: none. Operands start on 16 bytes and have row strides of whole 16 bytes.
-extern "C" int axb_fp8_gemm(const void* A, long long lda, const float* sa, long long ldsa, const void* B, long long ldb, const float* sb,
-                            long long sb_n, long long sb_k, int b_mn, void* C, long long ldc, int M, int N, int K, const void* A2,
-                            long long lda2, const void* B2, long long ldb2, int K2, int tile, int* status, void* stream) {
+// (b_mn: [K2, N]) bf16, K2 = 0: none. Operands start on 16 bytes and have row strides of whole 16 bytes. pdl: the launch before this one
+// is the one that quantised A; this one's start overlaps its end.
+static int fp8_gemm_entry(const void* A, long long lda, const float* sa, long long ldsa, const void* B, long long ldb, const float* sb,
+                          long long sb_n, long long sb_k, int b_mn, void* C, long long ldc, int M, int N, int K, const void* A2,
+                            long long lda2, const void* B2, long long ldb2, int K2, int tile, bool pdl, int* status, void* stream) {
   if (M <= 0 || N <= 0) return 0;
   auto bad = [](const void* q, long long bytes) { return (reinterpret_cast<uintptr_t>(q) & 15) != 0 || (bytes & 15) != 0; };
   if (K <= 0 || bad(A, lda) || bad(B, ldb) || ldsa < M) return -2;
@@ -396,8 +401,14 @@ extern "C" int axb_fp8_gemm(const void* A, long long lda, const float* sa, long 
   const long long band = (20ll << 20) / ((pair ? 256ll : 128ll) * K);   // A rows of a band: about 20 MB of the L2
   p.group_m = (int)(band < 2 ? 2 : (band > 16 ? 16 : band));
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (pair) return b_mn ? launch_fp8<true, true>(tA, tB, tA2, tB2, tC, p, st) : launch_fp8<true, false>(tA, tB, tA2, tB2, tC, p, st);
-  return b_mn ? launch_fp8<false, true>(tA, tB, tA2, tB2, tC, p, st) : launch_fp8<false, false>(tA, tB, tA2, tB2, tC, p, st);
+  if (pair) return b_mn ? launch_fp8<true, true>(tA, tB, tA2, tB2, tC, p, pdl, st) : launch_fp8<true, false>(tA, tB, tA2, tB2, tC, p, pdl, st);
+  return b_mn ? launch_fp8<false, true>(tA, tB, tA2, tB2, tC, p, pdl, st) : launch_fp8<false, false>(tA, tB, tA2, tB2, tC, p, pdl, st);
+}
+
+extern "C" int axb_fp8_gemm(const void* A, long long lda, const float* sa, long long ldsa, const void* B, long long ldb, const float* sb,
+                            long long sb_n, long long sb_k, int b_mn, void* C, long long ldc, int M, int N, int K, const void* A2,
+                            long long lda2, const void* B2, long long ldb2, int K2, int tile, int* status, void* stream) {
+  return fp8_gemm_entry(A, lda, sa, ldsa, B, ldb, sb, sb_n, sb_k, b_mn, C, ldc, M, N, K, A2, lda2, B2, ldb2, K2, tile, false, status, stream);
 }
 
 // y = x8 W8^T (b_mn: x8 W8) (+ X2 B2) of bf16 rows x [T, K] in one call. q: where the 8-bit rows go, T rows of K rounded up to 16 bytes and
@@ -416,5 +427,5 @@ extern "C" int axb_fp8_linear(const void* x, long long ldx, void* q, const void*
   if (rc) return rc;
   if (!b_mn && tile == 0)
     return axb_fp8_skinny(x, ldx, q, ldq, s, W, ldw, sw, sw_n, sw_k, y, N, T, N, K, X2, ldx2, B2, ldb2, K2, status, stream);
-  return axb_fp8_gemm(q, ldq, s, T, W, ldw, sw, sw_n, sw_k, b_mn, y, N, T, N, K, X2, ldx2, B2, ldb2, K2, tile, status, stream);
+  return fp8_gemm_entry(q, ldq, s, T, W, ldw, sw, sw_n, sw_k, b_mn, y, N, T, N, K, X2, ldx2, B2, ldb2, K2, tile, true, status, stream);
 }

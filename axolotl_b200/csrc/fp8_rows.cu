@@ -89,6 +89,7 @@ __global__ void __launch_bounds__(Q_ROWS * 32)
   const int lane = threadIdx.x & 31;
   const long long row = (long long)blockIdx.x * Q_ROWS + (threadIdx.x >> 5);
   const int c0 = blockIdx.y * Q_COLS;
+  pdl_launch_dependents();                       // a product of these rows may set itself up meanwhile
   if (row >= rows) return;                       // whole warps
   const T* xr = x + row * ldx;
   Eight<T> v[4];

@@ -7,6 +7,7 @@
 // Every block of 128 columns starts an accumulator of its own; four warps (a thread owns a weight row) add it to sums in registers,
 // times the weight's scale and the token's. The rows come as codes (csrc/fp8_rows.cu), or (FUSED) in bf16: then four warps quantise them
 // into the operand tile while the weight's bulk copies arrive, and the codes and their scales never reach memory. ops/fp8.py says when.
+// On quantised rows it is a dependent launch of the kernel that quantised them.
 #include <cuda_fp8.h>
 
 #include "axb_common.cuh"
@@ -105,16 +106,33 @@ __global__ void __launch_bounds__(FS_T, 2)
   float* part = reinterpret_cast<float*>(smem);     // partial tile, [token][128], in the ring after the last product
 
   if (warp == 0) {
+    auto load_w = [&](int kb, int s) {
+      const bool ext = kb >= nk_main;
+      mbar_expect_tx(&full[s], FUSED ? FS_P : C::STAGE);
+      tma_load_2d(smem + s * C::STAGE, ext ? &tmB2 : &tmW, &full[s], ext ? (kb - nk_main) * 64 : kb * 128, tile * 128);
+    };
+    auto load_x = [&](int kb, int s) {
+      const bool ext = kb >= nk_main;
+      if (!FUSED) tma_load_2d(smem + s * C::STAGE + FS_P, ext ? &tmX2 : &tmX, &full[s], ext ? (kb - nk_main) * 64 : kb * 128, 0);
+    };
+    // the weight does not come from the launch before this one: its first tiles are requested while the rows are quantised
+    const int pre = min(C::STAGES, kb1 - kb0);
+    for (int i = 0; i < pre; ++i) {
+      if (elect_one()) load_w(kb0 + i, i);
+      __syncwarp();
+    }
+    pdl_wait();
+    for (int i = 0; i < pre; ++i) {
+      if (elect_one()) load_x(kb0 + i, i);
+      __syncwarp();
+    }
     int s = 0;
-    uint32_t phase = 0;
-    for (int kb = kb0; kb < kb1; ++kb) {
-      if (!warp_all(mbar_wait(&empty[s], phase ^ 1, p.status, AXB_TIMEOUT_EMPTY))) break;
+    uint32_t phase = 0;                   // stage s is refilled once its first contents have been used
+    for (int kb = kb0 + pre; kb < kb1; ++kb) {
+      if (!warp_all(mbar_wait(&empty[s], phase, p.status, AXB_TIMEOUT_EMPTY))) break;
       if (elect_one()) {
-        const bool ext = kb >= nk_main;
-        const int k0 = ext ? (kb - nk_main) * 64 : kb * 128;
-        mbar_expect_tx(&full[s], FUSED ? FS_P : C::STAGE);
-        tma_load_2d(smem + s * C::STAGE, ext ? &tmB2 : &tmW, &full[s], k0, tile * 128);
-        if (!FUSED) tma_load_2d(smem + s * C::STAGE + FS_P, ext ? &tmX2 : &tmX, &full[s], k0, 0);
+        load_w(kb, s);
+        load_x(kb, s);
       }
       __syncwarp();
       if (++s == C::STAGES) {
@@ -204,6 +222,7 @@ __global__ void __launch_bounds__(FS_T, 2)
     for (int j = 0; j < NT; ++j)
       if (j < p.T) part[j * 128 + (warp & 3) * 32 + lane] = sum[j];
   } else if (!FUSED) {
+    pdl_wait();
     // the rows' scales into the ring, a quarter of the tokens a warp, as far ahead as the ring goes. (Not by the operands' `empty`: nothing
     // keeps these warps within one phase of it.)
     const int t = (warp - 6) * (NT / 4) + lane;
@@ -306,6 +325,7 @@ __global__ void __launch_bounds__(FS_T, 2)
       }
     }
   }
+  pdl_wait();                             // nothing is written before the launch before this one has ended
   if (cs > 1) cluster_sync();
   else __syncthreads();
   const uint32_t pbase = smem_u32(part);
@@ -343,7 +363,7 @@ int launch_fp8_skinny(const CUtensorMap (&m)[4], const Fp8SkinnyParams& p, int t
   auto kern = fp8_skinny_kernel<NT, FUSED>;
   static std::atomic<unsigned long long> allowed{0};
   if (const int rc = axb_allow_smem((const void*)kern, FsCfg<NT>::SMEM, allowed)) return rc;
-  AxbLaunch l(dim3((unsigned)(tiles * splits)), FS_T, FsCfg<NT>::SMEM, st, splits, false);
+  AxbLaunch l(dim3((unsigned)(tiles * splits)), FS_T, FsCfg<NT>::SMEM, st, splits, !FUSED);
   const cudaError_t e = cudaLaunchKernelEx(&l.cfg, kern, m[0], m[1], m[2], m[3], p);
   return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }
