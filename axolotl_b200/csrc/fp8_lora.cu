@@ -29,8 +29,10 @@ struct AxbFp8Lora {
   const void* qx;          // backward: 8-bit rows of x
   float* t32;              // backward scratch: [T, R] fp32, [T, R] bf16
   void* t;
-  float* dA;               // fp32 [R, K], [N, R] (null: not wanted); added to where add_* is set, else written
+  float* dA;               // fp32 [R, K] (null: not wanted), [N, R]; added to where add_* is set, else written
   float* dB;
+  void* dA16;              // their bf16 copies (null: none; dA and dB are then scratch without gaps)
+  void* dB16;
   const int* blocks;       // diagonal blocks of B
   int* status;
   long long ldx, ldw, sw_n, sw_k, lda, ldb, ldda, lddb;
@@ -50,8 +52,9 @@ extern "C" int axb_fp8_lora_bwd(const AxbFp8Lora* l, void* stream) {
   if (l->T <= 0) return 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const long long n = (long long)l->T * l->R;
-  cudaError_t e = cudaMemsetAsync(l->t32, 0, n * sizeof(float), st);
-  if (e == cudaSuccess && !l->add_dB) e = cudaMemset2DAsync(l->dB, l->lddb * sizeof(float), 0, l->R * sizeof(float), l->N, st);
+  const bool joined = !l->add_dB && l->dB == l->t32 + n && l->lddb == l->R;     // one block of zeros
+  cudaError_t e = cudaMemsetAsync(l->t32, 0, (n + (joined ? (long long)l->N * l->R : 0)) * sizeof(float), st);
+  if (e == cudaSuccess && !joined && !l->add_dB) e = cudaMemset2DAsync(l->dB, l->lddb * sizeof(float), 0, l->R * sizeof(float), l->N, st);
   if (e != cudaSuccess) return (int)e;
   int rc = axb_lora_bwd_dy(l->x, l->ldx, l->B, l->ldb, l->xa, l->R, l->t32, l->dB, l->lddb, l->T, l->N, l->R, l->blocks, l->n_blocks,
                            l->status, stream);
@@ -63,6 +66,8 @@ extern "C" int axb_fp8_lora_bwd(const AxbFp8Lora* l, void* stream) {
     const long long ldq = (l->K + 15ll) & ~15ll;
     rc = axb_fp8_adapter_grad(l->qx, ldq, reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(l->qx) + ldq * l->T), l->T, l->t,
                               l->R, l->dA, l->ldda, l->T, l->K, l->R, l->add_dA, l->status, stream);
+    if (!rc && l->dA16) rc = axb_cast_f32_to_bf16(l->dA, l->dA16, (long long)l->R * l->K, 1.f, stream);
   }
+  if (!rc && l->dB16) rc = axb_cast_f32_to_bf16(l->dB, l->dB16, (long long)l->N * l->R, 1.f, stream);
   return rc;
 }

@@ -199,6 +199,7 @@ def stream_ptr() -> int:
 
 
 _status = {}
+_status_at = {}
 
 
 def status_word(device=None) -> torch.Tensor:
@@ -211,6 +212,14 @@ def status_word(device=None) -> torch.Tensor:
         t = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", key))
         _status[key] = t
     return t
+
+
+def launch_args(index: int):
+    """(address of the status word, current stream) of a device that is the current one: the tail of a kernel call's arguments."""
+    at = _status_at.get(index)
+    if at is None:
+        at = _status_at[index] = status_word(torch.device("cuda", index)).data_ptr()
+    return at, torch._C._cuda_getCurrentRawStream(index)
 
 
 _STATUS_NAMES = {

@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes as C
+import functools
 from dataclasses import dataclass
 
 import torch
@@ -26,12 +27,13 @@ from . import _lib
 
 BLOCK = 128
 E4M3_MAX = 448.0
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
 def _device_of(t):
     """Launches go to the current device: makes it the tensor's where it is another one."""
-    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return contextlib.nullcontext() if t.device.index == _current_device() else torch.cuda.device(t.device)
 
 
 def _blocks(n: int) -> int:
@@ -58,7 +60,8 @@ def _check_scale(scale, shape, device, what):
 
 def _rows16(codes):
     """``codes`` with rows of whole 16 bytes: as they are, or laid out again."""
-    if codes.stride(1) == 1 and codes.stride(0) % 16 == 0 and codes.stride(0) >= codes.shape[1] and codes.data_ptr() % 16 == 0:
+    ld, unit = codes.stride()
+    if unit == 1 and ld % 16 == 0 and ld >= codes.shape[1] and codes.data_ptr() % 16 == 0:
         return codes
     out = _padded(*codes.shape, codes.device)
     out.view(torch.uint8).copy_(codes.view(torch.uint8))
@@ -90,15 +93,16 @@ def _pack(x):
     ld = (K + 15) & ~15
     if not x.is_cuda:
         return _pack_plain(x, ld)
-    if x.device.index != torch.cuda.current_device():
-        with torch.cuda.device(x.device):
+    device = x.device
+    if device.index != _current_device():
+        with torch.cuda.device(device):
             return _pack(x)
     if x.stride(1) != 1 and K > 1:
         x = x.contiguous()
-    q = torch.empty(T * (ld + 4 * _blocks(K)), dtype=torch.uint8, device=x.device)
+    q = torch.empty(T * (ld + 4 * _blocks(K)), dtype=torch.uint8, device=device)
     at = q.data_ptr()
     _lib.check_rc(_lib.cuda_lib().axb_fp8_quantize_rows(x.data_ptr(), x.stride(0), _DTYPES[x.dtype], at, ld, at + T * ld, T, T, K,
-                                                        _lib.stream_ptr()), "fp8_quantize_rows")
+                                                        torch._C._cuda_getCurrentRawStream(device.index)), "fp8_quantize_rows")
     return q
 
 
@@ -115,14 +119,15 @@ def _unpack(q, T, K, dtype):
     """The values of a block of ``_pack``, [T, K]."""
     if not q.is_cuda:
         return dequantize_fp8_rows(*_unpacked(q, T, K), dtype)
-    if q.device.index != torch.cuda.current_device():
-        with torch.cuda.device(q.device):
+    device = q.device
+    if device.index != _current_device():
+        with torch.cuda.device(device):
             return _unpack(q, T, K, dtype)
     ld = (K + 15) & ~15
     at = q.data_ptr()
-    out = torch.empty((T, K), dtype=dtype, device=q.device)
+    out = torch.empty((T, K), dtype=dtype, device=device)
     _lib.check_rc(_lib.cuda_lib().axb_fp8_dequantize_rows(at, ld, at + T * ld, T, out.data_ptr(), K, _DTYPES[dtype], T, K,
-                                                          _lib.stream_ptr()), "fp8_dequantize_rows")
+                                                          torch._C._cuda_getCurrentRawStream(device.index)), "fp8_dequantize_rows")
     return out
 
 
@@ -268,38 +273,40 @@ def _few(T, N, K):
 
 
 def _product(x, codes, scale, trans=False, a2=None, b2=None, keep=False):
-    """(x8 W8^T or x8 W8 (+ a2 b2) in bf16, block of ``_pack`` of x or None) of bf16 rows x [T, K]. One call: with at most 64 rows whose
-    codes nobody keeps, one launch."""
+    """(x8 W8^T or x8 W8 (+ a2 b2) in bf16, block of ``_pack`` of x or None) of bf16 rows x [T, K]. One call, and
+    for a few tokens whose codes nobody keeps one launch."""
     if not x.is_cuda:
         q = _pack(x)
         y = fp8_gemm(*_unpacked(q, *x.shape), codes, scale, trans_w=trans, a2=a2, b2=b2)
         return y, q
-    if x.device.index != torch.cuda.current_device():
-        with torch.cuda.device(x.device):
+    device = x.device
+    if device.index != _current_device():
+        with torch.cuda.device(device):
             return _product(x, codes, scale, trans, a2, b2, keep)
     T, K = x.shape
     N = codes.shape[1] if trans else codes.shape[0]
-    if x.stride(1) != 1 and K > 1:
+    ldx, unit = x.stride()
+    if unit != 1 and K > 1:
         x = x.contiguous()
+        ldx = K
     codes = _rows16(codes)
     sn, sk = scale.stride()
     if trans:
         sn, sk = sk, sn
-    K2 = 0
+    ext = (None, 0, None, 0, 0)
     if a2 is not None:
         from .gemm import _row_major_2d
 
-        a2, b2, K2 = _row_major_2d(a2), _row_major_2d(b2), a2.shape[1]
-    y = torch.empty((T, N), dtype=torch.bfloat16, device=x.device)
+        a2, b2 = _row_major_2d(a2), _row_major_2d(b2)
+        ext = (a2.data_ptr(), a2.stride(0), b2.data_ptr(), b2.stride(0), a2.shape[1])
+    few = 0 if trans or ext[4] % 8 else _few(T, N, K)
+    y = torch.empty((T, N), dtype=torch.bfloat16, device=device)
     q = None
-    few = 0 if trans or K2 % 8 else _few(T, N, K)
     if keep or few < 2:
-        q = torch.empty(T * (((K + 15) & ~15) + 4 * _blocks(K)), dtype=torch.uint8, device=x.device)
+        q = torch.empty(T * (((K + 15) & ~15) + 4 * _blocks(K)), dtype=torch.uint8, device=device)
     _lib.check_rc(_lib.cuda_lib().axb_fp8_linear(
-        x.data_ptr(), x.stride(0), None if q is None else q.data_ptr(), codes.data_ptr(), codes.stride(0), scale.data_ptr(), sn, sk,
-        trans, y.data_ptr(), T, N, K, None if K2 == 0 else a2.data_ptr(), 0 if K2 == 0 else a2.stride(0),
-        None if K2 == 0 else b2.data_ptr(), 0 if K2 == 0 else b2.stride(0), K2, 0 if few else _tile(T, N),
-        _lib.status_word(x.device).data_ptr(), _lib.stream_ptr()), "fp8_linear")
+        x.data_ptr(), ldx, None if q is None else q.data_ptr(), codes.data_ptr(), codes.stride(0), scale.data_ptr(), sn, sk, trans,
+        y.data_ptr(), T, N, K, *ext, 0 if few else _tile(T, N), *_lib.launch_args(device.index)), "fp8_linear")
     return y, q
 
 
@@ -323,7 +330,8 @@ class _Fp8LinearFn(torch.autograd.Function):
 
 class _Lora(C.Structure):
     """AxbFp8Lora of csrc/fp8_lora.cu."""
-    _fields_ = ([(n, C.c_void_p) for n in ("x", "q", "W", "sw", "A", "B", "xa", "y", "qx", "t32", "t", "dA", "dB", "blocks", "status")]
+    _fields_ = ([(n, C.c_void_p) for n in ("x", "q", "W", "sw", "A", "B", "xa", "y", "qx", "t32", "t", "dA", "dB", "dA16", "dB16", "blocks",
+                                        "status")]
                 + [(n, C.c_longlong) for n in ("ldx", "ldw", "sw_n", "sw_k", "lda", "ldb", "ldda", "lddb")]
                 + [(n, C.c_int) for n in ("T", "N", "K", "R", "tile", "n_blocks", "add_dA", "add_dB")] + [("scaling", C.c_float)])
 
@@ -338,6 +346,11 @@ def _lora_args(x, codes, scale, A16, B16, scaling, T, N, K, R, tile):
     return l
 
 
+@functools.lru_cache(64)
+def _flat_blocks(blocks):
+    return (C.c_int * (4 * len(blocks)))(*[int(v) for b in blocks for v in b])
+
+
 def _operand16(t):
     return t.dtype == torch.bfloat16 and t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0
 
@@ -347,7 +360,7 @@ def _lora_forward(x, codes, scale, A16, B16, scaling, keep):
     T, K = x.shape
     R, N = A16.shape[0], codes.shape[0]
     if not (T and R <= 128 and R % 8 == 0 and _operand16(x) and _operand16(A16) and _operand16(B16)
-            and x.device.index == torch.cuda.current_device()):
+            and x.device.index == _current_device()):
         from .lora import skinny_gemm
 
         xa = skinny_gemm(x, A16, alpha=scaling)            # [T, R], of the bf16 input
@@ -390,21 +403,29 @@ class _Fp8LoRALinearFn(torch.autograd.Function):
             # one pass over dy for t and dB, the product and dA behind it: one call
             codes = _rows16(codes)
             l = _lora_args(dy, codes, scale, A16, B16, ctx.scaling, T, N, K, R, _tile(T, K))
-            n = T * R
-            work = torch.empty(6 * n + (T * (((N + 15) & ~15) + 4 * _blocks(N)) if need[0] else 0), dtype=torch.uint8, device=dy.device)
-            l.t32, l.t, l.xa = work.data_ptr(), work.data_ptr() + 4 * n, xa.data_ptr()
+            n, tA, tB = T * R, getattr(A, "_axb_grad", None), getattr(B, "_axb_grad", None)
+            # scratch: t in fp32, dB in fp32 (where its place is elsewhere it is not used), t in bf16, dA in fp32, the rows of dy in 8 bits
+            low = [w is None and p.dtype == torch.bfloat16 for w, p in ((tA, A), (tB, B))]
+            at = [4 * n, 4 * N * R if low[1] else 0, 2 * n, 4 * R * K if need[3] and low[0] else 0]
+            work = torch.empty(sum(at) + (T * (((N + 15) & ~15) + 4 * _blocks(N)) if need[0] else 0), dtype=torch.uint8, device=dy.device)
+            l.t32 = p = work.data_ptr()
+            l.t, l.xa = p + at[0] + at[1], xa.data_ptr()
             if need[0]:
                 dx = torch.empty((T, K), dtype=torch.bfloat16, device=dy.device)
-                l.q, l.y = work.data_ptr() + 6 * n, dx.data_ptr()
-            tB = getattr(B, "_axb_grad", None)
-            dB = tB if tB is not None else torch.empty((N, R), dtype=torch.float32, device=dy.device)
-            l.dB, l.lddb, l.add_dB = dB.data_ptr(), dB.stride(0), tB is not None
-            tA = None
-            if need[3]:
-                tA = getattr(A, "_axb_grad", None)
+                l.q, l.y = p + sum(at), dx.data_ptr()
+            if low[1]:
+                dB = torch.empty((N, R), dtype=torch.bfloat16, device=dy.device)
+                l.dB, l.dB16, l.lddb = p + at[0], dB.data_ptr(), R
+            else:
+                dB = tB if tB is not None else torch.empty((N, R), dtype=torch.float32, device=dy.device)
+                l.dB, l.lddb, l.add_dB = dB.data_ptr(), dB.stride(0), tB is not None
+            if need[3] and low[0]:
+                dA = torch.empty((R, K), dtype=torch.bfloat16, device=dy.device)
+                l.qx, l.dA, l.dA16, l.ldda = q.data_ptr(), p + sum(at[:3]), dA.data_ptr(), K
+            elif need[3]:
                 dA = tA if tA is not None else torch.empty((R, K), dtype=torch.float32, device=dy.device)
                 l.qx, l.dA, l.ldda, l.add_dA = q.data_ptr(), dA.data_ptr(), dA.stride(0), tA is not None
-            flat = (C.c_int * (4 * len(ctx.blocks)))(*[int(v) for b in ctx.blocks for v in b])
+            flat = _flat_blocks(ctx.blocks)
             l.blocks, l.n_blocks = C.addressof(flat), len(ctx.blocks)
             _lib.check_rc(_lib.cuda_lib().axb_fp8_lora_bwd(C.byref(l), _lib.stream_ptr()), "fp8_lora_bwd")
             dA = None if dA is None or tA is not None else dA.to(A.dtype)
@@ -489,8 +510,10 @@ def fp8_linear(x, codes, scale, bias=None):
     _check_linear(x, codes, scale, "fp8_linear")
     if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
         return _shaped(_Fp8LinearFn.apply(_rows_of(x), codes, scale, bias), x)
-    y, _ = _product(_rows_of(x), codes, scale)
-    return _shaped(y if bias is None else y + bias, x)
+    y = _product(x if x.dim() == 2 else _rows_of(x), codes, scale)[0]
+    if bias is not None:
+        y = y + bias
+    return y if x.dim() == 2 and y.dtype == x.dtype else _shaped(y, x)
 
 
 def fp8_lora_linear(x, codes, scale, A, B, A16, B16, scaling, blocks, bias=None):

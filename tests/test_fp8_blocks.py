@@ -296,7 +296,8 @@ def test_linear_gradient_by_differences(dev):
 @pytest.mark.gpu
 @pytest.mark.parametrize("T,K,N,blocks", [(1, 256, 128, ((0, 128, 0, 8),)), (70, 520, 264, ((0, 200, 0, 8), (200, 64, 8, 8))),
                                           (600, 1024, 640, ((0, 640, 0, 16),)), (700, 264, 1032, ((128, 904, 0, 32),))])
-def test_lora_linear_and_its_gradients(T, K, N, blocks):
+@pytest.mark.parametrize("masters", [torch.float32, torch.bfloat16])
+def test_lora_linear_and_its_gradients(T, K, N, blocks, masters):
     R = sum(b[3] for b in blocks)
     x, dy = _make((T, K), 1, spread=0.5), _make((T, N), 2, spread=0.5) * 1e-2
     dy[: T // 3] = 0
@@ -306,7 +307,7 @@ def test_lora_linear_and_its_gradients(T, K, N, blocks):
     for r0, rows, c0, r in blocks:
         B[r0:r0 + rows, c0:c0 + r] = _make((rows, r), 5, torch.float32, 0.0) * 0.1
     A16, B16 = A.bfloat16(), B.bfloat16()
-    xl, Al, Bl = x.cuda().requires_grad_(True), A.cuda().requires_grad_(True), B.cuda().requires_grad_(True)
+    xl, Al, Bl = x.cuda().requires_grad_(True), A.to(masters).cuda().requires_grad_(True), B.to(masters).cuda().requires_grad_(True)
     y = fp8_lora_linear(xl, w, ws, Al, Bl, A16.cuda(), B16.cuda(), 2.0, blocks)
     dx, dA, dB = torch.autograd.grad(y, [xl, Al, Bl], dy.cuda())
     a, b, w8, x64, dy64 = A16.double(), B16.double(), _weight8(w, ws), x.double(), dy.double()
@@ -327,8 +328,10 @@ def test_lora_linear_and_its_gradients(T, K, N, blocks):
     want = dy8 @ w8 + tall @ a
     size = dy8.abs() @ w8.abs() + tall.abs() @ a.abs()
     near(dx, want, BF16 * want.abs() + (tall_e @ a.abs() + (N + R + 40) * EPS32 * size) * (1 + BF16), 4)
-    near(dA, tall.t() @ x8, tall_e.t() @ x8.abs() + (T + 8) * EPS32 * tall.abs().t() @ x8.abs(), 4)
-    wantB, offB = dy64.t() @ low, dy64.abs().t() @ low_e + (T + 8) * EPS32 * dy64.abs().t() @ low.abs()
+    assert dA.dtype == dB.dtype == masters
+    half = BF16 if masters == torch.bfloat16 else 0.0       # and the gradients' own rounding
+    near(dA, tall.t() @ x8, half * (1 + BF16) * (tall.t() @ x8).abs() + (1 + half) * tall_e.t() @ x8.abs() + (T + 8) * EPS32 * tall.abs().t() @ x8.abs(), 4)
+    wantB, offB = dy64.t() @ low, half * (1 + BF16) * (dy64.t() @ low).abs() + (1 + half) * dy64.abs().t() @ low_e + (T + 8) * EPS32 * dy64.abs().t() @ low.abs()
     for r0, rows, c0, r in blocks:
         near(dB[r0:r0 + rows, c0:c0 + r], wantB[r0:r0 + rows, c0:c0 + r], offB[r0:r0 + rows, c0:c0 + r], 4)
     assert (dB.cpu()[B == 0] == 0).all() or len(blocks) == 1
