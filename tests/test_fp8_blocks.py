@@ -208,7 +208,7 @@ def test_product_tiles_and_extension(tile, trans, rank, monkeypatch):
     """Both tile sizes whatever the rule picks, with and without the bf16 K-extension, more tiles than workers."""
     from axolotl_b200.ops import fp8
 
-    monkeypatch.setattr(fp8, "_tile", lambda M, N, *a: tile)
+    monkeypatch.setattr(fp8, "_tile", lambda *a: tile)
     for M, N, K in ((130, 264, 200), (2100, 2600, 256)):
         x = _make((M, K), M, spread=1.0).cuda()
         codes, scale = quantize_fp8_rows(x)
