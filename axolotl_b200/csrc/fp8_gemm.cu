@@ -16,7 +16,7 @@
 
 extern "C" int axb_fp8_quantize_rows(const void* x, long long ldx, int dtype, void* q, long long ldq, float* s, long long lds,
                                      long long rows, int K, void* stream);
-extern "C" int axb_fp8_skinny(const void* x, long long ldx, const void* q, long long ldq, const float* sx, const void* W, long long ldw,
+extern "C" int axb_fp8_skinny(const void* x, long long ldx, const void* q, long long ldq, const float* sx, long long ldsx, const void* W, long long ldw,
                               const float* sw, long long sw_n, long long sw_k, void* y, long long ldy, int T, int N, int K, const void* X2,
                               long long ldx2, const void* B2, long long ldb2, int K2, int* status, void* stream);
 
@@ -412,20 +412,20 @@ extern "C" int axb_fp8_gemm(const void* A, long long lda, const float* sa, long 
 }
 
 // y = x8 W8^T (b_mn: x8 W8) (+ X2 B2) of bf16 rows x [T, K] in one call. q: where the 8-bit rows go, T rows of K rounded up to 16 bytes and
-// behind them the scales, fp32 [ceil(K / 128)][T]; null: they are not kept (at most 64 rows, forward). The other arguments are those of
+// behind them the scales, fp32 [ceil(K / 128)][T rounded up to 4]; null: they are not kept (at most 64 rows, forward). The other arguments are those of
 // axb_fp8_gemm.
 extern "C" int axb_fp8_linear(const void* x, long long ldx, void* q, const void* W, long long ldw, const float* sw, long long sw_n,
                               long long sw_k, int b_mn, void* y, int T, int N, int K, const void* X2, long long ldx2, const void* B2,
                               long long ldb2, int K2, int tile, int* status, void* stream) {
   if (!q) {
     if (b_mn) return -2;
-    return axb_fp8_skinny(x, ldx, nullptr, 0, nullptr, W, ldw, sw, sw_n, sw_k, y, N, T, N, K, X2, ldx2, B2, ldb2, K2, status, stream);
+    return axb_fp8_skinny(x, ldx, nullptr, 0, nullptr, 0, W, ldw, sw, sw_n, sw_k, y, N, T, N, K, X2, ldx2, B2, ldb2, K2, status, stream);
   }
-  const long long ldq = (K + 15ll) & ~15ll;
+  const long long ldq = (K + 15ll) & ~15ll, lds = (T + 3ll) & ~3ll;
   float* s = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(q) + ldq * T);
-  int rc = axb_fp8_quantize_rows(x, ldx, 0, q, ldq, s, T, T, K, stream);
+  int rc = axb_fp8_quantize_rows(x, ldx, 0, q, ldq, s, lds, T, K, stream);
   if (rc) return rc;
   if (!b_mn && tile == 0)
-    return axb_fp8_skinny(x, ldx, q, ldq, s, W, ldw, sw, sw_n, sw_k, y, N, T, N, K, X2, ldx2, B2, ldb2, K2, status, stream);
-  return fp8_gemm_entry(q, ldq, s, T, W, ldw, sw, sw_n, sw_k, b_mn, y, N, T, N, K, X2, ldx2, B2, ldb2, K2, tile, true, status, stream);
+    return axb_fp8_skinny(x, ldx, q, ldq, s, lds, W, ldw, sw, sw_n, sw_k, y, N, T, N, K, X2, ldx2, B2, ldb2, K2, status, stream);
+  return fp8_gemm_entry(q, ldq, s, lds, W, ldw, sw, sw_n, sw_k, b_mn, y, N, T, N, K, X2, ldx2, B2, ldb2, K2, tile, true, status, stream);
 }

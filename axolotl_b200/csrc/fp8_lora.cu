@@ -63,8 +63,8 @@ extern "C" int axb_fp8_lora_bwd(const AxbFp8Lora* l, void* stream) {
     rc = axb_fp8_linear(l->x, l->ldx, l->q, l->W, l->ldw, l->sw, l->sw_k, l->sw_n, 1, l->y, l->T, l->K, l->N, l->t, l->R, l->A, l->lda, l->R,
                         l->tile, l->status, stream);
   if (!rc && l->dA) {
-    const long long ldq = (l->K + 15ll) & ~15ll;
-    rc = axb_fp8_adapter_grad(l->qx, ldq, reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(l->qx) + ldq * l->T), l->T, l->t,
+    const long long ldq = (l->K + 15ll) & ~15ll, lds = (l->T + 3ll) & ~3ll;      // the layout of axb_fp8_linear
+    rc = axb_fp8_adapter_grad(l->qx, ldq, reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(l->qx) + ldq * l->T), lds, l->t,
                               l->R, l->dA, l->ldda, l->T, l->K, l->R, l->add_dA, l->status, stream);
     if (!rc && l->dA16) rc = axb_cast_f32_to_bf16(l->dA, l->dA16, (long long)l->R * l->K, 1.f, stream);
   }

@@ -21,10 +21,10 @@ constexpr int FS_RING = 16;               // blocks whose row scales are held (s
 struct Fp8SkinnyParams {
   const __nv_bfloat16* x;
   const __nv_bfloat16* x2;                // bf16 extension of the tokens
-  const float* sx;                        // scales of quantised rows [block][T] (FUSED: not there)
+  const float* sx;                        // scales of quantised rows [block][ldsx] (FUSED: not there)
   const float* sw;
   __nv_bfloat16* y;
-  long long ldx, ldx2, sw_n, sw_k, ldy;
+  long long ldx, ldx2, ldsx, sw_n, sw_k, ldy;
   int T, N, K, K2, vec;                   // vec: rows of x start on 16 bytes
   int* status;
 };
@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(FS_T, 2)
     // keeps these warps within one phase of it.)
     const int t = (warp - 6) * (NT / 4) + lane;
     const bool mine = lane < NT / 4;
-    auto fetch = [&](int kb) { return mine && kb < nk_main && t < p.T ? __ldg(p.sx + (long long)kb * p.T + t) : 1.f; };
+    auto fetch = [&](int kb) { return mine && kb < nk_main && t < p.T ? __ldg(p.sx + kb * p.ldsx + t) : 1.f; };
     float next = fetch(kb0);
     for (int kb = kb0; kb < kb1; ++kb) {
       const int i = kb - kb0, slot = i % FS_RING;
@@ -380,9 +380,9 @@ int fp8_skinny_splits(int tiles, int nk) {
 }  // namespace
 
 // See the head of this file. x: bf16 [T, K], T <= 64; q (null: the rows are quantised by the kernel): their codes, rows of ldq bytes, and
-// sx: their scales [ceil(K / 128)][T]; W: codes [N, K], rows of ldw bytes, and their scales sw[(n / 128) * sw_n + b * sw_k]; y: bf16
+// sx: their scales [ceil(K / 128)][ldsx]; W: codes [N, K], rows of ldw bytes, and their scales sw[(n / 128) * sw_n + b * sw_k]; y: bf16
 // [T, N]; X2 [T, K2] and B2 [N, K2] bf16, K2 = 0: none. q, W, X2 and B2 start on 16 bytes and have row strides of whole 16 bytes.
-extern "C" int axb_fp8_skinny(const void* x, long long ldx, const void* q, long long ldq, const float* sx, const void* W, long long ldw,
+extern "C" int axb_fp8_skinny(const void* x, long long ldx, const void* q, long long ldq, const float* sx, long long ldsx, const void* W, long long ldw,
                               const float* sw, long long sw_n, long long sw_k, void* y, long long ldy, int T, int N, int K, const void* X2,
                               long long ldx2, const void* B2, long long ldb2, int K2, int* status, void* stream) {
   if (T <= 0 || N <= 0) return 0;
@@ -405,6 +405,7 @@ extern "C" int axb_fp8_skinny(const void* x, long long ldx, const void* q, long 
   p.y = (__nv_bfloat16*)y;
   p.ldx = ldx;
   p.ldx2 = ldx2;
+  p.ldsx = ldsx;
   p.sw_n = sw_n;
   p.sw_k = sw_k;
   p.ldy = ldy;

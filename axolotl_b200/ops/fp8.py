@@ -86,33 +86,42 @@ def quantize_fp8_rows(x: torch.Tensor):
     return _unpacked(_pack(x.detach()), *x.shape)
 
 
+def _lead(T, K):
+    """Row lengths of a block of ``_pack``: codes in bytes, scales in numbers."""
+    return (K + 15) & ~15, (T + 3) & ~3
+
+
+def _packed_size(T, K):
+    return T * ((K + 15) & ~15) + 4 * _blocks(K) * ((T + 3) & ~3)
+
+
 def _pack(x):
     """The 8-bit rows of x [T, K] as one block of bytes: T rows of codes, K rounded up to 16 bytes, and behind them the scales, fp32
-    [ceil(K / 128)][T]. What the layers and the checkpoint store keep."""
+    [ceil(K / 128)][T rounded up to 4]. What the layers and the checkpoint store keep."""
     T, K = x.shape
-    ld = (K + 15) & ~15
+    ld, lds = _lead(T, K)
     if not x.is_cuda:
-        return _pack_plain(x, ld)
+        return _pack_plain(x, ld, lds)
     device = x.device
     if device.index != _current_device():
         with torch.cuda.device(device):
             return _pack(x)
     if x.stride(1) != 1 and K > 1:
         x = x.contiguous()
-    q = torch.empty(T * (ld + 4 * _blocks(K)), dtype=torch.uint8, device=device)
+    q = torch.empty(_packed_size(T, K), dtype=torch.uint8, device=device)
     at = q.data_ptr()
-    _lib.check_rc(_lib.cuda_lib().axb_fp8_quantize_rows(x.data_ptr(), x.stride(0), _DTYPES[x.dtype], at, ld, at + T * ld, T, T, K,
+    _lib.check_rc(_lib.cuda_lib().axb_fp8_quantize_rows(x.data_ptr(), x.stride(0), _DTYPES[x.dtype], at, ld, at + T * ld, lds, T, K,
                                                         torch._C._cuda_getCurrentRawStream(device.index)), "fp8_quantize_rows")
     return q
 
 
 def _unpacked(q, T, K):
     """(codes [T, K], scales [ceil(K / 128), T]): views of a block of ``_pack``."""
-    ld = (K + 15) & ~15
+    ld, lds = _lead(T, K)
     if T == 0:
         return q.new_empty((0, K)).view(torch.float8_e4m3fn), torch.empty((_blocks(K), 0), device=q.device)
     codes = q[:T * ld].view(T, ld).view(torch.float8_e4m3fn)
-    return (codes if ld == K else codes[:, :K]), q[T * ld:].view(torch.float32).view(_blocks(K), T)
+    return (codes if ld == K else codes[:, :K]), q[T * ld:].view(torch.float32).view(_blocks(K), lds)[:, :T]
 
 
 def _unpack(q, T, K, dtype):
@@ -123,15 +132,15 @@ def _unpack(q, T, K, dtype):
     if device.index != _current_device():
         with torch.cuda.device(device):
             return _unpack(q, T, K, dtype)
-    ld = (K + 15) & ~15
+    ld, lds = _lead(T, K)
     at = q.data_ptr()
     out = torch.empty((T, K), dtype=dtype, device=device)
-    _lib.check_rc(_lib.cuda_lib().axb_fp8_dequantize_rows(at, ld, at + T * ld, T, out.data_ptr(), K, _DTYPES[dtype], T, K,
+    _lib.check_rc(_lib.cuda_lib().axb_fp8_dequantize_rows(at, ld, at + T * ld, lds, out.data_ptr(), K, _DTYPES[dtype], T, K,
                                                           torch._C._cuda_getCurrentRawStream(device.index)), "fp8_dequantize_rows")
     return out
 
 
-def _pack_plain(x, ld):
+def _pack_plain(x, ld, lds):
     T, K = x.shape
     kb = _blocks(K)
     v = torch.nn.functional.pad(x.float(), (0, kb * BLOCK - K)).view(T, kb, BLOCK)
@@ -142,7 +151,8 @@ def _pack_plain(x, ld):
     scale = torch.where(top > 0, torch.ldexp(torch.ones_like(top), e), torch.ones_like(top))
     v = v.clamp(-240 * 2.0 ** 120, 240 * 2.0 ** 120)
     codes = (v / scale[..., None]).to(torch.float8_e4m3fn).view(T, kb * BLOCK)[:, :ld]
-    return torch.cat([codes.reshape(-1).view(torch.uint8), scale.t().reshape(-1).view(torch.uint8)])
+    scale = torch.nn.functional.pad(scale.t(), (0, lds - T))
+    return torch.cat([codes.reshape(-1).view(torch.uint8), scale.reshape(-1).view(torch.uint8)])
 
 
 def dequantize_fp8_rows(codes: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = torch.bfloat16):
@@ -307,7 +317,7 @@ def _product(x, codes, scale, trans=False, a2=None, b2=None, keep=False):
     y = torch.empty((T, N), dtype=torch.bfloat16, device=device)
     q = None
     if keep or few < 2:
-        q = torch.empty(T * (((K + 15) & ~15) + 4 * _blocks(K)), dtype=torch.uint8, device=device)
+        q = torch.empty(_packed_size(T, K), dtype=torch.uint8, device=device)
     _lib.check_rc(_lib.cuda_lib().axb_fp8_linear(
         x.data_ptr(), ldx, None if q is None else q.data_ptr(), codes.data_ptr(), codes.stride(0), scale.data_ptr(), sn, sk, trans,
         y.data_ptr(), T, N, K, *ext, 0 if few else _tile(T, N, K), *_lib.launch_args(device.index)), "fp8_linear")
@@ -377,7 +387,7 @@ def _lora_forward(x, codes, scale, A16, B16, scaling, keep):
     xa = torch.empty((T, R), dtype=torch.bfloat16, device=x.device)
     l.y, l.xa, q = y.data_ptr(), xa.data_ptr(), None
     if keep or few < 2:
-        q = torch.empty(T * (((K + 15) & ~15) + 4 * _blocks(K)), dtype=torch.uint8, device=x.device)
+        q = torch.empty(_packed_size(T, K), dtype=torch.uint8, device=x.device)
         l.q = q.data_ptr()
     _lib.check_rc(_lib.cuda_lib().axb_fp8_lora_fwd(C.byref(l), _lib.stream_ptr()), "fp8_lora_fwd")
     return y, xa, q
@@ -411,7 +421,7 @@ class _Fp8LoRALinearFn(torch.autograd.Function):
             # scratch: t in fp32, dB in fp32 (where its place is elsewhere it is not used), t in bf16, dA in fp32, the rows of dy in 8 bits
             low = [w is None and p.dtype == torch.bfloat16 for w, p in ((tA, A), (tB, B))]
             at = [4 * n, 4 * N * R if low[1] else 0, 2 * n, 4 * R * K if need[3] and low[0] else 0]
-            work = torch.empty(sum(at) + (T * (((N + 15) & ~15) + 4 * _blocks(N)) if need[0] else 0), dtype=torch.uint8, device=dy.device)
+            work = torch.empty(sum(at) + (_packed_size(T, N) if need[0] else 0), dtype=torch.uint8, device=dy.device)
             l.t32 = p = work.data_ptr()
             l.t, l.xa = p + at[0] + at[1], xa.data_ptr()
             if need[0]:
@@ -439,8 +449,8 @@ class _Fp8LoRALinearFn(torch.autograd.Function):
         dx = _product(dy, codes, scale, trans=True, a2=t, b2=A16)[0] if need[0] else None
         if need[3]:
             tgt = getattr(A, "_axb_grad", None)
-            ld, at = (K + 15) & ~15, q.data_ptr()
-            buf = _adapter_grad(t, at, ld, at + T * ld, T, K, tgt)
+            (ld, lds), at = _lead(T, K), q.data_ptr()
+            buf = _adapter_grad(t, at, ld, at + T * ld, lds, K, tgt)
             dA = None if tgt is not None else buf.to(A.dtype)
         _, dB = _adapter_grads(None, B if need[4] else None, t, codes, dy, xa, ctx.blocks, dB_done, dB_fused)
         return dx, None, None, dA, dB, None, None, None, None, dbias
@@ -465,6 +475,9 @@ def fp8_adapter_grad(t, codes, row_scale, out=None):
     with _device_of(codes):
         codes = _rows16(codes)
         row_scale, lds = _row_scales(row_scale, T)
+        if lds % 4 or row_scale.data_ptr() % 16:            # read by bulk copies
+            row_scale = torch.nn.functional.pad(row_scale, (0, -T % 4))
+            lds = row_scale.shape[1]
         return _adapter_grad(t, codes.data_ptr(), codes.stride(0), row_scale.data_ptr(), lds, K, out)
 
 
