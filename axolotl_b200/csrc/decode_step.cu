@@ -21,15 +21,22 @@ extern "C" int axb_cache_attend(const void* qkv, long long ld, int q_col0, int k
 extern "C" int axb_rope_qk(void* qkv, const int* pos, const float* inv_freq, int T, int Hq, int Hk, int D, long long row_stride,
                            float sign, float attn_scale, const void* qn_w, const void* kn_w, float* rstd_out, float eps,
                            void* stream);
+extern "C" int axb_fp8_linear(const void* x, long long ldx, void* q, const void* W, long long ldw, const float* sw, long long sw_n,
+                              long long sw_k, int b_mn, void* y, int T, int N, int K, const void* X2, long long ldx2, const void* B2,
+                              long long ldb2, int K2, int tile, int* status, void* stream);
 extern "C" int axb_glu_fwd(const void* gu, void* h, long long T, int I, int kind, float limit, void* stream);
 
-// A projection y = x W^T (+ bias) (+ s (x A^T) B^T); A [rank, K], B [N, rank] row-major bf16, rank 0: no adapter.
+// A projection y = x W^T (+ bias) (+ s (x A^T) B^T); A [rank, K], B [N, rank] row-major bf16, rank 0: no adapter. fp8: W holds E4M3 codes,
+// rows of ldw bytes, with scales w8[n / 128 * w8_n + k / 128 * w8_k] and no bias; 1: its rows are quantised inside the product, 2: before
+// it, into the layer's q (`tile` as axb_fp8_linear takes it).
 struct AxbDecodeProj {
   const void* W;
   const void* bias;
   const void* A;
   const void* B;
-  int N, K, rank;
+  const float* w8;
+  long long ldw, w8_n, w8_k;
+  int N, K, rank, fp8, tile;
   float scaling;
 };
 
@@ -51,6 +58,7 @@ struct AxbDecodeLayer {
   void* gu;                // scratch [B, 2 I] (only where the activation is not fused)
   void* act;               // scratch [B, I]
   void* low;               // scratch [B, max rank]
+  void* q;                 // scratch of a projection with fp8 = 2
   void* k_cache;
   void* v_cache;
   const long long* seq;
@@ -66,13 +74,16 @@ struct AxbDecodeLayer {
 namespace {
 
 // y = x W^T with an optional adapter; glu: y = act(gate) * up
-int project(const AxbDecodeProj& p, const void* x, void* y, int B, void* low, bool glu, int kind, float limit, int* status,
+int project(const AxbDecodeProj& p, const void* x, void* y, int B, void* low, void* q, bool glu, int kind, float limit, int* status,
             void* stream) {
   if (p.rank > 0) {
     const int rc = axb_gemm_skinny(p.A, p.K, x, p.K, low, p.rank, p.rank, B, p.K, nullptr, 0, nullptr, 0, 0, p.scaling, nullptr, 0,
                                    0, 0, 0.f, 0, 0, 1, status, stream);
     if (rc) return rc;
   }
+  if (p.fp8)
+    return axb_fp8_linear(x, p.K, p.fp8 == 2 ? q : nullptr, p.W, p.ldw, p.w8, p.w8_n, p.w8_k, 0, y, B, p.N, p.K, low, p.rank, p.B, p.rank,
+                          p.rank, p.tile, status, stream);
   const int R = glu ? p.N / 2 : p.N;
   return axb_gemm_skinny(p.W, p.K, x, p.K, y, R, R, B, p.K, p.rank > 0 ? p.B : nullptr, p.rank, p.rank > 0 ? low : nullptr, p.rank,
                          p.rank, 1.f, p.bias, glu ? 2 : 0, 0, kind, limit, 0, 0, 1, status, stream);
@@ -87,7 +98,7 @@ extern "C" int axb_decode_layer(const AxbDecodeLayer* l, void* stream) {
                       : axb_rmsnorm_fwd(l->x, l->res_in, l->norm1, l->xn, l->res_in ? l->res_mid : nullptr, nullptr, B, H,
                                         l->eps1, l->off1, stream);
   const void* mid = l->res_in ? l->res_mid : l->x;
-  if (!rc) rc = project(l->qkv, l->xn, l->qkv_buf, B, l->low, false, 0, 0.f, l->status, stream);
+  if (!rc) rc = project(l->qkv, l->xn, l->qkv_buf, B, l->low, l->q, false, 0, 0.f, l->status, stream);
   const int nq = l->Hq * l->D, nk = l->Hk * l->D, W = nq + 2 * nk;
   const bool qk_norm = l->q_norm != nullptr || l->k_norm != nullptr;
   if (!rc && qk_norm)
@@ -97,12 +108,12 @@ extern "C" int axb_decode_layer(const AxbDecodeLayer* l, void* stream) {
     rc = axb_cache_attend(l->qkv_buf, W, 0, nq, nq + nk, l->k_cache, l->v_cache, l->rows, l->seq, l->lens, l->pos,
                           qk_norm ? nullptr : l->inv_freq, l->attn_scale, l->att, nq, B, l->Hq, l->Hk, l->D, l->max_len, l->scale,
                           l->window, 1, 0, qk_norm ? 0 : 1, l->status, stream);
-  if (!rc) rc = project(l->o, l->att, l->y, B, l->low, false, 0, 0.f, l->status, stream);
+  if (!rc) rc = project(l->o, l->att, l->y, B, l->low, l->q, false, 0, 0.f, l->status, stream);
   if (!rc) rc = axb_rmsnorm_fwd_pdl(l->y, mid, l->norm2, l->xn, l->res_out, B, H, l->eps2, l->off2, stream);
   const int I = l->gate_up.N / 2;
-  const bool fused = I % 64 == 0 && (l->glu_kind == 0 || l->glu_kind == 1) && !l->gate_up.bias;
-  if (!rc) rc = project(l->gate_up, l->xn, fused ? l->act : l->gu, B, l->low, fused, l->glu_kind, l->glu_limit, l->status, stream);
+  const bool fused = I % 64 == 0 && (l->glu_kind == 0 || l->glu_kind == 1) && !l->gate_up.bias && !l->gate_up.fp8;
+  if (!rc) rc = project(l->gate_up, l->xn, fused ? l->act : l->gu, B, l->low, l->q, fused, l->glu_kind, l->glu_limit, l->status, stream);
   if (!rc && !fused) rc = axb_glu_fwd(l->gu, l->act, B, I, l->glu_kind, l->glu_limit, stream);
-  if (!rc) rc = project(l->down, l->act, l->y, B, l->low, false, 0, 0.f, l->status, stream);
+  if (!rc) rc = project(l->down, l->act, l->y, B, l->low, l->q, false, 0, 0.f, l->status, stream);
   return rc;
 }

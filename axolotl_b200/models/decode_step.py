@@ -12,7 +12,7 @@ import ctypes as C
 import torch
 from torch.nn.modules import module as _nn
 
-from ..ops import _lib
+from ..ops import _lib, fp8
 from ..ops.functional import _ACT_KIND
 from .layers import FusedLinear, RMSNorm, adapters_enabled
 
@@ -20,13 +20,14 @@ _vp, _i32, _i64, _f32 = C.c_void_p, C.c_int, C.c_longlong, C.c_float
 
 
 class _Proj(C.Structure):
-    _fields_ = [("W", _vp), ("bias", _vp), ("A", _vp), ("B", _vp), ("N", _i32), ("K", _i32), ("rank", _i32), ("scaling", _f32)]
+    _fields_ = ([(n, _vp) for n in ("W", "bias", "A", "B", "w8")] + [(n, _i64) for n in ("ldw", "w8_n", "w8_k")]
+                + [(n, _i32) for n in ("N", "K", "rank", "fp8", "tile")] + [("scaling", _f32)])
 
 
 class _Layer(C.Structure):
     _fields_ = ([(n, _Proj) for n in ("qkv", "o", "gate_up", "down")]
                 + [(n, _vp) for n in ("norm1", "norm2", "q_norm", "k_norm", "x", "res_in", "res_mid", "res_out", "y", "xn", "qkv_buf",
-                                      "att", "gu", "act", "low", "k_cache", "v_cache", "seq", "lens", "pos", "inv_freq")]
+                                      "att", "gu", "act", "low", "q", "k_cache", "v_cache", "seq", "lens", "pos", "inv_freq")]
                 + [(n, _i64) for n in ("max_len", "rows")]
                 + [(n, _i32) for n in ("B", "Hq", "Hk", "D", "window", "glu_kind", "chained", "pad")]
                 + [(n, _f32) for n in ("eps1", "off1", "eps2", "off2", "attn_scale", "scale", "norm_eps", "glu_limit")]
@@ -48,19 +49,37 @@ def _dense16(t):
     return t.dtype == torch.bfloat16 and t.is_cuda and t.is_contiguous() and t.data_ptr() % 16 == 0
 
 
-def _proj(p, m, adapters):
-    """Fills ``p`` from a projection; False where it is not a dense one with at most a plain LoRA adapter."""
+def _coded(p, w, st, rows):
+    """Fills ``p`` from a weight in 8-bit blocks; False where its layout is another."""
+    N, K = w.shape
+    ld, unit = w.stride()
+    if not w.is_cuda or unit != 1 or ld % 16 or w.data_ptr() % 16 or N % 8 or K % 8 or st.scale.device != w.device:
+        return False
+    few = fp8._few(rows, N, K)
+    p.W, p.bias, p.N, p.K, p.rank = w.data_ptr(), None, N, K, 0
+    p.w8, p.ldw, p.fp8, p.tile = st.scale.data_ptr(), ld, 1 if few == 2 else 2, 0 if few else fp8._tile(rows, N, K)
+    p.w8_n, p.w8_k = st.scale.stride()
+    return True
+
+
+def _proj(p, m, adapters, rows):
+    """Fills ``p`` from a projection; False where it is not a dense one, or one in 8-bit blocks, with at most a plain LoRA adapter."""
     d = m.__dict__
     if not _bare(m, FusedLinear) or m.dora_magnitude is not None or m.mora_M is not None or d["qat"] is not None:
         return False
     w, bias, A = m._parameters["weight"], m.bias, m.lora_A
     extra = w.__dict__
-    if "_axb_quant" in extra or "_axb_shard" in extra or w.dim() != 2 or not _dense16(w):
+    st = extra.get("_axb_quant")
+    if "_axb_shard" in extra or w.dim() != 2 or (not _dense16(w) if st is None else not isinstance(st, fp8.Fp8State) or bias is not None):
         return False
     N, K = w.shape
-    if N % 8 or K % 8 or (bias is not None and not _dense16(bias)):
-        return False
-    p.W, p.bias, p.N, p.K, p.rank = w.data_ptr(), None if bias is None else bias.data_ptr(), N, K, 0
+    if st is not None:
+        if not _coded(p, w, st, rows):
+            return False
+    else:
+        if N % 8 or K % 8 or (bias is not None and not _dense16(bias)):
+            return False
+        p.W, p.bias, p.N, p.K, p.rank, p.fp8 = w.data_ptr(), None if bias is None else bias.data_ptr(), N, K, 0, 0
     if A is not None and not d["merged"] and adapters:
         if d["lora_dropout"] > 0.0 and d["training"]:
             return False
@@ -144,15 +163,15 @@ class DecodeStep:
 
     def _size(self, shape, h):
         """Scratch rows for layers of these widths (kept for the step: nearly always one set for all layers)."""
-        W, O, I, gu, rank = shape
+        W, O, I, gu, rank, q = shape
         cols = (self.H, self.H, W, O, I, gu, rank)
         at = [0]
         for c in cols:
             at.append(at[-1] + (self.B * c + 63) // 64 * 64)
-        t = torch.empty(at[-1], dtype=torch.bfloat16, device=h.device)
+        t = torch.empty(at[-1] + (q + 1) // 2, dtype=torch.bfloat16, device=h.device)
         self.keep.append(t)
         s, base = self.s, t.data_ptr()
-        s.res_mid, s.xn, s.qkv_buf, s.att, s.act, s.gu, s.low = (base + 2 * a for a in at[:-1])
+        s.res_mid, s.xn, s.qkv_buf, s.att, s.act, s.gu, s.low, s.q = (base + 2 * a for a in at)
         self.sized = shape
 
     def layer(self, layer, h, residual, inv_freq, attn_scale):
@@ -163,8 +182,9 @@ class DecodeStep:
         e, sub, s = a.__dict__, layer._modules, self.s
         Hq, Hk, D, on = e["Hq"], e["Hk"], e["D"], self.adapters
         gate_up = f._modules["gate_up_proj"]
-        if not (_proj(s.qkv, a._modules["qkv_proj"], on) and _proj(s.o, a._modules["o_proj"], on) and _proj(s.gate_up, gate_up, on)
-                and _proj(s.down, f._modules["down_proj"], on)):
+        B = self.B
+        if not (_proj(s.qkv, a._modules["qkv_proj"], on, B) and _proj(s.o, a._modules["o_proj"], on, B) and _proj(s.gate_up, gate_up, on, B)
+                and _proj(s.down, f._modules["down_proj"], on, B)):
             return None
         n1, n2 = sub["input_layernorm"], sub["post_attention_layernorm"]
         qn, kn = a.q_norm, a.k_norm
@@ -180,8 +200,9 @@ class DecodeStep:
                 or inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous()):
             return None
         kind = _ACT_KIND[f.act]
-        fused = I % 64 == 0 and kind < 2 and gate_up.bias is None
-        shape = (W, Hq * D, I, 0 if fused else 2 * I, max(s.qkv.rank, s.o.rank, s.gate_up.rank, s.down.rank))
+        fused = I % 64 == 0 and kind < 2 and gate_up.bias is None and not s.gate_up.fp8
+        q = max([fp8._packed_size(B, p.K) for p in (s.qkv, s.o, s.gate_up, s.down) if p.fp8 == 2], default=0)
+        shape = (W, Hq * D, I, 0 if fused else 2 * I, max(s.qkv.rank, s.o.rank, s.gate_up.rank, s.down.rank), q)
         if shape != self.sized:
             self._size(shape, h)
         s.norm1, s.norm2 = n1._parameters["weight"].data_ptr(), n2._parameters["weight"].data_ptr()

@@ -656,3 +656,52 @@ def test_lora_without_gradients_keeps_nothing():
     assert torch.equal(y, want) and y.grad_fn.saved_tensors[0] is None
     (dx,) = torch.autograd.grad(y, [xl], torch.ones_like(y))
     assert torch.isfinite(dx).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch", [1, 8, 40, 100])
+@pytest.mark.parametrize("lora", [False, True])
+def test_generation_step_in_one_call_per_layer(batch, lora, monkeypatch):
+    """A step of layers whose projections are in 8 bits (all of them, or some beside dense ones): the one-call form against the layers' own
+    forward, the same kernels on the same operands. What differs is the norm before a dependent launch and the rotary embedding inside the
+    attention launch: a few bf16 roundings (2^-8 each; 0.012 allows three), which the quantiser of the next product keeps or doubles on
+    the few values that then round to the next code."""
+    from axolotl_b200.models import decode_step
+    from axolotl_b200.models.config import preset
+    from axolotl_b200.models.kv_cache import KVCache, _DecodeMeta
+    from axolotl_b200.models.lora import ALL_LINEAR, LoraSpec, inject_lora, quantize_base_fp8_
+    from axolotl_b200.models.transformer import CausalLM
+    from axolotl_b200.ops import _lib
+
+    torch.manual_seed(5)
+    m = CausalLM(preset("tiny-llama", vocab_size=512, num_hidden_layers=3), dtype=torch.bfloat16, device="cuda").init_weights(0).eval()
+    m.layers[1].mlp.down_proj.quantize_fp8_()              # one alone in its layer
+    for n, f in list(m.fused_linears()):
+        if n.startswith(("layers.0.", "layers.2.")):
+            f.quantize_fp8_()
+    if lora:
+        inject_lora(m, LoraSpec(r=8, lora_alpha=16, target_modules=list(ALL_LINEAR)))
+        with torch.no_grad():
+            for _, f in m.fused_linears():
+                if f.lora_B is not None:
+                    for _, B in f.peft_tensors().values():
+                        B.normal_(0, 0.05)
+        m.refresh_lora_shadows()
+    pos = torch.randint(0, 60, (batch,), device="cuda")
+    tok = torch.randint(0, 512, (batch,), device="cuda")
+    at = m.layers[0].self_attn
+    k, v = torch.randn(2, 3, batch, 64, at.Hk * at.D, device="cuda").bfloat16()
+    done, outs = [], []
+    real = decode_step.DecodeStep.layer
+    monkeypatch.setattr(decode_step.DecodeStep, "layer", lambda self, *a: done.append(real(self, *a) if not force else None) or done[-1])
+    for force in (False, True):
+        cache = KVCache(m, batch, 64)
+        cache.k.copy_(k)
+        cache.v.copy_(v)
+        with torch.no_grad():
+            o = m(tok[None], pos.int()[None], attn_meta=_DecodeMeta(cache, torch.arange(batch, device="cuda"), pos, True), return_logits=True)
+        outs.append((o.logits.float(), cache.k.float(), cache.v.float()))
+    _lib.check_status()
+    assert [d is not None for d in done] == [True] * 3 + [False] * 3
+    for a, b in zip(*outs):
+        assert torch.isfinite(a).all() and ((a - b).norm() <= 0.012 * b.norm()).item()
