@@ -16,7 +16,7 @@ extern "C" int axb_fp8_linear(const void* x, long long ldx, void* q, const void*
 extern "C" int axb_fp8_adapter_grad(const void* q, long long ldq, const float* s, long long lds, const void* g, long long ldg, float* out,
                                     long long ldo, int T, int K, int R, int accumulate, int* status, void* stream);
 
-// Filled by ops/fp8.py field by field, in this order.
+// Packed by ops/fp8.py in this order.
 struct AxbFp8Lora {
   const void* x;           // forward: x [T, K]; backward: dy [T, N]; bf16, row stride ldx
   void* q;                 // its 8-bit rows (axb_fp8_linear; null in a forward pass that keeps none)
@@ -39,6 +39,7 @@ struct AxbFp8Lora {
   int T, N, K, R, tile, n_blocks, add_dA, add_dB;
   float scaling;
 };
+static_assert(sizeof(AxbFp8Lora) == 17 * 8 + 8 * 8 + 8 * 4 + 8, "no gaps but the last");
 
 extern "C" int axb_fp8_lora_fwd(const AxbFp8Lora* l, void* stream) {
   if (l->T <= 0) return 0;

@@ -46,8 +46,8 @@ _CUDA_SIGS = {
     "axb_fp8_quantize_rows": [vp, i64, i32, vp, i64, vp, i64, i64, i32, vp],
     "axb_fp8_dequantize_rows": [vp, i64, vp, i64, vp, i64, i32, i64, i32, vp],
     # A, lda, sa, ldsa, B, ldb, sb, sb_n, sb_k, b_mn, C, ldc, M, N, K, A2, lda2, B2, ldb2, K2, tile, status, stream
-    "axb_fp8_lora_fwd": [vp, vp],
-    "axb_fp8_lora_bwd": [vp, vp],
+    "axb_fp8_lora_fwd": [C.c_char_p, vp],      # AxbFp8Lora, stream
+    "axb_fp8_lora_bwd": [C.c_char_p, vp],
     # codes, ldq, scales, lds, g, ldg, out, ldo, T, K, R, accumulate, status, stream
     "axb_fp8_adapter_grad": [vp, i64, vp, i64, vp, i64, vp, i64, i32, i32, i32, i32, vp, vp],
     # x, ldx, codes and scales (null: not kept), W, ldw, sw, sw_n, sw_k, b_mn, y, T, N, K, X2, ldx2, B2, ldb2, K2, tile, status, stream

@@ -19,6 +19,7 @@ from __future__ import annotations
 import contextlib
 import ctypes as C
 import functools
+import struct
 from dataclasses import dataclass
 
 import torch
@@ -108,7 +109,7 @@ def _pack(x):
             return _pack(x)
     if x.stride(1) != 1 and K > 1:
         x = x.contiguous()
-    q = torch.empty(_packed_size(T, K), dtype=torch.uint8, device=device)
+    q = x.new_empty(_packed_size(T, K), dtype=torch.uint8)
     at = q.data_ptr()
     _lib.check_rc(_lib.cuda_lib().axb_fp8_quantize_rows(x.data_ptr(), x.stride(0), _DTYPES[x.dtype], at, ld, at + T * ld, lds, T, K,
                                                         torch._C._cuda_getCurrentRawStream(device.index)), "fp8_quantize_rows")
@@ -134,7 +135,7 @@ def _unpack(q, T, K, dtype):
             return _unpack(q, T, K, dtype)
     ld, lds = _lead(T, K)
     at = q.data_ptr()
-    out = torch.empty((T, K), dtype=dtype, device=device)
+    out = q.new_empty((T, K), dtype=dtype)
     _lib.check_rc(_lib.cuda_lib().axb_fp8_dequantize_rows(at, ld, at + T * ld, lds, out.data_ptr(), K, _DTYPES[dtype], T, K,
                                                           torch._C._cuda_getCurrentRawStream(device.index)), "fp8_dequantize_rows")
     return out
@@ -314,10 +315,8 @@ def _product(x, codes, scale, trans=False, a2=None, b2=None, keep=False):
         a2, b2 = _row_major_2d(a2), _row_major_2d(b2)
         ext = (a2.data_ptr(), a2.stride(0), b2.data_ptr(), b2.stride(0), a2.shape[1])
     few = 0 if trans or ext[4] % 8 else _few(T, N, K)
-    y = torch.empty((T, N), dtype=torch.bfloat16, device=device)
-    q = None
-    if keep or few < 2:
-        q = torch.empty(_packed_size(T, K), dtype=torch.uint8, device=device)
+    y = x.new_empty((T, N))
+    q = x.new_empty(_packed_size(T, K), dtype=torch.uint8) if keep or few < 2 else None
     _lib.check_rc(_lib.cuda_lib().axb_fp8_linear(
         x.data_ptr(), ldx, None if q is None else q.data_ptr(), codes.data_ptr(), codes.stride(0), scale.data_ptr(), sn, sk, trans,
         y.data_ptr(), T, N, K, *ext, 0 if few else _tile(T, N, K), *_lib.launch_args(device.index)), "fp8_linear")
@@ -342,22 +341,17 @@ class _Fp8LinearFn(torch.autograd.Function):
         return dx, None, None, dbias
 
 
-class _Lora(C.Structure):
-    """AxbFp8Lora of csrc/fp8_lora.cu."""
-    _fields_ = ([(n, C.c_void_p) for n in ("x", "q", "W", "sw", "A", "B", "xa", "y", "qx", "t32", "t", "dA", "dB", "dA16", "dB16", "blocks",
-                                        "status")]
-                + [(n, C.c_longlong) for n in ("ldx", "ldw", "sw_n", "sw_k", "lda", "ldb", "ldda", "lddb")]
-                + [(n, C.c_int) for n in ("T", "N", "K", "R", "tile", "n_blocks", "add_dA", "add_dB")] + [("scaling", C.c_float)])
+_LORA = struct.Struct("@17P8q8if")      # AxbFp8Lora of csrc/fp8_lora.cu
 
 
-def _lora_args(x, codes, scale, A16, B16, scaling, T, N, K, R, tile):
-    l = _Lora()
-    l.x, l.ldx, l.W, l.ldw, l.sw = x.data_ptr(), x.stride(0), codes.data_ptr(), codes.stride(0), scale.data_ptr()
-    l.sw_n, l.sw_k = scale.stride()
-    l.A, l.lda, l.B, l.ldb = A16.data_ptr(), A16.stride(0), B16.data_ptr(), B16.stride(0)
-    l.T, l.N, l.K, l.R, l.tile, l.scaling = T, N, K, R, tile, scaling
-    l.status = _lib.status_word(x.device).data_ptr()
-    return l
+def _lora_call(entry, x, codes, scale, A16, B16, scaling, sizes, q, xa, y, qx=0, t32=0, t=0, dA=0, dB=0, dA16=0, dB16=0, blocks=0,
+               ldda=0, lddb=0, n_blocks=0, add_dA=False, add_dB=False):
+    """One call of csrc/fp8_lora.cu; ``q`` .. ``blocks`` are addresses, ``sizes`` is (T, N, K, R, tile)."""
+    status, stream = _lib.launch_args(x.device.index)
+    args = _LORA.pack(x.data_ptr(), q, codes.data_ptr(), scale.data_ptr(), A16.data_ptr(), B16.data_ptr(), xa, y, qx, t32, t, dA, dB, dA16, dB16,
+                      blocks, status, x.stride(0), codes.stride(0), *scale.stride(), A16.stride(0), B16.stride(0), ldda, lddb, *sizes, n_blocks,
+                      add_dA, add_dB, scaling)
+    _lib.check_rc(entry(args, stream), "fp8_lora")
 
 
 @functools.lru_cache(64)
@@ -380,16 +374,11 @@ def _lora_forward(x, codes, scale, A16, B16, scaling, keep):
         xa = skinny_gemm(x, A16, alpha=scaling)            # [T, R], of the bf16 input
         y, q = _product(x, codes, scale, a2=xa, b2=B16, keep=keep)
         return y, xa, q
-    codes = _rows16(codes)
     few = _few(T, N, K)
-    l = _lora_args(x, codes, scale, A16, B16, scaling, T, N, K, R, 0 if few else _tile(T, N, K))
-    y = torch.empty((T, N), dtype=torch.bfloat16, device=x.device)
-    xa = torch.empty((T, R), dtype=torch.bfloat16, device=x.device)
-    l.y, l.xa, q = y.data_ptr(), xa.data_ptr(), None
-    if keep or few < 2:
-        q = torch.empty(_packed_size(T, K), dtype=torch.uint8, device=x.device)
-        l.q = q.data_ptr()
-    _lib.check_rc(_lib.cuda_lib().axb_fp8_lora_fwd(C.byref(l), _lib.stream_ptr()), "fp8_lora_fwd")
+    y, xa = x.new_empty((T, N)), x.new_empty((T, R))
+    q = x.new_empty(_packed_size(T, K), dtype=torch.uint8) if keep or few < 2 else None
+    _lora_call(_lib.cuda_lib().axb_fp8_lora_fwd, x, _rows16(codes), scale, A16, B16, scaling, (T, N, K, R, 0 if few else _tile(T, N, K)),
+               0 if q is None else q.data_ptr(), xa.data_ptr(), y.data_ptr())
     return y, xa, q
 
 
@@ -405,7 +394,7 @@ class _Fp8LoRALinearFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        from .lora import _adapter_grads, _t_and_dB, fused_dy_ok
+        from .lora import USE_FUSED_DY, _adapter_grads, _t_and_dB
 
         q, codes, scale, A, B, A16, B16, xa = ctx.saved_tensors
         need = ctx.needs_input_grad
@@ -413,37 +402,35 @@ class _Fp8LoRALinearFn(torch.autograd.Function):
         (T, N), K, R = dy.shape, codes.shape[1], A16.shape[0]
         dbias = dy.float().sum(0).to(ctx.bias_dtype) if need[9] else None
         dx = dA = dB = None
-        if need[4] and fused_dy_ok(dy, B16, xa) and R % 8 == 0 and all(map(_operand16, (dy, A16, B16, xa))) and len(ctx.blocks) <= 8:
-            # one pass over dy for t and dB, the product and dA behind it: one call
-            codes = _rows16(codes)
-            l = _lora_args(dy, codes, scale, A16, B16, ctx.scaling, T, N, K, R, _tile(T, K, N))
+        if (need[4] and USE_FUSED_DY and T and R <= 64 and R % 8 == 0 and len(ctx.blocks) <= 8 and xa.is_contiguous()
+                and all(map(_operand16, (dy, A16, B16, xa)))):
+            # one pass over dy for t and dB, the product and dA behind it: one call. Scratch: t in fp32, dB in fp32 (where its place is
+            # elsewhere it is not there), t in bf16, dA in fp32, the rows of dy in 8 bits
             n, tA, tB = T * R, getattr(A, "_axb_grad", None), getattr(B, "_axb_grad", None)
-            # scratch: t in fp32, dB in fp32 (where its place is elsewhere it is not used), t in bf16, dA in fp32, the rows of dy in 8 bits
             low = [w is None and p.dtype == torch.bfloat16 for w, p in ((tA, A), (tB, B))]
             at = [4 * n, 4 * N * R if low[1] else 0, 2 * n, 4 * R * K if need[3] and low[0] else 0]
-            work = torch.empty(sum(at) + (_packed_size(T, N) if need[0] else 0), dtype=torch.uint8, device=dy.device)
-            l.t32 = p = work.data_ptr()
-            l.t, l.xa = p + at[0] + at[1], xa.data_ptr()
+            work = dy.new_empty(sum(at) + (_packed_size(T, N) if need[0] else 0), dtype=torch.uint8)
+            p = work.data_ptr()
+            args = dict(t32=p, t=p + at[0] + at[1])
             if need[0]:
-                dx = torch.empty((T, K), dtype=torch.bfloat16, device=dy.device)
-                l.q, l.y = p + sum(at), dx.data_ptr()
+                dx = dy.new_empty((T, K))
             if low[1]:
-                dB = torch.empty((N, R), dtype=torch.bfloat16, device=dy.device)
-                l.dB, l.dB16, l.lddb = p + at[0], dB.data_ptr(), R
+                dB = dy.new_empty((N, R))
+                args.update(dB=p + at[0], dB16=dB.data_ptr(), lddb=R)
             else:
-                dB = tB if tB is not None else torch.empty((N, R), dtype=torch.float32, device=dy.device)
-                l.dB, l.lddb, l.add_dB = dB.data_ptr(), dB.stride(0), tB is not None
+                dB = tB if tB is not None else dy.new_empty((N, R), dtype=torch.float32)
+                args.update(dB=dB.data_ptr(), lddb=dB.stride(0), add_dB=tB is not None)
             if need[3] and low[0]:
-                dA = torch.empty((R, K), dtype=torch.bfloat16, device=dy.device)
-                l.qx, l.dA, l.dA16, l.ldda = q.data_ptr(), p + sum(at[:3]), dA.data_ptr(), K
+                dA = dy.new_empty((R, K))
+                args.update(qx=q.data_ptr(), dA=p + sum(at[:3]), dA16=dA.data_ptr(), ldda=K)
             elif need[3]:
-                dA = tA if tA is not None else torch.empty((R, K), dtype=torch.float32, device=dy.device)
-                l.qx, l.dA, l.ldda, l.add_dA = q.data_ptr(), dA.data_ptr(), dA.stride(0), tA is not None
+                dA = tA if tA is not None else dy.new_empty((R, K), dtype=torch.float32)
+                args.update(qx=q.data_ptr(), dA=dA.data_ptr(), ldda=dA.stride(0), add_dA=tA is not None)
             flat = _flat_blocks(ctx.blocks)
-            l.blocks, l.n_blocks = C.addressof(flat), len(ctx.blocks)
-            _lib.check_rc(_lib.cuda_lib().axb_fp8_lora_bwd(C.byref(l), _lib.stream_ptr()), "fp8_lora_bwd")
-            dA = None if dA is None or tA is not None else dA.to(A.dtype)
-            dB = None if tB is not None else dB.to(B.dtype)
+            _lora_call(_lib.cuda_lib().axb_fp8_lora_bwd, dy, _rows16(codes), scale, A16, B16, ctx.scaling, (T, N, K, R, _tile(T, K, N)),
+                       p + sum(at), xa.data_ptr(), 0 if dx is None else dx.data_ptr(), blocks=C.addressof(flat), n_blocks=len(ctx.blocks), **args)
+            dA = None if dA is None or tA is not None else dA if dA.dtype == A.dtype else dA.to(A.dtype)
+            dB = None if tB is not None else dB if dB.dtype == B.dtype else dB.to(B.dtype)
             return dx, None, None, dA, dB, None, None, None, None, dbias
         t, dB_fused, dB_done = _t_and_dB(dy, B, B16, xa, ctx.blocks, ctx.scaling, need[4])
         dx = _product(dy, codes, scale, trans=True, a2=t, b2=A16)[0] if need[0] else None

@@ -265,6 +265,32 @@ def bench_w4a16(rows):
                     f"fwd+dX: {2*t_deq*1e3 + t_f16*1e3 + t_b16*1e3:.0f} us (dequantise twice + GEMMs) -> {t_f4*1e3 + t_b4*1e3:.0f} us")
 
 
+def bench_fp8(rows):
+    """8-bit blocks at Llama-3-8B shapes: the product of bf16 rows with a frozen E4M3 weight (quantising included) and its input gradient
+    against the bf16 GEMM, few tokens, rows into codes and back, an adapter's gradient from the codes."""
+    from axolotl_b200.ops import fp8
+    from axolotl_b200.ops.gemm import gemm
+    tf, bw, src = _peaks()
+    dev = "cuda"
+    for T, K, N in ((1, 4096, 28672), (64, 14336, 4096), (777, 4096, 6144), (8192, 4096, 6144), (8192, 4096, 28672), (8192, 14336, 4096)):
+        x, dy = torch.randn(T, K, device=dev).bfloat16(), torch.randn(T, N, device=dev).bfloat16()
+        w = torch.randn(N, K, device=dev).bfloat16()
+        codes, scale = fp8.quantize_fp8_weight(w)
+        fl, by = 2.0 * T * N * K, N * K + 2.0 * T * (N + K)
+        t8 = time_cuda(lambda: fp8.fp8_linear(x, codes, scale))
+        b8 = time_cuda(lambda: fp8._product(dy, codes, scale, trans=True))
+        t16, b16 = time_cuda(lambda: gemm(x, w)), time_cuda(lambda: gemm(dy, w, trans_b=True))
+        rows.append(f"fp8 {T} x {K} by {N}: {t8*1e3:.1f} us ({fl/t8/1e9/tf:.2f} of {src} bf16 peak, {by/t8/1e6/bw:.2f} of HBM), bf16 {t16*1e3:.1f} us | "
+                    f"input gradient {b8*1e3:.1f} us ({fl/b8/1e9/tf:.2f}), bf16 {b16*1e3:.1f} us")
+    for T, K in ((8192, 4096), (8192, 14336), (32768, 4096)):
+        x, g = torch.randn(T, K, device=dev).bfloat16(), torch.randn(T, 16, device=dev).bfloat16()
+        codes, scale = fp8.quantize_fp8_rows(x)
+        tq, td = time_cuda(lambda: fp8.quantize_fp8_rows(x)), time_cuda(lambda: fp8.dequantize_fp8_rows(codes, scale))
+        ta = time_cuda(lambda: fp8.fp8_adapter_grad(g, codes, scale))
+        rows.append(f"fp8 rows {T} x {K}: quantise {tq*1e3:.1f} us ({3.0*T*K/tq/1e6/bw:.2f} of HBM), back {td*1e3:.1f} us ({3.0*T*K/td/1e6/bw:.2f}), "
+                    f"rank-16 adapter gradient {ta*1e3:.1f} us ({1.0*T*K/ta/1e6/bw:.2f})")
+
+
 def bench_decode(rows):
     """Single-query attention over a KV cache (memory-bound: one pass over the live cache) and
     end-to-end KV-cache generation on a randomly initialised Llama-3-8B."""
@@ -621,6 +647,8 @@ def main(argv):
         bench_decode(rows)
     if what in ("w4a16",):
         bench_w4a16(rows)
+    if what in ("fp8",):
+        bench_fp8(rows)
     if what in ("attn_wide",):
         bench_attn_wide(rows)
     if what in ("indexer",):
