@@ -69,6 +69,20 @@ def _rows16(codes):
     return out
 
 
+def _operand16(t):
+    return t.dtype == torch.bfloat16 and t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0
+
+
+def _operand(t, what):
+    """A bf16 matrix as bulk tensor copies read it: rows of whole 16 bytes, on 16 bytes."""
+    if t.dtype != torch.bfloat16:
+        raise TypeError(f"{what} takes bf16 matrices beside the codes, got {t.dtype}")
+    if _operand16(t):
+        return t
+    out = t.new_empty((t.shape[0], (t.shape[1] + 7) & ~7))[:, :t.shape[1]]
+    return out.copy_(t)
+
+
 def _row_scales(scale, rows):
     """(tensor, row stride) of the scales [blocks, rows] as the kernels read them."""
     if scale.stride(1) != 1 or (scale.shape[0] > 1 and scale.stride(0) < rows):
@@ -191,7 +205,7 @@ class Fp8State:
 @torch.no_grad()
 def quantize_fp8_weight(w: torch.Tensor):
     """w [N, K] -> (codes float8_e4m3fn [N, K] in rows of whole 16 bytes, scales fp32 [ceil(N / 128), ceil(K / 128)]): the block's largest
-    magnitude becomes 448. Done once, when a weight is loaded."""
+    finite magnitude becomes 448, NaN and infinities NaN codes. Done once, when a weight is loaded."""
     if w.dim() != 2 or 0 in w.shape:
         raise ValueError(f"quantize_fp8_weight takes a matrix that is not empty, got {tuple(w.shape)}")
     N, K = w.shape
@@ -200,7 +214,8 @@ def quantize_fp8_weight(w: torch.Tensor):
     for i in range(scale.shape[0]):                       # 128 rows at a time: no fp32 copy of the whole weight
         rows = w[i * BLOCK:(i + 1) * BLOCK].float()
         pad = torch.nn.functional.pad(rows, (0, scale.shape[1] * BLOCK - K)).view(rows.shape[0], -1, BLOCK)
-        s = pad.abs().amax((0, 2)) / E4M3_MAX
+        pad = torch.where(torch.isfinite(pad), pad, float("nan"))
+        s = pad.nan_to_num(nan=0.0).abs().amax((0, 2)) / E4M3_MAX
         s = torch.where(s > 0, s, torch.ones_like(s))
         scale[i] = s
         q = (pad / s[:, None]).clamp(-E4M3_MAX, E4M3_MAX).to(torch.float8_e4m3fn)
@@ -234,9 +249,11 @@ def fp8_gemm(codes, row_scale, w_codes, w_scale, *, trans_w=False, a2=None, b2=N
     _check_scale(row_scale, (_blocks(K), M), codes.device, "fp8_gemm")
     K2 = 0
     if a2 is not None:
+        if b2 is None or a2.dim() != 2 or a2.shape[0] != M or tuple(b2.shape) != ((a2.shape[1], N) if trans_w else (N, a2.shape[1])):
+            raise ValueError(f"fp8_gemm: extension {tuple(a2.shape)} x {None if b2 is None else tuple(b2.shape)} for a result [{M}, {N}]")
+        if a2.device != codes.device or b2.device != codes.device:
+            raise ValueError(f"fp8_gemm: extension on {a2.device} and {b2.device}, codes on {codes.device}")
         K2 = a2.shape[1]
-        if a2.shape[0] != M or tuple(b2.shape) != ((K2, N) if trans_w else (N, K2)):
-            raise ValueError(f"fp8_gemm: extension {tuple(a2.shape)} x {tuple(b2.shape)} for a result [{M}, {N}]")
     if not codes.is_cuda:
         w = w_codes.float() * w_scale.repeat_interleave(BLOCK, 0)[:w_codes.shape[0]].repeat_interleave(BLOCK, 1)[:, :w_codes.shape[1]]
         y = dequantize_fp8_rows(codes, row_scale, torch.float32) @ (w if trans_w else w.t())
@@ -247,11 +264,7 @@ def fp8_gemm(codes, row_scale, w_codes, w_scale, *, trans_w=False, a2=None, b2=N
         codes, w_codes = _rows16(codes), _rows16(w_codes)
         row_scale, lds = _row_scales(row_scale, M)
         if K2:
-            from .gemm import _row_major_2d
-
-            if a2.dtype != torch.bfloat16 or b2.dtype != torch.bfloat16:
-                raise TypeError("fp8_gemm: the K-extension is bf16")
-            a2, b2 = _row_major_2d(a2), _row_major_2d(b2)
+            a2, b2 = _operand(a2, "fp8_gemm"), _operand(b2, "fp8_gemm")
         out = torch.empty((M, N), dtype=torch.bfloat16, device=codes.device)
         sn, sk = (w_scale.stride(1), w_scale.stride(0)) if trans_w else w_scale.stride()
         _lib.check_rc(_lib.cuda_lib().axb_fp8_gemm(
@@ -300,6 +313,8 @@ def _product(x, codes, scale, trans=False, a2=None, b2=None, keep=False):
             return _product(x, codes, scale, trans, a2, b2, keep)
     T, K = x.shape
     N = codes.shape[1] if trans else codes.shape[0]
+    if T == 0:
+        return x.new_empty((0, N)), _pack(x) if keep else None
     ldx, unit = x.stride()
     if unit != 1 and K > 1:
         x = x.contiguous()
@@ -310,9 +325,7 @@ def _product(x, codes, scale, trans=False, a2=None, b2=None, keep=False):
         sn, sk = sk, sn
     ext = (None, 0, None, 0, 0)
     if a2 is not None:
-        from .gemm import _row_major_2d
-
-        a2, b2 = _row_major_2d(a2), _row_major_2d(b2)
+        a2, b2 = _operand(a2, "8-bit product"), _operand(b2, "8-bit product")
         ext = (a2.data_ptr(), a2.stride(0), b2.data_ptr(), b2.stride(0), a2.shape[1])
     few = 0 if trans or ext[4] % 8 else _few(T, N, K)
     y = x.new_empty((T, N))
@@ -354,13 +367,12 @@ def _lora_call(entry, x, codes, scale, A16, B16, scaling, sizes, q, xa, y, qx=0,
     _lib.check_rc(entry(args, stream), "fp8_lora")
 
 
-@functools.lru_cache(64)
-def _flat_blocks(blocks):
+@functools.lru_cache(256)
+def _flat_blocks(blocks, N, R):
+    """The diagonal blocks (row0, rows, column0, columns) of an adapter's B [N, R] as the kernels take them."""
+    if not blocks or any(len(b) != 4 or min(b) < 0 or b[0] + b[1] > N or b[2] + b[3] > R for b in blocks):
+        raise ValueError(f"adapter blocks {blocks} of a matrix [{N}, {R}]")
     return (C.c_int * (4 * len(blocks)))(*[int(v) for b in blocks for v in b])
-
-
-def _operand16(t):
-    return t.dtype == torch.bfloat16 and t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0
 
 
 def _lora_forward(x, codes, scale, A16, B16, scaling, keep):
@@ -388,7 +400,7 @@ class _Fp8LoRALinearFn(torch.autograd.Function):
         y, xa, q = _lora_forward(x, codes, scale, A16, B16, scaling, ctx.needs_input_grad[3])
         if bias is not None:
             y = y + bias
-        ctx.save_for_backward(q, codes, scale, A, B, A16, B16, xa)
+        ctx.save_for_backward(q if ctx.needs_input_grad[3] else None, codes, scale, A, B, A16, B16, xa)
         ctx.scaling, ctx.blocks, ctx.bias_dtype = scaling, blocks, None if bias is None else bias.dtype
         return y
 
@@ -398,7 +410,7 @@ class _Fp8LoRALinearFn(torch.autograd.Function):
 
         q, codes, scale, A, B, A16, B16, xa = ctx.saved_tensors
         need = ctx.needs_input_grad
-        dy = dy.contiguous()
+        dy = _operand(dy, "fp8_lora_linear")
         (T, N), K, R = dy.shape, codes.shape[1], A16.shape[0]
         dbias = dy.float().sum(0).to(ctx.bias_dtype) if need[9] else None
         dx = dA = dB = None
@@ -426,7 +438,7 @@ class _Fp8LoRALinearFn(torch.autograd.Function):
             elif need[3]:
                 dA = tA if tA is not None else dy.new_empty((R, K), dtype=torch.float32)
                 args.update(qx=q.data_ptr(), dA=dA.data_ptr(), ldda=dA.stride(0), add_dA=tA is not None)
-            flat = _flat_blocks(ctx.blocks)
+            flat = _flat_blocks(ctx.blocks, N, R)
             _lora_call(_lib.cuda_lib().axb_fp8_lora_bwd, dy, _rows16(codes), scale, A16, B16, ctx.scaling, (T, N, K, R, _tile(T, K, N)),
                        p + sum(at), xa.data_ptr(), 0 if dx is None else dx.data_ptr(), blocks=C.addressof(flat), n_blocks=len(ctx.blocks), **args)
             dA = None if dA is None or tA is not None else dA if dA.dtype == A.dtype else dA.to(A.dtype)
@@ -508,10 +520,17 @@ def _shaped(y, x):
     return y if x.dim() == 2 else y.view(*x.shape[:-1], y.shape[-1])
 
 
+def _no_rows(x, codes):
+    """The result of no rows, connected to ``x``."""
+    return x[..., :1].expand(*x.shape[:-1], codes.shape[0])
+
+
 def fp8_linear(x, codes, scale, bias=None):
     """``x8 W8^T (+ bias)`` of a frozen block-FP8 weight (codes [N, K], scales [ceil(N / 128), ceil(K / 128)]); ``x`` [..., K] in bf16. The
     input gradient is ``dy8 W8``; nothing of ``x`` is kept for it."""
     _check_linear(x, codes, scale, "fp8_linear")
+    if x.numel() == 0:
+        return _no_rows(x, codes)
     if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
         return _shaped(_Fp8LinearFn.apply(_rows_of(x), codes, scale, bias), x)
     y = _product(x if x.dim() == 2 else _rows_of(x), codes, scale)[0]
@@ -524,11 +543,23 @@ def fp8_lora_linear(x, codes, scale, A, B, A16, B16, scaling, blocks, bias=None)
     """``x8 W8^T + scaling (x A^T) B^T (+ bias)``: ``fp8_linear`` with the adapter of ``ops.lora.lora_linear`` (same arguments). The 8-bit
     rows of ``x`` are kept for ``dA = (scaling dy B)^T x8``."""
     _check_linear(x, codes, scale, "fp8_lora_linear")
+    if x.numel() == 0:
+        return _no_rows(x, codes)
     x2 = _rows_of(x)
     if not x.is_cuda:
         y = _Fp8LinearFn.apply(x2, codes, scale, bias).to(x.dtype)
         return _shaped(y + scaling * ((x2 @ A.to(x2.dtype).t()) @ B.to(x2.dtype).t()), x)
-    x2 = x2.contiguous()
+    N, K = codes.shape
+    R = A.shape[0]
+    if (A.shape != (R, K) or B.shape != (N, R) or A16.shape != A.shape or B16.shape != B.shape or A16.dtype != torch.bfloat16
+            or B16.dtype != torch.bfloat16 or not x.device == A.device == B.device == A16.device == B16.device):
+        raise ValueError(f"fp8_lora_linear: adapter {tuple(A.shape)} {tuple(B.shape)} with bf16 copies {A16.dtype} {tuple(A16.shape)} "
+                         f"{B16.dtype} {tuple(B16.shape)} for a weight [{N}, {K}] on {x.device}")
+    if R % 8:
+        raise ValueError(f"fp8_lora_linear: rank {R}, the device path needs a multiple of 8 (16-byte rows for the bulk tensor copies)")
+    blocks = tuple(map(tuple, blocks))
+    _flat_blocks(blocks, N, R)
+    x2, A16, B16 = (_operand(t, "fp8_lora_linear") for t in (x2, A16, B16))
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, A, B, bias)):
         return _shaped(_Fp8LoRALinearFn.apply(x2, codes, scale, A, B, A16, B16, float(scaling), blocks, bias), x)
     y = _lora_forward(x2, codes, scale, A16, B16, float(scaling), False)[0]

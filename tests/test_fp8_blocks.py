@@ -295,7 +295,7 @@ def test_linear_gradient_by_differences(dev):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("T,K,N,blocks", [(1, 256, 128, ((0, 128, 0, 8),)), (70, 520, 264, ((0, 200, 0, 8), (200, 64, 8, 8))),
-                                          (600, 1024, 640, ((0, 640, 0, 16),)), (700, 264, 1032, ((128, 904, 0, 32),))])
+                                          (600, 1024, 640, ((0, 640, 0, 16),)), (700, 264, 1032, ((128, 904, 0, 32),)), (90, 131, 77, ((0, 77, 0, 8),)), (20, 256, 128, ((0, 128, 0, 72),))])
 @pytest.mark.parametrize("masters", [torch.float32, torch.bfloat16])
 def test_lora_linear_and_its_gradients(T, K, N, blocks, masters):
     R = sum(b[3] for b in blocks)
@@ -705,3 +705,157 @@ def test_generation_step_in_one_call_per_layer(batch, lora, monkeypatch):
     assert [d is not None for d in done] == [True] * 3 + [False] * 3
     for a, b in zip(*outs):
         assert torch.isfinite(a).all() and ((a - b).norm() <= 0.012 * b.norm()).item()
+
+
+# ------------------------------------------------------------------ calls that ordinary use makes rarely
+@pytest.mark.parametrize("dev", DEVICES)
+def test_no_rows(dev):
+    w, ws = quantize_fp8_weight(torch.randn(64, 128).to(dev))
+    A, B = torch.randn(8, 128).bfloat16().to(dev), torch.randn(64, 8).bfloat16().to(dev)
+    for call in (lambda x: fp8_linear(x, w, ws), lambda x: fp8_lora_linear(x, w, ws, A, B, A, B, 1.0, ((0, 64, 0, 8),))):
+        x = torch.empty(2, 0, 128, dtype=torch.bfloat16, device=dev, requires_grad=True)
+        y = call(x)
+        assert y.shape == (2, 0, 64) and y.dtype == torch.bfloat16
+        y.sum().backward()
+        assert x.grad.shape == x.shape
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_weight_with_nan_and_infinity(dev):
+    w = torch.randn(140, 260)
+    w[3, 5], w[139, 259] = float("nan"), float("-inf")
+    codes, scale = quantize_fp8_weight(w.to(dev))
+    back = _weight8(codes, scale)
+    odd = ~torch.isfinite(w)
+    assert torch.isfinite(scale).all() and torch.equal(torch.isnan(back), odd)
+    s = scale.cpu().double().repeat_interleave(128, 0)[:140].repeat_interleave(128, 1)[:, :260]
+    ok = (back - w.double()).abs() <= torch.maximum(w.double().abs() * 2.0 ** -4, s * 2.0 ** -10) * (1 + 2.0 ** -20)
+    assert ok[~odd].all()
+
+
+def test_lora_refusals():
+    w, ws = quantize_fp8_weight(torch.randn(64, 128))
+    x, A, B = torch.randn(4, 128).bfloat16(), torch.randn(8, 128).bfloat16(), torch.randn(64, 8).bfloat16()
+    from axolotl_b200.ops.fp8 import _flat_blocks
+
+    for blocks in ((), ((0, 65, 0, 8),), ((0, 64, 4, 8),), ((-1, 8, 0, 8),), ((0, 64, 0),)):
+        with pytest.raises(ValueError):
+            _flat_blocks(blocks, 64, 8)
+    codes, scale = quantize_fp8_rows(x)
+    for a2, b2 in ((A[:4, :8], None), (A[:3, :8], B), (A[:4, :8].to("meta"), B)):
+        with pytest.raises(ValueError):
+            fp8_gemm(codes, scale, w, ws, a2=a2, b2=b2)
+
+
+@pytest.mark.gpu
+def test_lora_refusals_on_the_device():
+    w, ws = quantize_fp8_weight(torch.randn(64, 128).cuda())
+    x, A, B = torch.randn(4, 128).bfloat16().cuda(), torch.randn(8, 128).bfloat16().cuda(), torch.randn(64, 8).bfloat16().cuda()
+    blk = ((0, 64, 0, 8),)
+    for args in ((A[:, :64], B, A[:, :64], B), (A, B[:32], A, B[:32]), (A, B, A.float(), B), (A, B, A[:4], B), (A, B, A.cpu(), B), (A, B, A, B.cpu())):
+        with pytest.raises(ValueError):
+            fp8_lora_linear(x, w, ws, *args, 1.0, blk)
+    with pytest.raises(ValueError):
+        fp8_lora_linear(x, w, ws, A, B, A, B, 1.0, ((0, 64, 0, 16),))
+    with pytest.raises(TypeError):
+        fp8_linear(x.float(), w, ws)
+    with pytest.raises(ValueError):
+        fp8_linear(x, w.cpu(), ws.cpu())
+    with pytest.raises(TypeError):
+        fp8_gemm(*quantize_fp8_rows(x), w, ws, a2=A[:4, :8].float(), b2=B)
+    with pytest.raises(TypeError):
+        fp8_adapter_grad(torch.zeros(4, 8, device="cuda"), *quantize_fp8_rows(x))
+
+
+@pytest.mark.gpu
+def test_operands_off_a_16_byte_boundary():
+    """Inputs, gradients, adapters and extensions that start in the middle of a 16-byte vector give what aligned ones give."""
+    T, K, N, R = 300, 264, 136, 8
+
+    def off(t):                                            # the same values one element further on
+        wide = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)
+        wide[1:].copy_(t.reshape(-1))
+        return wide[1:].view(t.shape)
+
+    x, dy = _make((T, K), 1, spread=0.3).cuda(), _make((T, N), 2, spread=0.3).cuda()
+    w, ws = quantize_fp8_weight(_make((N, K), 3, torch.float32, 0.0).cuda())
+    A, B = _make((R, K), 4, spread=0.0).cuda() * 0.06, _make((N, R), 5, spread=0.0).cuda() * 0.1
+    assert off(x).data_ptr() % 16 and off(x).is_contiguous()
+    res = []
+    for f in (lambda t: t, off):
+        xl = f(x).requires_grad_(True)
+        y = fp8_linear(xl, w, ws)
+        Al, Bl = f(A).requires_grad_(True), f(B).requires_grad_(True)
+        z = fp8_lora_linear(f(x), w, ws, Al, Bl, f(A), f(B), 1.0, ((0, N, 0, R),))
+        codes, scale = quantize_fp8_rows(f(x))
+        res.append([y, torch.autograd.grad(y, [xl], f(dy))[0], z, *torch.autograd.grad(z, [Al, Bl], f(dy)),
+                    fp8_gemm(codes, scale, w, ws, a2=f(dy)[:, :5], b2=f(B)[:, :5]), fp8_adapter_grad(f(dy)[:, :7], codes, scale)])
+    for i, (a, b) in enumerate(zip(*res)):
+        if i in (3, 4):                                    # sums of atomics in any order, of t that may round to its neighbour (2^-7)
+            assert ((a.double() - b.double()).abs().max() <= 2.0 ** -6 * a.double().abs().max()).item()
+        else:
+            assert torch.equal(a, b), i
+
+
+@pytest.mark.gpu
+def test_captured_and_replayed_on_another_stream():
+    """Graphs of the products (every form), the adapter's layer with its backward pass and the checkpoint store, replayed on new inputs beside
+    one another: each gives what the eager call gives."""
+    from axolotl_b200.train.activation_memory import make_store
+
+    N, K, R = 264, 1032, 8
+    w, ws = quantize_fp8_weight(_make((N, K), 3, torch.float32, 0.0).cuda())
+    A, B = _make((R, K), 4, spread=0.0).cuda() * 0.06, _make((N, R), 5, spread=0.0).cuda() * 0.1
+    calls = []
+    for T in (1, 40, 64, 300):
+        calls.append((T, lambda x: fp8_linear(x, w, ws)))
+    calls.append((600, lambda x: fp8_lora_linear(x, w, ws, A, B, A, B, 1.0, ((0, N, 0, R),))))
+
+    def stored(x):
+        store = make_store("fp8", x.device)
+        return store.get(store.put(x))
+
+    def trained(x):
+        xl = x.detach().requires_grad_(True)
+        y = fp8_linear(xl, w, ws)
+        return torch.autograd.grad(y, [xl], torch.ones_like(y))[0]
+
+    calls += [(77, stored), (130, trained)]
+    stream = torch.cuda.Stream()
+    graphs = []
+    for i, (T, f) in enumerate(calls):
+        x = _make((T, K), i, spread=0.3).cuda()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            with torch.no_grad() if f is not trained else torch.enable_grad():
+                f(x)
+        stream.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            with torch.no_grad() if f is not trained else torch.enable_grad():
+                out = f(x)
+        graphs.append((g, x, out, f))
+    for i, (g, x, _, _) in enumerate(graphs):
+        x.copy_(_make(tuple(x.shape), 100 + i, spread=0.3))
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        for _ in range(2):
+            for g, _, _, _ in graphs:
+                g.replay()
+    torch.cuda.synchronize()
+    for i, (g, x, out, f) in enumerate(graphs):
+        with torch.no_grad() if f is not trained else torch.enable_grad():
+            assert torch.equal(out, f(x)), i
+
+
+@pytest.mark.gpu
+def test_results_repeat_bit_for_bit():
+    """Nothing but t and dB of an adapter is summed in an order that may change."""
+    x = _make((700, 1032), 1, spread=0.3).cuda()
+    w, ws = quantize_fp8_weight(_make((520, 1032), 2, torch.float32, 0.0).cuda())
+    codes, scale = quantize_fp8_rows(x)
+    t = _make((700, 16), 3, spread=0.0).cuda()
+    for f in (lambda: fp8_gemm(codes, scale, w, ws), lambda: fp8_linear(x[:5], w, ws), lambda: fp8_linear(x[:60], w, ws),
+              lambda: fp8_adapter_grad(t, codes, scale)):
+        first = f()
+        assert all(torch.equal(first, f()) for _ in range(5))
