@@ -7,7 +7,8 @@
 // Every block of 128 columns starts an accumulator of its own; four warps (a thread owns a weight row) add it to sums in registers,
 // times the weight's scale and the token's. The rows come as codes (csrc/fp8_rows.cu), or (FUSED) in bf16: then four warps quantise them
 // into the operand tile while the weight's bulk copies arrive, and the codes and their scales never reach memory. ops/fp8.py says when.
-// On quantised rows it is a dependent launch of the kernel that quantised them.
+// On quantised rows it is a dependent launch of the kernel that quantised them. One token by 4096 x 4096 8.3 us (codes in the L2), by
+// 4096 x 28672 25 us (4.7 TB/s); 64 tokens, 14336 x 4096, 20 us.
 #include <cuda_fp8.h>
 
 #include "axb_common.cuh"
