@@ -341,7 +341,7 @@ class _Fp8LinearFn(torch.autograd.Function):
     def forward(ctx, x, codes, scale, bias):
         y, _ = _product(x, codes, scale)
         if bias is not None:
-            y = y + bias
+            y += bias                                     # in place: bf16 whatever the bias is in, and so is the gradient that comes back
         ctx.save_for_backward(codes, scale)               # the weight is frozen: nothing of x is needed again
         ctx.bias_dtype = None if bias is None else bias.dtype
         return y
@@ -399,7 +399,7 @@ class _Fp8LoRALinearFn(torch.autograd.Function):
     def forward(ctx, x, codes, scale, A, B, A16, B16, scaling, blocks, bias):
         y, xa, q = _lora_forward(x, codes, scale, A16, B16, scaling, ctx.needs_input_grad[3])
         if bias is not None:
-            y = y + bias
+            y += bias
         ctx.save_for_backward(q if ctx.needs_input_grad[3] else None, codes, scale, A, B, A16, B16, xa)
         ctx.scaling, ctx.blocks, ctx.bias_dtype = scaling, blocks, None if bias is None else bias.dtype
         return y
@@ -497,8 +497,10 @@ def _adapter_grad(t, q, ldq, s, lds, K, out):
     return out
 
 
-def _check_linear(x, codes, scale, what):
+def _check_linear(x, codes, scale, bias, what):
     cs, ss = codes.shape, scale.shape
+    if bias is not None and (bias.shape != cs[:1] or bias.device != x.device):
+        raise ValueError(f"{what}: a bias {tuple(bias.shape)} on {bias.device} for a weight {tuple(cs)} and an input on {x.device}")
     if (len(cs) == 2 and len(ss) == 2 and cs[0] and cs[1] and x.dim() and x.shape[-1] == cs[1] and codes.dtype == torch.float8_e4m3fn
             and scale.dtype == torch.float32 and ss[0] == _blocks(cs[0]) and ss[1] == _blocks(cs[1]) and x.device == codes.device
             and x.device == scale.device and (x.dtype == torch.bfloat16 or not x.is_cuda)):
@@ -528,21 +530,21 @@ def _no_rows(x, codes):
 def fp8_linear(x, codes, scale, bias=None):
     """``x8 W8^T (+ bias)`` of a frozen block-FP8 weight (codes [N, K], scales [ceil(N / 128), ceil(K / 128)]); ``x`` [..., K] in bf16. The
     input gradient is ``dy8 W8``; nothing of ``x`` is kept for it."""
-    _check_linear(x, codes, scale, "fp8_linear")
+    _check_linear(x, codes, scale, bias, "fp8_linear")
     if x.numel() == 0:
         return _no_rows(x, codes)
     if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
         return _shaped(_Fp8LinearFn.apply(_rows_of(x), codes, scale, bias), x)
     y = _product(x if x.dim() == 2 else _rows_of(x), codes, scale)[0]
     if bias is not None:
-        y = y + bias
+        y += bias
     return y if x.dim() == 2 and y.dtype == x.dtype else _shaped(y, x)
 
 
 def fp8_lora_linear(x, codes, scale, A, B, A16, B16, scaling, blocks, bias=None):
     """``x8 W8^T + scaling (x A^T) B^T (+ bias)``: ``fp8_linear`` with the adapter of ``ops.lora.lora_linear`` (same arguments). The 8-bit
     rows of ``x`` are kept for ``dA = (scaling dy B)^T x8``."""
-    _check_linear(x, codes, scale, "fp8_lora_linear")
+    _check_linear(x, codes, scale, bias, "fp8_lora_linear")
     if x.numel() == 0:
         return _no_rows(x, codes)
     x2 = _rows_of(x)
@@ -563,4 +565,6 @@ def fp8_lora_linear(x, codes, scale, A, B, A16, B16, scaling, blocks, bias=None)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, A, B, bias)):
         return _shaped(_Fp8LoRALinearFn.apply(x2, codes, scale, A, B, A16, B16, float(scaling), blocks, bias), x)
     y = _lora_forward(x2, codes, scale, A16, B16, float(scaling), False)[0]
-    return _shaped(y if bias is None else y + bias, x)
+    if bias is not None:
+        y += bias
+    return _shaped(y, x)

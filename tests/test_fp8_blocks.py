@@ -859,3 +859,33 @@ def test_results_repeat_bit_for_bit():
               lambda: fp8_adapter_grad(t, codes, scale)):
         first = f()
         assert all(torch.equal(first, f()) for _ in range(5))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_bias_in_another_type(dtype, dev):
+    """The result and the gradient that comes back stay bf16: the sum is rounded once, and dx is what it is without a bias."""
+    T, K, N, R = 40, 256, 64, 8
+    x, dy = _make((T, K), 1, spread=0.0).to(dev), _make((T, N), 2, spread=0.0).to(dev)
+    w, ws = quantize_fp8_weight(_make((N, K), 3, torch.float32, 0.0).to(dev))
+    A, B = (_make((R, K), 4, spread=0.0) * 0.06).to(dev), (_make((N, R), 5, spread=0.0) * 0.1).to(dev)
+    bias = _make((1, N), 6, torch.float32, 0.0)[0].to(dtype).to(dev)
+    for f in (lambda x, b: fp8_linear(x, w, ws, b), lambda x, b: fp8_lora_linear(x, w, ws, A, B, A, B, 1.0, ((0, N, 0, R),), b)):
+        x0, xb, b = x.clone().requires_grad_(True), x.clone().requires_grad_(True), bias.clone().requires_grad_(True)
+        y0, yb = f(x0, None), f(xb, b)
+        assert yb.dtype == torch.bfloat16
+        (d0,) = torch.autograd.grad(y0, [x0], dy)
+        db, d1 = torch.autograd.grad(yb, [b, xb], dy)
+        assert db.dtype == dtype       # the adapter's t is summed in any order and may round to its neighbour (2^-7)
+        assert ((d0.double() - d1.double()).abs().max() <= 2.0 ** -6 * d0.double().abs().max()).item()
+        want = dy.double().sum(0)
+        half = torch.finfo(dtype).eps / 2
+        assert ((db.double() - want).abs() <= half * want.abs() + T * EPS32 * dy.double().abs().sum(0) * (1 + half)).all()
+        with torch.no_grad():
+            assert torch.equal(f(x, bias), yb)
+    assert torch.equal(fp8_linear(x, w, ws, bias), (fp8_linear(x, w, ws).float() + bias.float()).bfloat16())
+    for wrong in (bias[:1], bias[None], bias.repeat(2)):
+        with pytest.raises(ValueError):
+            fp8_linear(x, w, ws, wrong)
+        with pytest.raises(ValueError):
+            fp8_lora_linear(x, w, ws, A, B, A, B, 1.0, ((0, N, 0, R),), wrong)
