@@ -23,7 +23,7 @@ from ..ops import fp8
 
 
 class _Handle:
-    __slots__ = ("shape", "dtype", "device", "host", "event", "gpu", "gpu_event", "prev", "path", "future", "coded", "nbytes")
+    __slots__ = ("shape", "dtype", "device", "host", "event", "gpu", "gpu_event", "prev", "path", "future", "coded", "stream", "nbytes")
 
     def __init__(self):
         self.host = self.event = self.gpu = self.gpu_event = self.prev = self.path = self.future = None
@@ -161,6 +161,7 @@ class Fp8Store:
     def put(self, t: torch.Tensor) -> _Handle:
         h = _Handle()
         h.shape, h.dtype, h.device = t.shape, t.dtype, t.device
+        h.stream = torch._C._cuda_getCurrentRawStream(t.device.index) if t.is_cuda else None
         if t.dtype not in (torch.bfloat16, torch.float16, torch.float32) or t.numel() == 0 or t.dim() == 0:
             h.gpu, h.coded = t.detach(), False            # kept as it is
         else:
@@ -174,6 +175,10 @@ class Fp8Store:
         kept, h.gpu = h.gpu, None
         if kept is None:
             raise RuntimeError("this checkpoint has been given back already")
+        if h.stream is not None and h.stream != torch._C._cuda_getCurrentRawStream(h.device.index):
+            now = torch.cuda.current_stream(h.device)         # another stream than the one that wrote the codes
+            now.wait_stream(torch.cuda.ExternalStream(h.stream, h.device))
+            kept.record_stream(now)
         if not h.coded:
             return kept
         K = h.shape[-1]

@@ -454,7 +454,8 @@ def _train(cfg, dataset_meta: TrainDatasetMeta | None = None):
         if ao in (True, "legacy", "disk"):
             model.offload_saved_store = model.ckpt_store   # also park what autograd saves outside the layers
         if ao:
-            LOG.info("activation offloading: checkpointed layer inputs go to %s", "disk" if ao == "disk" else "pinned host memory")
+            LOG.info("activation offloading: checkpointed layer inputs go to %s",
+                     {"disk": "disk", "fp8": "8-bit codes on the device"}.get(ao, "pinned host memory"))
     if cfg.get("layer_offloading"):
         from .activation_memory import LayerOffloader
 

@@ -889,3 +889,29 @@ def test_bias_in_another_type(dtype, dev):
             fp8_linear(x, w, ws, wrong)
         with pytest.raises(ValueError):
             fp8_lora_linear(x, w, ws, A, B, A, B, 1.0, ((0, N, 0, R),), wrong)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("coded", [True, False])
+def test_store_taken_back_on_another_stream(coded):
+    """What one stream stores, another takes back: it waits for the codes, and their memory is not given out again while it reads them."""
+    from axolotl_b200.train.activation_memory import make_store
+
+    x = _make((512, 1024), 1, spread=0.3).cuda()
+    x = x if coded else x.double()
+    want = dequantize_fp8_rows(*quantize_fp8_rows(x)) if coded else x.clone()
+    store, side = make_store("fp8", x.device), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    late = torch.zeros_like(x)
+    torch.cuda._sleep(20_000_000)                          # some 10 ms
+    late.copy_(x)
+    h = store.put(late)
+    kept = h.gpu.data_ptr()
+    del late
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)
+        got = store.get(h)
+        got = got if coded else got.clone()
+    fresh = [torch.full((want.numel() * (1 if coded else 8) + 16384 * coded,), 0x55, dtype=torch.uint8, device="cuda") for _ in range(4)]
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and kept and fresh
