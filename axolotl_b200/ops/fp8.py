@@ -23,6 +23,7 @@ import struct
 from dataclasses import dataclass
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -336,10 +337,23 @@ def _product(x, codes, scale, trans=False, a2=None, b2=None, keep=False):
     return y, q
 
 
+def _as_codes(w):
+    """The codes of a weight given as they are, or as the bytes of a frozen parameter. Autograd then saves the parameter and no view of
+    its data, so that data which leave the device between the two passes are not kept alive there."""
+    return w.data.view(torch.float8_e4m3fn) if w.dtype == torch.uint8 else w
+
+
+def _once(backward):
+    """A backward pass without a second derivative; the wrapper that refuses one costs the host 2 us and is entered where a graph of the
+    backward pass is asked for."""
+    refusing = once_differentiable(backward)
+    return lambda ctx, dy: (refusing if torch.is_grad_enabled() else backward)(ctx, dy)
+
+
 class _Fp8LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, codes, scale, bias):
-        y, _ = _product(x, codes, scale)
+        y, _ = _product(x, _as_codes(codes), scale)
         if bias is not None:
             y += bias                                     # in place: bf16 whatever the bias is in, and so is the gradient that comes back
         ctx.save_for_backward(codes, scale)               # the weight is frozen: nothing of x is needed again
@@ -347,9 +361,10 @@ class _Fp8LinearFn(torch.autograd.Function):
         return y
 
     @staticmethod
+    @_once
     def backward(ctx, dy):
         codes, scale = ctx.saved_tensors
-        dx = _product(dy, codes, scale, trans=True)[0] if ctx.needs_input_grad[0] else None
+        dx = _product(dy, _as_codes(codes), scale, trans=True)[0] if ctx.needs_input_grad[0] else None
         dbias = dy.float().sum(0).to(ctx.bias_dtype) if ctx.needs_input_grad[3] else None
         return dx, None, None, dbias
 
@@ -397,7 +412,7 @@ def _lora_forward(x, codes, scale, A16, B16, scaling, keep):
 class _Fp8LoRALinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, codes, scale, A, B, A16, B16, scaling, blocks, bias):
-        y, xa, q = _lora_forward(x, codes, scale, A16, B16, scaling, ctx.needs_input_grad[3])
+        y, xa, q = _lora_forward(x, _as_codes(codes), scale, A16, B16, scaling, ctx.needs_input_grad[3])
         if bias is not None:
             y += bias
         ctx.save_for_backward(q if ctx.needs_input_grad[3] else None, codes, scale, A, B, A16, B16, xa)
@@ -405,10 +420,12 @@ class _Fp8LoRALinearFn(torch.autograd.Function):
         return y
 
     @staticmethod
+    @_once
     def backward(ctx, dy):
         from .lora import USE_FUSED_DY, _adapter_grads, _t_and_dB
 
         q, codes, scale, A, B, A16, B16, xa = ctx.saved_tensors
+        codes = _as_codes(codes)
         need = ctx.needs_input_grad
         dy = _operand(dy, "fp8_lora_linear")
         (T, N), K, R = dy.shape, codes.shape[1], A16.shape[0]
@@ -501,11 +518,11 @@ def _check_linear(x, codes, scale, bias, what):
     cs, ss = codes.shape, scale.shape
     if bias is not None and (bias.shape != cs[:1] or bias.device != x.device):
         raise ValueError(f"{what}: a bias {tuple(bias.shape)} on {bias.device} for a weight {tuple(cs)} and an input on {x.device}")
-    if (len(cs) == 2 and len(ss) == 2 and cs[0] and cs[1] and x.dim() and x.shape[-1] == cs[1] and codes.dtype == torch.float8_e4m3fn
-            and scale.dtype == torch.float32 and ss[0] == _blocks(cs[0]) and ss[1] == _blocks(cs[1]) and x.device == codes.device
+    if (len(cs) == 2 and len(ss) == 2 and cs[0] and cs[1] and x.dim() and x.shape[-1] == cs[1]
+            and codes.dtype in (torch.float8_e4m3fn, torch.uint8) and scale.dtype == torch.float32 and ss[0] == _blocks(cs[0]) and ss[1] == _blocks(cs[1]) and x.device == codes.device
             and x.device == scale.device and (x.dtype == torch.bfloat16 or not x.is_cuda)):
         return
-    _check_weight(codes, scale, what)
+    _check_weight(_as_codes(codes), scale, what)
     if 0 in cs or x.dim() < 1 or x.shape[-1] != cs[1]:
         raise ValueError(f"{what}: input {tuple(x.shape)} for a weight {tuple(cs)}")
     if x.device != codes.device:
@@ -528,14 +545,14 @@ def _no_rows(x, codes):
 
 
 def fp8_linear(x, codes, scale, bias=None):
-    """``x8 W8^T (+ bias)`` of a frozen block-FP8 weight (codes [N, K], scales [ceil(N / 128), ceil(K / 128)]); ``x`` [..., K] in bf16. The
-    input gradient is ``dy8 W8``; nothing of ``x`` is kept for it."""
+    """``x8 W8^T (+ bias)`` of a frozen block-FP8 weight (codes [N, K], float8_e4m3fn or the same as bytes, and scales [ceil(N / 128),
+    ceil(K / 128)]); ``x`` [..., K] in bf16. The input gradient is ``dy8 W8``; nothing of ``x`` is kept for it."""
     _check_linear(x, codes, scale, bias, "fp8_linear")
     if x.numel() == 0:
         return _no_rows(x, codes)
     if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
         return _shaped(_Fp8LinearFn.apply(_rows_of(x), codes, scale, bias), x)
-    y = _product(x if x.dim() == 2 else _rows_of(x), codes, scale)[0]
+    y = _product(x if x.dim() == 2 else _rows_of(x), _as_codes(codes), scale)[0]
     if bias is not None:
         y += bias
     return y if x.dim() == 2 and y.dtype == x.dtype else _shaped(y, x)
@@ -564,7 +581,7 @@ def fp8_lora_linear(x, codes, scale, A, B, A16, B16, scaling, blocks, bias=None)
     x2, A16, B16 = (_operand(t, "fp8_lora_linear") for t in (x2, A16, B16))
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, A, B, bias)):
         return _shaped(_Fp8LoRALinearFn.apply(x2, codes, scale, A, B, A16, B16, float(scaling), blocks, bias), x)
-    y = _lora_forward(x2, codes, scale, A16, B16, float(scaling), False)[0]
+    y = _lora_forward(x2, _as_codes(codes), scale, A16, B16, float(scaling), False)[0]
     if bias is not None:
         y += bias
     return _shaped(y, x)

@@ -300,7 +300,7 @@ def linear(x, W, bias=None):
     """``x @ W^T (+ bias)``; 2-D or N-D ``x``. CPU tensors use torch ops directly; a weight in 8-bit blocks takes ``fp8_linear``."""
     st = fp8_state(W)
     if st is not None:
-        return fp8_linear(x, W.data.view(torch.float8_e4m3fn), st.scale, bias)
+        return fp8_linear(x, W, st.scale, bias)
     if not x.is_cuda:
         return torch.nn.functional.linear(x, _cpu_weight(W, x.dtype), None if bias is None else bias.to(x.dtype))
     shp = x.shape
@@ -315,7 +315,7 @@ def lora_linear(x, W, A, B, A16, B16, scaling, blocks, bias=None, dropout_p=0.0,
     x2 = x.reshape(-1, shp[-1])
     st = fp8_state(W)
     if st is not None and not (dropout_p > 0.0 and training):
-        return fp8_lora_linear(x, W.data.view(torch.float8_e4m3fn), st.scale, A, B, A16, B16, scaling, blocks, bias)
+        return fp8_lora_linear(x, W, st.scale, A, B, A16, B16, scaling, blocks, bias)
     if not x.is_cuda or (dropout_p > 0.0 and training):
         xd = torch.nn.functional.dropout(x2, dropout_p, training) if dropout_p > 0.0 else x2
         if x.is_cuda:

@@ -915,3 +915,100 @@ def test_store_taken_back_on_another_stream(coded):
     fresh = [torch.full((want.numel() * (1 if coded else 8) + 16384 * coded,), 0x55, dtype=torch.uint8, device="cuda") for _ in range(4)]
     torch.cuda.synchronize()
     assert torch.equal(got, want) and kept and fresh
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_frozen_parameter_moves_between_the_passes(dev):
+    """Autograd saves the frozen parameter itself: data that leave after the forward pass are let go, and come back for the backward pass."""
+    from axolotl_b200.models.layers import FusedLinear
+
+    m = FusedLinear(256, [128], ["a"], dtype=torch.bfloat16, device=dev)
+    with torch.no_grad():
+        m.weight.copy_(_make((128, 256), 1, spread=0.0))
+    m.quantize_fp8_()
+    x, dy = _make((30, 256), 2, spread=0.0).to(dev), _make((30, 128), 3, spread=0.0).to(dev)
+    x0 = x.clone().requires_grad_(True)
+    (want,) = torch.autograd.grad(m(x0), [x0], dy)
+    x1 = x.clone().requires_grad_(True)
+    y = m(x1)
+    kept = m.weight.data.clone()
+    m.weight.data = torch.empty(0, dtype=torch.uint8, device=dev)
+    m.weight.data = kept
+    assert any(t is m.weight for t in y.grad_fn.saved_tensors)
+    (got,) = torch.autograd.grad(y, [x1], dy)
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_second_derivatives_are_refused(dev):
+    w, ws = quantize_fp8_weight(_make((64, 128), 3, torch.float32, 0.0).to(dev))
+    x = _make((4, 128), 1, spread=0.0).to(dev).requires_grad_(True)
+    (dx,) = torch.autograd.grad(fp8_linear(x, w, ws).float().pow(2).sum(), [x], create_graph=True)
+    with pytest.raises(RuntimeError):
+        dx.float().sum().backward()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_layer_offloading_of_8_bit_layers(dev):
+    """Frozen layers that live in host memory give the gradients of resident ones."""
+    from axolotl_b200.models.config import preset
+    from axolotl_b200.models.lora import LoraSpec, inject_lora, quantize_base_fp8_
+    from axolotl_b200.models.transformer import CausalLM
+    from axolotl_b200.train.activation_memory import LayerOffloader
+
+    cfg = preset("tiny-llama", num_hidden_layers=3, vocab_size=512)
+    grads = []
+    for offload in (False, True):
+        m = CausalLM(cfg, dtype=torch.bfloat16 if dev == "cuda" else torch.float32, device=dev).init_weights(0)
+        quantize_base_fp8_(m)
+        torch.manual_seed(1)
+        inject_lora(m, LoraSpec(r=8, lora_alpha=16, target_modules=["q_proj", "o_proj", "gate_proj", "up_proj", "down_proj"]))
+        with torch.no_grad():
+            for _, f in m.fused_linears():
+                if f.lora_B is not None:
+                    for _, B in f.peft_tensors().values():
+                        B.normal_(0, 0.05)
+        m.refresh_lora_shadows()
+        m.train()
+        if offload:
+            LayerOffloader(m, dev)
+        ids = torch.randint(0, 512, (1, 96), generator=torch.Generator().manual_seed(2)).to(dev)
+        m(ids, labels=ids).loss.backward()
+        grads.append({n: p.grad.float() for n, p in m.named_parameters() if p.grad is not None})
+    assert grads[0].keys() == grads[1].keys() and grads[0]
+    for n, g in grads[0].items():
+        assert ((g - grads[1][n]).norm() <= 2.0 ** -6 * g.norm()).item(), n
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """Rows behind 2^31 values are those of a short call: codes, values, products, both gradients and the checkpoint."""
+    from axolotl_b200.train.activation_memory import make_store
+
+    T, K, N, R, n = (1 << 18) + 5, 8200, 72, 8, 9
+    assert (T - n) * K > 1 << 31
+    x = torch.empty(T, K, dtype=torch.bfloat16, device="cuda").normal_()
+    tail = x[T - n:].clone()
+    codes, scale = quantize_fp8_rows(x)
+    c, s = quantize_fp8_rows(tail)
+    assert torch.equal(codes[T - n:].view(torch.uint8), c.view(torch.uint8)) and torch.equal(scale[:, T - n:], s)
+    want = dequantize_fp8_rows(c, s)
+    assert torch.equal(dequantize_fp8_rows(codes, scale)[T - n:], want)
+    store = make_store("fp8", "cuda")
+    assert torch.equal(store.get(store.put(x))[T - n:], want)
+    t = torch.zeros(T, R, dtype=torch.bfloat16, device="cuda")
+    t[T - n:] = _make((n, R), 1, spread=0.0).cuda()
+    t64 = t[T - n:].cpu().double()
+    exact, size = t64.t() @ want.cpu().double(), t64.abs().t() @ want.cpu().double().abs()
+    assert ((fp8_adapter_grad(t, codes, scale).cpu().double() - exact).abs() <= (n + 8) * EPS32 * size).all()
+    del codes, scale
+    w, ws = quantize_fp8_weight(_make((N, K), 3, torch.float32, 0.0).cuda())
+    dy = torch.zeros(T, N, dtype=torch.bfloat16, device="cuda")
+    dy[T - n:] = _make((n, N), 4, spread=0.0).cuda()
+    xl = x.requires_grad_(True)
+    y = fp8_linear(xl, w, ws)
+    (dx,) = torch.autograd.grad(y, [xl], dy)
+    w8 = _weight8(w, ws)
+    _assert_product(y[T - n:], want.cpu().double(), w8.t())
+    _assert_product(dx[T - n:], _rows8(dy[T - n:].cpu()), w8)
+    assert not dx[:T - n].any().item()
