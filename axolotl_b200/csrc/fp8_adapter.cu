@@ -233,8 +233,8 @@ __global__ void __launch_bounds__(FA_T, 2)
 }
 
 template <int NR>
-int launch_adapter_grad(const CUtensorMap& q, const CUtensorMap& sc, const CUtensorMap& g, const Fp8AdapterParams& p, int tiles, int chunks, int splits,
-                        cudaStream_t st) {
+int launch_adapter_grad(const CUtensorMap& q, const CUtensorMap& sc, const CUtensorMap& g, const Fp8AdapterParams& p, int tiles, int chunks,
+                        int splits, cudaStream_t st) {
   auto kern = fp8_adapter_grad_kernel<NR>;
   static std::atomic<unsigned long long> allowed{0};
   if (const int rc = axb_allow_smem((const void*)kern, FA_SMEM, allowed)) return rc;

@@ -50,8 +50,7 @@ _CUDA_SIGS = {
     "axb_fp8_lora_bwd": [C.c_char_p, vp],
     # codes, ldq, scales, lds, g, ldg, out, ldo, T, K, R, accumulate, status, stream
     "axb_fp8_adapter_grad": [vp, i64, vp, i64, vp, i64, vp, i64, i32, i32, i32, i32, vp, vp],
-    # x, ldx, codes and scales (null: not kept), W, ldw, sw, sw_n, sw_k, b_mn, y, T, N, K, X2, ldx2, B2, ldb2, K2, tile, status, stream
-    "axb_fp8_linear": [vp, i64, vp, vp, i64, vp, i64, i64, i32, vp, i32, i32, i32, vp, i64, vp, i64, i32, i32, vp, vp],
+    "axb_fp8_linear_packed": [C.c_char_p],     # AxbFp8Linear
     "axb_fp8_gemm": [vp, i64, vp, i64, vp, i64, vp, i64, i64, i32, vp, i64, i32, i32, i32, vp, i64, vp, i64, i32, i32, vp, vp],
     "axb_nvfp4_dequant_batched": [vp, vp, vp, vp, i64, i64, i64, vp, vp],
     # A, lda, W, A2, lda2, W2, C, ldc, E, N, K, K2, trans_w, alpha, out_mode, bn, blk_expert, n_blocks, max_blocks, status, stream

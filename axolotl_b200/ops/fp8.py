@@ -301,6 +301,9 @@ def _few(T, N, K):
     return 0 if T > 32 and tiles > 70 else 1
 
 
+_LINEAR = struct.Struct("@9P6q6i")      # AxbFp8Linear of csrc/fp8_gemm.cu
+
+
 def _product(x, codes, scale, trans=False, a2=None, b2=None, keep=False):
     """(x8 W8^T or x8 W8 (+ a2 b2) in bf16, block of ``_pack`` of x or None) of bf16 rows x [T, K]. One call, and
     for a few tokens whose codes nobody keeps one launch."""
@@ -324,16 +327,17 @@ def _product(x, codes, scale, trans=False, a2=None, b2=None, keep=False):
     sn, sk = scale.stride()
     if trans:
         sn, sk = sk, sn
-    ext = (None, 0, None, 0, 0)
+    a, lda, b, ldb, K2 = 0, 0, 0, 0, 0
     if a2 is not None:
         a2, b2 = _operand(a2, "8-bit product"), _operand(b2, "8-bit product")
-        ext = (a2.data_ptr(), a2.stride(0), b2.data_ptr(), b2.stride(0), a2.shape[1])
-    few = 0 if trans or ext[4] % 8 else _few(T, N, K)
+        a, lda, b, ldb, K2 = a2.data_ptr(), a2.stride(0), b2.data_ptr(), b2.stride(0), a2.shape[1]
+    few = 0 if trans or K2 % 8 else _few(T, N, K)
     y = x.new_empty((T, N))
     q = x.new_empty(_packed_size(T, K), dtype=torch.uint8) if keep or few < 2 else None
-    _lib.check_rc(_lib.cuda_lib().axb_fp8_linear(
-        x.data_ptr(), ldx, None if q is None else q.data_ptr(), codes.data_ptr(), codes.stride(0), scale.data_ptr(), sn, sk, trans,
-        y.data_ptr(), T, N, K, *ext, 0 if few else _tile(T, N, K), *_lib.launch_args(device.index)), "fp8_linear")
+    status, stream = _lib.launch_args(device.index)
+    _lib.check_rc(_lib.cuda_lib().axb_fp8_linear_packed(_LINEAR.pack(
+        x.data_ptr(), 0 if q is None else q.data_ptr(), codes.data_ptr(), scale.data_ptr(), y.data_ptr(), a, b, status, stream, ldx,
+        codes.stride(0), sn, sk, lda, ldb, T, N, K, K2, 0 if few else _tile(T, N, K), trans)), "fp8_linear")
     return y, q
 
 
@@ -509,8 +513,9 @@ def _adapter_grad(t, q, ldq, s, lds, K, out):
     add = out is not None
     if not add:
         out = torch.empty((R, K), dtype=torch.float32, device=t.device)
-    _lib.check_rc(_lib.cuda_lib().axb_fp8_adapter_grad(q, ldq, s, lds, t.data_ptr(), t.stride(0), out.data_ptr(), out.stride(0) if R > 1 else K, T, K, R,
-                                                       add, _lib.status_word(t.device).data_ptr(), _lib.stream_ptr()), "fp8_adapter_grad")
+    _lib.check_rc(_lib.cuda_lib().axb_fp8_adapter_grad(
+        q, ldq, s, lds, t.data_ptr(), t.stride(0), out.data_ptr(), out.stride(0) if R > 1 else K, T, K, R, add,
+        _lib.status_word(t.device).data_ptr(), _lib.stream_ptr()), "fp8_adapter_grad")
     return out
 
 
