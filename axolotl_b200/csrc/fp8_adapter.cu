@@ -24,6 +24,7 @@ static_assert(64 * 128 * 4 <= FA_STAGES * (FA_Q + FA_G), "the partial tile reuse
 
 struct Fp8AdapterParams {
   float* out;
+  __nv_bfloat16* out16;     // instead of out: the sums rounded once
   long long ldo;
   int T, K, R, accumulate, vec;
   int* status;
@@ -209,6 +210,16 @@ __global__ void __launch_bounds__(FA_T, 2)
       a.z += u.z;
       a.w += u.w;
     }
+    if (p.out16) {
+      __nv_bfloat16* o = p.out16 + (long long)(r0 + rr) * p.ldo + k;
+      if (p.vec && k + 4 <= p.K) {
+        *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w));
+      } else {
+        const float v[4] = {a.x, a.y, a.z, a.w};
+        for (int j = 0; j < 4 && k + j < p.K; ++j) o[j] = __float2bfloat16(v[j]);
+      }
+      continue;
+    }
     float* o = p.out + (long long)(r0 + rr) * p.ldo + k;
     if (p.vec && k + 4 <= p.K) {
       if (p.accumulate) {
@@ -245,10 +256,10 @@ int launch_adapter_grad(const CUtensorMap& q, const CUtensorMap& sc, const CUten
 
 }  // namespace
 
-// q: codes [T, K], rows of ldq bytes; s: fp32 [ceil(K / 128)][lds]; g: bf16 [T, R], row stride ldg; out: fp32 [R, K], row stride ldo, added
-// to (accumulate) or written. q, s and g start on 16 bytes and have row strides of whole 16 bytes.
-extern "C" int axb_fp8_adapter_grad(const void* q, long long ldq, const float* s, long long lds, const void* g, long long ldg, float* out,
-                                    long long ldo, int T, int K, int R, int accumulate, int* status, void* stream) {
+// q: codes [T, K], rows of ldq bytes; s: fp32 [ceil(K / 128)][lds]; g: bf16 [T, R], row stride ldg; out: [R, K], row stride ldo; kind 0:
+// fp32, written, 1: fp32, added to, 2: bf16, written. q, s and g start on 16 bytes and have row strides of whole 16 bytes.
+extern "C" int axb_fp8_adapter_grad(const void* q, long long ldq, const float* s, long long lds, const void* g, long long ldg, void* out,
+                                    long long ldo, int T, int K, int R, int kind, int* status, void* stream) {
   if (K <= 0 || R <= 0) return 0;
   auto bad = [](const void* v, long long bytes) { return (reinterpret_cast<uintptr_t>(v) & 15) != 0 || (bytes & 15) != 0; };
   if (T <= 0 || bad(q, ldq) || bad(s, 4 * lds) || bad(g, 2 * ldg) || lds < T || ldo < K) return -2;
@@ -265,12 +276,13 @@ extern "C" int axb_fp8_adapter_grad(const void* q, long long ldq, const float* s
   for (const auto& z : sizes)
     if (splits == 1 && (long long)tiles * chunks <= z[1] && steps >= 2 * z[0]) splits = z[0];
   Fp8AdapterParams p = {};
-  p.out = out;
+  p.out = reinterpret_cast<float*>(out);
+  p.out16 = kind == 2 ? reinterpret_cast<__nv_bfloat16*>(out) : nullptr;
   p.ldo = ldo;
   p.T = T;
   p.K = K;
   p.R = R;
-  p.accumulate = accumulate;
+  p.accumulate = kind == 1;
   p.vec = (ldo & 3) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
   p.status = status;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);

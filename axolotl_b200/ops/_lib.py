@@ -42,15 +42,16 @@ _CUDA_SIGS = {
     "axb_moe_combine_dw": [vp, vp, vp, vp, i64, i32, i32, vp],
     "axb_nf4_dequant": [vp, vp, vp, i64, i32, vp],
     "axb_fp8_block_dequant": [vp, vp, vp, i64, i64, i32, vp],
-    # x, ldx, dtype, codes, ldq, scales, lds, rows, K, stream; back: codes, ldq, scales, lds, x, ldx, dtype, rows, K, stream
-    "axb_fp8_quantize_rows": [vp, i64, i32, vp, i64, vp, i64, i64, i32, vp],
+    "axb_fp8_pack_rows": [C.c_char_p],         # AxbFp8Rows
+    "axb_fp8_unpack_rows": [C.c_char_p],
+    # codes, ldq, scales, lds, x, ldx, dtype, rows, K, stream
     "axb_fp8_dequantize_rows": [vp, i64, vp, i64, vp, i64, i32, i64, i32, vp],
-    # A, lda, sa, ldsa, B, ldb, sb, sb_n, sb_k, b_mn, C, ldc, M, N, K, A2, lda2, B2, ldb2, K2, tile, status, stream
     "axb_fp8_lora_fwd": [C.c_char_p, vp],      # AxbFp8Lora, stream
     "axb_fp8_lora_bwd": [C.c_char_p, vp],
     # codes, ldq, scales, lds, g, ldg, out, ldo, T, K, R, accumulate, status, stream
     "axb_fp8_adapter_grad": [vp, i64, vp, i64, vp, i64, vp, i64, i32, i32, i32, i32, vp, vp],
     "axb_fp8_linear_packed": [C.c_char_p],     # AxbFp8Linear
+    # A, lda, sa, ldsa, B, ldb, sb, sb_n, sb_k, b_mn, C, ldc, M, N, K, A2, lda2, B2, ldb2, K2, tile, status, stream
     "axb_fp8_gemm": [vp, i64, vp, i64, vp, i64, vp, i64, i64, i32, vp, i64, i32, i32, i32, vp, i64, vp, i64, i32, i32, vp, vp],
     "axb_nvfp4_dequant_batched": [vp, vp, vp, vp, i64, i64, i64, vp, vp],
     # A, lda, W, A2, lda2, W2, C, ldc, E, N, K, K2, trans_w, alpha, out_mode, bn, blk_expert, n_blocks, max_blocks, status, stream

@@ -111,13 +111,15 @@ def _packed_size(T, K):
     return T * ((K + 15) & ~15) + 4 * _blocks(K) * ((T + 3) & ~3)
 
 
+_ROWS = struct.Struct("@3P2q2i")        # AxbFp8Rows of csrc/fp8_rows.cu
+
+
 def _pack(x):
     """The 8-bit rows of x [T, K] as one block of bytes: T rows of codes, K rounded up to 16 bytes, and behind them the scales, fp32
     [ceil(K / 128)][T rounded up to 4]. What the layers and the checkpoint store keep."""
     T, K = x.shape
-    ld, lds = _lead(T, K)
     if not x.is_cuda:
-        return _pack_plain(x, ld, lds)
+        return _pack_plain(x, *_lead(T, K))
     device = x.device
     if device.index != _current_device():
         with torch.cuda.device(device):
@@ -125,9 +127,8 @@ def _pack(x):
     if x.stride(1) != 1 and K > 1:
         x = x.contiguous()
     q = x.new_empty(_packed_size(T, K), dtype=torch.uint8)
-    at = q.data_ptr()
-    _lib.check_rc(_lib.cuda_lib().axb_fp8_quantize_rows(x.data_ptr(), x.stride(0), _DTYPES[x.dtype], at, ld, at + T * ld, lds, T, K,
-                                                        torch._C._cuda_getCurrentRawStream(device.index)), "fp8_quantize_rows")
+    _lib.check_rc(_lib.cuda_lib().axb_fp8_pack_rows(_ROWS.pack(x.data_ptr(), q.data_ptr(), torch._C._cuda_getCurrentRawStream(device.index),
+                                                               x.stride(0), T, K, _DTYPES[x.dtype])), "fp8_quantize_rows")
     return q
 
 
@@ -148,11 +149,9 @@ def _unpack(q, T, K, dtype):
     if device.index != _current_device():
         with torch.cuda.device(device):
             return _unpack(q, T, K, dtype)
-    ld, lds = _lead(T, K)
-    at = q.data_ptr()
     out = q.new_empty((T, K), dtype=dtype)
-    _lib.check_rc(_lib.cuda_lib().axb_fp8_dequantize_rows(at, ld, at + T * ld, lds, out.data_ptr(), K, _DTYPES[dtype], T, K,
-                                                          torch._C._cuda_getCurrentRawStream(device.index)), "fp8_dequantize_rows")
+    _lib.check_rc(_lib.cuda_lib().axb_fp8_unpack_rows(_ROWS.pack(out.data_ptr(), q.data_ptr(), torch._C._cuda_getCurrentRawStream(device.index),
+                                                                 K, T, K, _DTYPES[dtype])), "fp8_dequantize_rows")
     return out
 
 
@@ -373,16 +372,16 @@ class _Fp8LinearFn(torch.autograd.Function):
         return dx, None, None, dbias
 
 
-_LORA = struct.Struct("@17P8q8if")      # AxbFp8Lora of csrc/fp8_lora.cu
+_LORA = struct.Struct("@16P8q9if")      # AxbFp8Lora of csrc/fp8_lora.cu
 
 
-def _lora_call(entry, x, codes, scale, A16, B16, scaling, sizes, q, xa, y, qx=0, t32=0, t=0, dA=0, dB=0, dA16=0, dB16=0, blocks=0,
-               ldda=0, lddb=0, n_blocks=0, add_dA=False, add_dB=False):
+def _lora_call(entry, x, codes, scale, A16, B16, scaling, sizes, q, xa, y, qx=0, t32=0, t=0, dA=0, dB=0, dB16=0, blocks=0,
+               ldda=0, lddb=0, n_blocks=0, add_dA=False, add_dB=False, dA_bf16=False):
     """One call of csrc/fp8_lora.cu; ``q`` .. ``blocks`` are addresses, ``sizes`` is (T, N, K, R, tile)."""
     status, stream = _lib.launch_args(x.device.index)
-    args = _LORA.pack(x.data_ptr(), q, codes.data_ptr(), scale.data_ptr(), A16.data_ptr(), B16.data_ptr(), xa, y, qx, t32, t, dA, dB, dA16, dB16,
+    args = _LORA.pack(x.data_ptr(), q, codes.data_ptr(), scale.data_ptr(), A16.data_ptr(), B16.data_ptr(), xa, y, qx, t32, t, dA, dB, dB16,
                       blocks, status, x.stride(0), codes.stride(0), *scale.stride(), A16.stride(0), B16.stride(0), ldda, lddb, *sizes, n_blocks,
-                      add_dA, add_dB, scaling)
+                      add_dA, add_dB, dA_bf16, scaling)
     _lib.check_rc(entry(args, stream), "fp8_lora")
 
 
@@ -438,10 +437,10 @@ class _Fp8LoRALinearFn(torch.autograd.Function):
         if (need[4] and USE_FUSED_DY and T and R <= 64 and R % 8 == 0 and len(ctx.blocks) <= 8 and xa.is_contiguous()
                 and all(map(_operand16, (dy, A16, B16, xa)))):
             # one pass over dy for t and dB, the product and dA behind it: one call. Scratch: t in fp32, dB in fp32 (where its place is
-            # elsewhere it is not there), t in bf16, dA in fp32, the rows of dy in 8 bits
+            # elsewhere it is not there), t in bf16, the rows of dy in 8 bits
             n, tA, tB = T * R, getattr(A, "_axb_grad", None), getattr(B, "_axb_grad", None)
             low = [w is None and p.dtype == torch.bfloat16 for w, p in ((tA, A), (tB, B))]
-            at = [4 * n, 4 * N * R if low[1] else 0, 2 * n, 4 * R * K if need[3] and low[0] else 0]
+            at = [4 * n, 4 * N * R if low[1] else 0, 2 * n]
             work = dy.new_empty(sum(at) + (_packed_size(T, N) if need[0] else 0), dtype=torch.uint8)
             p = work.data_ptr()
             args = dict(t32=p, t=p + at[0] + at[1])
@@ -455,7 +454,7 @@ class _Fp8LoRALinearFn(torch.autograd.Function):
                 args.update(dB=dB.data_ptr(), lddb=dB.stride(0), add_dB=tB is not None)
             if need[3] and low[0]:
                 dA = dy.new_empty((R, K))
-                args.update(qx=q.data_ptr(), dA=p + sum(at[:3]), dA16=dA.data_ptr(), ldda=K)
+                args.update(qx=q.data_ptr(), dA=dA.data_ptr(), ldda=K, dA_bf16=True)
             elif need[3]:
                 dA = tA if tA is not None else dy.new_empty((R, K), dtype=torch.float32)
                 args.update(qx=q.data_ptr(), dA=dA.data_ptr(), ldda=dA.stride(0), add_dA=tA is not None)
