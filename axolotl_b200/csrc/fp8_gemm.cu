@@ -418,7 +418,7 @@ extern "C" int axb_fp8_gemm(const void* A, long long lda, const float* sa, long 
   return fp8_gemm_entry(A, lda, sa, ldsa, B, ldb, sb, sb_n, sb_k, b_mn, C, ldc, M, N, K, A2, lda2, B2, ldb2, K2, tile, false, status, stream);
 }
 
-// y = x8 W8^T (b_mn: x8 W8) (+ X2 B2) of bf16 rows x [T, K] in one call. q: where the 8-bit rows go, T rows of K rounded up to 16 bytes and
+// y = x8 W8^T (b_mn: x8 W8) (+ X2 B2) of bf16 rows x [T, K] (null: the launch before this one has put them into q) in one call. q: where the 8-bit rows go, T rows of K rounded up to 16 bytes and
 // behind them the scales, fp32 [ceil(K / 128)][T rounded up to 4]; null: they are not kept (at most 64 rows, forward). The other
 // arguments are those of axb_fp8_gemm.
 extern "C" int axb_fp8_linear(const void* x, long long ldx, void* q, const void* W, long long ldw, const float* sw, long long sw_n,
@@ -430,7 +430,7 @@ extern "C" int axb_fp8_linear(const void* x, long long ldx, void* q, const void*
   }
   const long long ldq = (K + 15ll) & ~15ll, lds = (T + 3ll) & ~3ll;
   float* s = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(q) + ldq * T);
-  int rc = axb_fp8_quantize_rows(x, ldx, 0, q, ldq, s, lds, T, K, stream);
+  const int rc = x ? axb_fp8_quantize_rows(x, ldx, 0, q, ldq, s, lds, T, K, stream) : 0;
   if (rc) return rc;
   if (!b_mn && tile == 0)
     return axb_fp8_skinny(x, ldx, q, ldq, s, lds, W, ldw, sw, sw_n, sw_k, y, N, T, N, K, X2, ldx2, B2, ldb2, K2, status, stream);

@@ -10,6 +10,8 @@ extern "C" int axb_gemm_skinny(const void* P, long long ldp, const void* S, long
 extern "C" int axb_lora_bwd_dy(const void* dy, long long ld_dy, const void* B, long long ld_b, const void* xa, long long ld_xa, float* t32,
                                float* dB32, long long ldb32, int T, int N, int R, const int* blocks, int n_lora_blocks, int* status,
                                void* stream);
+extern "C" int axb_fp8_quantize_low(const void* x, long long ldx, const void* A, long long lda, void* q, long long ldq, float* s, long long lds,
+                                    void* xa, long long ldxa, int T, int K, int R, float scale, int* status, void* stream);
 extern "C" int axb_fp8_linear(const void* x, long long ldx, void* q, const void* W, long long ldw, const float* sw, long long sw_n,
                               long long sw_k, int b_mn, void* y, int T, int N, int K, const void* X2, long long ldx2, const void* B2,
                               long long ldb2, int K2, int tile, int* status, void* stream);
@@ -58,9 +60,17 @@ static_assert(sizeof(AxbFp8Lora) == 16 * 8 + 8 * 8 + 10 * 4, "no gaps");
 
 extern "C" int axb_fp8_lora_fwd(const AxbFp8Lora* l, void* stream) {
   if (l->T <= 0) return 0;
-  const int rc = axb_gemm_skinny(l->x, l->ldx, l->A, l->lda, l->xa, l->R, l->T, l->R, l->K, nullptr, 0, nullptr, 0, 0, l->scaling, nullptr,
-                                 1, 0, 0, 0.f, 1, 0, 0, l->status, stream);
-  return rc ? rc : axb_fp8_linear(l->x, l->ldx, l->q, l->W, l->ldw, l->sw, l->sw_n, l->sw_k, 0, l->y, l->T, l->N, l->K, l->xa, l->R, l->B,
+  const bool one = l->q && l->R <= 64;         // xa and the 8-bit rows in one pass over x
+  int rc;
+  if (one) {
+    const long long ldq = (l->K + 15ll) & ~15ll;
+    rc = axb_fp8_quantize_low(l->x, l->ldx, l->A, l->lda, l->q, ldq, reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(l->q) + ldq * l->T),
+                              (l->T + 3ll) & ~3ll, l->xa, l->R, l->T, l->K, l->R, l->scaling, l->status, stream);
+  } else {
+    rc = axb_gemm_skinny(l->x, l->ldx, l->A, l->lda, l->xa, l->R, l->T, l->R, l->K, nullptr, 0, nullptr, 0, 0, l->scaling, nullptr, 1, 0, 0,
+                         0.f, 1, 0, 0, l->status, stream);
+  }
+  return rc ? rc : axb_fp8_linear(one ? nullptr : l->x, l->ldx, l->q, l->W, l->ldw, l->sw, l->sw_n, l->sw_k, 0, l->y, l->T, l->N, l->K, l->xa, l->R, l->B,
                                   l->ldb, l->R, l->tile, l->status, stream);
 }
 

@@ -10,77 +10,12 @@
 //
 // Bound: HBM, 2 bytes read and 1 written per value (and the other way round); a warp takes 1024 columns of a row with all its
 // 16-byte loads in flight, eight neighbouring rows share a block so that their 4-byte scales fill whole sectors.
-#include <cuda_fp16.h>
-#include <cuda_fp8.h>
-
-#include "axb_common.cuh"
+#include "fp8_rows.cuh"
 
 namespace {
 
 constexpr int Q_ROWS = 8;          // rows (warps) of a block
 constexpr int Q_COLS = 1024;       // columns of a warp: four vectors of eight values for every lane
-
-template <typename T>
-AXB_DEVICE float to_f32(T v);
-template <>
-AXB_DEVICE float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <>
-AXB_DEVICE float to_f32(__half v) { return __half2float(v); }
-template <>
-AXB_DEVICE float to_f32(float v) { return v; }
-template <typename T>
-AXB_DEVICE T from_f32(float v);
-template <>
-AXB_DEVICE __nv_bfloat16 from_f32(float v) { return __float2bfloat16(v); }
-template <>
-AXB_DEVICE __half from_f32(float v) { return __float2half(v); }
-template <>
-AXB_DEVICE float from_f32(float v) { return v; }
-
-// Eight values of a row as they are stored. The largest magnitude is taken in the stored type, two values an instruction: with every
-// value widened first the kernel was bound by its arithmetic (32768 x 4096 in bf16: 112 us, 70 us like this, 5.8 TB/s).
-template <typename T>
-struct Eight {
-  uint4 raw[sizeof(T) / 2];
-  AXB_DEVICE void load(const T* p) {
-#pragma unroll
-    for (int h = 0; h < (int)sizeof(T) / 2; ++h) raw[h] = __ldg(reinterpret_cast<const uint4*>(p) + h);
-  }
-  AXB_DEVICE void load_some(const T* p, int n) {     // the first n, zeros behind them
-#pragma unroll
-    for (int h = 0; h < (int)sizeof(T) / 2; ++h) raw[h] = make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j < n) reinterpret_cast<T*>(raw)[j] = p[j];
-  }
-  AXB_DEVICE float at(int j) const { return to_f32<T>(reinterpret_cast<const T*>(raw)[j]); }
-  AXB_DEVICE float top() const;                      // of those that are not NaN (NaN: there is none)
-};
-template <>
-AXB_DEVICE float Eight<__nv_bfloat16>::top() const {
-  const __nv_bfloat162* v = reinterpret_cast<const __nv_bfloat162*>(raw);
-  const __nv_bfloat162 m = __hmax2(__hmax2(__habs2(v[0]), __habs2(v[1])), __hmax2(__habs2(v[2]), __habs2(v[3])));
-  return __bfloat162float(__hmax(m.x, m.y));
-}
-template <>
-AXB_DEVICE float Eight<__half>::top() const {
-  const __half2* v = reinterpret_cast<const __half2*>(raw);
-  const __half2 m = __hmax2(__hmax2(__habs2(v[0]), __habs2(v[1])), __hmax2(__habs2(v[2]), __habs2(v[3])));
-  return __half2float(__hmax(__low2half(m), __high2half(m)));
-}
-template <>
-AXB_DEVICE float Eight<float>::top() const {
-  float m = fabsf(at(0));
-#pragma unroll
-  for (int j = 1; j < 8; ++j) m = fmaxf(m, fabsf(at(j)));
-  return m;
-}
-
-AXB_DEVICE float group_max(float m) {     // over the 16 lanes that hold a block of 128 columns
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  return m;
-}
 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(Q_ROWS * 32)
@@ -99,41 +34,15 @@ __global__ void __launch_bounds__(Q_ROWS * 32)
     if (VEC && c + 8 <= K) v[i].load(xr + c);
     else v[i].load_some(xr + c, K - c);
   }
+  uint2 w[4];
+  int e[4];
+  codes4(v, w, e);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int c = c0 + i * 256 + lane * 8;
-    if (c0 + i * 256 >= K) break;                // the whole warp
-    float top = group_max(v[i].top());
-    float f[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = v[i].at(j);
-    if (__any_sync(0xffffffffu, !(top <= 3.402823466e38f))) {
-      // an infinity, or nothing but NaN: the maximum of the finite values, and NaN for the others
-      float m = 0.f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (fabsf(f[j]) <= 3.402823466e38f) m = fmaxf(m, fabsf(f[j]));
-        else f[j] = __uint_as_float(0x7FC00000u);
-      }
-      top = group_max(m);
-    }
-    const int e = fp8_scale_exponent(top);
-    const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
-    if (e >= 247) {                              // scale 2^120: the code 256 would stand for 2^128
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (fabsf(f[j]) > 240.f * 0x1p120f) f[j] = copysignf(240.f * 0x1p120f, f[j]);
-    }
-    uint32_t w[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(f[4 * h] * inv, f[4 * h + 1] * inv), __NV_SATFINITE, __NV_E4M3);
-      const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(f[4 * h + 2] * inv, f[4 * h + 3] * inv), __NV_SATFINITE, __NV_E4M3);
-      w[h] = lo | (hi << 16);
-    }
     // rows of codes start on 16 bytes and are padded to them, so a vector that begins inside a row ends inside its padding
-    if (c < K) *reinterpret_cast<uint2*>(q + row * ldq + c) = make_uint2(w[0], w[1]);
-    if ((lane & 15) == 0 && c < K) s[(long long)(c >> 7) * lds + row] = __uint_as_float((uint32_t)e << 23);
+    if (c < K) *reinterpret_cast<uint2*>(q + row * ldq + c) = w[i];
+    if ((lane & 15) == 0 && c < K) s[(long long)(c >> 7) * lds + row] = __uint_as_float((uint32_t)e[i] << 23);
   }
 }
 

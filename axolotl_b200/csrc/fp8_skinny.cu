@@ -211,7 +211,8 @@ __global__ void __launch_bounds__(FS_T, 2)
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(&tempty[buf]);
-        if (!FUSED) mbar_arrive(&freed[i % FS_RING]);
+        // a block late: this one's scales may still be on their way to the sums, which nothing orders before the arrival
+        if (!FUSED && i > 0) mbar_arrive(&freed[(i - 1) % FS_RING]);
       }
       if (++buf == C::BUFS) {
         buf = 0;

@@ -950,14 +950,17 @@ def test_second_derivatives_are_refused(dev):
 
 @pytest.mark.parametrize("dev", DEVICES)
 def test_layer_offloading_of_8_bit_layers(dev):
-    """Frozen layers that live in host memory give the gradients of resident ones."""
+    """Frozen layers that live in host memory give the loss and the gradients of resident ones. On the device the sums of t are atomic: t may
+    round to its neighbour (2^-8). A value that is off by d of itself takes another code with a probability of d / step, and is off by a
+    step (at most 2^-3) then: sqrt(2^-8 2^-3) = 2.2 % rms at each quantisation of a gradient. It passes four of them a layer, 12 in all:
+    sqrt(12) 2.2 % = 8 %."""
     from axolotl_b200.models.config import preset
     from axolotl_b200.models.lora import LoraSpec, inject_lora, quantize_base_fp8_
     from axolotl_b200.models.transformer import CausalLM
     from axolotl_b200.train.activation_memory import LayerOffloader
 
     cfg = preset("tiny-llama", num_hidden_layers=3, vocab_size=512)
-    grads = []
+    grads, losses = [], []
     for offload in (False, True):
         m = CausalLM(cfg, dtype=torch.bfloat16 if dev == "cuda" else torch.float32, device=dev).init_weights(0)
         quantize_base_fp8_(m)
@@ -973,11 +976,13 @@ def test_layer_offloading_of_8_bit_layers(dev):
         if offload:
             LayerOffloader(m, dev)
         ids = torch.randint(0, 512, (1, 96), generator=torch.Generator().manual_seed(2)).to(dev)
-        m(ids, labels=ids).loss.backward()
+        loss = m(ids, labels=ids).loss
+        loss.backward()
+        losses.append(loss.item())
         grads.append({n: p.grad.float() for n, p in m.named_parameters() if p.grad is not None})
-    assert grads[0].keys() == grads[1].keys() and grads[0]
+    assert losses[0] == losses[1] and grads[0].keys() == grads[1].keys() and grads[0]
     for n, g in grads[0].items():
-        assert ((g - grads[1][n]).norm() <= 2.0 ** -6 * g.norm()).item(), n
+        assert ((g - grads[1][n]).norm() <= 0.08 * g.norm()).item(), n
 
 
 @pytest.mark.gpu
