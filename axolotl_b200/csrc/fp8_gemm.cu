@@ -418,9 +418,9 @@ extern "C" int axb_fp8_gemm(const void* A, long long lda, const float* sa, long 
   return fp8_gemm_entry(A, lda, sa, ldsa, B, ldb, sb, sb_n, sb_k, b_mn, C, ldc, M, N, K, A2, lda2, B2, ldb2, K2, tile, false, status, stream);
 }
 
-// y = x8 W8^T (b_mn: x8 W8) (+ X2 B2) of bf16 rows x [T, K] (null: the launch before this one has put them into q) in one call. q: where the 8-bit rows go, T rows of K rounded up to 16 bytes and
-// behind them the scales, fp32 [ceil(K / 128)][T rounded up to 4]; null: they are not kept (at most 64 rows, forward). The other
-// arguments are those of axb_fp8_gemm.
+// y = x8 W8^T (b_mn: x8 W8) (+ X2 B2) of bf16 rows x [T, K] in one call. q: where the 8-bit rows go, T rows of K rounded up to 16 bytes and
+// behind them the scales, fp32 [ceil(K / 128)][T rounded up to 4]; null: they are not kept (at most 64 rows, forward). x null: the launch
+// before this one has put them there. The other arguments are those of axb_fp8_gemm.
 extern "C" int axb_fp8_linear(const void* x, long long ldx, void* q, const void* W, long long ldw, const float* sw, long long sw_n,
                               long long sw_k, int b_mn, void* y, int T, int N, int K, const void* X2, long long ldx2, const void* B2,
                               long long ldb2, int K2, int tile, int* status, void* stream) {

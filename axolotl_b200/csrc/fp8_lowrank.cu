@@ -4,7 +4,8 @@
 // Bound: HBM, 2 bytes read and 1 written per value. A step is 128 rows x 128 columns: bulk copies bring it in as the K-major 128-row
 // operand of tcgen05.mma (A's block is the other one, N = 16 .. 64), and eight warps read the same tile back for the codes, a
 // conflict-free 16 bytes a lane. They hand the stage back as soon as the values are in registers. K is split over a cluster, whose partial
-// products meet in distributed shared memory in a fixed order.
+// products meet in distributed shared memory in a fixed order. What it measures: 8192 x 14336, rank 16, 67 us, 5.9 TB/s and some 7 us of
+// start, join and end; 960 x 4096 12.3 us. No faster: eight quantising warps of eight passes, five stages for one CTA of an SM.
 #include "fp8_rows.cuh"
 
 namespace {
@@ -200,7 +201,21 @@ int launch_fp8_quantize_low(const CUtensorMap& x, const CUtensorMap& a, const Fp
   return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }
 
+// CTAs of a tile: eight while every cluster gets SMs to itself (14 of them), four elsewhere; two blocks at least to each CTA
+int fp8_low_splits(int tiles, int nk) { return tiles <= 14 && nk >= 16 ? 8 : nk >= 8 ? 4 : nk >= 4 ? 2 : 1; }
+
 }  // namespace
+
+// Whether one pass beats the quantiser and a low-rank product of its own (both over x). One pass: 1.03 us for each block of a CTA and each
+// CTA that an SM holds (148 SMs take 35 clusters of four), and 8.2 us around them. Two: 11 us and 0.65 for a million values, over 128 rows
+// (up to there the product is not split: 23 us at 4096 columns, 55 at 14336). Microseconds, one / two, rank 16: 960 x 4096 12.3 / 12.4,
+// 960 x 14336 22.6 / 19.6, 2000 x 14336 35.7 / 28.7, 4000 x 14336 41.0 / 54.5, 5000 x 4096 23.9 / 20.6, 8192 x 14336 67 / 102.
+extern "C" int axb_fp8_low_pays(int T, int K) {
+  if (T <= 128) return 1;
+  const int tiles = (T + 127) / 128, nk = (K + 127) / 128, splits = fp8_low_splits(tiles, nk);
+  const double load = splits == 8 || tiles <= 35 ? 1. : tiles <= 70 ? 2. : tiles / 35.;
+  return 8.2 + 1.03 * load * ((nk + splits - 1) / splits) <= 11. + 0.65e-6 * T * K;
+}
 
 // x: bf16 [T, K], row stride ldx; A: bf16 [R, K], row stride lda, R <= 64 and a multiple of 8; q: codes, rows of ldq bytes; s: fp32 [ceil(K /
 // 128)][lds]; xa: bf16 [T, R], row stride ldxa. x, A, q and xa start on 16 bytes and have row strides of whole 16 bytes.
@@ -226,9 +241,7 @@ extern "C" int axb_fp8_quantize_low(const void* x, long long ldx, const void* A,
   p.R = R;
   p.scale = scale;
   p.status = status;
-  const int tiles = (T + 127) / 128, nk = (K + 127) / 128;
-  // K of a tile over the largest cluster that leaves two blocks to each CTA, up to eight where few tiles leave SMs idle and four elsewhere
-  const int splits = tiles <= 18 && nk >= 16 ? 8 : nk >= 8 ? 4 : nk >= 4 ? 2 : 1;
+  const int tiles = (T + 127) / 128, splits = fp8_low_splits(tiles, (K + 127) / 128);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (NR == 16) return launch_fp8_quantize_low<16>(tX, tA, p, tiles, splits, st);
   if (NR == 32) return launch_fp8_quantize_low<32>(tX, tA, p, tiles, splits, st);

@@ -1017,3 +1017,33 @@ def test_offsets_past_32_bits():
     _assert_product(y[T - n:], want.cpu().double(), w8.t())
     _assert_product(dx[T - n:], _rows8(dy[T - n:].cpu()), w8)
     assert not dx[:T - n].any().item()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,K,R", [(1, 264, 8), (65, 8, 16), (129, 200, 24), (300, 904, 40), (960, 4096, 16), (2053, 2056, 32), (4100, 4104, 16),
+                                   (4100, 4104, 64), (9000, 1288, 16)])
+def test_codes_and_low_rank_product_in_one_pass(T, K, R):
+    """What the forward pass keeps: the codes are those of the quantiser, bit for bit and every time, and s x A^T is that of the values
+    before they were coded; rows with NaN and infinities stay to themselves."""
+    x = _make((T, K), T + K, spread=0.5)
+    if T > 64:
+        x[7, 3], x[64, 5], x[T - 1, K - 1] = float("nan"), float("inf"), float("-inf")
+    A, N = _make((R, K), 4, spread=0.0) * K ** -0.5, 40
+    B = torch.zeros(N, R, dtype=torch.bfloat16, device="cuda")
+    w, ws = quantize_fp8_weight(_make((N, K), 3, torch.float32, 0.0).cuda())
+    xd, Al, Ad = x.cuda(), A.cuda().requires_grad_(True), A.cuda()
+    codes, scale = quantize_fp8_rows(xd)
+    from axolotl_b200.ops.fp8 import _unpacked
+
+    for i in range(8):
+        y = fp8_lora_linear(xd, w, ws, Al, B, Ad, B, 0.5, ((0, N, 0, R),))
+        q, xa = y.grad_fn.saved_tensors[0], y.grad_fn.saved_tensors[7]
+        c, s = _unpacked(q, T, K)
+        assert torch.equal(c.view(torch.uint8), codes.view(torch.uint8)) and torch.equal(s, scale), i
+        first = xa if i == 0 else first
+        assert torch.equal(xa.view(torch.int16), first.view(torch.int16)), i
+    want, size = 0.5 * xd.double() @ Ad.double().t(), 0.5 * xd.double().abs() @ Ad.double().abs().t()
+    ok = torch.isfinite(xd).all(1)
+    diff = (xa.double() - want).abs()
+    assert (diff <= BF16 * want.abs() + (K + 8) * EPS32 * size * (1 + BF16) + 1e-38)[ok].all()
+    assert not torch.isfinite(xa[~ok]).any()
