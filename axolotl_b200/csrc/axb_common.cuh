@@ -598,6 +598,16 @@ inline int axb_allow_smem(const void* kern, int bytes, std::atomic<unsigned long
   if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
   return (int)e;
 }
+// CTAs that share the long axis of a tile as one cluster: the largest size of which the chip holds a cluster for every tile at once with two
+// CTAs on an SM (counted: 33 clusters of eight, 44 of six, 50 of five, 70 of four, 92 of three, 148 of two), two steps at least to a CTA.
+// Microseconds of 8192 rows in fp8_adapter.cu, with the next smaller power of two / with this: 40 tiles 32.8 / 24.8, 50 32.8 / 28.7, 88
+// 57.4 / 41.5; one tile more than a size holds costs as much again (96 tiles in threes 62).
+inline int axb_cluster_split(long long tiles, int steps) {
+  const int sizes[][2] = {{8, 33}, {6, 44}, {5, 50}, {4, 70}, {3, 92}, {2, 148}};
+  for (const auto& s : sizes)
+    if (tiles <= s[1] && steps >= 2 * s[0]) return s[0];
+  return 1;
+}
 // Launch attributes of a clustered and / or dependent launch (cluster = CTAs per cluster along x, 0 = none).
 struct AxbLaunch {
   cudaLaunchConfig_t cfg = {};

@@ -270,11 +270,7 @@ extern "C" int axb_fp8_adapter_grad(const void* q, long long ldq, const float* s
   if (rc) return -100 - rc;
   const int tiles = (K + 127) / 128, chunks = (R + 63) / 64, steps = (T + FA_ROWS - 1) / FA_ROWS;
   if (chunks > 65535) return -2;
-  // rows of a tile over the largest cluster of which the chip holds one per tile at once (33 of eight, 70 of four, 148 of two)
-  const int sizes[][2] = {{8, 33}, {4, 70}, {2, 148}};
-  int splits = 1;
-  for (const auto& z : sizes)
-    if (splits == 1 && (long long)tiles * chunks <= z[1] && steps >= 2 * z[0]) splits = z[0];
+  const int splits = axb_cluster_split((long long)tiles * chunks, steps);
   Fp8AdapterParams p = {};
   p.out = reinterpret_cast<float*>(out);
   p.out16 = kind == 2 ? reinterpret_cast<__nv_bfloat16*>(out) : nullptr;

@@ -370,15 +370,6 @@ int launch_fp8_skinny(const CUtensorMap (&m)[4], const Fp8SkinnyParams& p, int t
   return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }
 
-// CTAs per tile: the largest cluster of which the chip holds one per tile at once (33 clusters of eight, 70 of four, 148 of two), at
-// least two blocks for each CTA
-int fp8_skinny_splits(int tiles, int nk) {
-  const int sizes[][2] = {{8, 33}, {4, 70}, {2, 148}};
-  for (const auto& s : sizes)
-    if (tiles <= s[1] && nk >= 2 * s[0]) return s[0];
-  return 1;
-}
-
 }  // namespace
 
 // See the head of this file. x: bf16 [T, K], T <= 64; q (null: the rows are quantised by the kernel): their codes, rows of ldq bytes, and
@@ -417,7 +408,7 @@ extern "C" int axb_fp8_skinny(const void* x, long long ldx, const void* q, long 
   p.K2 = K2 > 0 ? K2 : 0;
   p.vec = !bad(x, 2 * ldx);
   p.status = status;
-  const int tiles = (N + 127) / 128, nk = (K + 127) / 128 + (p.K2 + 63) / 64, splits = fp8_skinny_splits(tiles, nk);
+  const int tiles = (N + 127) / 128, nk = (K + 127) / 128 + (p.K2 + 63) / 64, splits = axb_cluster_split(tiles, nk);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (q) {
     if (NT == 16) return launch_fp8_skinny<16, false>(m, p, tiles, splits, st);

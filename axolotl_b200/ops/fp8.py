@@ -293,8 +293,9 @@ def _few(T, N, K):
     if T > 64:
         return 0
     tiles, nk = (N + 127) >> 7, (K + 127) >> 7
-    # CTAs of a tile: fp8_skinny_splits
-    splits = 8 if tiles <= 33 and nk >= 16 else 4 if tiles <= 70 and nk >= 8 else 2 if tiles <= 148 and nk >= 4 else 1
+    # axb_cluster_split of csrc/axb_common.cuh
+    splits = (8 if tiles <= 33 and nk >= 16 else 6 if tiles <= 44 and nk >= 12 else 5 if tiles <= 50 and nk >= 10 else
+              4 if tiles <= 70 and nk >= 8 else 3 if tiles <= 92 and nk >= 6 else 2 if tiles <= 148 and nk >= 4 else 1)
     if -(-nk // splits) * (1 if T <= 16 else 2 if T <= 32 else 4) <= 16:
         return 2
     return 0 if T > 32 and tiles > 70 else 1

@@ -1047,3 +1047,22 @@ def test_codes_and_low_rank_product_in_one_pass(T, K, R):
     diff = (xa.double() - want).abs()
     assert (diff <= BF16 * want.abs() + (K + 8) * EPS32 * size * (1 + BF16) + 1e-38)[ok].all()
     assert not torch.isfinite(xa[~ok]).any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,N,K", [(5, 4616, 1544), (20, 6280, 1288), (33, 9224, 776), (64, 4616, 4104), (64, 6280, 3336), (50, 9224, 2056)])
+def test_few_tokens_over_clusters_of_three_five_and_six(T, N, K):
+    x = _make((T, K), T + K, spread=0.5)
+    w, ws = quantize_fp8_weight(_make((N, K), 3, torch.float32, 0.0).cuda())
+    _assert_product(fp8_linear(x.cuda(), w, ws), _rows8(x), _weight8(w, ws).t())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,K", [(800, 4616), (1300, 5512), (700, 6280), (400, 9224), (390, 11656)])
+def test_adapter_gradient_over_clusters_of_three_five_and_six(T, K):
+    x, t = _make((T, K), T + K, spread=0.5), _make((T, 16), 2, spread=0.5)
+    codes, scale = quantize_fp8_rows(x.cuda())
+    want, size = t.double().t() @ _rows8(x), t.double().abs().t() @ _rows8(x).abs()
+    got = fp8_adapter_grad(t.cuda(), codes, scale)
+    assert ((got.cpu().double() - want).abs() <= (T + 8) * EPS32 * size * (1 + 2.0 ** -20)).all()
+    assert torch.equal(got, fp8_adapter_grad(t.cuda(), codes, scale))
