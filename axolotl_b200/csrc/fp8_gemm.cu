@@ -9,9 +9,9 @@
 // The scales change every 128 columns of K, so an accumulator cannot stay in TMEM: the four MMAs of a block start a new one, and
 // eight epilogue warps add it, times its scale, to fp32 sums in registers while the tensor cores work on the next. A thread owns a
 // row: one scale for all its columns of a weight block.
-// Tiles: 256 x 256 by a CTA pair, 128 x 128 by one CTA. In the pair a block is two products of 128 columns with two accumulators each
-// (columns of both CTAs' B rows: 64 h .. of either), one for each half of the epilogue warps, so that one half drains its
-// accumulator while the other's is computed.
+// Tiles: 256 x 256 or 256 x 128 by a CTA pair, 128 x 128 by one CTA (ops/fp8.py says when). In the largest a block is two products of 128
+// columns with two accumulators each (columns of both CTAs' B rows: 64 h .. of either), one for each half of the epilogue warps, so
+// that one half drains its accumulator while the other's is computed; in the others one product with four.
 //
 // Bound: the epilogue's turn of a block. TMEM reads (110 cycles) and multiply-adds (250, half a packed one a cycle and partition) follow
 // one another in a warp behind some 500 cycles of waits, arrivals and scale loads, against 512 of the tensor cores and as many of the
@@ -23,8 +23,8 @@
 
 extern "C" int axb_fp8_quantize_rows(const void* x, long long ldx, int dtype, void* q, long long ldq, float* s, long long lds,
                                      long long rows, int K, void* stream);
-extern "C" int axb_fp8_skinny(const void* x, long long ldx, const void* q, long long ldq, const float* sx, long long ldsx, const void* W, long long ldw,
-                              const float* sw, long long sw_n, long long sw_k, void* y, long long ldy, int T, int N, int K, const void* X2,
+extern "C" int axb_fp8_skinny(const void* x, long long ldx, const void* q, long long ldq, const float* sx, long long ldsx, const void* W,
+                              long long ldw, const float* sw, long long sw_n, long long sw_k, void* y, long long ldy, int T, int N, int K, const void* X2,
                               long long ldx2, const void* B2, long long ldb2, int K2, int* status, void* stream);
 
 namespace {
@@ -32,10 +32,9 @@ namespace {
 constexpr int G_THREADS = 320;                 // TMA, MMA, eight epilogue warps
 constexpr int G_BK = 128;                      // bytes of a K block: 128 codes, or 64 bf16 of the extension
 constexpr int G_OP = 128 * G_BK;               // an operand tile of a CTA
-constexpr int G_STAGE = 2 * G_OP;
-constexpr int G_STAGES = 6;
+constexpr int G_RING = 6 * 2 * G_OP;
 constexpr int G_EPI = 8 * 4096;                // per epilogue warp: 32 rows x 64 bf16
-constexpr int G_SMEM = G_STAGES * G_STAGE + G_EPI + 1024 + 256;
+constexpr int G_SMEM = G_RING + G_EPI + 1024 + 256;
 
 struct Fp8GemmParams {
   const float* sa;
@@ -78,19 +77,20 @@ AXB_DEVICE void fp8_tile(int tile, int num_m, int num_n, int group_m, int& m_blk
   n_blk = in / rows;
 }
 
-template <bool PAIR, bool B_MN>
+template <int CTAS, int SETS, bool B_MN>
 __global__ void __launch_bounds__(G_THREADS, 1)
     fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ CUtensorMap tmA2, const __grid_constant__ CUtensorMap tmB2,
                     const __grid_constant__ CUtensorMap tmC, const Fp8GemmParams p) {
-  constexpr int CTAS = PAIR ? 2 : 1;
-  constexpr int TILE = 128 * CTAS;             // rows and columns of a tile
-  constexpr int SETS = CTAS;                   // products of 128 columns a block
-  constexpr int BUFS = 4 / SETS;               // accumulators of each
+  constexpr bool PAIR = CTAS == 2;
+  constexpr int TILE_M = 128 * CTAS, TILE_N = 128 * SETS;       // SETS products of 128 columns a block
+  constexpr int BN = TILE_N / CTAS;            // columns whose B a CTA brings in
+  constexpr int G_STAGE = G_OP + BN * G_BK, G_STAGES = G_RING / G_STAGE;
+  constexpr int BUFS = 4 / SETS;               // accumulators of each product
   constexpr int GROUPS = SETS;                 // groups of 64 columns that an epilogue warp owns
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint8_t* sEpi = smem + G_STAGES * G_STAGE;
+  uint8_t* sEpi = smem + G_RING;
   uint64_t* full = reinterpret_cast<uint64_t*>(sEpi + G_EPI);   // leader's: both CTAs' loads of the stage
   uint64_t* empty = full + G_STAGES;                            // one per CTA
   uint64_t* tfull = empty + G_STAGES;                           // [set][buffer], one per CTA
@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(G_THREADS, 1)
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
   const int rank = PAIR ? (int)cluster_ctarank() : 0;
   const int worker = blockIdx.x / CTAS, workers = gridDim.x / CTAS;
-  const int num_m = (p.M + TILE - 1) / TILE, num_n = (p.N + TILE - 1) / TILE, tiles = num_m * num_n;
+  const int num_m = (p.M + TILE_M - 1) / TILE_M, num_n = (p.N + TILE_N - 1) / TILE_N, tiles = num_m * num_n;
   const int nk_main = (p.K + 127) / 128, nk = nk_main + (p.K2 + 63) / 64;
 
   if (threadIdx.x == 0) {
@@ -109,7 +109,7 @@ __global__ void __launch_bounds__(G_THREADS, 1)
     }
     for (int s = 0; s < 4; ++s) {
       mbar_init(&tfull[s], 1);
-      mbar_init(&tempty[s], 8);
+      mbar_init(&tempty[s], 8 * CTAS / SETS);
     }
     mbar_fence_init();
     tma_prefetch_desc(&tmA);
@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(G_THREADS, 1)
     for (int tile = worker; tile < tiles && ok; tile += workers) {
       int m_blk, n_blk;
       fp8_tile(tile, num_m, num_n, p.group_m, m_blk, n_blk);
-      const int m0 = m_blk * TILE + rank * 128, n0 = n_blk * TILE + rank * 128;
+      const int m0 = m_blk * TILE_M + rank * 128, n0 = n_blk * TILE_N + rank * BN;
       for (int kb = 0; kb < nk; ++kb) {
         if (!warp_all(mbar_wait(&empty[stage], phase ^ 1, p.status, AXB_TIMEOUT_EMPTY))) {
           ok = false;
@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(G_THREADS, 1)
           load(a, ext ? &tmA2 : &tmA, ka, m0);
           if (B_MN) {
             load(b, mb, n0, ka);
-            load(b + G_OP / 2, mb, n0 + 64, ka);
+            if (BN > 64) load(b + G_OP / 2, mb, n0 + 64, ka);
           } else {
             load(b, mb, ka, n0);
           }
@@ -172,8 +172,8 @@ __global__ void __launch_bounds__(G_THREADS, 1)
     }
   } else if (warp == 1) {
     if (rank == 0) {
-      constexpr uint32_t id8 = make_idesc_e4m3(TILE, 128, B_MN ? 1 : 0);
-      constexpr uint32_t id16 = make_idesc_bf16(TILE, 128, 0, B_MN ? 1 : 0);
+      constexpr uint32_t id8 = make_idesc_e4m3(TILE_M, 128, B_MN ? 1 : 0);
+      constexpr uint32_t id16 = make_idesc_bf16(TILE_M, 128, 0, B_MN ? 1 : 0);
       const uint64_t base_a = make_smem_desc_sw128(smem_u32(smem), 16, 1024);
       // MN-major: two chunks of 64 columns (64-byte rows of codes, 128-byte rows of bf16), G_OP / 2 apart
       const uint64_t base_b8 = B_MN ? make_smem_desc_sw64(smem_u32(smem + G_OP), G_OP / 2) : base_a + G_OP / 16;
@@ -239,8 +239,8 @@ __global__ void __launch_bounds__(G_THREADS, 1)
   } else {
     const int quad = warp & 3, half = (warp - 2) >> 2;
     uint8_t* stg = sEpi + (warp - 2) * 4096;
-    const int set = PAIR ? half : 0;
-    const uint32_t t_base = tmem + (uint32_t(quad * 32) << 16) + (PAIR ? set * BUFS * 128 : half * 64);
+    const int set = SETS == 2 ? half : 0;
+    const uint32_t t_base = tmem + (uint32_t(quad * 32) << 16) + (SETS == 2 ? set * BUFS * 128 : half * 64);
     const long long step_a = p.ldsa * 4, step_b = p.sb_k * 4;   // bytes: the address arithmetic stays off the multipliers
     int buf = 0;
     uint32_t buf_phase = 0;
@@ -248,8 +248,8 @@ __global__ void __launch_bounds__(G_THREADS, 1)
     for (int tile = worker; tile < tiles && ok; tile += workers) {
       int m_blk, n_blk;
       fp8_tile(tile, num_m, num_n, p.group_m, m_blk, n_blk);
-      const int row0 = m_blk * TILE + rank * 128 + quad * 32, row = row0 + lane;
-      const int col0 = n_blk * TILE + half * 64;                // group g: col0 + 128 g ..
+      const int row0 = m_blk * TILE_M + rank * 128 + quad * 32, row = row0 + lane;
+      const int col0 = n_blk * TILE_N + half * 64;                // group g: col0 + 128 g ..
       const bool live = row < p.M;
       const float* sa = p.sa + (live ? row : 0);
       const float* sb = p.sb + (long long)(col0 >> 7) * p.sb_n;
@@ -351,16 +351,15 @@ int fp8_sm_count() {
   return n > 1 ? n : 148;
 }
 
-template <bool PAIR, bool B_MN>
+template <int CTAS, int SETS, bool B_MN>
 int launch_fp8(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& a2, const CUtensorMap& b2, const CUtensorMap& c,
                const Fp8GemmParams& p, bool pdl, cudaStream_t st) {
-  constexpr int CTAS = PAIR ? 2 : 1, TILE = 128 * CTAS;
-  auto kern = fp8_gemm_kernel<PAIR, B_MN>;
+  auto kern = fp8_gemm_kernel<CTAS, SETS, B_MN>;
   static std::atomic<unsigned long long> allowed{0};
   if (const int rc = axb_allow_smem((const void*)kern, G_SMEM, allowed)) return rc;
-  const long long tiles = (long long)((p.M + TILE - 1) / TILE) * ((p.N + TILE - 1) / TILE);
+  const long long tiles = (long long)((p.M + 128 * CTAS - 1) / (128 * CTAS)) * ((p.N + 128 * SETS - 1) / (128 * SETS));
   const long long workers = tiles < fp8_sm_count() / CTAS ? tiles : fp8_sm_count() / CTAS;
-  AxbLaunch l(dim3((unsigned)(workers * CTAS)), G_THREADS, G_SMEM, st, PAIR ? 2 : 0, pdl);
+  AxbLaunch l(dim3((unsigned)(workers * CTAS)), G_THREADS, G_SMEM, st, CTAS == 2 ? 2 : 0, pdl);
   const cudaError_t e = cudaLaunchKernelEx(&l.cfg, kern, a, b, a2, b2, c, p);
   return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }
@@ -378,15 +377,16 @@ static int fp8_gemm_entry(const void* A, long long lda, const float* sa, long lo
   auto bad = [](const void* q, long long bytes) { return (reinterpret_cast<uintptr_t>(q) & 15) != 0 || (bytes & 15) != 0; };
   if (K <= 0 || bad(A, lda) || bad(B, ldb) || ldsa < M) return -2;
   if (K2 > 0 && (bad(A2, 2 * lda2) || bad(B2, 2 * ldb2))) return -2;
-  const bool pair = tile == 256;
+  const bool pair = tile != 128;
+  const int bn = tile == 192 ? 64 : 128;
   CUtensorMap tA, tB, tA2, tB2, tC;
   int rc = axb_make_tmap_2d(&tA, A, M, K, lda, 128, 128, 1);
-  if (!rc) rc = b_mn ? axb_make_tmap_2d(&tB, B, K, N, ldb, 128, 64, 1, false, true) : axb_make_tmap_2d(&tB, B, N, K, ldb, 128, 128, 1);
+  if (!rc) rc = b_mn ? axb_make_tmap_2d(&tB, B, K, N, ldb, 128, 64, 1, false, true) : axb_make_tmap_2d(&tB, B, N, K, ldb, bn, 128, 1);
   tA2 = tC = tA;
   tB2 = tB;
   if (!rc && K2 > 0) {
     rc = axb_make_tmap_2d(&tA2, A2, M, K2, lda2, 128, 64);
-    if (!rc) rc = b_mn ? axb_make_tmap_2d(&tB2, B2, K2, N, ldb2, 64, 64) : axb_make_tmap_2d(&tB2, B2, N, K2, ldb2, 128, 64);
+    if (!rc) rc = b_mn ? axb_make_tmap_2d(&tB2, B2, K2, N, ldb2, 64, 64) : axb_make_tmap_2d(&tB2, B2, N, K2, ldb2, bn, 64);
   }
   const int tma_store = !bad(C, 2 * ldc);
   if (!rc && tma_store) rc = axb_make_tmap_2d(&tC, C, M, N, ldc, 32, 64);
@@ -408,8 +408,10 @@ static int fp8_gemm_entry(const void* A, long long lda, const float* sa, long lo
   const long long band = (20ll << 20) / ((pair ? 256ll : 128ll) * K);   // A rows of a band: about 20 MB of the L2
   p.group_m = (int)(band < 2 ? 2 : (band > 16 ? 16 : band));
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (pair) return b_mn ? launch_fp8<true, true>(tA, tB, tA2, tB2, tC, p, pdl, st) : launch_fp8<true, false>(tA, tB, tA2, tB2, tC, p, pdl, st);
-  return b_mn ? launch_fp8<false, true>(tA, tB, tA2, tB2, tC, p, pdl, st) : launch_fp8<false, false>(tA, tB, tA2, tB2, tC, p, pdl, st);
+  auto run = [&](auto kmajor, auto mnmajor) { return (b_mn ? mnmajor : kmajor)(tA, tB, tA2, tB2, tC, p, pdl, st); };
+  if (tile == 256) return run(launch_fp8<2, 2, false>, launch_fp8<2, 2, true>);
+  if (tile == 192) return run(launch_fp8<2, 1, false>, launch_fp8<2, 1, true>);
+  return run(launch_fp8<1, 1, false>, launch_fp8<1, 1, true>);
 }
 
 extern "C" int axb_fp8_gemm(const void* A, long long lda, const float* sa, long long ldsa, const void* B, long long ldb, const float* sb,

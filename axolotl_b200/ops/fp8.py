@@ -275,12 +275,15 @@ def fp8_gemm(codes, row_scale, w_codes, w_scale, *, trans_w=False, a2=None, b2=N
 
 
 def _tile(M, N, K) -> int:
-    """256 x 256 tiles of a CTA pair or 128 x 128: waves x (microseconds per block of K + microseconds per tile), by least squares over 68
-    products of 65 to 8192 rows. Within 0.3 % of the better of the two on average; 5.5 % with pairs from one wave on. 376 x 5512 by 1304
-    15.7 / 14.8 us (128 / 256), 1531 x 2904 by 2008 22.6 / 18.5, 636 x 680 by 608 14.6 / 15.7, 8192 x 28672 by 4096 993 / 830."""
-    nk = (K + 127) >> 7
-    small = -(-(((M + 127) >> 7) * ((N + 127) >> 7)) // 148) * (0.321 * nk + 0.85) + 1.3
-    return 256 if -(-(((M + 255) >> 8) * ((N + 255) >> 8)) // 74) * (0.394 * nk + 2.53) < small else 128
+    """Tiles of 256 x 256 (256) or 256 x 128 (192) by a CTA pair, or of 128 x 128: waves x (microseconds per block of K + microseconds per
+    tile), by least squares over 105 products of 65 to 8192 rows; what it picks is 0.9 % above the best of the three on average (3.5 %
+    without the middle one). 361 x 3048 by 6784 33.5 / 26.2 / 34.0 us (128 / 192 / 256), 3600 x 344 by 8304 35.6 / 31.1 / 35.6, 376 x 5512
+    by 1304 15.7 / - / 14.8, 636 x 680 by 608 14.6 / - / 15.7, 8192 x 28672 by 4096 993 / - / 830."""
+    nk, m1, m2, n1 = (K + 127) >> 7, (M + 127) >> 7, (M + 255) >> 8, (N + 127) >> 7
+    small = -(-m1 * n1 // 148) * (0.326 * nk + 0.74) + 1.1
+    mid = -(-m2 * n1 // 74) * (0.265 * nk + 0.73) + 1.8
+    big = -(-m2 * ((N + 255) >> 8) // 74) * (0.393 * nk + 2.33)
+    return 256 if big <= small and big <= mid else 192 if mid <= small else 128
 
 
 def _few(T, N, K):

@@ -201,11 +201,11 @@ def test_product(M, N, K, trans, dev):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("tile", [128, 256])
+@pytest.mark.parametrize("tile", [128, 192, 256])
 @pytest.mark.parametrize("trans", [False, True])
 @pytest.mark.parametrize("rank", [0, 8, 16, 72])
 def test_product_tiles_and_extension(tile, trans, rank, monkeypatch):
-    """Both tile sizes whatever the rule picks, with and without the bf16 K-extension, more tiles than workers."""
+    """Every tile size whatever the rule picks, with and without the bf16 K-extension, more tiles than workers."""
     from axolotl_b200.ops import fp8
 
     monkeypatch.setattr(fp8, "_tile", lambda *a: tile)
