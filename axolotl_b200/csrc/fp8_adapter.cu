@@ -5,8 +5,8 @@
 // are widened first: eight warps turn a tile of 64 rows x 128 columns into bf16 (exact: four significant bits and a power of two) as the
 // MN-major 128-row operand of tcgen05.mma, g is the other one, 64 of its columns at a time. The rows are split over a cluster whose partial
 // sums meet in distributed shared memory in a fixed order: no atomics, the same bits every time.
-// What it measures: 8192 x 14336, rank 16, 60 us (2 TB/s of codes; expanding the rows and a bf16 product took 122), bound by the integer
-// pipe of the SMs that hold two of the 224 CTAs, some seven instructions a code; 8192 x 4096 23 us.
+// What it measures: 8192 x 14336, rank 16, 57 us (2 TB/s of codes; expanding the rows and a bf16 product took 122), bound by the integer
+// pipe of the SMs that hold two of the 224 CTAs, some seven instructions a code; 8192 x 11008 41.5 us, 8192 x 4096 20.6.
 #include "axb_common.cuh"
 
 namespace {

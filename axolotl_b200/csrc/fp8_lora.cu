@@ -1,6 +1,6 @@
 // A projection in 8-bit blocks with an adapter (ops/fp8.py) as one host call each way: a short training row spends less time on the device
-// than the interpreter needs to issue the launches one by one (960 x 4096 by 6144, rank 16, forward and backward: kernels 112 us; 253 us
-// with them issued from Python, 177 like this, 49 of it autograd's own).
+// than the interpreter needs to issue the launches one by one (960 x 4096 by 6144, rank 16, forward and backward: kernels 106 us; 253 us
+// with them issued from Python, 175 like this, 49 of it autograd's own).
 #include "axb_common.cuh"
 
 extern "C" int axb_gemm_skinny(const void* P, long long ldp, const void* S, long long lds, void* C, long long ldc, int R, int N,

@@ -4,7 +4,7 @@
 // Bound: HBM, 2 bytes read and 1 written per value. A step is 128 rows x 128 columns: bulk copies bring it in as the K-major 128-row
 // operand of tcgen05.mma (A's block is the other one, N = 16 .. 64), and eight warps read the same tile back for the codes, a
 // conflict-free 16 bytes a lane. They hand the stage back as soon as the values are in registers. K is split over a cluster, whose partial
-// products meet in distributed shared memory in a fixed order. What it measures: 8192 x 14336, rank 16, 67 us, 5.9 TB/s and some 7 us of
+// products meet in distributed shared memory in a fixed order. What it measures: 8192 x 14336, rank 16, 67 us: 5.9 TB/s and some 7 us of
 // start, join and end; 960 x 4096 12.3 us. No faster: eight quantising warps of eight passes, five stages for one CTA of an SM.
 #include "fp8_rows.cuh"
 

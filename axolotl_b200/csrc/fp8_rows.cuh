@@ -22,7 +22,7 @@ AXB_DEVICE void put2(__half* o, float2 f) { *reinterpret_cast<__half2*>(o) = __f
 AXB_DEVICE void put2(float* o, float2 f) { *reinterpret_cast<float2*>(o) = f; }
 
 // Eight values of a row as they are stored. The largest magnitude is taken in the stored type, two values an instruction: with every
-// value widened first the kernel was bound by its arithmetic (32768 x 4096 in bf16: 112 us, 70 us like this, 5.8 TB/s).
+// value widened first the kernel was bound by its arithmetic (32768 x 4096 in bf16: 112 us, 70 like this, 64 with codes4 below).
 template <typename T>
 struct Eight {
   uint4 raw[sizeof(T) / 2];
