@@ -24,8 +24,8 @@
 extern "C" int axb_fp8_quantize_rows(const void* x, long long ldx, int dtype, void* q, long long ldq, float* s, long long lds,
                                      long long rows, int K, void* stream);
 extern "C" int axb_fp8_skinny(const void* x, long long ldx, const void* q, long long ldq, const float* sx, long long ldsx, const void* W,
-                              long long ldw, const float* sw, long long sw_n, long long sw_k, void* y, long long ldy, int T, int N, int K, const void* X2,
-                              long long ldx2, const void* B2, long long ldb2, int K2, int* status, void* stream);
+                              long long ldw, const float* sw, long long sw_n, long long sw_k, void* y, long long ldy, int T, int N, int K,
+                              const void* X2, long long ldx2, const void* B2, long long ldb2, int K2, int* status, void* stream);
 
 namespace {
 

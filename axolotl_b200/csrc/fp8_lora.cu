@@ -71,8 +71,8 @@ extern "C" int axb_fp8_lora_fwd(const AxbFp8Lora* l, void* stream) {
     rc = axb_gemm_skinny(l->x, l->ldx, l->A, l->lda, l->xa, l->R, l->T, l->R, l->K, nullptr, 0, nullptr, 0, 0, l->scaling, nullptr, 1, 0, 0,
                          0.f, 1, 0, 0, l->status, stream);
   }
-  return rc ? rc : axb_fp8_linear(one ? nullptr : l->x, l->ldx, l->q, l->W, l->ldw, l->sw, l->sw_n, l->sw_k, 0, l->y, l->T, l->N, l->K, l->xa, l->R, l->B,
-                                  l->ldb, l->R, l->tile, l->status, stream);
+  return rc ? rc : axb_fp8_linear(one ? nullptr : l->x, l->ldx, l->q, l->W, l->ldw, l->sw, l->sw_n, l->sw_k, 0, l->y, l->T, l->N, l->K, l->xa,
+                                  l->R, l->B, l->ldb, l->R, l->tile, l->status, stream);
 }
 
 extern "C" int axb_fp8_lora_bwd(const AxbFp8Lora* l, void* stream) {

@@ -376,8 +376,8 @@ int launch_fp8_skinny(const CUtensorMap (&m)[4], const Fp8SkinnyParams& p, int t
 // sx: their scales [ceil(K / 128)][ldsx]; W: codes [N, K], rows of ldw bytes, and their scales sw[(n / 128) * sw_n + b * sw_k]; y: bf16
 // [T, N]; X2 [T, K2] and B2 [N, K2] bf16, K2 = 0: none. q, W, X2 and B2 start on 16 bytes and have row strides of whole 16 bytes.
 extern "C" int axb_fp8_skinny(const void* x, long long ldx, const void* q, long long ldq, const float* sx, long long ldsx, const void* W,
-                              long long ldw, const float* sw, long long sw_n, long long sw_k, void* y, long long ldy, int T, int N, int K, const void* X2,
-                              long long ldx2, const void* B2, long long ldb2, int K2, int* status, void* stream) {
+                              long long ldw, const float* sw, long long sw_n, long long sw_k, void* y, long long ldy, int T, int N, int K,
+                              const void* X2, long long ldx2, const void* B2, long long ldb2, int K2, int* status, void* stream) {
   if (T <= 0 || N <= 0) return 0;
   auto bad = [](const void* a, long long bytes) { return (reinterpret_cast<uintptr_t>(a) & 15) != 0 || (bytes & 15) != 0; };
   if (T > 64 || K <= 0 || bad(W, ldw) || (q && bad(q, ldq))) return -2;

@@ -527,7 +527,8 @@ def _check_linear(x, codes, scale, bias, what):
     if bias is not None and (bias.shape != cs[:1] or bias.device != x.device):
         raise ValueError(f"{what}: a bias {tuple(bias.shape)} on {bias.device} for a weight {tuple(cs)} and an input on {x.device}")
     if (len(cs) == 2 and len(ss) == 2 and cs[0] and cs[1] and x.dim() and x.shape[-1] == cs[1]
-            and codes.dtype in (torch.float8_e4m3fn, torch.uint8) and scale.dtype == torch.float32 and ss[0] == _blocks(cs[0]) and ss[1] == _blocks(cs[1]) and x.device == codes.device
+            and codes.dtype in (torch.float8_e4m3fn, torch.uint8) and scale.dtype == torch.float32 and ss[0] == _blocks(cs[0])
+            and ss[1] == _blocks(cs[1]) and x.device == codes.device
             and x.device == scale.device and (x.dtype == torch.bfloat16 or not x.is_cuda)):
         return
     _check_weight(_as_codes(codes), scale, what)
@@ -547,9 +548,12 @@ def _shaped(y, x):
     return y if x.dim() == 2 else y.view(*x.shape[:-1], y.shape[-1])
 
 
-def _no_rows(x, codes):
-    """The result of no rows, connected to ``x``."""
-    return x[..., :1].expand(*x.shape[:-1], codes.shape[0])
+def _no_rows(x, codes, bias, A=None, B=None):
+    """The result of no rows, connected to all that learns."""
+    y = x[..., :1].expand(*x.shape[:-1], codes.shape[0])
+    if A is not None:
+        y = y + (x @ A.to(x.dtype).t()) @ B.to(x.dtype).t()
+    return y if bias is None else y + bias.to(x.dtype)
 
 
 def fp8_linear(x, codes, scale, bias=None):
@@ -557,7 +561,7 @@ def fp8_linear(x, codes, scale, bias=None):
     ceil(K / 128)]); ``x`` [..., K] in bf16. The input gradient is ``dy8 W8``; nothing of ``x`` is kept for it."""
     _check_linear(x, codes, scale, bias, "fp8_linear")
     if x.numel() == 0:
-        return _no_rows(x, codes)
+        return _no_rows(x, codes, bias)
     if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
         return _shaped(_Fp8LinearFn.apply(_rows_of(x), codes, scale, bias), x)
     y = _product(x if x.dim() == 2 else _rows_of(x), _as_codes(codes), scale)[0]
@@ -571,7 +575,7 @@ def fp8_lora_linear(x, codes, scale, A, B, A16, B16, scaling, blocks, bias=None)
     rows of ``x`` are kept for ``dA = (scaling dy B)^T x8``."""
     _check_linear(x, codes, scale, bias, "fp8_lora_linear")
     if x.numel() == 0:
-        return _no_rows(x, codes)
+        return _no_rows(x, codes, bias, A, B)
     x2 = _rows_of(x)
     if not x.is_cuda:
         y = _Fp8LinearFn.apply(x2, codes, scale, bias).to(x.dtype)

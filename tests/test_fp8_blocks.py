@@ -295,7 +295,8 @@ def test_linear_gradient_by_differences(dev):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("T,K,N,blocks", [(1, 256, 128, ((0, 128, 0, 8),)), (70, 520, 264, ((0, 200, 0, 8), (200, 64, 8, 8))),
-                                          (600, 1024, 640, ((0, 640, 0, 16),)), (700, 264, 1032, ((128, 904, 0, 32),)), (90, 131, 77, ((0, 77, 0, 8),)), (20, 256, 128, ((0, 128, 0, 72),))])
+                                          (600, 1024, 640, ((0, 640, 0, 16),)), (700, 264, 1032, ((128, 904, 0, 32),)),
+                                          (90, 131, 77, ((0, 77, 0, 8),)), (20, 256, 128, ((0, 128, 0, 72),))])
 @pytest.mark.parametrize("masters", [torch.float32, torch.bfloat16])
 def test_lora_linear_and_its_gradients(T, K, N, blocks, masters):
     R = sum(b[3] for b in blocks)
@@ -330,8 +331,10 @@ def test_lora_linear_and_its_gradients(T, K, N, blocks, masters):
     near(dx, want, BF16 * want.abs() + (tall_e @ a.abs() + (N + R + 40) * EPS32 * size) * (1 + BF16), 4)
     assert dA.dtype == dB.dtype == masters
     half = BF16 if masters == torch.bfloat16 else 0.0       # and the gradients' own rounding
-    near(dA, tall.t() @ x8, half * (1 + BF16) * (tall.t() @ x8).abs() + (1 + half) * tall_e.t() @ x8.abs() + (T + 8) * EPS32 * tall.abs().t() @ x8.abs(), 4)
-    wantB, offB = dy64.t() @ low, half * (1 + BF16) * (dy64.t() @ low).abs() + (1 + half) * dy64.abs().t() @ low_e + (T + 8) * EPS32 * dy64.abs().t() @ low.abs()
+    want, size = tall.t() @ x8, tall.abs().t() @ x8.abs()
+    near(dA, want, half * (1 + BF16) * want.abs() + (1 + half) * tall_e.t() @ x8.abs() + (T + 8) * EPS32 * size, 4)
+    wantB, size = dy64.t() @ low, dy64.abs().t() @ low.abs()
+    offB = half * (1 + BF16) * wantB.abs() + (1 + half) * dy64.abs().t() @ low_e + (T + 8) * EPS32 * size
     for r0, rows, c0, r in blocks:
         near(dB[r0:r0 + rows, c0:c0 + r], wantB[r0:r0 + rows, c0:c0 + r], offB[r0:r0 + rows, c0:c0 + r], 4)
     assert (dB.cpu()[B == 0] == 0).all() or len(blocks) == 1
@@ -752,7 +755,8 @@ def test_lora_refusals_on_the_device():
     w, ws = quantize_fp8_weight(torch.randn(64, 128).cuda())
     x, A, B = torch.randn(4, 128).bfloat16().cuda(), torch.randn(8, 128).bfloat16().cuda(), torch.randn(64, 8).bfloat16().cuda()
     blk = ((0, 64, 0, 8),)
-    for args in ((A[:, :64], B, A[:, :64], B), (A, B[:32], A, B[:32]), (A, B, A.float(), B), (A, B, A[:4], B), (A, B, A.cpu(), B), (A, B, A, B.cpu())):
+    for args in ((A[:, :64], B, A[:, :64], B), (A, B[:32], A, B[:32]), (A, B, A.float(), B), (A, B, A[:4], B), (A, B, A.cpu(), B),
+                 (A, B, A, B.cpu())):
         with pytest.raises(ValueError):
             fp8_lora_linear(x, w, ws, *args, 1.0, blk)
     with pytest.raises(ValueError):
@@ -1066,3 +1070,75 @@ def test_adapter_gradient_over_clusters_of_three_five_and_six(T, K):
     got = fp8_adapter_grad(t.cuda(), codes, scale)
     assert ((got.cpu().double() - want).abs() <= (T + 8) * EPS32 * size * (1 + 2.0 ** -20)).all()
     assert torch.equal(got, fp8_adapter_grad(t.cuda(), codes, scale))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_no_rows_reach_all_that_learns(dev):
+    """Frozen inputs without rows: the adapter and the bias receive zeros."""
+    w, ws = quantize_fp8_weight(torch.randn(64, 128).to(dev))
+    A, B = (torch.randn(s).to(dev).requires_grad_(True) for s in ((8, 128), (64, 8)))
+    bias = torch.randn(64, device=dev, requires_grad=True)
+    x = torch.empty(0, 128, dtype=torch.bfloat16, device=dev)
+    y = fp8_lora_linear(x, w, ws, A, B, A.detach().bfloat16(), B.detach().bfloat16(), 1.0, ((0, 64, 0, 8),), bias)
+    assert y.shape == (0, 64) and y.dtype == torch.bfloat16
+    for g in (*torch.autograd.grad(y.sum(), [A, B, bias]), *torch.autograd.grad(fp8_linear(x, w, ws, bias).sum(), [bias])):
+        assert not g.any()
+
+
+@pytest.mark.gpu
+def test_adapter_layer_captured_forward_and_backward():
+    """A graph of the adapter's layer both ways, replayed on other inputs, beside the eager call."""
+    T, K, N, R = 1000, 1160, 328, 16
+    w, ws = quantize_fp8_weight(_make((N, K), 3, torch.float32, 0.0).cuda())
+    A, B = _make((R, K), 4, spread=0.0).cuda() * 0.06, _make((N, R), 5, spread=0.0).cuda() * 0.1
+    x, dy = _make((T, K), 1, spread=0.3).cuda(), _make((T, N), 2, spread=0.3).cuda()
+
+    def both():
+        xl, a, b = x.detach().requires_grad_(True), A.detach().requires_grad_(True), B.detach().requires_grad_(True)
+        y = fp8_lora_linear(xl, w, ws, a, b, A, B, 0.5, ((0, N, 0, R),))
+        return [y, *torch.autograd.grad(y, [xl, a, b], dy)]
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        both()
+    stream.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=stream):
+        outs = both()
+    for seed in (11, 12):
+        x.copy_(_make((T, K), seed, spread=0.3))
+        dy.copy_(_make((T, N), seed + 1, spread=0.3))
+        g.replay()
+        torch.cuda.synchronize()
+        got = [o.detach().clone() for o in outs]
+        want = both()
+        assert torch.equal(got[0], want[0])
+        for a, b in zip(got[1:], want[1:]):                # t and dB are summed in any order and may round to their neighbours (2^-7)
+            assert ((a.double() - b.detach().double()).abs().max() <= 2.0 ** -6 * b.detach().double().abs().max()).item()
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once():
+    """Calls of every form in flight on two streams give what they give alone."""
+    N, K, R = 1160, 2056, 16
+    w, ws = quantize_fp8_weight(_make((N, K), 3, torch.float32, 0.0).cuda())
+    A, B = _make((R, K), 4, spread=0.0).cuda() * 0.06, _make((N, R), 5, spread=0.0).cuda() * 0.1
+    xs = [_make((T, K), T, spread=0.3).cuda() for T in (1, 40, 64, 200, 1200)]
+    t = _make((1200, R), 6, spread=0.0).cuda()
+    codes, scale = quantize_fp8_rows(xs[-1])
+    Al = A.clone().requires_grad_(True)
+    calls = [lambda x=x: fp8_linear(x, w, ws) for x in xs]
+    calls += [lambda x=x: fp8_lora_linear(x, w, ws, Al, B, A, B, 1.0, ((0, N, 0, R),)) for x in xs]
+    calls += [lambda: fp8_adapter_grad(t, codes, scale), lambda: quantize_fp8_rows(xs[-1])[0].view(torch.uint8)]
+    alone = [f() for f in calls]
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    for _ in range(4):
+        for s, o, order in zip(streams, outs, (calls, calls[::-1])):
+            with torch.cuda.stream(s):
+                o.append([f() for f in order])
+    torch.cuda.synchronize()
+    for o, order in zip(outs, (alone, alone[::-1])):
+        for run in o:
+            assert all(torch.equal(a, b) for a, b in zip(run, order))
