@@ -202,14 +202,18 @@ __global__ void __launch_bounds__(FA_T, 2)
   for (int i = rank * FA_T + tid; i < rows * 32; i += cs * FA_T) {
     const int rr = i >> 5, c = (i & 31) * 4, k = tile * 128 + c;
     if (k >= p.K) continue;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int q = 0; q < cs; ++q) {
-      const float4 u = cs == 1 ? *reinterpret_cast<const float4*>(part + rr * 128 + c) : ld_cluster_f32x4(mapa_u32(pbase + (rr * 128 + c) * 4, q));
-      a.x += u.x;
-      a.y += u.y;
-      a.z += u.z;
-      a.w += u.w;
-    }
+    float4 u[8], a = make_float4(0.f, 0.f, 0.f, 0.f);    // all on their way before the first is added
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (q < cs) u[q] = cs == 1 ? *reinterpret_cast<const float4*>(part + rr * 128 + c) : ld_cluster_f32x4(mapa_u32(pbase + (rr * 128 + c) * 4, q));
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (q < cs) {
+        a.x += u[q].x;
+        a.y += u[q].y;
+        a.z += u[q].z;
+        a.w += u[q].w;
+      }
     if (p.out16) {
       __nv_bfloat16* o = p.out16 + (long long)(r0 + rr) * p.ldo + k;
       if (p.vec && k + 4 <= p.K) {
@@ -223,11 +227,11 @@ __global__ void __launch_bounds__(FA_T, 2)
     float* o = p.out + (long long)(r0 + rr) * p.ldo + k;
     if (p.vec && k + 4 <= p.K) {
       if (p.accumulate) {
-        const float4 u = *reinterpret_cast<const float4*>(o);
-        a.x += u.x;
-        a.y += u.y;
-        a.z += u.z;
-        a.w += u.w;
+        const float4 b = *reinterpret_cast<const float4*>(o);
+        a.x += b.x;
+        a.y += b.y;
+        a.z += b.z;
+        a.w += b.w;
       }
       *reinterpret_cast<float4*>(o) = a;
     } else {

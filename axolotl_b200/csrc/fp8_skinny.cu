@@ -178,9 +178,9 @@ __global__ void __launch_bounds__(FS_T, 2)
   } else if (warp < 6) {
     const float* sw = p.sw + (long long)tile * p.sw_n;
     const uint32_t t_base = tmem + (uint32_t((warp & 3) * 32) << 16);
-    float sum[NT];
+    uint64_t sum[NT / 2];                 // two tokens each
 #pragma unroll
-    for (int j = 0; j < NT; ++j) sum[j] = 0.f;
+    for (int j = 0; j < NT / 2; ++j) sum[j] = 0ull;
     float mine = 0.f;                     // lane l: the weight's scale of block kb0 + l, kb0 + 32 + l, ..
     int buf = 0;
     uint32_t buf_phase = 0;
@@ -188,6 +188,7 @@ __global__ void __launch_bounds__(FS_T, 2)
       const int i = kb - kb0;
       if ((i & 31) == 0) mine = kb + lane < nk_main ? __ldg(sw + (kb + lane) * p.sw_k) : 1.f;
       const float w = __shfl_sync(0xffffffffu, mine, i & 31);
+      const uint64_t ww = pack_f32x2(w, w);
       if (!warp_all(mbar_wait(&tfull[buf], buf_phase, p.status, AXB_TIMEOUT_TMEM_FULL) &&
                     mbar_wait(&ready[i % FS_RING], (uint32_t)(i / FS_RING) & 1, p.status, AXB_TIMEOUT_GENERIC)))
         break;
@@ -201,10 +202,9 @@ __global__ void __launch_bounds__(FS_T, 2)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const float4 s4 = sx[c * 4 + j];
-          sum[c * 16 + 4 * j] += __uint_as_float(r[4 * j]) * (w * s4.x);
-          sum[c * 16 + 4 * j + 1] += __uint_as_float(r[4 * j + 1]) * (w * s4.y);
-          sum[c * 16 + 4 * j + 2] += __uint_as_float(r[4 * j + 2]) * (w * s4.z);
-          sum[c * 16 + 4 * j + 3] += __uint_as_float(r[4 * j + 3]) * (w * s4.w);
+          uint64_t* to = sum + c * 8 + 2 * j;
+          to[0] = fma_f32x2(pack_b32x2(r[4 * j], r[4 * j + 1]), mul_f32x2(ww, pack_f32x2(s4.x, s4.y)), to[0]);
+          to[1] = fma_f32x2(pack_b32x2(r[4 * j + 2], r[4 * j + 3]), mul_f32x2(ww, pack_f32x2(s4.z, s4.w)), to[1]);
         }
       }
       tc_fence_before();
@@ -221,8 +221,10 @@ __global__ void __launch_bounds__(FS_T, 2)
     }
     // this warp has seen the last product end, and with it every read and write of the ring
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
-      if (j < p.T) part[j * 128 + (warp & 3) * 32 + lane] = sum[j];
+    for (int j = 0; j < NT; ++j) {
+      const float2 two = unpack_f32x2(sum[j >> 1]);
+      if (j < p.T) part[j * 128 + (warp & 3) * 32 + lane] = j & 1 ? two.y : two.x;
+    }
   } else if (!FUSED) {
     pdl_wait();
     // the rows' scales into the ring, a quarter of the tokens a warp, as far ahead as the ring goes. (Not by the operands' `empty`: nothing
@@ -335,14 +337,18 @@ __global__ void __launch_bounds__(FS_T, 2)
   for (int i = rank * FS_T + tid; i < p.T * 32; i += cs * FS_T) {
     const int t = i >> 5, r = (i & 31) * 4, n = tile * 128 + r;
     if (n >= p.N) continue;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int q = 0; q < cs; ++q) {
-      const float4 u = cs == 1 ? *reinterpret_cast<const float4*>(part + t * 128 + r) : ld_cluster_f32x4(mapa_u32(pbase + (t * 128 + r) * 4, q));
-      a.x += u.x;
-      a.y += u.y;
-      a.z += u.z;
-      a.w += u.w;
-    }
+    float4 u[8], a = make_float4(0.f, 0.f, 0.f, 0.f);    // all on their way before the first is added
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (q < cs) u[q] = cs == 1 ? *reinterpret_cast<const float4*>(part + t * 128 + r) : ld_cluster_f32x4(mapa_u32(pbase + (t * 128 + r) * 4, q));
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      if (q < cs) {
+        a.x += u[q].x;
+        a.y += u[q].y;
+        a.z += u[q].z;
+        a.w += u[q].w;
+      }
     __nv_bfloat16* y = p.y + (long long)t * p.ldy + n;
     if (vec && n + 4 <= p.N) {
       *reinterpret_cast<uint2*>(y) = make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w));
