@@ -334,6 +334,14 @@ def load_pretrained(path: str, dtype=torch.bfloat16, device="cpu", config: Model
     return model
 
 
+def _dense(m) -> torch.Tensor:
+    """A projection's weight as it is written: as it is, or expanded from its codes (4-bit or 8-bit blocks) and brought to the host, so that
+    one expanded weight at a time is on the device."""
+    if getattr(m.weight, "_axb_quant", None) is None:
+        return m.weight.detach()
+    return m._dense_weight().cpu()
+
+
 def sharded_state_dict(model: CausalLM, rank: int) -> tuple[dict, list[str]]:
     """This rank's part of a SHARDED state dict under HF names, and the list of tensors that are split on
     dim 0. A row-sharded fused weight (q|k|v, gate|up) holds rows [rank * n, (rank + 1) * n) of the fused
@@ -435,8 +443,8 @@ def _lfm2_state_dict(model, sd):
             pre = f"model.layers.{i}"
             for k in [k for k in sd if k.startswith(pre + ".self_attn.")]:
                 sd.pop(k)
-            out[f"{pre}.conv.in_proj.weight"] = mx.in_proj.weight.detach()
-            out[f"{pre}.conv.out_proj.weight"] = mx.out_proj.weight.detach()
+            out[f"{pre}.conv.in_proj.weight"] = _dense(mx.in_proj)
+            out[f"{pre}.conv.out_proj.weight"] = _dense(mx.out_proj)
             out[f"{pre}.conv.conv.weight"] = mx.conv_weight.detach()[:, None, :]
             if mx.conv_bias is not None:
                 out[f"{pre}.conv.in_proj.bias"] = mx.in_proj.bias.detach()
@@ -528,8 +536,8 @@ def _llama4_out(model, sd):
 
 
 def _mamba_tensors(pre, mx, sd):
-    sd[f"{pre}.mamba.in_proj.weight"] = mx.in_proj.weight.detach()
-    sd[f"{pre}.mamba.out_proj.weight"] = mx.out_proj.weight.detach()
+    sd[f"{pre}.mamba.in_proj.weight"] = _dense(mx.in_proj)
+    sd[f"{pre}.mamba.out_proj.weight"] = _dense(mx.out_proj)
     if mx.in_proj.bias is not None:
         sd[f"{pre}.mamba.in_proj.bias"] = mx.in_proj.bias.detach()
     if mx.out_proj.bias is not None:
@@ -558,9 +566,10 @@ def _nemotron_h_state_dict(model):
             sd.update({k.replace(".mamba.", ".mixer."): v for k, v in tmp.items()})
         else:
             for fl in ([mx.qkv_proj, mx.o_proj] if layer.kind == "attention" else [mx.up_proj, mx.down_proj]):
+                w = _dense(fl)
                 for sub in fl.names:
                     r0, r1 = fl.row_range(sub)
-                    sd[f"{pre}.mixer.{sub}.weight"] = fl.weight.detach()[r0:r1]
+                    sd[f"{pre}.mixer.{sub}.weight"] = w[r0:r1]
                     if fl.bias is not None:
                         sd[f"{pre}.mixer.{sub}.bias"] = fl.bias.detach()[r0:r1]
     return sd
@@ -620,15 +629,17 @@ def _bamba_state_dict(model, sd):
                 _mamba_tensors(pre, mx, sd)
             else:
                 for fl in (mx.qkv_proj, mx.o_proj):
+                    w = _dense(fl)
                     for sub in fl.names:
                         r0, r1 = fl.row_range(sub)
-                        sd[f"{pre}.self_attn.{sub}.weight"] = fl.weight.detach()[r0:r1]
+                        sd[f"{pre}.self_attn.{sub}.weight"] = w[r0:r1]
                         if fl.bias is not None:
                             sd[f"{pre}.self_attn.{sub}.bias"] = fl.bias.detach()[r0:r1]
         for fl in (layer.mlp.gate_up_proj, layer.mlp.down_proj):
+            w = _dense(fl)
             for sub in fl.names:
                 r0, r1 = fl.row_range(sub)
-                sd[f"{pre}.feed_forward.{sub}.weight"] = fl.weight.detach()[r0:r1]
+                sd[f"{pre}.feed_forward.{sub}.weight"] = w[r0:r1]
     return sd
 
 
@@ -641,13 +652,14 @@ def _qwen3_next_out(model, sd):
             for k in [k for k in sd if k.startswith(pre + ".self_attn.")]:
                 sd.pop(k)
             if mx.flat:
+                w = _dense(mx.in_proj)
                 for sub in mx.in_proj.names:
                     r0, r1 = mx.in_proj.row_range(sub)
-                    sd[f"{pre}.linear_attn.{sub}.weight"] = mx.in_proj.weight.detach()[r0:r1]
+                    sd[f"{pre}.linear_attn.{sub}.weight"] = w[r0:r1]
             else:
-                sd[f"{pre}.linear_attn.in_proj_qkvz.weight"] = mx.in_proj_qkvz.weight.detach()
-                sd[f"{pre}.linear_attn.in_proj_ba.weight"] = mx.in_proj_ba.weight.detach()
-            sd[f"{pre}.linear_attn.out_proj.weight"] = mx.out_proj.weight.detach()
+                sd[f"{pre}.linear_attn.in_proj_qkvz.weight"] = _dense(mx.in_proj_qkvz)
+                sd[f"{pre}.linear_attn.in_proj_ba.weight"] = _dense(mx.in_proj_ba)
+            sd[f"{pre}.linear_attn.out_proj.weight"] = _dense(mx.out_proj)
             sd[f"{pre}.linear_attn.conv1d.weight"] = mx.conv_weight.detach()[:, None, :]
             sd[f"{pre}.linear_attn.norm.weight"] = mx.norm_weight.detach()
             sd[f"{pre}.linear_attn.dt_bias"] = mx.dt_bias.detach()
@@ -668,8 +680,8 @@ def _granite_hybrid_state_dict(model, sd):
             sd[f"{pre}.{nm}.weight"] = getattr(layer, nm).weight.detach()
         mx = layer.self_attn
         if type(mx).__name__ == "Mamba2Mixer":
-            sd[f"{pre}.mamba.in_proj.weight"] = mx.in_proj.weight.detach()
-            sd[f"{pre}.mamba.out_proj.weight"] = mx.out_proj.weight.detach()
+            sd[f"{pre}.mamba.in_proj.weight"] = _dense(mx.in_proj)
+            sd[f"{pre}.mamba.out_proj.weight"] = _dense(mx.out_proj)
             if mx.in_proj.bias is not None:
                 sd[f"{pre}.mamba.in_proj.bias"] = mx.in_proj.bias.detach()
                 sd[f"{pre}.mamba.out_proj.bias"] = mx.out_proj.bias.detach()
@@ -681,15 +693,16 @@ def _granite_hybrid_state_dict(model, sd):
                 sd[f"{pre}.mamba.{leaf}"] = getattr(mx, leaf).detach()
         else:
             for fl in (mx.qkv_proj, mx.o_proj):
+                w = _dense(fl)
                 for sub in fl.names:
                     r0, r1 = fl.row_range(sub)
-                    sd[f"{pre}.self_attn.{sub}.weight"] = fl.weight.detach()[r0:r1]
+                    sd[f"{pre}.self_attn.{sub}.weight"] = w[r0:r1]
         mlp = layer.mlp
         is_moe = isinstance(getattr(mlp, "experts", None), Experts)
         shared = getattr(mlp, "shared_experts", None) if is_moe else mlp
         if shared is not None:
-            sd[f"{pre}.shared_mlp.input_linear.weight"] = shared.gate_up_proj.weight.detach()
-            sd[f"{pre}.shared_mlp.output_linear.weight"] = shared.down_proj.weight.detach()
+            sd[f"{pre}.shared_mlp.input_linear.weight"] = _dense(shared.gate_up_proj)
+            sd[f"{pre}.shared_mlp.output_linear.weight"] = _dense(shared.down_proj)
         if isinstance(getattr(mlp, "experts", None), Experts):
             sd[f"{pre}.block_sparse_moe.input_linear.weight"] = mlp.experts.gate_up_proj.detach()
             sd[f"{pre}.block_sparse_moe.output_linear.weight"] = mlp.experts.down_proj.detach()
@@ -772,9 +785,10 @@ def hf_state_dict(model: CausalLM, per_expert: bool = False) -> dict:
             sd[f"model.{name}.k_norm.bias"] = m.k_norm_bias.detach()
         if isinstance(m, FusedLinear):
             parent = name.rsplit(".", 1)[0]
+            w = _dense(m)
             for sub in m.names:
                 r0, r1 = m.row_range(sub)
-                sd[f"model.{parent}.{sub}.weight"] = m.weight.detach()[r0:r1]
+                sd[f"model.{parent}.{sub}.weight"] = w[r0:r1]
                 if m.bias is not None:
                     sd[f"model.{parent}.{sub}.bias"] = m.bias.detach()[r0:r1]
         elif name.endswith(("input_layernorm", "post_attention_layernorm", "pre_feedforward_layernorm", "post_feedforward_layernorm",

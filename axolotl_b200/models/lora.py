@@ -427,7 +427,8 @@ def load_adapter(model, adapter_dir: str, strict: bool = True) -> LoraSpec:
 
 @torch.no_grad()
 def merge_and_unload(model):
-    """Folds every adapter into its base weight (W += s * B A) and removes the adapters."""
+    """Folds every adapter into its base weight (W += s * B A) and removes the adapters. What comes out is a dense model: frozen weights
+    held as codes are expanded whether they carry an adapter or not."""
     if getattr(model, "embed_lora_At", None) is not None:
         model.merge_embedding_lora_()
     if getattr(model, "token_rows", None) is not None:
@@ -440,6 +441,8 @@ def merge_and_unload(model):
             m.merge_lora_()
             m.lora_A = m.lora_B = m.lora_A16 = m.lora_B16 = None
             m.lora_blocks, m.lora_names, m.merged = (), [], False
+        if isinstance(m, FusedLinear):
+            m.dequantize_()
     for m in model.modules():
         if isinstance(m, Experts) and m.lora is not None:
             if m.nvfp4 is not None:
