@@ -39,6 +39,10 @@ _FUSED_OF = {"q_proj": "qkv_proj", "k_proj": "qkv_proj", "v_proj": "qkv_proj", "
 def load_state_into(model: CausalLM, named_tensors, strict: bool = True):
     """Streams (hf_name, tensor) pairs into the model. Returns the set of missing parameter slots."""
     mods = dict(model.named_modules())
+    for n, m in mods.items():
+        if isinstance(m, FusedLinear) and getattr(m.weight, "_axb_quant", None) is not None:
+            raise ValueError(f"{n} holds codes, which a checkpoint's values cannot be copied over: load the model before its base weights are "
+                             "quantised")
     filled = set()
     expert_parts = {}
     mxfp4_parts = {}

@@ -81,3 +81,19 @@ def test_written_weights_are_expanded(preset_kw, dev, tmp_path):
         if n.startswith("layers."):
             w8 = _weight8(m)
             assert ((back[n].weight.detach().double() - w8).abs() <= (BF16 if dev == "cuda" else EPS32) * w8.abs()).all(), n
+
+
+@pytest.mark.parametrize("quantize", ["fp8", "nf4"])
+def test_loading_into_coded_weights_is_refused(quantize):
+    """A checkpoint's values are no codes: a model takes them before it is coded, and the codes stay what they were."""
+    from axolotl_b200.io.hf import hf_state_dict, load_state_into
+    from axolotl_b200.models.lora import quantize_base_fp8_, quantize_base_nf4_
+
+    model = _model()
+    sd = {k: v.clone() for k, v in hf_state_dict(model).items()}
+    load_state_into(model, sd.items())
+    (quantize_base_fp8_ if quantize == "fp8" else quantize_base_nf4_)(model)
+    before = {n: m.weight.data.clone() for n, m in model.fused_linears()}
+    with pytest.raises(ValueError, match="codes"):
+        load_state_into(model, sd.items())
+    assert all(torch.equal(m.weight.data, before[n]) for n, m in model.fused_linears())
