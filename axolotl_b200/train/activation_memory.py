@@ -26,7 +26,7 @@ class _Handle:
     __slots__ = ("shape", "dtype", "device", "host", "event", "gpu", "gpu_event", "prev", "path", "future", "coded", "stream", "nbytes")
 
     def __init__(self):
-        self.host = self.event = self.gpu = self.gpu_event = self.prev = self.path = self.future = None
+        self.host = self.event = self.gpu = self.gpu_event = self.prev = self.path = self.future = self.stream = None
 
 
 class HostStore:
@@ -161,12 +161,14 @@ class Fp8Store:
     def put(self, t: torch.Tensor) -> _Handle:
         h = _Handle()
         h.shape, h.dtype, h.device = t.shape, t.dtype, t.device
-        h.stream = torch._C._cuda_getCurrentRawStream(t.device.index) if t.is_cuda else None
         if t.dtype not in (torch.bfloat16, torch.float16, torch.float32) or t.numel() == 0 or t.dim() == 0:
             h.gpu, h.coded = t.detach(), False            # kept as it is
         else:
             t = t.detach()
             h.gpu, h.coded = fp8._pack(t if t.dim() == 2 else t.reshape(-1, t.shape[-1])), True
+        if t.is_cuda:                                     # an event, since a handle of the stream says too little: that of the default
+            now = torch.cuda.current_stream(t.device)     # stream is 0, like no handle, and others may be gone when the codes are wanted
+            h.stream, h.event = now.cuda_stream, now.record_event()
         h.nbytes = h.gpu.numel() * h.gpu.element_size()
         self.bytes_out += h.nbytes
         return h
@@ -175,9 +177,9 @@ class Fp8Store:
         kept, h.gpu = h.gpu, None
         if kept is None:
             raise RuntimeError("this checkpoint has been given back already")
-        if h.stream is not None and h.stream != torch._C._cuda_getCurrentRawStream(h.device.index):
-            now = torch.cuda.current_stream(h.device)         # another stream than the one that wrote the codes
-            now.wait_stream(torch.cuda.ExternalStream(h.stream, h.device))
+        if h.event is not None and h.stream != torch._C._cuda_getCurrentRawStream(h.device.index):
+            now = torch.cuda.current_stream(h.device)     # another stream than the one that wrote the codes
+            now.wait_event(h.event)
             kept.record_stream(now)
         if not h.coded:
             return kept

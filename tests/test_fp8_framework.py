@@ -97,3 +97,88 @@ def test_loading_into_coded_weights_is_refused(quantize):
     with pytest.raises(ValueError, match="codes"):
         load_state_into(model, sd.items())
     assert all(torch.equal(m.weight.data, before[n]) for n, m in model.fused_linears())
+
+
+# ------------------------------------------------------------------ the checkpoint store on several streams
+def _values(x):
+    from axolotl_b200.ops.fp8 import dequantize_fp8_rows, quantize_fp8_rows
+
+    return dequantize_fp8_rows(*quantize_fp8_rows(x)) if x.dtype == torch.bfloat16 else x.clone()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("coded", [True, False])
+@pytest.mark.parametrize("producer,consumer", [("default", "side"), ("side", "default"), ("side", "other")])
+def test_store_waits_for_the_stream_that_wrote(producer, consumer, coded):
+    """Only the producing stream is behind: some 25 ms of sleep lie before the tensor and its codes are written, none before they are taken
+    back. The memory that the codes come to lie in holds other bytes before."""
+    from axolotl_b200.train.activation_memory import make_store
+
+    streams = {"default": torch.cuda.default_stream(), "side": torch.cuda.Stream(), "other": torch.cuda.Stream()}
+    src, dst = streams[producer], streams[consumer]
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(512, 1024, generator=g).bfloat16().cuda()
+    x = x if coded else x.double()
+    want, store = _values(x), make_store("fp8", x.device)
+    with torch.cuda.stream(src):
+        late = torch.full_like(x, 3.0)
+        scrap = [torch.full((n,), 0x38, dtype=torch.uint8, device="cuda") for n in (512 * 1024 + 8 * 512 * 4, 512 * 1024 * 8)]
+    torch.cuda.synchronize()
+    del scrap
+    with torch.cuda.stream(src):
+        torch.cuda._sleep(50_000_000)
+        late.copy_(x)
+        h = store.put(late)
+    with torch.cuda.stream(dst):
+        got = store.get(h).clone()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("coded", [True, False])
+@pytest.mark.parametrize("producer", ["default", "side"])
+def test_store_keeps_its_memory_while_another_stream_reads(producer, coded):
+    """The producer has ended, the consumer is behind: the codes' memory is not given out again before the consumer has read it."""
+    from axolotl_b200.train.activation_memory import make_store
+
+    src, dst = torch.cuda.default_stream() if producer == "default" else torch.cuda.Stream(), torch.cuda.Stream()
+    x = torch.randn(512, 1024, generator=torch.Generator().manual_seed(1)).bfloat16().cuda()
+    x = x if coded else x.double()
+    want, store = _values(x), make_store("fp8", x.device)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(src):
+        late = x.clone()
+        h = store.put(late)
+        size = h.gpu.numel() * h.gpu.element_size()
+        del late
+    src.synchronize()
+    with torch.cuda.stream(dst):
+        torch.cuda._sleep(50_000_000)
+        got = store.get(h).clone()
+    with torch.cuda.stream(src):
+        fresh = [torch.full((size,), 0x55, dtype=torch.uint8, device="cuda") for _ in range(4)]
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and fresh
+
+
+@pytest.mark.gpu
+def test_store_on_two_streams_of_one_captured_graph():
+    """Put on the capturing stream and taken back on one that it forks, every replay with new values."""
+    from axolotl_b200.train.activation_memory import make_store
+
+    x = torch.zeros(300, 520, dtype=torch.bfloat16, device="cuda")
+    store, side = make_store("fp8", x.device), torch.cuda.Stream()
+    _values(x)
+    graph, out = torch.cuda.CUDAGraph(), torch.zeros_like(x)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        h = store.put(x)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            out.copy_(store.get(h))
+        torch.cuda.current_stream().wait_stream(side)
+    for seed in (1, 2):
+        x.copy_(torch.randn(x.shape, generator=torch.Generator().manual_seed(seed)))
+        graph.replay()
+        assert torch.equal(out, _values(x))
