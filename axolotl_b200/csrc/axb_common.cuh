@@ -368,6 +368,13 @@ AXB_DEVICE void tmem_st_32x16(uint32_t taddr, const uint32_t (&r)[16]) {
 // call pdl_wait() before it touches anything the predecessor writes or reads. Both are no-ops in a plain launch.
 AXB_DEVICE void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 AXB_DEVICE void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// What the launch before this one writes while this one is there already, read behind pdl_wait(). The non-coherent load (__ldg) is for data
+// that nothing writes while the kernel lives: the compiler may move it ahead of the wait.
+AXB_DEVICE float ld_after_wait(const float* p) {
+  float v;
+  asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p));
+  return v;
+}
 
 // ------------------------------------------------------------------ distributed shared memory
 AXB_DEVICE uint32_t cluster_nctarank() {

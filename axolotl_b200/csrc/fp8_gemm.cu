@@ -257,14 +257,14 @@ __global__ void __launch_bounds__(G_THREADS, 1)
       uint64_t sum[GROUPS * 32];
 #pragma unroll
       for (int j = 0; j < GROUPS * 32; ++j) sum[j] = 0ull;
-      float na = __ldg(sa), nb0 = __ldg(sb), nb1 = GROUPS > 1 ? __ldg(sb2) : 0.f;   // the next block's, requested a block ahead
+      float na = ld_after_wait(sa), nb0 = __ldg(sb), nb1 = GROUPS > 1 ? __ldg(sb2) : 0.f;   // the next block's, requested a block ahead
       for (int kb = 0; kb < nk; ++kb) {
         const float s0 = na * nb0, s1 = na * nb1;
         na = nb0 = nb1 = 1.f;
         if (kb + 1 < nk_main) {
           sa = at_bytes(sa, step_a);
           sb = at_bytes(sb, step_b);
-          na = __ldg(sa);
+          na = ld_after_wait(sa);
           nb0 = __ldg(sb);
           if (GROUPS > 1) nb1 = __ldg(sb2 = at_bytes(sb2, step_b));
         }

@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(FS_T, 2)
     // keeps these warps within one phase of it.)
     const int t = (warp - 6) * (NT / 4) + lane;
     const bool mine = lane < NT / 4;
-    auto fetch = [&](int kb) { return mine && kb < nk_main && t < p.T ? __ldg(p.sx + kb * p.ldsx + t) : 1.f; };
+    auto fetch = [&](int kb) { return mine && kb < nk_main && t < p.T ? ld_after_wait(p.sx + kb * p.ldsx + t) : 1.f; };
     float next = fetch(kb0);
     for (int kb = kb0; kb < kb1; ++kb) {
       const int i = kb - kb0, slot = i % FS_RING;

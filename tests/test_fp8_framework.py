@@ -182,3 +182,25 @@ def test_store_on_two_streams_of_one_captured_graph():
         x.copy_(torch.randn(x.shape, generator=torch.Generator().manual_seed(seed)))
         graph.replay()
         assert torch.equal(out, _values(x))
+
+
+# ------------------------------------------------------------------ dependent launches
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,K,N", [(40, 8192, 512), (300, 2048, 1024), (2100, 1024, 2600)])
+def test_products_see_the_rows_of_the_launch_before_them(T, K, N):
+    """Codes and scales of one call lie where those of the call before lay, and their scales are far apart: a product, which starts while its
+    rows are still being quantised, gives for each what it gives alone."""
+    from axolotl_b200.ops import fp8
+
+    g = torch.Generator().manual_seed(T)
+    w, ws = fp8.quantize_fp8_weight(torch.randn(N, K, generator=g).cuda())
+    rows = [(torch.randn(T, K, generator=g) * 2.0 ** e).bfloat16().cuda() for e in (0, -20, 20, 7)]
+    alone = []
+    for x in rows:
+        alone.append(fp8._product(x, w, ws, keep=True)[0])
+        torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    together = [fp8._product(rows[i % 4], w, ws, keep=True)[0] for i in range(32)]
+    torch.cuda.synchronize()
+    for i, y in enumerate(together):
+        assert torch.equal(y, alone[i % 4]), i
