@@ -349,6 +349,10 @@ class FusedLinear(nn.Module):
         super()._apply(fn, *a, **kw)
         if st is not None:   # nn.Module._apply may rebuild the parameter object: carry the state along
             self.weight._axb_quant = st.to(self.weight.device)
+            from ..ops import fp8
+
+            if isinstance(st, fp8.Fp8State) and self.weight.dim() == 2:   # a move drops the padding of rows that are not whole 16 bytes: laid out again once, here
+                self.weight.data = fp8._rows16(self.weight.data.view(torch.float8_e4m3fn)).view(torch.uint8)
         if self.lora_A is not None:
             self.lora_A16 = None
             self.refresh_shadows()

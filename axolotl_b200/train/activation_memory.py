@@ -302,6 +302,16 @@ class OffloadSavedTensors:
         return self._ctx.__exit__(*exc)
 
 
+def _whole_rows(t):
+    """A matrix with the padding of its rows (8-bit codes start each row on 16 bytes), any other tensor as it is."""
+    if t.dim() != 2 or t.stride(1) != 1 or not 0 < (t.stride(0) - t.shape[1]) * t.element_size() < 16:
+        return t
+    ld = t.stride(0)
+    if t.storage_offset() + t.shape[0] * ld > t.untyped_storage().nbytes() // t.element_size():
+        return t
+    return t.as_strided((t.shape[0], ld), (ld, 1))
+
+
 class LayerOffloader:
     """Frozen decoder-layer weights live in pinned host memory; a layer's weights are copied to the device on
     a side stream before the layer runs (forward, recomputation and backward) and dropped afterwards, with
@@ -319,9 +329,10 @@ class LayerOffloader:
             for p in layer.parameters():
                 if p.requires_grad or getattr(p, "_axb_shard", None) is not None:
                     continue
-                h = torch.empty(p.shape, dtype=p.dtype, pin_memory=self.cuda)
-                h.copy_(p.detach())
-                entry.append((p, h))
+                full = _whole_rows(p.detach())
+                h = torch.empty(full.shape, dtype=p.dtype, pin_memory=self.cuda)
+                h.copy_(full)
+                entry.append((p, h[:, :p.shape[1]] if h.shape != p.shape else h))
                 p.data = torch.empty(0, dtype=p.dtype, device=self.device)
             self.host.append(entry)
             layer.register_forward_pre_hook(lambda m, a, i=i: self._enter(i, +1))
@@ -336,14 +347,17 @@ class LayerOffloader:
         if self.cuda:
             with torch.cuda.stream(self.stream):
                 for p, h in self.host[i]:
-                    p.data = torch.empty(h.shape, dtype=h.dtype, device=self.device)
-                    p.data.copy_(h, non_blocking=True)
+                    full = _whole_rows(h)
+                    d = torch.empty(full.shape, dtype=h.dtype, device=self.device)
+                    d.copy_(full, non_blocking=True)
+                    p.data = d if full is h else d[:, :h.shape[1]]
                 ev = torch.cuda.Event()
                 ev.record(self.stream)
             self.ready[i] = ev
         else:
             for p, h in self.host[i]:
-                p.data = h.clone()
+                full = _whole_rows(h)
+                p.data = h.clone() if full is h else full.clone()[:, :h.shape[1]]
 
     def _enter(self, i, direction):
         if direction < 0:

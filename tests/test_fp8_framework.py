@@ -204,3 +204,50 @@ def test_products_see_the_rows_of_the_launch_before_them(T, K, N):
     torch.cuda.synchronize()
     for i, y in enumerate(together):
         assert torch.equal(y, alone[i % 4]), i
+
+
+# ------------------------------------------------------------------ rows of whole 16 bytes
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("K", [2008, 200, 256])
+def test_codes_keep_their_row_layout_when_they_move(K, dev):
+    """Rows of codes start on 16 bytes as they were laid out when the weight was quantised, wherever the module goes: no product lays the
+    weight out again."""
+    from axolotl_b200.models.layers import FusedLinear
+    from axolotl_b200.ops import fp8
+
+    m = FusedLinear(K, [40], ["a"], dtype=torch.float32, device="cpu")
+    with torch.no_grad():
+        m.weight.copy_(torch.randn(40, K, generator=torch.Generator().manual_seed(1)))
+    m.quantize_fp8_()
+    codes, scale = m.weight.data.clone(), m.weight._axb_quant.scale.clone()
+    moves = [lambda: m._apply(lambda t: t.clone(memory_format=torch.contiguous_format)), lambda: m.to(dev), lambda: m.to(torch.bfloat16),
+             lambda: m.cpu(), lambda: m.to(dev)]
+    for move in moves:
+        move()
+        w = m.weight
+        assert w.stride(1) == 1 and w.stride(0) % 16 == 0 and w.data_ptr() % 16 == 0 and not w.requires_grad
+        assert torch.equal(w.data.cpu(), codes) and torch.equal(w._axb_quant.scale.cpu(), scale) and w._axb_quant.scale.device == w.device
+        assert fp8._rows16(w.data.view(torch.float8_e4m3fn)).data_ptr() == w.data_ptr()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_codes_keep_their_row_layout_under_layer_offloading(dev):
+    """The host copy has the rows' padding, and so has what comes back."""
+    from axolotl_b200.models.lora import LoraSpec, inject_lora, quantize_base_fp8_
+    from axolotl_b200.train.activation_memory import LayerOffloader
+
+    m = _model(dev, layers=3, intermediate_size=200)          # down: rows of 200 codes
+    quantize_base_fp8_(m)
+    inject_lora(m, LoraSpec(r=8, lora_alpha=16, target_modules=["q_proj"]))
+    ids = torch.randint(0, 512, (1, 32), generator=torch.Generator().manual_seed(2)).to(dev)
+    want = m(ids, labels=ids).loss.item()
+    seen = []
+    off = LayerOffloader(m, dev)
+    for layer in m.layers:
+        w = layer.mlp.down_proj.weight
+        assert w.numel() == 0
+        layer.mlp.down_proj.register_forward_pre_hook(lambda mod, a: seen.append((tuple(mod.weight.shape), mod.weight.stride())))
+    loss = m(ids, labels=ids).loss
+    loss.backward()
+    assert loss.item() == want and seen and all(shape[1] == 200 and stride == (208, 1) for shape, stride in seen)
+    assert off.bytes_per_layer
