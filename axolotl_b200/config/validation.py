@@ -96,6 +96,8 @@ def validate(cfg: dict, capabilities: dict | None = None) -> list[str]:
             raise ValueError("`base_weights_fp8` holds frozen projections: it requires `adapter: lora`")
         if (g("tensor_parallel_size") or 1) > 1:
             raise ValueError("8-bit base weights cannot be combined with tensor parallelism")
+        if g("relora"):
+            raise ValueError("`relora` folds its adapters into the base weights, which `base_weights_fp8` holds as codes")
     if ad == "llama-adapter":
         raise ValueError("`adapter: llama-adapter` is not supported")
     if g("lora_dropout") and (g("lora_mlp_kernel") or g("lora_qkv_kernel") or g("lora_o_kernel")):

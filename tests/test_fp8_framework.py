@@ -251,3 +251,18 @@ def test_codes_keep_their_row_layout_under_layer_offloading(dev):
     loss.backward()
     assert loss.item() == want and seen and all(shape[1] == 200 and stride == (208, 1) for shape, stride in seen)
     assert off.bytes_per_layer
+
+
+# ------------------------------------------------------------------ configuration
+BASE = {"model_preset": "tiny-llama", "adapter": "lora", "lora_r": 8, "lora_alpha": 16, "lora_target_linear": True, "sequence_len": 64,
+        "micro_batch_size": 1, "gradient_accumulation_steps": 1, "max_steps": 1, "learning_rate": 1e-3, "output_dir": "unused",
+        "device": "cpu", "datasets": [{"path": "synthetic", "type": "_synthetic"}], "base_weights_fp8": True}
+
+
+def test_restarts_that_fold_into_codes_are_refused():
+    from axolotl_b200.config.load import load_cfg
+
+    relora = {"relora": True, "jagged_restart_steps": 100}
+    with pytest.raises(ValueError, match="base_weights_fp8"):
+        load_cfg({**BASE, **relora})
+    assert load_cfg({**BASE, **relora, "base_weights_fp8": False})["relora"]
