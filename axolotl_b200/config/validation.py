@@ -5,6 +5,26 @@ spellings in place; warnings are returned as strings."""
 from __future__ import annotations
 
 import os
+import re
+
+
+# the projections of the decoder layers, of every family
+_PROJECTIONS = ([f"self_attn.{n}" for n in ("qkv_proj", "o_proj", "out_gate", "q_proj", "q_a_proj", "q_b_proj", "kv_a_proj_with_mqa", "kv_b_proj",
+                                            "in_proj", "out_proj", "in_proj_qkvz", "in_proj_ba", "indexer.wq_b", "indexer.wk",
+                                            "indexer.weights_proj")]
+                + [f"{m}.{n}" for m in ("mlp", "mlp.shared_expert", "mlp.shared_experts", "mixer") for n in ("gate_up_proj", "up_proj", "down_proj")]
+                + [f"{m}.{n}" for m in ("mixer", "mamba") for n in ("qkv_proj", "o_proj", "in_proj", "out_proj")]
+                + ["per_layer_input_gate", "per_layer_projection"])
+
+
+def refuse_trained_codes(cfg: dict, names) -> None:
+    """``base_weights_fp8`` holds the weights of these names as codes, which take no gradient: refuses the keys that would train one."""
+    trained = [(k, re.compile(p)) for k, p in (("unfrozen_parameters", p) for p in cfg.get("unfrozen_parameters") or [])]
+    trained += [("lora_modules_to_save", re.compile(re.escape(p))) for p in cfg.get("lora_modules_to_save") or []]
+    for n in names if trained else ():
+        for key, pattern in trained:
+            if pattern.search(n):
+                raise ValueError(f"`{key}` {pattern.pattern!r} would train {n}, which `base_weights_fp8` holds as codes")
 
 
 def validate(cfg: dict, capabilities: dict | None = None) -> list[str]:
@@ -98,6 +118,7 @@ def validate(cfg: dict, capabilities: dict | None = None) -> list[str]:
             raise ValueError("8-bit base weights cannot be combined with tensor parallelism")
         if g("relora"):
             raise ValueError("`relora` folds its adapters into the base weights, which `base_weights_fp8` holds as codes")
+        refuse_trained_codes(cfg, (f"layers.{i}.{n}.weight" for i in range(256) for n in _PROJECTIONS))
     if ad == "llama-adapter":
         raise ValueError("`adapter: llama-adapter` is not supported")
     if g("lora_dropout") and (g("lora_mlp_kernel") or g("lora_qkv_kernel") or g("lora_o_kernel")):

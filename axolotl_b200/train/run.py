@@ -123,8 +123,10 @@ def setup_adapter(cfg, model):
         saved = quantize_base_nf4_(model, double_quant=qcfg.get("bnb_4bit_use_double_quant", True) is not False)
         LOG.info("base projections stored as NF4: %.2f GiB saved", saved / 1024 ** 3)
     if cfg.get("base_weights_fp8"):
+        from ..config.validation import refuse_trained_codes
         from ..models.lora import quantize_base_fp8_
 
+        refuse_trained_codes(cfg, [n + ".weight" for n, _ in model.fused_linears() if n.startswith("layers.")])
         saved = quantize_base_fp8_(model)
         LOG.info("base projections stored in 8-bit blocks: %.2f GiB saved", saved / 1024 ** 3)
     adapter_dtype = torch.float32 if cfg.get("peft_autocast_adapter_dtype", True) is not False else model.dtype

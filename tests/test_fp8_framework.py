@@ -266,3 +266,35 @@ def test_restarts_that_fold_into_codes_are_refused():
     with pytest.raises(ValueError, match="base_weights_fp8"):
         load_cfg({**BASE, **relora})
     assert load_cfg({**BASE, **relora, "base_weights_fp8": False})["relora"]
+
+
+@pytest.mark.parametrize("key,bad,good", [
+    ("unfrozen_parameters", [r"layers\.1\.mlp\.down_proj"], [r"layers\.\d+\.input_layernorm", "embed_tokens"]),
+    ("unfrozen_parameters", ["embed_tokens", r"^layers\.0\."], ["^norm"]),
+    ("unfrozen_parameters", [r"qkv_proj\.weight$"], [r"qkv_proj\.bias$"]),
+    ("unfrozen_parameters", [r"layers\.37\.self_attn\.kv_b_proj"], ["lm_head"]),
+    ("lora_modules_to_save", ["down_proj"], ["embed_tokens", "lm_head"]),
+    ("lora_modules_to_save", ["mlp"], ["layernorm"])])
+def test_training_a_coded_projection_is_refused(key, bad, good):
+    """Codes take no gradient: what would train them is refused with the configuration, before a model is loaded."""
+    from axolotl_b200.config.load import load_cfg
+
+    with pytest.raises(ValueError, match="base_weights_fp8"):
+        load_cfg({**BASE, key: bad})
+    assert list(load_cfg({**BASE, key: good})[key]) == good
+    assert list(load_cfg({**BASE, "base_weights_fp8": False, key: bad})[key]) == bad
+
+
+def test_training_a_coded_projection_is_refused_by_its_own_name():
+    """A plugin may name parameters after the configuration was checked, and a family may have projections of other names: the model's own
+    names are checked before a weight is coded."""
+    from axolotl_b200.config.load import load_cfg
+    from axolotl_b200.train.run import setup_adapter
+
+    model = _model()
+    model.layers[1].other_proj, model.layers[1].mlp.down_proj = model.layers[1].mlp.down_proj, None
+    cfg = load_cfg(dict(BASE))
+    cfg["unfrozen_parameters"] = ["other_proj"]
+    with pytest.raises(ValueError, match="layers.1.other_proj.weight"):
+        setup_adapter(cfg, model)
+    assert all(m.weight.is_floating_point() for _, m in model.fused_linears())
