@@ -18,7 +18,9 @@ template <>
 AXB_DEVICE float to_f32(float v) { return v; }
 // two neighbouring values as they are stored
 AXB_DEVICE void put2(__nv_bfloat16* o, float2 f) { *reinterpret_cast<uint32_t*>(o) = pack_bf16x2(f.x, f.y); }
-AXB_DEVICE void put2(__half* o, float2 f) { *reinterpret_cast<__half2*>(o) = __floats2half2_rn(f.x, f.y); }
+// The largest fp16 numbers have a code that stands for 2^16, which fp16 does not have: its largest one, so that they stay finite.
+AXB_DEVICE float in_fp16(float v) { return fabsf(v) == 65536.f ? copysignf(65504.f, v) : v; }
+AXB_DEVICE void put2(__half* o, float2 f) { *reinterpret_cast<__half2*>(o) = __floats2half2_rn(in_fp16(f.x), in_fp16(f.y)); }
 AXB_DEVICE void put2(float* o, float2 f) { *reinterpret_cast<float2*>(o) = f; }
 
 // Eight values of a row as they are stored. The largest magnitude is taken in the stored type, two values an instruction: with every

@@ -171,14 +171,16 @@ def _pack_plain(x, ld, lds):
 
 
 def dequantize_fp8_rows(codes: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = torch.bfloat16):
-    """The values that the codes of ``quantize_fp8_rows`` stand for (exact in bf16 and fp32), [rows, columns]."""
+    """The values that the codes of ``quantize_fp8_rows`` stand for (exact in bf16 and fp32), [rows, columns]. In fp16 2^16, the nearest code
+    of that type's largest values, comes back as the largest one, 65504."""
     _check_codes(codes, "dequantize_fp8_rows")
     T, K = codes.shape
     _check_scale(scale, (_blocks(K), T), codes.device, "dequantize_fp8_rows")
     if dtype not in _DTYPES:
         raise TypeError(f"dequantize_fp8_rows gives bfloat16, float16 or float32, not {dtype}")
     if not codes.is_cuda:
-        return (codes.float() * scale.t().repeat_interleave(BLOCK, 1)[:, :K]).to(dtype)
+        v = codes.float() * scale.t().repeat_interleave(BLOCK, 1)[:, :K]
+        return (torch.where(v.abs() == 65536, torch.copysign(torch.full_like(v, 65504.0), v), v) if dtype == torch.float16 else v).to(dtype)
     with _device_of(codes):
         codes = _rows16(codes)
         scale, lds = _row_scales(scale, T)

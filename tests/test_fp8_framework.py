@@ -298,3 +298,29 @@ def test_training_a_coded_projection_is_refused_by_its_own_name():
     with pytest.raises(ValueError, match="layers.1.other_proj.weight"):
         setup_adapter(cfg, model)
     assert all(m.weight.is_floating_point() for _, m in model.fused_linears())
+
+
+# ------------------------------------------------------------------ rows in fp16
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("K", [264, 131])
+def test_finite_values_of_fp16_stay_finite(K, dev):
+    """From 248 * 2^8 on the nearest code stands for 2^16, which fp16 does not have: its largest number comes back, half a step of E4M3 off
+    at most. What is further beyond overflows as in any conversion."""
+    from axolotl_b200.ops.fp8 import dequantize_fp8_rows, quantize_fp8_rows
+    from axolotl_b200.train.activation_memory import make_store
+
+    x = torch.zeros(3, K, dtype=torch.float16)
+    x[0, :6] = torch.tensor([65504.0, -65504.0, 63488.0, 63456.0, -61440.0, 3.0])
+    x[1, 128:131] = torch.tensor([-65504.0, 1.0, 65472.0])
+    x[2, 0] = float("inf")
+    want = x.clone()
+    want[0, :6] = torch.tensor([65504.0, -65504.0, 65504.0, 61440.0, -61440.0, 3.0])     # 248 lies in the middle: to even, 256; scale 2^8
+    want[1, 128:131] = torch.tensor([-65504.0, 1.0, 65504.0])
+    codes, scale = quantize_fp8_rows(x.to(dev))
+    back = dequantize_fp8_rows(codes, scale, torch.float16).cpu()
+    assert torch.isnan(back[2, 0]) and back[2, 1:].abs().sum() == 0 and torch.equal(back[:2], want[:2])
+    assert dequantize_fp8_rows(codes, scale, torch.float32)[0, 0].item() == 65536.0       # what the code stands for
+    store = make_store("fp8", dev)
+    assert torch.equal(store.get(store.put(x.to(dev)))[:2].cpu(), want[:2])
+    big = torch.full((1, K), 1e5, dtype=torch.float32, device=dev)
+    assert torch.isinf(dequantize_fp8_rows(*quantize_fp8_rows(big), dtype=torch.float16)).all()
