@@ -250,9 +250,10 @@ def fp8_gemm(codes, row_scale, w_codes, w_scale, *, trans_w=False, a2=None, b2=N
         raise ValueError(f"fp8_gemm: rows of {K} columns on {codes.device} against a weight of {Kw} on {w_codes.device}")
     _check_scale(row_scale, (_blocks(K), M), codes.device, "fp8_gemm")
     K2 = 0
-    if a2 is not None:
-        if b2 is None or a2.dim() != 2 or a2.shape[0] != M or tuple(b2.shape) != ((a2.shape[1], N) if trans_w else (N, a2.shape[1])):
-            raise ValueError(f"fp8_gemm: extension {tuple(a2.shape)} x {None if b2 is None else tuple(b2.shape)} for a result [{M}, {N}]")
+    if a2 is not None or b2 is not None:
+        if a2 is None or b2 is None or a2.dim() != 2 or a2.shape[0] != M or tuple(b2.shape) != ((a2.shape[1], N) if trans_w else (N, a2.shape[1])):
+            raise ValueError("fp8_gemm: extension " + " x ".join(str(t if t is None else tuple(t.shape)) for t in (a2, b2))
+                             + f" for a result [{M}, {N}]")
         if a2.device != codes.device or b2.device != codes.device:
             raise ValueError(f"fp8_gemm: extension on {a2.device} and {b2.device}, codes on {codes.device}")
         K2 = a2.shape[1]

@@ -324,3 +324,15 @@ def test_finite_values_of_fp16_stay_finite(K, dev):
     assert torch.equal(store.get(store.put(x.to(dev)))[:2].cpu(), want[:2])
     big = torch.full((1, K), 1e5, dtype=torch.float32, device=dev)
     assert torch.isinf(dequantize_fp8_rows(*quantize_fp8_rows(big), dtype=torch.float16)).all()
+
+
+# ------------------------------------------------------------------ arguments
+@pytest.mark.parametrize("dev", DEVICES)
+def test_half_an_extension_is_refused(dev):
+    from axolotl_b200.ops.fp8 import fp8_gemm, quantize_fp8_rows, quantize_fp8_weight
+
+    codes, scale = quantize_fp8_rows(torch.ones(4, 128, device=dev).bfloat16())
+    w, ws = quantize_fp8_weight(torch.ones(64, 128, device=dev))
+    for kw in (dict(b2=torch.zeros(64, 8, device=dev).bfloat16()), dict(a2=torch.zeros(4, 8, device=dev).bfloat16())):
+        with pytest.raises(ValueError, match="extension"):
+            fp8_gemm(codes, scale, w, ws, **kw)
