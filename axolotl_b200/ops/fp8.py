@@ -514,8 +514,7 @@ def _adapter_grad(t, q, ldq, s, lds, K, out):
         return torch.zeros((R, K), dtype=torch.float32, device=t.device) if out is None else out
     if out is not None and out.stride(1) != 1:
         return out.add_(_adapter_grad(t, q, ldq, s, lds, K, None))
-    if t.stride(1) != 1 or t.stride(0) % 8 or t.data_ptr() % 16:
-        t = torch.nn.functional.pad(t, (0, -R % 8))[:, :R] if R % 8 else t.contiguous()
+    t = _operand(t, "fp8_adapter_grad")
     add = out is not None
     if not add:
         out = torch.empty((R, K), dtype=torch.float32, device=t.device)

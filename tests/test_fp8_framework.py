@@ -336,3 +336,22 @@ def test_half_an_extension_is_refused(dev):
     for kw in (dict(b2=torch.zeros(64, 8, device=dev).bfloat16()), dict(a2=torch.zeros(4, 8, device=dev).bfloat16())):
         with pytest.raises(ValueError, match="extension"):
             fp8_gemm(codes, scale, w, ws, **kw)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("T", [1, 70, 200])
+def test_adapter_gradient_of_rows_in_any_layout(T, dev):
+    """t as one row for all tokens, as overlapping rows, as columns of a wider matrix and transposed: what it gives laid out plainly. The
+    factors are small integers and the rows their own codes, so that every sum is exact."""
+    from axolotl_b200.ops.fp8 import fp8_adapter_grad, quantize_fp8_rows
+
+    g = torch.Generator().manual_seed(T)
+    x = torch.randint(-2, 3, (T, 264), generator=g).bfloat16().to(dev)
+    codes, scale = quantize_fp8_rows(x)
+    flat = torch.randint(-2, 3, (T * 40 + 64,), generator=g).bfloat16().to(dev)
+    for t in (flat[:16].expand(T, 16), flat.as_strided((T, 16), (8, 1)), flat[:T * 40].view(T, 40)[:, 3:19],
+              flat[:T * 16].view(16, T).t(), flat[:1].expand(T, 1), flat[:T * 9].view(T, 9)):
+        want = t.cpu().double().t() @ x.cpu().double()
+        assert torch.equal(fp8_adapter_grad(t, codes, scale).cpu().double(), want), t.stride()
+        out = torch.ones(want.shape, device=dev)
+        assert torch.equal(fp8_adapter_grad(t, codes, scale, out=out).cpu().double(), want + 1)
