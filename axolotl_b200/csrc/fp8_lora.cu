@@ -7,9 +7,9 @@ extern "C" int axb_gemm_skinny(const void* P, long long ldp, const void* S, long
                                int K, const void* P2, long long ldp2, const void* S2, long long lds2, int K2, float alpha,
                                const void* bias, int out_mode, int out_f32, int glu_kind, float glu_limit, int p_dep, int splits,
                                int pdl, int* status, void* stream);
-extern "C" int axb_lora_bwd_dy(const void* dy, long long ld_dy, const void* B, long long ld_b, const void* xa, long long ld_xa, float* t32,
-                               float* dB32, long long ldb32, int T, int N, int R, const int* blocks, int n_lora_blocks, int* status,
-                               void* stream);
+extern "C" int axb_lora_bwd_dy_parts(const void* dy, long long ld_dy, const void* B, long long ld_b, const void* xa, long long ld_xa,
+                                     float* t_parts, float* dB_parts, int T, int N, int R, const int* blocks, int n_lora_blocks, int splits,
+                                     int* status, void* stream);
 extern "C" int axb_fp8_low_pays(int T, int K);
 extern "C" int axb_fp8_quantize_low(const void* x, long long ldx, const void* A, long long lda, void* q, long long ldq, float* s, long long lds,
                                     void* xa, long long ldxa, int T, int K, int R, float scale, int* status, void* stream);
@@ -21,16 +21,82 @@ extern "C" int axb_fp8_adapter_grad(const void* q, long long ldq, const float* s
 
 namespace {
 
-// bf16 of `scale` times a and of b, one after the other in memory (n4 and m4 groups of four): t and the gradient of B in one launch
-__global__ void __launch_bounds__(256) fp8_lora_cast_kernel(const float4* __restrict__ a, const float4* __restrict__ b, uint2* __restrict__ a16,
-                                                            uint2* __restrict__ b16, long long n4, long long m4, float scale) {
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n4 + m4) return;
-  const float4 v = i < n4 ? a[i] : b[i - n4];
-  const float s = i < n4 ? scale : 1.f;
-  const uint2 o = make_uint2(pack_bf16x2(v.x * s, v.y * s), pack_bf16x2(v.z * s, v.w * s));
-  if (i < n4) a16[i] = o;
-  else b16[i - n4] = o;
+constexpr int JOIN_ROWS = 8192;           // rows of dy whose parts are there at once (16 row chunks of csrc/lora_fused.cu)
+
+struct JoinParams {
+  const float4* t_parts;                  // [splits][T, R]
+  const float4* dB_parts;                 // [chunks][N, R]; nothing outside the diagonal blocks
+  uint2* t;                               // bf16 [T, R]: scale x the sum
+  const float* dB_old;                    // what the sum is added to (null: nothing); row strides ld
+  float* dB;                              // fp32 (null: none)
+  uint2* dB16;                            // bf16 [N, R] (null: none)
+  long long ld;
+  int T, N, R, splits, chunks, n_blocks;
+  int row0[8], rows[8], r0[8], r[8];
+  float scale;
+};
+
+// The sum of `count` parts at p, p + stride, .. by four lanes (l, l + 8, l + 16, l + 24), each every fourth of them, then across the lanes:
+// the same order every time.
+AXB_DEVICE float4 join4(const float4* p, long long stride, int count, bool any) {
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (any) {
+#pragma unroll 4
+    for (int s = (threadIdx.x & 31) >> 3; s < count; s += 4) {
+      const float4 v = __ldg(p + s * stride);
+      a.x += v.x;
+      a.y += v.y;
+      a.z += v.z;
+      a.w += v.w;
+    }
+  }
+#pragma unroll
+  for (int o = 8; o < 32; o <<= 1) {
+    a.x += __shfl_xor_sync(0xffffffffu, a.x, o);
+    a.y += __shfl_xor_sync(0xffffffffu, a.y, o);
+    a.z += __shfl_xor_sync(0xffffffffu, a.z, o);
+    a.w += __shfl_xor_sync(0xffffffffu, a.w, o);
+  }
+  return a;
+}
+
+// t and the gradient of B from the parts of csrc/lora_fused.cu, four neighbouring values of a row for four lanes. Bound: the parts' bytes,
+// most of them still in the L2 (8192 x 14336, rank 16: 9 x 0.5 MB of t, 16 x 0.9 MB of B).
+__global__ void __launch_bounds__(256) fp8_lora_join_kernel(const __grid_constant__ JoinParams p) {
+  const int lane = threadIdx.x & 31, q = p.R >> 2;
+  const long long n = (long long)p.T * q, n8 = (n + 7) & ~7ll, m = (long long)p.N * q;
+  const long long u = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * 8 + (lane & 7);      // a warp is all t or all B
+  if (u < n8) {
+    const float4 a = join4(p.t_parts + u, n, p.splits, u < n);
+    if (lane < 8 && u < n) p.t[u] = make_uint2(pack_bf16x2(a.x * p.scale, a.y * p.scale), pack_bf16x2(a.z * p.scale, a.w * p.scale));
+    return;
+  }
+  const long long i = u - n8;
+  const int row = (int)(i / q), c = (int)(i % q) * 4;
+  int lo = 0, hi = 0;                     // columns of this row's block
+  for (int b = 0; b < p.n_blocks; ++b)
+    if (i < m && row >= p.row0[b] && row < p.row0[b] + p.rows[b]) {
+      lo = p.r0[b];
+      hi = p.r0[b] + p.r[b];
+    }
+  const bool any = c < hi && c + 4 > lo;
+  const float4 a = join4(p.dB_parts + i, m, p.chunks, any);
+  if (lane >= 8 || i >= m) return;
+  const float in[4] = {a.x, a.y, a.z, a.w};
+  float v[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    v[j] = (c + j >= lo && c + j < hi ? in[j] : 0.f) + (p.dB_old ? p.dB_old[row * p.ld + c + j] : 0.f);
+  if (p.dB) {
+    float* o = p.dB + row * p.ld + c;
+    if ((p.ld & 3) == 0 && (reinterpret_cast<uintptr_t>(p.dB) & 15) == 0) {
+      *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[j] = v[j];
+    }
+  }
+  if (p.dB16) p.dB16[i] = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
 }
 
 }  // namespace
@@ -46,18 +112,20 @@ struct AxbFp8Lora {
   void* xa;                // scaling x A^T, bf16 [T, R]: written by the forward pass, read by the backward pass
   void* y;                 // y [T, N], or dx [T, K] (null: not wanted)
   const void* qx;          // backward: 8-bit rows of x
-  float* t32;              // backward scratch: [T, R] fp32, [T, R] bf16
+  float* t_parts;          // backward scratch: fp32 [splits][min(T, 8192), R], [ceil of that many rows / 512][N, R]; bf16 [T, R]
+  float* dB_parts;
   void* t;
   void* dA;                // [R, K] (null: not wanted), fp32 or, where dA_bf16 is set, bf16
   float* dB;               // fp32 [N, R]; both are added to where add_* is set, else written
-  void* dB16;              // its bf16 copy (null: none; dB is then scratch without gaps)
+  void* dB16;              // bf16 [N, R] instead of dB (null: none; dB is then scratch of row stride R, wanted beyond 8192 rows)
   const int* blocks;       // diagonal blocks of B
   int* status;
   long long ldx, ldw, sw_n, sw_k, lda, ldb, ldda, lddb;
-  int T, N, K, R, tile, n_blocks, add_dA, add_dB, dA_bf16;
+  int T, N, K, R, tile, n_blocks, splits, add_dA, add_dB, dA_bf16;
   float scaling;
+  int pad;
 };
-static_assert(sizeof(AxbFp8Lora) == 16 * 8 + 8 * 8 + 10 * 4, "no gaps");
+static_assert(sizeof(AxbFp8Lora) == 17 * 8 + 8 * 8 + 12 * 4, "no gaps");
 
 extern "C" int axb_fp8_lora_fwd(const AxbFp8Lora* l, void* stream) {
   if (l->T <= 0) return 0;
@@ -78,18 +146,40 @@ extern "C" int axb_fp8_lora_fwd(const AxbFp8Lora* l, void* stream) {
 extern "C" int axb_fp8_lora_bwd(const AxbFp8Lora* l, void* stream) {
   if (l->T <= 0) return 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const long long n = (long long)l->T * l->R;
-  const bool joined = !l->add_dB && l->dB == l->t32 + n && l->lddb == l->R;     // one block of zeros
-  cudaError_t e = cudaMemsetAsync(l->t32, 0, (n + (joined ? (long long)l->N * l->R : 0)) * sizeof(float), st);
-  if (e == cudaSuccess && !joined && !l->add_dB) e = cudaMemset2DAsync(l->dB, l->lddb * sizeof(float), 0, l->R * sizeof(float), l->N, st);
-  if (e != cudaSuccess) return (int)e;
-  int rc = axb_lora_bwd_dy(l->x, l->ldx, l->B, l->ldb, l->xa, l->R, l->t32, l->dB, l->lddb, l->T, l->N, l->R, l->blocks, l->n_blocks,
-                           l->status, stream);
-  if (rc) return rc;
-  const long long n4 = n / 4, m4 = l->dB16 ? (long long)l->N * l->R / 4 : 0;      // R is a multiple of 8
-  fp8_lora_cast_kernel<<<(unsigned)((n4 + m4 + 255) / 256), 256, 0, st>>>((const float4*)l->t32, (const float4*)l->dB, (uint2*)l->t,
-                                                                           (uint2*)l->dB16, n4, m4, l->scaling);
-  rc = (int)cudaGetLastError();
+  if (l->n_blocks < 1 || l->n_blocks > 8 || (l->T > JOIN_ROWS && !l->dB)) return -2;
+  int rc = 0;
+  JoinParams p = {};
+  p.t_parts = reinterpret_cast<const float4*>(l->t_parts);
+  p.dB_parts = reinterpret_cast<const float4*>(l->dB_parts);
+  p.ld = l->dB16 ? l->R : l->lddb;
+  p.N = l->N;
+  p.R = l->R;
+  p.splits = l->splits;
+  p.n_blocks = l->n_blocks;
+  p.scale = l->scaling;
+  for (int b = 0; b < l->n_blocks; ++b) {
+    p.row0[b] = l->blocks[4 * b];
+    p.rows[b] = l->blocks[4 * b + 1];
+    p.r0[b] = l->blocks[4 * b + 2];
+    p.r[b] = l->blocks[4 * b + 3];
+  }
+  for (int row = 0; row < l->T && !rc; row += JOIN_ROWS) {        // the parts of 8192 rows at a time: some 64 N R bytes of scratch
+    const bool first = row == 0, last = l->T - row <= JOIN_ROWS;
+    p.T = last ? l->T - row : JOIN_ROWS;
+    p.chunks = (p.T + 511) / 512;
+    const long long at = (long long)row * l->R;
+    rc = axb_lora_bwd_dy_parts(static_cast<const char*>(l->x) + 2ll * row * l->ldx, l->ldx, l->B, l->ldb,
+                               static_cast<const char*>(l->xa) + 2 * at, l->R, l->t_parts, l->dB_parts, p.T, l->N, l->R, l->blocks,
+                               l->n_blocks, l->splits, l->status, stream);
+    if (rc) break;
+    p.t = reinterpret_cast<uint2*>(static_cast<char*>(l->t) + 2 * at);
+    p.dB_old = first && (l->dB16 || !l->add_dB) ? nullptr : l->dB;
+    p.dB = l->dB16 && last ? nullptr : l->dB;
+    p.dB16 = last ? reinterpret_cast<uint2*>(l->dB16) : nullptr;
+    const long long groups = (((long long)p.T * (p.R >> 2) + 7) & ~7ll) + (long long)p.N * (p.R >> 2);
+    fp8_lora_join_kernel<<<(unsigned)((groups + 63) / 64), 256, 0, st>>>(p);
+    rc = (int)cudaGetLastError();
+  }
   if (!rc && l->y)
     rc = axb_fp8_linear(l->x, l->ldx, l->q, l->W, l->ldw, l->sw, l->sw_k, l->sw_n, 1, l->y, l->T, l->K, l->N, l->t, l->R, l->A, l->lda, l->R,
                         l->tile, l->status, stream);

@@ -15,7 +15,8 @@
 //   warp 0 (one lane): TMA producer   - xa sub-tiles once, then per column block the B tile and 4 dY tiles
 //   warp 1 (one lane): MMA issuer     - t accumulators (4 x R columns of TMEM) live for the whole CTA,
 //                                       dB accumulators are double buffered per column block
-//   warps 2-5        : epilogue       - fp32 reductions into t32 / dB32 (several CTAs share every row)
+//   warps 2-5        : epilogue       - fp32 reductions into t32 / dB32 (several CTAs share every row), or (PARTS) stores: what a CTA
+//                                       has summed goes to a place of its own, and the caller adds the parts in a fixed order
 #include "axb_common.cuh"
 
 namespace {
@@ -32,14 +33,15 @@ struct LoraBwdParams {
   int T, N, R, Rpad;
   int n_blocks;        // ceil(N / 128)
   int n_splits;        // CTAs along N
-  float* t32;          // [T, R]
-  float* dB32;         // [N, ldb32]
+  float* t32;          // [T, R]; PARTS: [n_splits][T, R]
+  float* dB32;         // [N, ldb32]; PARTS: [row chunks][N, R]
   long long ldb32;
   int n_lora_blocks;
   int blk_row0[8], blk_rows[8], blk_r0[8], blk_r[8];
   int* status;
 };
 
+template <bool PARTS>
 __global__ void __launch_bounds__(LF_THREADS, 1)
     lora_bwd_dy_kernel(const __grid_constant__ CUtensorMap tmDY, const __grid_constant__ CUtensorMap tmB,
                        const __grid_constant__ CUtensorMap tmXA, const LoraBwdParams p) {
@@ -201,10 +203,20 @@ __global__ void __launch_bounds__(LF_THREADS, 1)
           tmem_ld_32x16(t_addr + c, v);
           tmem_ld_wait();
           if (n < p.N && c < r0 + r && c + 16 > r0) {
-            float* dst = p.dB32 + (long long)n * p.ldb32 + c;
+            float* dst = PARTS ? p.dB32 + ((long long)t_chunk * p.N + n) * p.R + c : p.dB32 + (long long)n * p.ldb32 + c;
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-              if (c + j >= r0 && c + j < r0 + r) atomicAdd(dst + j, __uint_as_float(v[j]));
+            for (int j = 0; j < 16; j += 4) {
+              if (PARTS && c + j >= r0 && c + j + 4 <= r0 + r) {       // R is a multiple of 8
+                *reinterpret_cast<uint4*>(dst + j) = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+                continue;
+              }
+#pragma unroll
+              for (int i = j; i < j + 4; ++i)
+                if (c + i >= r0 && c + i < r0 + r) {
+                  if constexpr (PARTS) dst[i] = __uint_as_float(v[i]);
+                  else atomicAdd(dst + i, __uint_as_float(v[i]));
+                }
+            }
           }
         }
         tc_fence_before();
@@ -221,10 +233,17 @@ __global__ void __launch_bounds__(LF_THREADS, 1)
             tmem_ld_32x16(t_addr + c, v);
             tmem_ld_wait();
             if (t < p.T) {
-              float* dst = p.t32 + (long long)t * p.R + c;
+              float* dst = p.t32 + ((PARTS ? (long long)split * p.T : 0) + t) * p.R + c;
 #pragma unroll
-              for (int j = 0; j < 16; ++j)
-                if (c + j < p.R) atomicAdd(dst + j, __uint_as_float(v[j]));
+              for (int j = 0; j < 16; j += 4) {
+                if (PARTS) {                                           // R is a multiple of 8
+                  if (c + j < p.R) *reinterpret_cast<uint4*>(dst + j) = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+                  continue;
+                }
+#pragma unroll
+                for (int i = j; i < j + 4; ++i)
+                  if (c + i < p.R) atomicAdd(dst + i, __uint_as_float(v[i]));
+              }
             }
           }
         }
@@ -239,15 +258,9 @@ __global__ void __launch_bounds__(LF_THREADS, 1)
   }
 }
 
-}  // namespace
-
-// dY [T, N] (ld_dy), B [N, R] (ld_b), xa [T, R] (ld_xa): bf16 row-major, R <= 64, all leading dimensions
-// multiples of 8. t32 [T, R] and dB32 [N, ldb32] are fp32 and are ACCUMULATED into (zero t32 first).
-// blocks: n_blocks x (row0, rows, r0, r) diagonal blocks of B (HOST array of 4 * n_blocks ints).
-extern "C" int axb_lora_bwd_dy(const void* dy, long long ld_dy, const void* B, long long ld_b, const void* xa,
-                               long long ld_xa, float* t32, float* dB32, long long ldb32, int T, int N, int R,
-                               const int* blocks, int n_lora_blocks, int* status, void* stream) {
-  if (T <= 0 || N <= 0 || R <= 0) return 0;
+template <bool PARTS>
+int launch_lora_bwd_dy(const void* dy, long long ld_dy, const void* B, long long ld_b, const void* xa, long long ld_xa, float* t32, float* dB32,
+                       long long ldb32, int T, int N, int R, const int* blocks, int n_lora_blocks, int splits, int* status, void* stream) {
   if (R > 64 || n_lora_blocks < 1 || n_lora_blocks > 8) return -3;
   if ((ld_dy & 7) || (ld_b & 7) || (ld_xa & 7)) return -2;
   CUtensorMap tDY, tB, tXA;
@@ -260,13 +273,7 @@ extern "C" int axb_lora_bwd_dy(const void* dy, long long ld_dy, const void* B, l
   p.T = T; p.N = N; p.R = R; p.Rpad = (R + 15) & ~15;
   p.n_blocks = (N + 127) / 128;
   const int t_chunks = (T + LF_ROWS - 1) / LF_ROWS;
-  int dev = 0, sms = 148;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  int splits = sms / t_chunks;
-  if (splits < 1) splits = 1;
-  if (splits > p.n_blocks) splits = p.n_blocks;
-  p.n_splits = splits;
+  p.n_splits = splits < 1 ? 1 : (splits > p.n_blocks ? p.n_blocks : splits);
   p.t32 = t32; p.dB32 = dB32; p.ldb32 = ldb32;
   p.n_lora_blocks = n_lora_blocks;
   for (int b = 0; b < n_lora_blocks; ++b) {
@@ -274,12 +281,36 @@ extern "C" int axb_lora_bwd_dy(const void* dy, long long ld_dy, const void* B, l
     p.blk_r0[b] = blocks[4 * b + 2]; p.blk_r[b] = blocks[4 * b + 3];
   }
   p.status = status;
-  static bool attr_set = false;
-  if (!attr_set) {
-    cudaError_t e = cudaFuncSetAttribute(lora_bwd_dy_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, LF_SMEM);
-    if (e != cudaSuccess) return (int)e;
-    attr_set = true;
-  }
-  lora_bwd_dy_kernel<<<t_chunks * splits, LF_THREADS, LF_SMEM, reinterpret_cast<cudaStream_t>(stream)>>>(tDY, tB, tXA, p);
+  static std::atomic<unsigned long long> allowed{0};
+  if (const int e = axb_allow_smem((const void*)lora_bwd_dy_kernel<PARTS>, LF_SMEM, allowed)) return e;
+  lora_bwd_dy_kernel<PARTS><<<t_chunks * p.n_splits, LF_THREADS, LF_SMEM, reinterpret_cast<cudaStream_t>(stream)>>>(tDY, tB, tXA, p);
   return (int)cudaGetLastError();
+}
+
+}  // namespace
+
+// dY [T, N] (ld_dy), B [N, R] (ld_b), xa [T, R] (ld_xa): bf16 row-major, R <= 64, all leading dimensions
+// multiples of 8. t32 [T, R] and dB32 [N, ldb32] are fp32 and are ACCUMULATED into (zero t32 first).
+// blocks: n_blocks x (row0, rows, r0, r) diagonal blocks of B (HOST array of 4 * n_blocks ints).
+extern "C" int axb_lora_bwd_dy(const void* dy, long long ld_dy, const void* B, long long ld_b, const void* xa,
+                               long long ld_xa, float* t32, float* dB32, long long ldb32, int T, int N, int R,
+                               const int* blocks, int n_lora_blocks, int* status, void* stream) {
+  if (T <= 0 || N <= 0 || R <= 0) return 0;
+  int dev = 0, sms = 148;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return launch_lora_bwd_dy<false>(dy, ld_dy, B, ld_b, xa, ld_xa, t32, dB32, ldb32, T, N, R, blocks, n_lora_blocks,
+                                   sms / ((T + LF_ROWS - 1) / LF_ROWS), status, stream);
+}
+
+// The same sums in parts, each written once by one CTA: t_parts fp32 [splits][T, R], dB_parts fp32 [ceil(T / 512)][N, R], of which only the
+// columns of the diagonal blocks are written; R a multiple of 8, both on 16 bytes, 1 <= splits <= ceil(N / 128). Added in a fixed order they
+// are the same bits every time.
+extern "C" int axb_lora_bwd_dy_parts(const void* dy, long long ld_dy, const void* B, long long ld_b, const void* xa, long long ld_xa,
+                                     float* t_parts, float* dB_parts, int T, int N, int R, const int* blocks, int n_lora_blocks, int splits,
+                                     int* status, void* stream) {
+  if (T <= 0 || N <= 0 || R <= 0) return 0;
+  if ((R & 7) || splits < 1 || splits > (N + 127) / 128) return -2;
+  if ((reinterpret_cast<uintptr_t>(t_parts) | reinterpret_cast<uintptr_t>(dB_parts)) & 15) return -2;
+  return launch_lora_bwd_dy<true>(dy, ld_dy, B, ld_b, xa, ld_xa, t_parts, dB_parts, R, T, N, R, blocks, n_lora_blocks, splits, status, stream);
 }

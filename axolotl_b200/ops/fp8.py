@@ -379,16 +379,16 @@ class _Fp8LinearFn(torch.autograd.Function):
         return dx, None, None, dbias
 
 
-_LORA = struct.Struct("@16P8q9if")      # AxbFp8Lora of csrc/fp8_lora.cu
+_LORA = struct.Struct("@17P8q10ifi")      # AxbFp8Lora of csrc/fp8_lora.cu
 
 
-def _lora_call(entry, x, codes, scale, A16, B16, scaling, sizes, q, xa, y, qx=0, t32=0, t=0, dA=0, dB=0, dB16=0, blocks=0,
-               ldda=0, lddb=0, n_blocks=0, add_dA=False, add_dB=False, dA_bf16=False):
+def _lora_call(entry, x, codes, scale, A16, B16, scaling, sizes, q, xa, y, qx=0, t_parts=0, dB_parts=0, t=0, dA=0, dB=0, dB16=0, blocks=0,
+               ldda=0, lddb=0, n_blocks=0, splits=0, add_dA=False, add_dB=False, dA_bf16=False):
     """One call of csrc/fp8_lora.cu; ``q`` .. ``blocks`` are addresses, ``sizes`` is (T, N, K, R, tile)."""
     status, stream = _lib.launch_args(x.device.index)
-    args = _LORA.pack(x.data_ptr(), q, codes.data_ptr(), scale.data_ptr(), A16.data_ptr(), B16.data_ptr(), xa, y, qx, t32, t, dA, dB, dB16,
-                      blocks, status, x.stride(0), codes.stride(0), *scale.stride(), A16.stride(0), B16.stride(0), ldda, lddb, *sizes, n_blocks,
-                      add_dA, add_dB, dA_bf16, scaling)
+    args = _LORA.pack(x.data_ptr(), q, codes.data_ptr(), scale.data_ptr(), A16.data_ptr(), B16.data_ptr(), xa, y, qx, t_parts, dB_parts, t, dA,
+                      dB, dB16, blocks, status, x.stride(0), codes.stride(0), *scale.stride(), A16.stride(0), B16.stride(0), ldda, lddb, *sizes,
+                      n_blocks, splits, add_dA, add_dB, dA_bf16, scaling, 0)
     _lib.check_rc(entry(args, stream), "fp8_lora")
 
 
@@ -443,19 +443,23 @@ class _Fp8LoRALinearFn(torch.autograd.Function):
         dx = dA = dB = None
         if (need[4] and USE_FUSED_DY and T and R <= 64 and R % 8 == 0 and len(ctx.blocks) <= 8 and xa.is_contiguous()
                 and all(map(_operand16, (dy, A16, B16, xa)))):
-            # one pass over dy for t and dB, the product and dA behind it: one call. Scratch: t in fp32, dB in fp32 (where its place is
-            # elsewhere it is not there), t in bf16, the rows of dy in 8 bits
-            n, tA, tB = T * R, getattr(A, "_axb_grad", None), getattr(B, "_axb_grad", None)
+            # one pass over dy for t and dB, the product and dA behind it: one call. Scratch: the parts of t and of dB (a CTA of
+            # csrc/lora_fused.cu holds 512 rows and one of `splits` ranges of dy's columns), dB in fp32 (where more than 8192 rows are summed
+            # into a bf16 one), t in bf16, the rows of dy in 8 bits
+            tA, tB = getattr(A, "_axb_grad", None), getattr(B, "_axb_grad", None)
             low = [w is None and p.dtype == torch.bfloat16 for w, p in ((tA, A), (tB, B))]
-            at = [4 * n, 4 * N * R if low[1] else 0, 2 * n]
+            rows = min(T, 8192)
+            chunks = -(-rows // 512)
+            splits = min(148 // chunks, _blocks(N))
+            at = [4 * splits * rows * R, 4 * chunks * N * R, 4 * N * R if low[1] and T > rows else 0, 2 * T * R]
             work = dy.new_empty(sum(at) + (_packed_size(T, N) if need[0] else 0), dtype=torch.uint8)
             p = work.data_ptr()
-            args = dict(t32=p, t=p + at[0] + at[1])
+            args = dict(t_parts=p, dB_parts=p + at[0], t=p + sum(at[:3]), splits=splits)
             if need[0]:
                 dx = dy.new_empty((T, K))
             if low[1]:
                 dB = dy.new_empty((N, R))
-                args.update(dB=p + at[0], dB16=dB.data_ptr(), lddb=R)
+                args.update(dB=p + at[0] + at[1] if at[2] else 0, dB16=dB.data_ptr(), lddb=R)
             else:
                 dB = tB if tB is not None else dy.new_empty((N, R), dtype=torch.float32)
                 args.update(dB=dB.data_ptr(), lddb=dB.stride(0), add_dB=tB is not None)

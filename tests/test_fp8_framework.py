@@ -355,3 +355,111 @@ def test_adapter_gradient_of_rows_in_any_layout(T, dev):
         assert torch.equal(fp8_adapter_grad(t, codes, scale).cpu().double(), want), t.stride()
         out = torch.ones(want.shape, device=dev)
         assert torch.equal(fp8_adapter_grad(t, codes, scale, out=out).cpu().double(), want + 1)
+
+
+# ------------------------------------------------------------------ adapters
+def _rows8(x):
+    from axolotl_b200.ops.fp8 import dequantize_fp8_rows, quantize_fp8_rows
+
+    return dequantize_fp8_rows(*quantize_fp8_rows(x.cpu()), dtype=torch.float32).double()
+
+
+def _adapter(N, K, blocks, seed=1):
+    """(A, B) in fp32 with bf16 values, B block diagonal."""
+    g = torch.Generator().manual_seed(seed)
+    R = sum(b[3] for b in blocks)
+    A, B = (torch.randn(R, K, generator=g) * K ** -0.5).bfloat16().float(), torch.zeros(N, R)
+    for r0, rows, c0, r in blocks:
+        B[r0:r0 + rows, c0:c0 + r] = (torch.randn(rows, r, generator=g) * 0.1).bfloat16().float()
+    return A, B
+
+
+QKV = ((0, 256, 0, 16), (256, 64, 16, 16), (320, 64, 32, 16))                    # q | k | v, rank 16 each
+ADAPTERS = [(1, 264, 384, QKV), (513, 264, 384, QKV), (960, 520, 640, ((0, 640, 0, 16),)), (700, 136, 264, ((0, 100, 0, 3), (100, 150, 3, 5))),
+            (130, 264, 520, ((0, 264, 0, 32), (264, 256, 32, 32))), (8192, 136, 128, ((0, 128, 0, 8),)), (8200, 136, 264, ((8, 200, 0, 8),)),
+            (17000, 136, 384, QKV)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("masters", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,K,N,blocks", ADAPTERS)
+def test_adapter_gradients_repeat_and_are_what_they_are(T, K, N, blocks, masters):
+    """The sums over column ranges and row chunks are joined in one order: the same bits every time. Against 64 bits: s x A^T and s dy B are
+    held in bf16 (2^-8 of themselves and their sums in fp32), each sum of n products is off by n 2^-23 of the sum of magnitudes."""
+    from axolotl_b200.ops.fp8 import fp8_lora_linear, quantize_fp8_weight
+
+    g = torch.Generator().manual_seed(T)
+    x, dy = torch.randn(T, K, generator=g).bfloat16(), (torch.randn(T, N, generator=g) * 1e-2).bfloat16()
+    w, ws = quantize_fp8_weight(torch.randn(N, K, generator=g).cuda())
+    A, B = _adapter(N, K, blocks)
+    leaves = [x.cuda().requires_grad_(True)] + [t.to(masters).cuda().requires_grad_(True) for t in (A, B)]
+    A16, B16 = A.bfloat16().cuda(), B.bfloat16().cuda()
+    runs = []
+    for _ in range(4):
+        y = fp8_lora_linear(leaves[0], w, ws, leaves[1], leaves[2], A16, B16, 2.0, blocks)
+        runs.append([y.detach(), *torch.autograd.grad(y, leaves, dy.cuda())])
+    assert all(torch.equal(a, b) for r in runs[1:] for a, b in zip(runs[0], r))
+    y, dx, dA, dB = (t.cpu().double() for t in runs[0])
+    a, b, x64, d64, x8 = A.double(), B.double(), x.double(), dy.double(), _rows8(x)
+    low, tall = 2 * x64 @ a.t(), 2 * d64 @ b
+    low_e = BF16 * low.abs() + (K + 2) * EPS32 * 2 * x64.abs() @ a.abs().t()
+    tall_e = BF16 * tall.abs() + (N + 2) * EPS32 * 2 * d64.abs() @ b.abs()
+    half = BF16 if masters == torch.bfloat16 else 0.0
+    for got, want, off, size in ((dA, tall.t() @ x8, tall_e.t() @ x8.abs(), tall.abs().t() @ x8.abs()),
+                                 (dB, d64.t() @ low, d64.abs().t() @ low_e, d64.abs().t() @ low.abs())):
+        tol = half * (1 + BF16) * want.abs() + (1 + half) * off + (T + 32) * EPS32 * size
+        if got is dB:
+            inside = torch.zeros(N, B.shape[1], dtype=torch.bool)
+            for r0, rows, c0, r in blocks:
+                inside[r0:r0 + rows, c0:c0 + r] = True
+            assert (got[~inside] == 0).all()
+            want, tol = want * inside, tol * inside
+        assert ((got - want).abs() <= tol + 1e-30).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [300, 8200])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_adapter_gradients_add_to_flat_buffers_in_order(T, shift):
+    """Gradients that are added where the optimizer keeps them, at any address: twice the same pass is one pass and its own sum, and what
+    lies beside the buffer and outside the blocks stays."""
+    from axolotl_b200.ops.fp8 import fp8_lora_linear, quantize_fp8_weight
+
+    K, N, R = 264, 384, 48
+    g = torch.Generator().manual_seed(T)
+    x, dy = torch.randn(T, K, generator=g).bfloat16().cuda(), (torch.randn(T, N, generator=g) * 1e-2).bfloat16().cuda()
+    w, ws = quantize_fp8_weight(torch.randn(N, K, generator=g).cuda())
+    A, B = (t.cuda().requires_grad_(True) for t in _adapter(N, K, QKV))
+    A16, B16 = A.detach().bfloat16(), B.detach().bfloat16()
+    fresh = torch.autograd.grad(fp8_lora_linear(x, w, ws, A, B, A16, B16, 2.0, QKV), [A, B], dy)
+    for start in (0.0, 3.0):
+        flat = [torch.full((t.numel() + 2,), start, device="cuda") for t in (A, B)]
+        A._axb_grad, B._axb_grad = (f[shift:shift + t.numel()].view(t.shape) for f, t in zip(flat, (A, B)))
+        torch.autograd.backward(fp8_lora_linear(x, w, ws, A, B, A16, B16, 2.0, QKV), dy)
+        for f, got, t in zip(flat, (A._axb_grad, B._axb_grad), fresh):
+            # the sum is added at once, or (more than 8192 rows of dB) in two parts: one rounding each
+            tol = EPS32 * 2 * (t.abs() + start) if start or T > 8192 else torch.zeros_like(t)
+            assert ((got - t - start).abs() <= tol).all()
+            assert (f[:shift] == start).all() and (f[shift + t.numel():] == start).all()
+        outside = torch.ones(N, R, dtype=torch.bool, device="cuda")
+        for r0, rows, c0, r in QKV:
+            outside[r0:r0 + rows, c0:c0 + r] = False
+        assert (B._axb_grad[outside] == start).all()
+    del A._axb_grad, B._axb_grad
+
+
+@pytest.mark.gpu
+def test_adapter_layer_on_a_second_device():
+    if torch.cuda.device_count() < 2:
+        pytest.skip("one device")
+    from axolotl_b200.ops.fp8 import fp8_lora_linear, quantize_fp8_weight
+
+    got = []
+    for dev in ("cuda:0", "cuda:1"):
+        g = torch.Generator().manual_seed(1)
+        x, dy = torch.randn(70, 264, generator=g).bfloat16().to(dev).requires_grad_(True), torch.randn(70, 384, generator=g).bfloat16().to(dev)
+        w, ws = quantize_fp8_weight(torch.randn(384, 264, generator=g).to(dev))
+        A, B = (t.to(dev).requires_grad_(True) for t in _adapter(384, 264, QKV))
+        y = fp8_lora_linear(x, w, ws, A, B, A.detach().bfloat16(), B.detach().bfloat16(), 2.0, QKV)
+        got.append([t.cpu() for t in (y, *torch.autograd.grad(y, [x, A, B], dy))])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
