@@ -552,6 +552,14 @@ AXB_DEVICE float2 unpack_bf16x2(uint32_t u) {
   return __bfloat1622float2(v);
 }
 
+// two fp32 values as bf16, and what that leaves of them as bf16 too (together off by at most 2^-16 of the value)
+AXB_DEVICE uint32_t split_bf16x2(float x, float y, uint32_t& low) {
+  const uint32_t h = pack_bf16x2(x, y);
+  const float2 f = unpack_bf16x2(h);
+  low = pack_bf16x2(x - f.x, y - f.y);
+  return h;
+}
+
 // two fp32 values in a register pair: one instruction each, rounded like the scalar ones
 AXB_DEVICE uint64_t pack_b32x2(uint32_t a, uint32_t b) {
   uint64_t r;

@@ -3,7 +3,8 @@
 //
 // Bound: one pass over the codes (HBM), half of what the bf16 rows would take. The scales lie along the contracted axis, so the codes
 // are widened first: eight warps turn a tile of 64 rows x 128 columns into bf16 (exact: four significant bits and a power of two) as the
-// MN-major 128-row operand of tcgen05.mma, g is the other one, 64 of its columns at a time. The rows are split over a cluster whose partial
+// MN-major 128-row operand of tcgen05.mma, g is the other one, 64 of its columns at a time; TWO: g comes as two bf16 numbers, and both
+// products go to the same sums. The rows are split over a cluster whose partial
 // sums meet in distributed shared memory in a fixed order: no atomics, the same bits every time.
 // What it measures: 8192 x 14336, rank 16, 57 us (2 TB/s of codes; expanding the rows and a bf16 product took 122), bound by the integer
 // pipe of the SMs that hold two of the 224 CTAs, some seven instructions a code; 8192 x 11008 41.5 us, 8192 x 4096 20.6.
@@ -15,12 +16,17 @@ constexpr int FA_T = 320;                 // TMA, MMA, eight widening warps
 constexpr int FA_ROWS = 64;               // rows of a step
 constexpr int FA_Q = FA_ROWS * 128;       // codes of a step
 constexpr int FA_G = FA_ROWS * 128;       // g of a step: 64 columns in bf16
-constexpr int FA_STAGES = 4;
 constexpr int FA_X = FA_ROWS * 256;       // widened tile: two chunks of 64 columns
 constexpr int FA_XBUFS = 2;
 constexpr int FA_S = FA_ROWS * 4;         // scales of a step
-constexpr int FA_SMEM = FA_STAGES * (FA_Q + FA_G + FA_S) + FA_XBUFS * FA_X + 1024 + 256;
-static_assert(64 * 128 * 4 <= FA_STAGES * (FA_Q + FA_G), "the partial tile reuses the ring");
+template <bool TWO>
+struct FaCfg {
+  static constexpr int STAGES = TWO ? 3 : 4;            // two CTAs of an SM
+  static constexpr int STAGE = FA_Q + FA_G * (TWO ? 2 : 1);
+  static constexpr int SMEM = STAGES * (STAGE + FA_S) + FA_XBUFS * FA_X + 1024 + 256;
+  static_assert(64 * 128 * 4 <= STAGES * STAGE, "the partial tile reuses the ring");
+  static_assert(2 * (SMEM + 1024) <= 228 * 1024, "two CTAs of an SM");
+};
 
 struct Fp8AdapterParams {
   float* out;
@@ -41,13 +47,14 @@ AXB_DEVICE uint32_t widen2(uint32_t h, __nv_bfloat162 sc) {
   return *reinterpret_cast<uint32_t*>(&v);
 }
 
-template <int NR>
+template <int NR, bool TWO>
 __global__ void __launch_bounds__(FA_T, 2)
     fp8_adapter_grad_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmS,
-                            const __grid_constant__ CUtensorMap tmG, const Fp8AdapterParams p) {
+                            const __grid_constant__ CUtensorMap tmG, const __grid_constant__ CUtensorMap tmL, const Fp8AdapterParams p) {
+  constexpr int FA_STAGES = FaCfg<TWO>::STAGES, FA_STAGE = FaCfg<TWO>::STAGE;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint8_t* sX = smem + FA_STAGES * (FA_Q + FA_G);
+  uint8_t* sX = smem + FA_STAGES * FA_STAGE;
   float* sS = reinterpret_cast<float*>(sX + FA_XBUFS * FA_X);
   uint64_t* full = reinterpret_cast<uint64_t*>(sS + FA_STAGES * FA_ROWS);   // codes, scales and g have arrived
   uint64_t* empty = full + FA_STAGES;                                   // the product that read g has ended
@@ -90,11 +97,12 @@ __global__ void __launch_bounds__(FA_T, 2)
     for (int t = t0; t < t1; ++t) {
       if (!warp_all(mbar_wait(&empty[s], phase ^ 1, p.status, AXB_TIMEOUT_EMPTY))) break;
       if (elect_one()) {
-        uint8_t* dst = smem + s * (FA_Q + FA_G);
-        mbar_expect_tx(&full[s], FA_Q + FA_G + FA_S);
+        uint8_t* dst = smem + s * FA_STAGE;
+        mbar_expect_tx(&full[s], FA_STAGE + FA_S);
         tma_load_2d(sS + s * FA_ROWS, &tmS, &full[s], t * FA_ROWS, tile);
         tma_load_2d(dst, &tmQ, &full[s], tile * 128, t * FA_ROWS);
         tma_load_2d(dst + FA_Q, &tmG, &full[s], r0, t * FA_ROWS);
+        if constexpr (TWO) tma_load_2d(dst + FA_Q + FA_G, &tmL, &full[s], r0, t * FA_ROWS);
       }
       __syncwarp();
       if (++s == FA_STAGES) {
@@ -114,11 +122,15 @@ __global__ void __launch_bounds__(FA_T, 2)
                     mbar_wait(&full[s], (uint32_t)((t - t0) / FA_STAGES) & 1, p.status, AXB_TIMEOUT_FULL)))
         break;
       tc_fence_after();
-      const uint64_t x = base_x + (uint32_t)(b * (FA_X / 16)), g = base_g + (uint32_t)(s * ((FA_Q + FA_G) / 16));
+      const uint64_t x = base_x + (uint32_t)(b * (FA_X / 16)), g = base_g + (uint32_t)(s * (FA_STAGE / 16));
       if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < FA_ROWS / 16; ++kk)
           umma_f16(tmem, x + kk * (2048 / 16), g + kk * (2048 / 16), idesc, t > t0 || kk > 0 ? 1u : 0u);
+        if constexpr (TWO) {
+#pragma unroll
+          for (int kk = 0; kk < FA_ROWS / 16; ++kk) umma_f16(tmem, x + kk * (2048 / 16), g + (FA_G + kk * 2048) / 16, idesc, 1u);
+        }
         umma_commit(&empty[s]);
         umma_commit(&xempty[b]);
         if (t == t1 - 1) umma_commit(done);
@@ -139,7 +151,7 @@ __global__ void __launch_bounds__(FA_T, 2)
       if (!warp_all(mbar_wait(&full[s], phase, p.status, AXB_TIMEOUT_FULL) &&
                     mbar_wait(&xempty[b], xphase ^ 1, p.status, AXB_TIMEOUT_EMPTY)))
         break;
-      const uint8_t* src = smem + s * (FA_Q + FA_G);
+      const uint8_t* src = smem + s * FA_STAGE;
       uint8_t* dst = sX + b * FA_X + (c16 >> 2) * (FA_X / 2);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -247,30 +259,32 @@ __global__ void __launch_bounds__(FA_T, 2)
   }
 }
 
-template <int NR>
-int launch_adapter_grad(const CUtensorMap& q, const CUtensorMap& sc, const CUtensorMap& g, const Fp8AdapterParams& p, int tiles, int chunks,
+template <int NR, bool TWO>
+int launch_adapter_grad(const CUtensorMap& q, const CUtensorMap& sc, const CUtensorMap& g, const CUtensorMap& lo, const Fp8AdapterParams& p, int tiles, int chunks,
                         int splits, cudaStream_t st) {
-  auto kern = fp8_adapter_grad_kernel<NR>;
+  auto kern = fp8_adapter_grad_kernel<NR, TWO>;
   static std::atomic<unsigned long long> allowed{0};
-  if (const int rc = axb_allow_smem((const void*)kern, FA_SMEM, allowed)) return rc;
-  AxbLaunch l(dim3((unsigned)(tiles * splits), (unsigned)chunks), FA_T, FA_SMEM, st, splits, false);
-  const cudaError_t e = cudaLaunchKernelEx(&l.cfg, kern, q, sc, g, p);
+  if (const int rc = axb_allow_smem((const void*)kern, FaCfg<TWO>::SMEM, allowed)) return rc;
+  AxbLaunch l(dim3((unsigned)(tiles * splits), (unsigned)chunks), FA_T, FaCfg<TWO>::SMEM, st, splits, false);
+  const cudaError_t e = cudaLaunchKernelEx(&l.cfg, kern, q, sc, g, lo, p);
   return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }
 
 }  // namespace
 
-// q: codes [T, K], rows of ldq bytes; s: fp32 [ceil(K / 128)][lds]; g: bf16 [T, R], row stride ldg; out: [R, K], row stride ldo; kind 0:
-// fp32, written, 1: fp32, added to, 2: bf16, written. q, s and g start on 16 bytes and have row strides of whole 16 bytes.
-extern "C" int axb_fp8_adapter_grad(const void* q, long long ldq, const float* s, long long lds, const void* g, long long ldg, void* out,
-                                    long long ldo, int T, int K, int R, int kind, int* status, void* stream) {
+// q: codes [T, K], rows of ldq bytes; s: fp32 [ceil(K / 128)][lds]; g: bf16 [T, R], row stride ldg; g_lo: the same, added to it (null: none);
+// out: [R, K], row stride ldo; kind 0: fp32, written, 1: fp32, added to, 2: bf16, written. q, s, g and g_lo start on 16 bytes and have row strides of whole 16 bytes.
+extern "C" int axb_fp8_adapter_grad(const void* q, long long ldq, const float* s, long long lds, const void* g, const void* g_lo,
+                                    long long ldg, void* out, long long ldo, int T, int K, int R, int kind, int* status, void* stream) {
   if (K <= 0 || R <= 0) return 0;
   auto bad = [](const void* v, long long bytes) { return (reinterpret_cast<uintptr_t>(v) & 15) != 0 || (bytes & 15) != 0; };
-  if (T <= 0 || bad(q, ldq) || bad(s, 4 * lds) || bad(g, 2 * ldg) || lds < T || ldo < K) return -2;
-  CUtensorMap tQ, tS, tG;
+  if (T <= 0 || bad(q, ldq) || bad(s, 4 * lds) || bad(g, 2 * ldg) || bad(g_lo, 0) || lds < T || ldo < K) return -2;
+  CUtensorMap tQ, tS, tG, tL;
   int rc = axb_make_tmap_2d(&tQ, q, T, K, ldq, FA_ROWS, 128, 1, false);
   if (!rc) rc = axb_make_tmap_2d(&tS, s, (K + 127) / 128, T, lds, 1, FA_ROWS, 4, false);
   if (!rc) rc = axb_make_tmap_2d(&tG, g, T, R, ldg, FA_ROWS, 64);
+  tL = tG;
+  if (!rc && g_lo) rc = axb_make_tmap_2d(&tL, g_lo, T, R, ldg, FA_ROWS, 64);
   if (rc) return -100 - rc;
   const int tiles = (K + 127) / 128, chunks = (R + 63) / 64, steps = (T + FA_ROWS - 1) / FA_ROWS;
   if (chunks > 65535) return -2;
@@ -286,7 +300,8 @@ extern "C" int axb_fp8_adapter_grad(const void* q, long long ldq, const float* s
   p.vec = (ldo & 3) == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
   p.status = status;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (R <= 16) return launch_adapter_grad<16>(tQ, tS, tG, p, tiles, chunks, splits, st);
-  if (R <= 32) return launch_adapter_grad<32>(tQ, tS, tG, p, tiles, chunks, splits, st);
-  return launch_adapter_grad<64>(tQ, tS, tG, p, tiles, chunks, splits, st);
+  auto run = [&](auto one, auto two) { return (g_lo ? two : one)(tQ, tS, tG, tL, p, tiles, chunks, splits, st); };
+  if (R <= 16) return run(launch_adapter_grad<16, false>, launch_adapter_grad<16, true>);
+  if (R <= 32) return run(launch_adapter_grad<32, false>, launch_adapter_grad<32, true>);
+  return run(launch_adapter_grad<64, false>, launch_adapter_grad<64, true>);
 }

@@ -7,17 +7,17 @@ extern "C" int axb_gemm_skinny(const void* P, long long ldp, const void* S, long
                                int K, const void* P2, long long ldp2, const void* S2, long long lds2, int K2, float alpha,
                                const void* bias, int out_mode, int out_f32, int glu_kind, float glu_limit, int p_dep, int splits,
                                int pdl, int* status, void* stream);
-extern "C" int axb_lora_bwd_dy_parts(const void* dy, long long ld_dy, const void* B, long long ld_b, const void* xa, long long ld_xa,
-                                     float* t_parts, float* dB_parts, int T, int N, int R, const int* blocks, int n_lora_blocks, int splits,
+extern "C" int axb_lora_bwd_dy_parts(const void* dy, long long ld_dy, const void* B, long long ld_b, const void* xa, const void* xa_lo,
+                                     long long ld_xa, float* t_parts, float* dB_parts, int T, int N, int R, const int* blocks, int n_lora_blocks, int splits,
                                      int* status, void* stream);
 extern "C" int axb_fp8_low_pays(int T, int K);
 extern "C" int axb_fp8_quantize_low(const void* x, long long ldx, const void* A, long long lda, void* q, long long ldq, float* s, long long lds,
-                                    void* xa, long long ldxa, int T, int K, int R, float scale, int* status, void* stream);
+                                    void* xa, void* xa_lo, long long ldxa, int T, int K, int R, float scale, int* status, void* stream);
 extern "C" int axb_fp8_linear(const void* x, long long ldx, void* q, const void* W, long long ldw, const float* sw, long long sw_n,
                               long long sw_k, int b_mn, void* y, int T, int N, int K, const void* X2, long long ldx2, const void* B2,
                               long long ldb2, int K2, int tile, int* status, void* stream);
-extern "C" int axb_fp8_adapter_grad(const void* q, long long ldq, const float* s, long long lds, const void* g, long long ldg, void* out,
-                                    long long ldo, int T, int K, int R, int kind, int* status, void* stream);
+extern "C" int axb_fp8_adapter_grad(const void* q, long long ldq, const float* s, long long lds, const void* g, const void* g_lo,
+                                    long long ldg, void* out, long long ldo, int T, int K, int R, int kind, int* status, void* stream);
 
 namespace {
 
@@ -26,7 +26,8 @@ constexpr int JOIN_ROWS = 8192;           // rows of dy whose parts are there at
 struct JoinParams {
   const float4* t_parts;                  // [splits][T, R]
   const float4* dB_parts;                 // [chunks][N, R]; nothing outside the diagonal blocks
-  uint2* t;                               // bf16 [T, R]: scale x the sum
+  uint2* t;                               // scale x the sum [T, R] as two bf16 numbers
+  uint2* t_lo;
   const float* dB_old;                    // what the sum is added to (null: nothing); row strides ld
   float* dB;                              // fp32 (null: none)
   uint2* dB16;                            // bf16 [N, R] (null: none)
@@ -68,7 +69,13 @@ __global__ void __launch_bounds__(256) fp8_lora_join_kernel(const __grid_constan
   const long long u = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * 8 + (lane & 7);      // a warp is all t or all B
   if (u < n8) {
     const float4 a = join4(p.t_parts + u, n, p.splits, u < n);
-    if (lane < 8 && u < n) p.t[u] = make_uint2(pack_bf16x2(a.x * p.scale, a.y * p.scale), pack_bf16x2(a.z * p.scale, a.w * p.scale));
+    if (lane < 8 && u < n) {
+      uint2 h, l;
+      h.x = split_bf16x2(a.x * p.scale, a.y * p.scale, l.x);
+      h.y = split_bf16x2(a.z * p.scale, a.w * p.scale, l.y);
+      p.t[u] = h;
+      p.t_lo[u] = l;
+    }
     return;
   }
   const long long i = u - n8;
@@ -109,10 +116,11 @@ struct AxbFp8Lora {
   const float* sw;
   const void* A;           // bf16 [R, K], [N, R]
   const void* B;
-  void* xa;                // scaling x A^T, bf16 [T, R]: written by the forward pass, read by the backward pass
+  void* xa;                // scaling x A^T, bf16 [T, R]: written by the forward pass, read by the backward pass. two: what that leaves of the
+                           // fp32 sums, in bf16, T rows behind it
   void* y;                 // y [T, N], or dx [T, K] (null: not wanted)
   const void* qx;          // backward: 8-bit rows of x
-  float* t_parts;          // backward scratch: fp32 [splits][min(T, 8192), R], [ceil of that many rows / 512][N, R]; bf16 [T, R]
+  float* t_parts;          // backward scratch: fp32 [splits][min(T, 8192), R], [ceil of that many rows / 512][N, R]; bf16 [2][T, R]
   float* dB_parts;
   void* t;
   void* dA;                // [R, K] (null: not wanted), fp32 or, where dA_bf16 is set, bf16
@@ -123,7 +131,7 @@ struct AxbFp8Lora {
   long long ldx, ldw, sw_n, sw_k, lda, ldb, ldda, lddb;
   int T, N, K, R, tile, n_blocks, splits, add_dA, add_dB, dA_bf16;
   float scaling;
-  int pad;
+  int two;                 // always in a backward pass
 };
 static_assert(sizeof(AxbFp8Lora) == 17 * 8 + 8 * 8 + 12 * 4, "no gaps");
 
@@ -134,10 +142,11 @@ extern "C" int axb_fp8_lora_fwd(const AxbFp8Lora* l, void* stream) {
   if (one) {
     const long long ldq = (l->K + 15ll) & ~15ll;
     rc = axb_fp8_quantize_low(l->x, l->ldx, l->A, l->lda, l->q, ldq, reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(l->q) + ldq * l->T),
-                              (l->T + 3ll) & ~3ll, l->xa, l->R, l->T, l->K, l->R, l->scaling, l->status, stream);
+                              (l->T + 3ll) & ~3ll, l->xa, l->two ? static_cast<char*>(l->xa) + 2ll * l->T * l->R : nullptr,
+                              l->R, l->T, l->K, l->R, l->scaling, l->status, stream);
   } else {
-    rc = axb_gemm_skinny(l->x, l->ldx, l->A, l->lda, l->xa, l->R, l->T, l->R, l->K, nullptr, 0, nullptr, 0, 0, l->scaling, nullptr, 1, 0, 0,
-                         0.f, 1, 0, 0, l->status, stream);
+    rc = axb_gemm_skinny(l->x, l->ldx, l->A, l->lda, l->xa, l->R, l->T, l->R, l->K, nullptr, 0, nullptr, 0, 0, l->scaling, nullptr, 1,
+                         l->two ? 2 : 0, 0, 0.f, 1, 0, 0, l->status, stream);
   }
   return rc ? rc : axb_fp8_linear(one ? nullptr : l->x, l->ldx, l->q, l->W, l->ldw, l->sw, l->sw_n, l->sw_k, 0, l->y, l->T, l->N, l->K, l->xa,
                                   l->R, l->B, l->ldb, l->R, l->tile, l->status, stream);
@@ -148,6 +157,7 @@ extern "C" int axb_fp8_lora_bwd(const AxbFp8Lora* l, void* stream) {
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (l->n_blocks < 1 || l->n_blocks > 8 || (l->T > JOIN_ROWS && !l->dB)) return -2;
   int rc = 0;
+  const long long n = (long long)l->T * l->R;
   JoinParams p = {};
   p.t_parts = reinterpret_cast<const float4*>(l->t_parts);
   p.dB_parts = reinterpret_cast<const float4*>(l->dB_parts);
@@ -169,10 +179,11 @@ extern "C" int axb_fp8_lora_bwd(const AxbFp8Lora* l, void* stream) {
     p.chunks = (p.T + 511) / 512;
     const long long at = (long long)row * l->R;
     rc = axb_lora_bwd_dy_parts(static_cast<const char*>(l->x) + 2ll * row * l->ldx, l->ldx, l->B, l->ldb,
-                               static_cast<const char*>(l->xa) + 2 * at, l->R, l->t_parts, l->dB_parts, p.T, l->N, l->R, l->blocks,
+                               static_cast<const char*>(l->xa) + 2 * at, static_cast<const char*>(l->xa) + 2 * (n + at), l->R, l->t_parts, l->dB_parts, p.T, l->N, l->R, l->blocks,
                                l->n_blocks, l->splits, l->status, stream);
     if (rc) break;
     p.t = reinterpret_cast<uint2*>(static_cast<char*>(l->t) + 2 * at);
+    p.t_lo = reinterpret_cast<uint2*>(static_cast<char*>(l->t) + 2 * (n + at));
     p.dB_old = first && (l->dB16 || !l->add_dB) ? nullptr : l->dB;
     p.dB = l->dB16 && last ? nullptr : l->dB;
     p.dB16 = last ? reinterpret_cast<uint2*>(l->dB16) : nullptr;
@@ -186,7 +197,7 @@ extern "C" int axb_fp8_lora_bwd(const AxbFp8Lora* l, void* stream) {
   if (!rc && l->dA) {
     const long long ldq = (l->K + 15ll) & ~15ll, lds = (l->T + 3ll) & ~3ll;      // the layout of axb_fp8_linear
     rc = axb_fp8_adapter_grad(l->qx, ldq, reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(l->qx) + ldq * l->T), lds, l->t,
-                              l->R, l->dA, l->ldda, l->T, l->K, l->R, l->dA_bf16 ? 2 : l->add_dA, l->status, stream);
+                              static_cast<const char*>(l->t) + 2 * n, l->R, l->dA, l->ldda, l->T, l->K, l->R, l->dA_bf16 ? 2 : l->add_dA, l->status, stream);
   }
   return rc;
 }

@@ -20,6 +20,7 @@ struct Fp8LowParams {
   uint8_t* q;
   float* s;
   __nv_bfloat16* xa;
+  __nv_bfloat16* xa_lo;                   // what the bf16 xa leaves, in bf16 (null: not wanted)
   long long ldq, lds, ldxa;
   int T, K, R;
   float scale;
@@ -178,10 +179,11 @@ __global__ void __launch_bounds__(FL_T, 2)
     for (int k = 0; k < cs; ++k)
 #pragma unroll
       for (int j = 0; j < 8; ++j) a[j] += cs == 1 ? part[(c + j) * 128 + r] : ld_cluster_f32(mapa_u32(pbase + ((c + j) * 128 + r) * 4, k));
-    uint32_t o[4];
+    uint32_t o[4], l[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] = pack_bf16x2(a[2 * j] * p.scale, a[2 * j + 1] * p.scale);
+    for (int j = 0; j < 4; ++j) o[j] = split_bf16x2(a[2 * j] * p.scale, a[2 * j + 1] * p.scale, l[j]);
     *reinterpret_cast<uint4*>(p.xa + (row0 + r) * p.ldxa + c) = make_uint4(o[0], o[1], o[2], o[3]);
+    if (p.xa_lo) *reinterpret_cast<uint4*>(p.xa_lo + (row0 + r) * p.ldxa + c) = make_uint4(l[0], l[1], l[2], l[3]);
   }
   if (cs > 1) cluster_sync();             // peers may still read this CTA's partial product
   else __syncthreads();
@@ -218,12 +220,13 @@ extern "C" int axb_fp8_low_pays(int T, int K) {
 }
 
 // x: bf16 [T, K], row stride ldx; A: bf16 [R, K], row stride lda, R <= 64 and a multiple of 8; q: codes, rows of ldq bytes; s: fp32 [ceil(K /
-// 128)][lds]; xa: bf16 [T, R], row stride ldxa. x, A, q and xa start on 16 bytes and have row strides of whole 16 bytes.
+// 128)][lds]; xa: bf16 [T, R], row stride ldxa; xa_lo: the same, what xa leaves of the fp32 sums (null: not wanted). x, A, q, xa and xa_lo start
+// on 16 bytes and have row strides of whole 16 bytes.
 extern "C" int axb_fp8_quantize_low(const void* x, long long ldx, const void* A, long long lda, void* q, long long ldq, float* s, long long lds,
-                                    void* xa, long long ldxa, int T, int K, int R, float scale, int* status, void* stream) {
+                                    void* xa, void* xa_lo, long long ldxa, int T, int K, int R, float scale, int* status, void* stream) {
   if (T <= 0 || K <= 0) return 0;
   auto bad = [](const void* a, long long bytes) { return (reinterpret_cast<uintptr_t>(a) & 15) != 0 || (bytes & 15) != 0; };
-  if (R <= 0 || R > 64 || (R & 7) || bad(x, 2 * ldx) || bad(A, 2 * lda) || bad(q, ldq) || bad(xa, 2 * ldxa) || ldq < K || lds < T) return -2;
+  if (R <= 0 || R > 64 || (R & 7) || bad(x, 2 * ldx) || bad(A, 2 * lda) || bad(q, ldq) || bad(xa, 2 * ldxa) || bad(xa_lo, 0) || ldq < K || lds < T) return -2;
   const int NR = R <= 16 ? 16 : (R <= 32 ? 32 : 64);
   CUtensorMap tX, tA;
   int rc = axb_make_tmap_2d(&tX, x, T, K, ldx, 128, 64);
@@ -233,6 +236,7 @@ extern "C" int axb_fp8_quantize_low(const void* x, long long ldx, const void* A,
   p.q = reinterpret_cast<uint8_t*>(q);
   p.s = s;
   p.xa = reinterpret_cast<__nv_bfloat16*>(xa);
+  p.xa_lo = reinterpret_cast<__nv_bfloat16*>(xa_lo);
   p.ldq = ldq;
   p.lds = lds;
   p.ldxa = ldxa;

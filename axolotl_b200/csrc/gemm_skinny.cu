@@ -27,6 +27,7 @@ struct SkinnyParams {
   int R, N, K, K2;             // out_mode 2: R counts the I columns of h
   float alpha;
   int out_mode, out_f32, p_dep;
+  int two;                     // out_mode 1: what the bf16 result leaves, in bf16, R rows behind it
   int glu_kind;
   float glu_limit;
   int* status;
@@ -204,7 +205,13 @@ __global__ void __launch_bounds__(SK_T)
       for (int j = 0; j < 4; ++j) {
         if (n0 + j >= p.N) break;
         if (p.out_f32) reinterpret_cast<float*>(p.C)[row * p.ldc + n0 + j] = v[j] * p.alpha;
-        else reinterpret_cast<__nv_bfloat16*>(p.C)[row * p.ldc + n0 + j] = __float2bfloat16(v[j] * p.alpha);
+        else {
+          const float o = v[j] * p.alpha;
+          const __nv_bfloat16 hi = __float2bfloat16(o);
+          __nv_bfloat16* c = reinterpret_cast<__nv_bfloat16*>(p.C) + row * p.ldc + n0 + j;
+          *c = hi;
+          if (p.two) c[p.R * p.ldc] = __float2bfloat16(o - __bfloat162float(hi));
+        }
       }
     }
   } else {
@@ -281,13 +288,15 @@ int pick_splits(int tiles, int nk) {
 
 // See the head of this file. P [R, K] (out_mode 2: [2R, K]), S [N, K], P2 / S2 the K-extension (K2 = 0: none); rows of all four
 // are 16-byte aligned with strides that are multiples of 8 elements. p_dep: P, too, is written by the launch before this one.
+// out_f32: 0 a bf16 result, 1 fp32, 2 (out_mode 1, N <= 128) two bf16 numbers, the second R rows behind the first.
 // splits: 0 = chosen by pick_splits. pdl: the launch may overlap the end of its predecessor.
 extern "C" int axb_gemm_skinny(const void* P, long long ldp, const void* S, long long lds, void* C, long long ldc, int R, int N,
                                int K, const void* P2, long long ldp2, const void* S2, long long lds2, int K2, float alpha,
                                const void* bias, int out_mode, int out_f32, int glu_kind, float glu_limit, int p_dep, int splits,
                                int pdl, int* status, void* stream) {
   if (R <= 0 || N <= 0 || (K <= 0 && K2 <= 0)) return 0;
-  if (N > 256 || out_mode < 0 || out_mode > 2 || splits < 0 || splits > 8) return -2;
+  if (N > 256 || out_mode < 0 || out_mode > 2 || splits < 0 || splits > 8 || out_f32 > 2) return -2;
+  if (out_f32 == 2 && (out_mode != 1 || N > 128)) return -2;
   if (out_mode == 2 && (out_f32 || (R % 64) || glu_kind < 0 || glu_kind > 1)) return -2;
   if (K <= 0) return -2;
   if (N > 128) {
@@ -321,7 +330,8 @@ extern "C" int axb_gemm_skinny(const void* P, long long ldp, const void* S, long
   p.K2 = K2 > 0 ? K2 : 0;
   p.alpha = alpha;
   p.out_mode = out_mode;
-  p.out_f32 = out_f32;
+  p.out_f32 = out_f32 == 1;
+  p.two = out_f32 == 2;
   p.p_dep = p_dep;
   p.glu_kind = glu_kind;
   p.glu_limit = glu_limit;

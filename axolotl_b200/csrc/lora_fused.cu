@@ -24,10 +24,16 @@ namespace {
 constexpr int LF_THREADS = 192;
 constexpr int LF_ROWS = 512;                 // token rows per CTA
 constexpr int LF_SUB = 4;                    // 128-row sub-tiles
-constexpr int LF_DY_STAGES = 3;
 constexpr int LF_DY_BYTES = 128 * 128 * 2;   // two 64-column halves of 128 rows x 128 bytes
 constexpr int LF_SMALL_BYTES = 128 * 64 * 2; // [128 rows, 64 columns] tile of xa / B (columns >= R are zero)
-constexpr int LF_SMEM = LF_DY_STAGES * LF_DY_BYTES + LF_SUB * LF_SMALL_BYTES + 2 * LF_SMALL_BYTES + 1024 + 256;
+// PARTS: xa comes as two bf16 numbers (high and low halves), whose tiles take the place of a stage of dY
+template <bool PARTS>
+struct LfCfg {
+  static constexpr int DY_STAGES = PARTS ? 2 : 3;
+  static constexpr int XA_TILES = LF_SUB * (PARTS ? 2 : 1);
+  static constexpr int SMEM = DY_STAGES * LF_DY_BYTES + XA_TILES * LF_SMALL_BYTES + 2 * LF_SMALL_BYTES + 1024 + 256;
+  static_assert(SMEM <= 227 * 1024, "shared memory of a CTA");
+};
 
 struct LoraBwdParams {
   int T, N, R, Rpad;
@@ -44,12 +50,13 @@ struct LoraBwdParams {
 template <bool PARTS>
 __global__ void __launch_bounds__(LF_THREADS, 1)
     lora_bwd_dy_kernel(const __grid_constant__ CUtensorMap tmDY, const __grid_constant__ CUtensorMap tmB,
-                       const __grid_constant__ CUtensorMap tmXA, const LoraBwdParams p) {
+                       const __grid_constant__ CUtensorMap tmXA, const __grid_constant__ CUtensorMap tmXL, const LoraBwdParams p) {
+  constexpr int LF_DY_STAGES = LfCfg<PARTS>::DY_STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* sDY = smem;
   uint8_t* sXA = smem + LF_DY_STAGES * LF_DY_BYTES;
-  uint8_t* sB = sXA + LF_SUB * LF_SMALL_BYTES;
+  uint8_t* sB = sXA + LfCfg<PARTS>::XA_TILES * LF_SMALL_BYTES;       // low halves of xa: LF_SUB tiles behind the high ones
   uint64_t* bars = reinterpret_cast<uint64_t*>(sB + 2 * LF_SMALL_BYTES);
   uint64_t* dy_full = bars;                     // [3]
   uint64_t* dy_empty = bars + 3;                // [3]
@@ -69,7 +76,7 @@ __global__ void __launch_bounds__(LF_THREADS, 1)
   const int n_sub = min(LF_SUB, (p.T - row0 + 127) / 128);
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < 3; ++s) {
+    for (int s = 0; s < LF_DY_STAGES; ++s) {
       mbar_init(&dy_full[s], 1);
       mbar_init(&dy_empty[s], 1);
     }
@@ -96,10 +103,14 @@ __global__ void __launch_bounds__(LF_THREADS, 1)
   if (nb1 > nb0 && n_sub > 0) {
     if (warp == 0) {
       if (elect_one()) {
-        mbar_expect_tx(xa_full, n_sub * LF_SMALL_BYTES);
+        mbar_expect_tx(xa_full, n_sub * (PARTS ? 2 : 1) * LF_SMALL_BYTES);
         for (int s = 0; s < n_sub; ++s) {
           tma_load_2d(sXA + s * LF_SMALL_BYTES, &tmXA, xa_full, 0, row0 + s * 128);
           tma_load_2d(sXA + s * LF_SMALL_BYTES + 8192, &tmXA, xa_full, 0, row0 + s * 128 + 64);
+          if constexpr (PARTS) {
+            tma_load_2d(sXA + (LF_SUB + s) * LF_SMALL_BYTES, &tmXL, xa_full, 0, row0 + s * 128);
+            tma_load_2d(sXA + (LF_SUB + s) * LF_SMALL_BYTES + 8192, &tmXL, xa_full, 0, row0 + s * 128 + 64);
+          }
         }
       }
       __syncwarp();
@@ -168,6 +179,11 @@ __global__ void __launch_bounds__(LF_THREADS, 1)
 #pragma unroll
             for (int kk = 0; kk < 8; ++kk)
               umma_f16(d_db, da2 + kk * (2048 / 16), db2 + kk * (2048 / 16), idesc2, (s > 0 || kk > 0) ? 1u : 0u);
+            if constexpr (PARTS) {
+#pragma unroll
+              for (int kk = 0; kk < 8; ++kk)
+                umma_f16(d_db, da2 + kk * (2048 / 16), db2 + (LF_SUB * LF_SMALL_BYTES + kk * 2048) / 16, idesc2, 1u);
+            }
             umma_commit(&dy_empty[stage]);
             if (s == n_sub - 1) {
               umma_commit(&db_full[bb]);
@@ -259,15 +275,17 @@ __global__ void __launch_bounds__(LF_THREADS, 1)
 }
 
 template <bool PARTS>
-int launch_lora_bwd_dy(const void* dy, long long ld_dy, const void* B, long long ld_b, const void* xa, long long ld_xa, float* t32, float* dB32,
-                       long long ldb32, int T, int N, int R, const int* blocks, int n_lora_blocks, int splits, int* status, void* stream) {
+int launch_lora_bwd_dy(const void* dy, long long ld_dy, const void* B, long long ld_b, const void* xa, const void* xa_lo, long long ld_xa,
+                       float* t32, float* dB32, long long ldb32, int T, int N, int R, const int* blocks, int n_lora_blocks, int splits, int* status, void* stream) {
   if (R > 64 || n_lora_blocks < 1 || n_lora_blocks > 8) return -3;
   if ((ld_dy & 7) || (ld_b & 7) || (ld_xa & 7)) return -2;
-  CUtensorMap tDY, tB, tXA;
+  CUtensorMap tDY, tB, tXA, tXL;
   int rc = 0;
   rc |= axb_make_tmap_2d(&tDY, dy, T, N, ld_dy, 128, 64);
   rc |= axb_make_tmap_2d(&tB, B, N, R, ld_b, 64, 64);
   rc |= axb_make_tmap_2d(&tXA, xa, T, R, ld_xa, 64, 64);
+  tXL = tXA;
+  if (PARTS) rc |= axb_make_tmap_2d(&tXL, xa_lo, T, R, ld_xa, 64, 64);
   if (rc) return -4;
   LoraBwdParams p = {};
   p.T = T; p.N = N; p.R = R; p.Rpad = (R + 15) & ~15;
@@ -282,8 +300,8 @@ int launch_lora_bwd_dy(const void* dy, long long ld_dy, const void* B, long long
   }
   p.status = status;
   static std::atomic<unsigned long long> allowed{0};
-  if (const int e = axb_allow_smem((const void*)lora_bwd_dy_kernel<PARTS>, LF_SMEM, allowed)) return e;
-  lora_bwd_dy_kernel<PARTS><<<t_chunks * p.n_splits, LF_THREADS, LF_SMEM, reinterpret_cast<cudaStream_t>(stream)>>>(tDY, tB, tXA, p);
+  if (const int e = axb_allow_smem((const void*)lora_bwd_dy_kernel<PARTS>, LfCfg<PARTS>::SMEM, allowed)) return e;
+  lora_bwd_dy_kernel<PARTS><<<t_chunks * p.n_splits, LF_THREADS, LfCfg<PARTS>::SMEM, reinterpret_cast<cudaStream_t>(stream)>>>(tDY, tB, tXA, tXL, p);
   return (int)cudaGetLastError();
 }
 
@@ -299,18 +317,18 @@ extern "C" int axb_lora_bwd_dy(const void* dy, long long ld_dy, const void* B, l
   int dev = 0, sms = 148;
   cudaGetDevice(&dev);
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return launch_lora_bwd_dy<false>(dy, ld_dy, B, ld_b, xa, ld_xa, t32, dB32, ldb32, T, N, R, blocks, n_lora_blocks,
+  return launch_lora_bwd_dy<false>(dy, ld_dy, B, ld_b, xa, nullptr, ld_xa, t32, dB32, ldb32, T, N, R, blocks, n_lora_blocks,
                                    sms / ((T + LF_ROWS - 1) / LF_ROWS), status, stream);
 }
 
-// The same sums in parts, each written once by one CTA: t_parts fp32 [splits][T, R], dB_parts fp32 [ceil(T / 512)][N, R], of which only the
+// The same sums of an xa that is given as two bf16 numbers (xa + xa_lo), in parts, each written once by one CTA: t_parts fp32 [splits][T, R], dB_parts fp32 [ceil(T / 512)][N, R], of which only the
 // columns of the diagonal blocks are written; R a multiple of 8, both on 16 bytes, 1 <= splits <= ceil(N / 128). Added in a fixed order they
 // are the same bits every time.
-extern "C" int axb_lora_bwd_dy_parts(const void* dy, long long ld_dy, const void* B, long long ld_b, const void* xa, long long ld_xa,
-                                     float* t_parts, float* dB_parts, int T, int N, int R, const int* blocks, int n_lora_blocks, int splits,
+extern "C" int axb_lora_bwd_dy_parts(const void* dy, long long ld_dy, const void* B, long long ld_b, const void* xa, const void* xa_lo,
+                                     long long ld_xa, float* t_parts, float* dB_parts, int T, int N, int R, const int* blocks, int n_lora_blocks, int splits,
                                      int* status, void* stream) {
   if (T <= 0 || N <= 0 || R <= 0) return 0;
   if ((R & 7) || splits < 1 || splits > (N + 127) / 128) return -2;
   if ((reinterpret_cast<uintptr_t>(t_parts) | reinterpret_cast<uintptr_t>(dB_parts)) & 15) return -2;
-  return launch_lora_bwd_dy<true>(dy, ld_dy, B, ld_b, xa, ld_xa, t_parts, dB_parts, R, T, N, R, blocks, n_lora_blocks, splits, status, stream);
+  return launch_lora_bwd_dy<true>(dy, ld_dy, B, ld_b, xa, xa_lo, ld_xa, t_parts, dB_parts, R, T, N, R, blocks, n_lora_blocks, splits, status, stream);
 }

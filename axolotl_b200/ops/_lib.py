@@ -48,8 +48,8 @@ _CUDA_SIGS = {
     "axb_fp8_dequantize_rows": [vp, i64, vp, i64, vp, i64, i32, i64, i32, vp],
     "axb_fp8_lora_fwd": [C.c_char_p, vp],      # AxbFp8Lora, stream
     "axb_fp8_lora_bwd": [C.c_char_p, vp],
-    # codes, ldq, scales, lds, g, ldg, out, ldo, T, K, R, accumulate, status, stream
-    "axb_fp8_adapter_grad": [vp, i64, vp, i64, vp, i64, vp, i64, i32, i32, i32, i32, vp, vp],
+    # codes, ldq, scales, lds, g, g_lo, ldg, out, ldo, T, K, R, accumulate, status, stream
+    "axb_fp8_adapter_grad": [vp, i64, vp, i64, vp, vp, i64, vp, i64, i32, i32, i32, i32, vp, vp],
     "axb_fp8_linear_packed": [C.c_char_p],     # AxbFp8Linear
     # A, lda, sa, ldsa, B, ldb, sb, sb_n, sb_k, b_mn, C, ldc, M, N, K, A2, lda2, B2, ldb2, K2, tile, status, stream
     "axb_fp8_gemm": [vp, i64, vp, i64, vp, i64, vp, i64, i64, i32, vp, i64, i32, i32, i32, vp, i64, vp, i64, i32, i32, vp, vp],

@@ -383,12 +383,12 @@ _LORA = struct.Struct("@17P8q10ifi")      # AxbFp8Lora of csrc/fp8_lora.cu
 
 
 def _lora_call(entry, x, codes, scale, A16, B16, scaling, sizes, q, xa, y, qx=0, t_parts=0, dB_parts=0, t=0, dA=0, dB=0, dB16=0, blocks=0,
-               ldda=0, lddb=0, n_blocks=0, splits=0, add_dA=False, add_dB=False, dA_bf16=False):
+               ldda=0, lddb=0, n_blocks=0, splits=0, add_dA=False, add_dB=False, dA_bf16=False, two=True):
     """One call of csrc/fp8_lora.cu; ``q`` .. ``blocks`` are addresses, ``sizes`` is (T, N, K, R, tile)."""
     status, stream = _lib.launch_args(x.device.index)
     args = _LORA.pack(x.data_ptr(), q, codes.data_ptr(), scale.data_ptr(), A16.data_ptr(), B16.data_ptr(), xa, y, qx, t_parts, dB_parts, t, dA,
                       dB, dB16, blocks, status, x.stride(0), codes.stride(0), *scale.stride(), A16.stride(0), B16.stride(0), ldda, lddb, *sizes,
-                      n_blocks, splits, add_dA, add_dB, dA_bf16, scaling, 0)
+                      n_blocks, splits, add_dA, add_dB, dA_bf16, scaling, two)
     _lib.check_rc(entry(args, stream), "fp8_lora")
 
 
@@ -400,29 +400,33 @@ def _flat_blocks(blocks, N, R):
     return (C.c_int * (4 * len(blocks)))(*[int(v) for b in blocks for v in b])
 
 
-def _lora_forward(x, codes, scale, A16, B16, scaling, keep):
-    """(y, scaling x A^T, block of ``_pack`` of x or None): one call where the operands are what the kernels read as they are."""
+def _lora_forward(x, codes, scale, A16, B16, scaling, keep, two):
+    """(y, scaling x A^T, block of ``_pack`` of x or None): one call up to rank 128. Where a gradient may follow, the low-rank product comes
+    up to rank 64 as two bf16 numbers [2, T, R], the second what the first leaves of the fp32 sums."""
+    if x.device.index != _current_device():
+        with torch.cuda.device(x.device):
+            return _lora_forward(x, codes, scale, A16, B16, scaling, keep, two)
     T, K = x.shape
     R, N = A16.shape[0], codes.shape[0]
-    if not (T and R <= 128 and R % 8 == 0 and _operand16(x) and _operand16(A16) and _operand16(B16)
-            and x.device.index == _current_device()):
+    if R > 128:
         from .lora import skinny_gemm
 
         xa = skinny_gemm(x, A16, alpha=scaling)            # [T, R], of the bf16 input
         y, q = _product(x, codes, scale, a2=xa, b2=B16, keep=keep)
         return y, xa, q
     few = _few(T, N, K)
-    y, xa = x.new_empty((T, N)), x.new_empty((T, R))
+    two = two and R <= 64
+    y, xa = x.new_empty((T, N)), x.new_empty((2, T, R) if two else (T, R))
     q = x.new_empty(_packed_size(T, K), dtype=torch.uint8) if keep or few < 2 else None
     _lora_call(_lib.cuda_lib().axb_fp8_lora_fwd, x, _rows16(codes), scale, A16, B16, scaling, (T, N, K, R, 0 if few else _tile(T, N, K)),
-               0 if q is None else q.data_ptr(), xa.data_ptr(), y.data_ptr())
+               0 if q is None else q.data_ptr(), xa.data_ptr(), y.data_ptr(), two=two)
     return y, xa, q
 
 
 class _Fp8LoRALinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, codes, scale, A, B, A16, B16, scaling, blocks, bias):
-        y, xa, q = _lora_forward(x, _as_codes(codes), scale, A16, B16, scaling, ctx.needs_input_grad[3])
+        y, xa, q = _lora_forward(x, _as_codes(codes), scale, A16, B16, scaling, ctx.needs_input_grad[3], ctx.needs_input_grad[4])
         if bias is not None:
             y += bias
         ctx.save_for_backward(q if ctx.needs_input_grad[3] else None, codes, scale, A, B, A16, B16, xa)
@@ -441,17 +445,16 @@ class _Fp8LoRALinearFn(torch.autograd.Function):
         (T, N), K, R = dy.shape, codes.shape[1], A16.shape[0]
         dbias = dy.float().sum(0).to(ctx.bias_dtype) if need[9] else None
         dx = dA = dB = None
-        if (need[4] and USE_FUSED_DY and T and R <= 64 and R % 8 == 0 and len(ctx.blocks) <= 8 and xa.is_contiguous()
-                and all(map(_operand16, (dy, A16, B16, xa)))):
+        if need[4] and USE_FUSED_DY and R <= 64 and len(ctx.blocks) <= 8:
             # one pass over dy for t and dB, the product and dA behind it: one call. Scratch: the parts of t and of dB (a CTA of
             # csrc/lora_fused.cu holds 512 rows and one of `splits` ranges of dy's columns), dB in fp32 (where more than 8192 rows are summed
-            # into a bf16 one), t in bf16, the rows of dy in 8 bits
+            # into a bf16 one), t as two bf16 numbers, the rows of dy in 8 bits
             tA, tB = getattr(A, "_axb_grad", None), getattr(B, "_axb_grad", None)
             low = [w is None and p.dtype == torch.bfloat16 for w, p in ((tA, A), (tB, B))]
             rows = min(T, 8192)
             chunks = -(-rows // 512)
             splits = min(148 // chunks, _blocks(N))
-            at = [4 * splits * rows * R, 4 * chunks * N * R, 4 * N * R if low[1] and T > rows else 0, 2 * T * R]
+            at = [4 * splits * rows * R, 4 * chunks * N * R, 4 * N * R if low[1] and T > rows else 0, 4 * T * R]
             work = dy.new_empty(sum(at) + (_packed_size(T, N) if need[0] else 0), dtype=torch.uint8)
             p = work.data_ptr()
             args = dict(t_parts=p, dB_parts=p + at[0], t=p + sum(at[:3]), splits=splits)
@@ -475,6 +478,7 @@ class _Fp8LoRALinearFn(torch.autograd.Function):
             dA = None if dA is None or tA is not None else dA if dA.dtype == A.dtype else dA.to(A.dtype)
             dB = None if tB is not None else dB if dB.dtype == B.dtype else dB.to(B.dtype)
             return dx, None, None, dA, dB, None, None, None, None, dbias
+        xa = xa[0] if xa.dim() == 3 else xa
         t, dB_fused, dB_done = _t_and_dB(dy, B, B16, xa, ctx.blocks, ctx.scaling, need[4])
         dx = _product(dy, codes, scale, trans=True, a2=t, b2=A16)[0] if need[0] else None
         if need[3]:
@@ -523,7 +527,7 @@ def _adapter_grad(t, q, ldq, s, lds, K, out):
     if not add:
         out = torch.empty((R, K), dtype=torch.float32, device=t.device)
     _lib.check_rc(_lib.cuda_lib().axb_fp8_adapter_grad(
-        q, ldq, s, lds, t.data_ptr(), t.stride(0), out.data_ptr(), out.stride(0) if R > 1 else K, T, K, R, add,
+        q, ldq, s, lds, t.data_ptr(), None, t.stride(0), out.data_ptr(), out.stride(0) if R > 1 else K, T, K, R, add,
         _lib.status_word(t.device).data_ptr(), _lib.stream_ptr()), "fp8_adapter_grad")
     return out
 
@@ -599,7 +603,7 @@ def fp8_lora_linear(x, codes, scale, A, B, A16, B16, scaling, blocks, bias=None)
     x2, A16, B16 = (_operand(t, "fp8_lora_linear") for t in (x2, A16, B16))
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, A, B, bias)):
         return _shaped(_Fp8LoRALinearFn.apply(x2, codes, scale, A, B, A16, B16, float(scaling), blocks, bias), x)
-    y = _lora_forward(x2, _as_codes(codes), scale, A16, B16, float(scaling), False)[0]
+    y = _lora_forward(x2, _as_codes(codes), scale, A16, B16, float(scaling), False, False)[0]
     if bias is not None:
         y += bias
     return _shaped(y, x)

@@ -463,3 +463,28 @@ def test_adapter_layer_on_a_second_device():
         y = fp8_lora_linear(x, w, ws, A, B, A.detach().bfloat16(), B.detach().bfloat16(), 2.0, QKV)
         got.append([t.cpu() for t in (y, *torch.autograd.grad(y, [x, A, B], dy))])
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,K,N,blocks", [(1, 136, 384, QKV), (40, 4096, 256, ((0, 256, 0, 64),)), (520, 264, 640, ((0, 640, 0, 16),)),
+                                          (700, 2056, 384, QKV), (1000, 14336, 256, ((0, 256, 0, 32),)), (8300, 136, 264, ((0, 264, 0, 8),))])
+def test_adapter_gradients_see_the_sums_in_sixteen_bits(T, K, N, blocks):
+    """dA and dB of fp32 masters: s dy B and s x A^T enter as two bf16 numbers, which are off by 2^-16 of the value together, so that what is
+    left is the sums' own error in fp32."""
+    from axolotl_b200.ops.fp8 import fp8_lora_linear, quantize_fp8_weight
+
+    g = torch.Generator().manual_seed(T)
+    x, dy = torch.randn(T, K, generator=g).bfloat16(), (torch.randn(T, N, generator=g) * 1e-2).bfloat16()
+    w, ws = quantize_fp8_weight(torch.randn(N, K, generator=g).cuda())
+    A, B = _adapter(N, K, blocks)
+    Al, Bl = A.cuda().requires_grad_(True), B.cuda().requires_grad_(True)
+    y = fp8_lora_linear(x.cuda(), w, ws, Al, Bl, A.bfloat16().cuda(), B.bfloat16().cuda(), 2.0, blocks)
+    dA, dB = (t.cpu().double() for t in torch.autograd.grad(y, [Al, Bl], dy.cuda()))
+    a, b, x64, d64, x8 = A.double(), B.double(), x.double(), dy.double(), _rows8(x)
+    low, tall = 2 * x64 @ a.t(), 2 * d64 @ b
+    low_e = 2.0 ** -16 * low.abs() + (K + 16) * EPS32 * 2 * x64.abs() @ a.abs().t()
+    tall_e = 2.0 ** -16 * tall.abs() + (N + 160) * EPS32 * 2 * d64.abs() @ b.abs()          # parts of up to 148 column ranges
+    assert ((dA - tall.t() @ x8).abs() <= tall_e.t() @ x8.abs() + (2 * T + 32) * EPS32 * tall.abs().t() @ x8.abs() + 1e-30).all()
+    for r0, rows, c0, r in blocks:
+        d, l, e = d64[:, r0:r0 + rows], low[:, c0:c0 + r], low_e[:, c0:c0 + r]
+        assert ((dB[r0:r0 + rows, c0:c0 + r] - d.t() @ l).abs() <= d.abs().t() @ e + (2 * T + 64) * EPS32 * d.abs().t() @ l.abs() + 1e-30).all()
