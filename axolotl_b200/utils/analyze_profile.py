@@ -18,8 +18,8 @@ import re
 CATEGORIES = [
     ("grouped gemm (MoE)", r"grouped_gemm_kernel"),
     ("gemm (tcgen05)", r"gemm_bf16_(tcgen05|pair)_kernel|gather_only_kernel"),
-    ("8-bit products", r"fp8_(gemm|skinny|adapter_grad)_kernel"),
-    ("8-bit rows", r"fp8_(de)?quantize_rows_kernel"),
+    ("8-bit products", r"fp8_(gemm|skinny|adapter_grad|lora_join)_kernel"),
+    ("8-bit rows", r"fp8_(de)?quantize_(rows|low)_kernel"),
     ("attention fwd", r"flash_fwd_kernel"),
     ("attention bwd", r"flash_bwd_kernel|attn_delta_kernel|dq_convert_kernel"),
     ("loss", r"ce_fwd_bwd_kernel"),

@@ -488,3 +488,20 @@ def test_adapter_gradients_see_the_sums_in_sixteen_bits(T, K, N, blocks):
     for r0, rows, c0, r in blocks:
         d, l, e = d64[:, r0:r0 + rows], low[:, c0:c0 + r], low_e[:, c0:c0 + r]
         assert ((dB[r0:r0 + rows, c0:c0 + r] - d.t() @ l).abs() <= d.abs().t() @ e + (2 * T + 64) * EPS32 * d.abs().t() @ l.abs() + 1e-30).all()
+
+
+# ------------------------------------------------------------------ profiles
+def test_every_kernel_of_the_8_bit_blocks_has_a_category():
+    import pathlib
+    import re
+
+    import axolotl_b200
+    from axolotl_b200.utils.analyze_profile import categorize
+
+    names = set()
+    for f in sorted((pathlib.Path(axolotl_b200.__file__).parent / "csrc").glob("fp8_*.cu")):
+        names |= set(re.findall(r"\b(fp8_\w+_kernel)\s*\(", f.read_text()))
+    assert len(names) >= 6
+    for n in names:
+        where = [c for c, (count, _) in categorize([(f"void (anonymous namespace)::{n}<16, true>(...)", 1.0)]).items() if count]
+        assert where in (["8-bit products"], ["8-bit rows"]), n
