@@ -552,11 +552,13 @@ AXB_DEVICE float2 unpack_bf16x2(uint32_t u) {
   return __bfloat1622float2(v);
 }
 
+// what bf16 leaves of an fp32 value (nothing of one that is not finite there)
+AXB_DEVICE float left_by_bf16(float x, float hi) { return fabsf(hi) <= 3.402823466e38f ? x - hi : 0.f; }
 // two fp32 values as bf16, and what that leaves of them as bf16 too (together off by at most 2^-16 of the value)
 AXB_DEVICE uint32_t split_bf16x2(float x, float y, uint32_t& low) {
   const uint32_t h = pack_bf16x2(x, y);
   const float2 f = unpack_bf16x2(h);
-  low = pack_bf16x2(x - f.x, y - f.y);
+  low = pack_bf16x2(left_by_bf16(x, f.x), left_by_bf16(y, f.y));
   return h;
 }
 

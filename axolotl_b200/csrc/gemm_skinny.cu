@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(SK_T)
           const __nv_bfloat16 hi = __float2bfloat16(o);
           __nv_bfloat16* c = reinterpret_cast<__nv_bfloat16*>(p.C) + row * p.ldc + n0 + j;
           *c = hi;
-          if (p.two) c[p.R * p.ldc] = __float2bfloat16(o - __bfloat162float(hi));
+          if (p.two) c[p.R * p.ldc] = __float2bfloat16(left_by_bf16(o, __bfloat162float(hi)));
         }
       }
     }

@@ -505,3 +505,24 @@ def test_every_kernel_of_the_8_bit_blocks_has_a_category():
     for n in names:
         where = [c for c, (count, _) in categorize([(f"void (anonymous namespace)::{n}<16, true>(...)", 1.0)]).items() if count]
         assert where in (["8-bit products"], ["8-bit rows"]), n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K", [264, 14336])
+def test_infinities_stay_infinities_in_the_gradient_of_b(K):
+    """An infinite x A^T has nothing that bf16 leaves of it: dB is infinite where the formula says so, and no NaN."""
+    from axolotl_b200.ops.fp8 import fp8_lora_linear, quantize_fp8_weight
+
+    T, N, R = 200, 128, 16
+    g = torch.Generator().manual_seed(1)
+    x, dy = torch.randn(T, K, generator=g).bfloat16(), torch.randn(T, N, generator=g).bfloat16()
+    dy[dy == 0] = 1
+    x[77, 5] = float("inf")
+    w, ws = quantize_fp8_weight(torch.randn(N, K, generator=g).cuda())
+    A, B = _adapter(N, K, ((0, N, 0, R),))
+    A[:, 5] = torch.where(A[:, 5] == 0, 1.0, A[:, 5])
+    B0 = B.cuda().requires_grad_(True)
+    y = fp8_lora_linear(x.cuda(), w, ws, A.cuda(), B0, A.bfloat16().cuda(), B.bfloat16().cuda(), 2.0, ((0, N, 0, R),))
+    (dB,) = torch.autograd.grad(y, [B0], dy.cuda())
+    want = dy[77].double()[:, None].sign() * A.double()[:, 5].sign()[None] * float("inf")
+    assert torch.equal(dB.cpu().double(), want)
