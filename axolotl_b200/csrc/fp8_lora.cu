@@ -10,7 +10,7 @@ extern "C" int axb_gemm_skinny(const void* P, long long ldp, const void* S, long
 extern "C" int axb_lora_bwd_dy_parts(const void* dy, long long ld_dy, const void* B, long long ld_b, const void* xa, const void* xa_lo,
                                      long long ld_xa, float* t_parts, float* dB_parts, int T, int N, int R, const int* blocks, int n_lora_blocks, int splits,
                                      int* status, void* stream);
-extern "C" int axb_fp8_low_pays(int T, int K);
+extern "C" int axb_fp8_low_pays(int T, int K, int R);
 extern "C" int axb_fp8_quantize_low(const void* x, long long ldx, const void* A, long long lda, void* q, long long ldq, float* s, long long lds,
                                     void* xa, void* xa_lo, long long ldxa, int T, int K, int R, float scale, int* status, void* stream);
 extern "C" int axb_fp8_linear(const void* x, long long ldx, void* q, const void* W, long long ldw, const float* sw, long long sw_n,
@@ -137,7 +137,7 @@ static_assert(sizeof(AxbFp8Lora) == 17 * 8 + 8 * 8 + 12 * 4, "no gaps");
 
 extern "C" int axb_fp8_lora_fwd(const AxbFp8Lora* l, void* stream) {
   if (l->T <= 0) return 0;
-  const bool one = l->q && l->R <= 64 && axb_fp8_low_pays(l->T, l->K);         // xa and the 8-bit rows in one pass over x
+  const bool one = l->q && l->R <= 64 && axb_fp8_low_pays(l->T, l->K, l->R);         // xa and the 8-bit rows in one pass over x
   int rc;
   if (one) {
     const long long ldq = (l->K + 15ll) & ~15ll;

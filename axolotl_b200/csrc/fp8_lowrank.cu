@@ -208,15 +208,16 @@ int fp8_low_splits(int tiles, int nk) { return tiles <= 14 && nk >= 16 ? 8 : nk 
 
 }  // namespace
 
-// Whether one pass beats the quantiser and a low-rank product of its own (both over x). One pass: 1.03 us for each block of a CTA and each
-// CTA that an SM holds (148 SMs take 35 clusters of four), and 8.2 us around them. Two: 11 us and 0.65 for a million values, over 128 rows
-// (up to there the product is not split: 23 us at 4096 columns, 55 at 14336). Microseconds, one / two, rank 16: 960 x 4096 12.3 / 12.4,
-// 960 x 14336 22.6 / 19.6, 2000 x 14336 35.7 / 28.7, 4000 x 14336 41.0 / 54.5, 5000 x 4096 23.9 / 20.6, 8192 x 14336 67 / 102.
-extern "C" int axb_fp8_low_pays(int T, int K) {
-  if (T <= 128) return 1;
+// Whether one pass beats the quantiser and a low-rank product of its own (both over x). One pass: 1.09 us for each block of a CTA and each
+// CTA that an SM holds (148 SMs take 35 clusters of four), and 9.1 us around them, whatever the rank. Two: 10.6 us, 0.79 for a million values
+// and 0.087 for each column of xa. By least squares over 300 shapes of 16 to 8192 rows, 2048 to 14336 columns and ranks 8 to 64 (x not in the
+// L2); what it picks is 0.2 % above the better one on average, 10 % at most. Microseconds, one / two, rank 16: 64 x 14336 22.7 / 14.5,
+// 960 x 4096 14.4 / 14.4, 960 x 14336 24.6 / 22.5, 2000 x 14336 39.0 / 33.3, 5000 x 4096 24.7 / 26.3, 8192 x 14336 67.8 / 102.6; rank 48:
+// 700 x 8192 18.6 / 21.3, 2000 x 4096 18.5 / 22.5, 2000 x 14336 41.1 / 38.3, 8192 x 4096 28.9 / 43.0.
+extern "C" int axb_fp8_low_pays(int T, int K, int R) {
   const int tiles = (T + 127) / 128, nk = (K + 127) / 128, splits = fp8_low_splits(tiles, nk);
   const double load = splits == 8 || tiles <= 35 ? 1. : tiles <= 70 ? 2. : tiles / 35.;
-  return 8.2 + 1.03 * load * ((nk + splits - 1) / splits) <= 11. + 0.65e-6 * T * K;
+  return 9.1 + 1.09 * load * ((nk + splits - 1) / splits) <= 10.6 + 0.79e-6 * T * K + 0.087 * R;
 }
 
 // x: bf16 [T, K], row stride ldx; A: bf16 [R, K], row stride lda, R <= 64 and a multiple of 8; q: codes, rows of ldq bytes; s: fp32 [ceil(K /

@@ -526,3 +526,22 @@ def test_infinities_stay_infinities_in_the_gradient_of_b(K):
     (dB,) = torch.autograd.grad(y, [B0], dy.cuda())
     want = dy[77].double()[:, None].sign() * A.double()[:, 5].sign()[None] * float("inf")
     assert torch.equal(dB.cpu().double(), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,K,R", [(64, 14336, 16), (64, 2048, 48), (700, 8192, 48), (700, 8192, 8), (2000, 4096, 64), (2000, 4096, 8)])
+def test_one_pass_and_two_keep_the_same(T, K, R):
+    """On both sides of the rule that picks one pass over x or two: the codes are the quantiser's, s x A^T is its sum to 2^-16 of itself."""
+    from axolotl_b200.ops.fp8 import _unpacked, fp8_lora_linear, quantize_fp8_rows, quantize_fp8_weight
+
+    g = torch.Generator().manual_seed(T + R)
+    x = torch.randn(T, K, generator=g).bfloat16().cuda()
+    A, B = _adapter(64, K, ((0, 64, 0, R),))
+    w, ws = quantize_fp8_weight(torch.randn(64, K, generator=g).cuda())
+    A, B = A.cuda().requires_grad_(True), B.cuda().requires_grad_(True)
+    y = fp8_lora_linear(x, w, ws, A, B, A.detach().bfloat16(), B.detach().bfloat16(), 0.5, ((0, 64, 0, R),))
+    q, xa = y.grad_fn.saved_tensors[0], y.grad_fn.saved_tensors[7]
+    (c, s), (codes, scale) = _unpacked(q, T, K), quantize_fp8_rows(x)
+    assert torch.equal(c.view(torch.uint8), codes.view(torch.uint8)) and torch.equal(s, scale) and xa.shape == (2, T, R)
+    want, size = 0.5 * x.double() @ A.double().t(), 0.5 * x.double().abs() @ A.double().abs().t()
+    assert ((xa.double().sum(0) - want).abs() <= 2.0 ** -16 * want.abs() + (K + 16) * EPS32 * size).all()
