@@ -545,3 +545,51 @@ def test_one_pass_and_two_keep_the_same(T, K, R):
     assert torch.equal(c.view(torch.uint8), codes.view(torch.uint8)) and torch.equal(s, scale) and xa.shape == (2, T, R)
     want, size = 0.5 * x.double() @ A.double().t(), 0.5 * x.double().abs() @ A.double().abs().t()
     assert ((xa.double().sum(0) - want).abs() <= 2.0 ** -16 * want.abs() + (K + 16) * EPS32 * size).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 50, 960])
+@pytest.mark.parametrize("names,outs,r", [(["q_proj", "k_proj", "v_proj"], [512, 128, 128], 16), (["gate_proj", "up_proj"], [704, 704], 16),
+                                          (["q_proj", "k_proj", "v_proj"], [264, 72, 72], 8), (["o_proj"], [520], 64)])
+def test_stacked_adapters_of_a_coded_projection(T, names, outs, r):
+    """A fused projection as a model has it: the adapters of q | k | v (rank 48 for 16 each) or gate | up stacked, B block diagonal, fp32
+    masters with bf16 copies, gradients into the masters or into flat buffers. Against the definition in 64 bits."""
+    from axolotl_b200.models.layers import FusedLinear
+
+    K, N = 520, sum(outs)
+    g = torch.Generator().manual_seed(T)
+    m = FusedLinear(K, outs, names, dtype=torch.bfloat16, device="cuda")
+    with torch.no_grad():
+        m.weight.copy_(torch.randn(N, K, generator=g))
+    m.quantize_fp8_()
+    m.add_lora(r, 2 * r, targets=names)
+    with torch.no_grad():
+        for A, B in m.peft_tensors().values():
+            B.copy_(torch.randn(B.shape, generator=g) * 0.1)
+    m.refresh_shadows()
+    m.train()
+    assert m.lora_A.dtype == torch.float32 and m.lora_A.shape == (r * len(names), K) and len(m.lora_blocks) == len(names)
+    x, dy = torch.randn(T, K, generator=g).bfloat16(), (torch.randn(T, N, generator=g) * 1e-2).bfloat16()
+    xl = x.cuda().requires_grad_(True)
+    y = m(xl)
+    dx, dA, dB = torch.autograd.grad(y, [xl, m.lora_A, m.lora_B], dy.cuda())
+    a, b = m.lora_A16.cpu().double(), m.lora_B16.cpu().double()
+    w8, x64, d64, x8, d8, R = _weight8(m), x.double(), dy.double(), _rows8(x), _rows8(dy), a.shape[0]
+    low, tall = m.scaling * x64 @ a.t(), m.scaling * d64 @ b
+    low_s, tall_s = (K + 16) * EPS32 * m.scaling * x64.abs() @ a.abs().t(), (N + 160) * EPS32 * m.scaling * d64.abs() @ b.abs()
+    for got, want, off, size, n in (
+            (y, x8 @ w8.t() + low @ b.t(), (BF16 * low.abs() + low_s) @ b.abs().t(), x8.abs() @ w8.abs().t() + low.abs() @ b.abs().t(), K),
+            (dx, d8 @ w8 + tall @ a, (BF16 * tall.abs() + tall_s) @ a.abs(), d8.abs() @ w8.abs() + tall.abs() @ a.abs(), N)):
+        tol = BF16 * want.abs() + (1 + BF16) * (off + (n + R + 64) * EPS32 * size)
+        assert ((got.detach().cpu().double() - want).abs() <= tol + 1e-30).all()
+    assert ((dA.cpu().double() - tall.t() @ x8).abs() <= (2.0 ** -16 * tall.abs() + tall_s).t() @ x8.abs()
+            + (2 * T + 32) * EPS32 * tall.abs().t() @ x8.abs() + 1e-30).all()
+    inside = torch.zeros(N, R, dtype=torch.bool)
+    for r0, rows, c0, k in m.lora_blocks:
+        inside[r0:r0 + rows, c0:c0 + k] = True
+    offB = d64.abs().t() @ (2.0 ** -16 * low.abs() + low_s) + (2 * T + 64) * EPS32 * d64.abs().t() @ low.abs() + 1e-30
+    assert ((dB.cpu().double() - d64.t() @ low).abs() <= offB)[inside].all() and not dB.cpu()[~inside].any()
+    m.lora_A._axb_grad, m.lora_B._axb_grad = torch.zeros_like(m.lora_A), torch.zeros_like(m.lora_B)
+    xl.grad = None
+    m(xl).backward(dy.cuda())
+    assert m.lora_A.grad is None and torch.equal(m.lora_A._axb_grad, dA) and torch.equal(m.lora_B._axb_grad, dB) and torch.equal(xl.grad, dx)
