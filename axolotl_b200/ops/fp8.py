@@ -292,17 +292,19 @@ def _tile(M, N, K) -> int:
 def _few(T, N, K):
     """How the product of a few tokens runs: 2 in one launch, quantising inside (csrc/fp8_skinny.cu), 1 by the same kernel on rows that a
     launch before it has quantised, 0 by tiles. Inside, every CTA quantises the blocks of its part of K, 16 tokens at a time: some
-    0.5 us each, against 3 us for the launch that does it once. Microseconds, inside / before / tiles: 24 x 4096 by 4096 (4 blocks a
-    CTA, two passes) 16.5 / 20.2 / 21.5; 16 x 4096 by 6144 (8, one) 15.9 / 19.0 / 21.5, 64 (four) 27.0 / 21.4 / 22.8; 1 x 4096 by 28672
-    (32, one) 32.6 / 29.7 / 47.6; 64 x 14336 by 4096 (14, four) 37.8 / 29.4 / 46.4; 64 x 4096 by 28672, where the tiles fill the chip
-    by themselves, 66.1 / 39.5 / 34.8."""
+    0.5 us each, against 3 us, most of them the host's, for the launch that does it once. Microseconds among others, inside / before /
+    tiles, weights not in the L2: 1 x 4096 by 4096 (4 blocks a CTA, one pass) 10.9 / 15.6 / 17.5; 24 x 2048 by 11264 (6, two) 14.4 / 15.3 /
+    15.5; 1 x 14336 by 4096 (14, one) 18.5 / 17.5 / 40.9, 16 tokens 22.6 / 18.6 / 36.7; 64 x 4096 by 4096 (4, four) 18.5 / 15.6 / 16.9; 1 x
+    4096 by 28672 (32, one) 31.5 / 24.7 / 43.0; 64 x 14336 by 4096 (14, four) 36.9 / 24.5 / 41.0; 48 x 2048 by 11264 18.8 / 15.5 / 16.0 (on
+    the device 18.0 / 14.2 / 12.3) and 64 x 4096 by 28672 66.6 / 34.8 / 30.4, where the tiles fill the chip by themselves. Replayed from a
+    graph the launch before is the better one from some 6 blocks on: 24 x 4096 by 4096 11.5 / 10.8."""
     if T > 64:
         return 0
     tiles, nk = (N + 127) >> 7, (K + 127) >> 7
     # axb_cluster_split of csrc/axb_common.cuh
     splits = (8 if tiles <= 33 and nk >= 16 else 6 if tiles <= 44 and nk >= 12 else 5 if tiles <= 50 and nk >= 10 else
               4 if tiles <= 70 and nk >= 8 else 3 if tiles <= 92 and nk >= 6 else 2 if tiles <= 148 and nk >= 4 else 1)
-    if -(-nk // splits) * (1 if T <= 16 else 2 if T <= 32 else 4) <= 16:
+    if -(-nk // splits) * (1 if T <= 16 else 2 if T <= 32 else 4) <= 12:
         return 2
     return 0 if T > 32 and tiles > 70 else 1
 

@@ -593,3 +593,16 @@ def test_stacked_adapters_of_a_coded_projection(T, names, outs, r):
     xl.grad = None
     m(xl).backward(dy.cuda())
     assert m.lora_A.grad is None and torch.equal(m.lora_A._axb_grad, dA) and torch.equal(m.lora_B._axb_grad, dB) and torch.equal(xl.grad, dx)
+
+
+def test_few_tokens_take_the_form_that_measured_best():
+    """Forms that were timed side by side among other calls (tokens, rows of codes, columns): inside the product up to 12 blocks a CTA and pass,
+    before it from 14 on, by tiles where more than 32 tokens meet enough of them."""
+    from axolotl_b200.ops.fp8 import _few
+
+    for form, shapes in ((2, [(1, 4096, 4096), (1, 2048, 8192), (24, 11264, 2048), (24, 4096, 4096), (48, 2048, 2048), (64, 2048, 2048)]),
+                         (1, [(1, 4096, 14336), (16, 4096, 14336), (24, 6144, 4096), (24, 2048, 8192), (48, 4096, 4096), (64, 4096, 4096),
+                              (1, 28672, 4096), (64, 4096, 14336), (64, 6144, 4096)]),
+                         (0, [(48, 11264, 2048), (64, 28672, 4096), (65, 4096, 4096)])):
+        for shape in shapes:
+            assert _few(*shape) == form, shape
