@@ -10,6 +10,7 @@ those buffers, so adapter checkpoints stay PEFT compatible
 """
 from __future__ import annotations
 
+import copy
 import math
 
 import torch
@@ -344,15 +345,29 @@ class FusedLinear(nn.Module):
         self.weight.copy_((self.weight.float() + delta).to(self.weight.dtype))
         self.merged = True
 
+    def _carry_quant(self, st):
+        """Puts the state of a coded weight on the parameter that has taken its place. 8-bit codes are laid out again, once, where a copy has
+        dropped the padding of rows that are not whole 16 bytes."""
+        from ..ops import fp8
+
+        self.weight._axb_quant = st
+        if isinstance(st, fp8.Fp8State) and self.weight.dim() == 2:
+            self.weight.data = fp8._rows16(self.weight.data.view(torch.float8_e4m3fn)).view(torch.uint8)
+
+    def __deepcopy__(self, memo):
+        new = self.__class__.__new__(self.__class__)
+        memo[id(self)] = new
+        new.__setstate__(copy.deepcopy(self.__dict__, memo))
+        st = getattr(self.weight, "_axb_quant", None)
+        if st is not None:   # a parameter's copy has none of its attributes
+            new._carry_quant(copy.deepcopy(st, memo))
+        return new
+
     def _apply(self, fn, *a, **kw):
         st = getattr(self.weight, "_axb_quant", None)
         super()._apply(fn, *a, **kw)
         if st is not None:   # nn.Module._apply may rebuild the parameter object: carry the state along
-            self.weight._axb_quant = st.to(self.weight.device)
-            from ..ops import fp8
-
-            if isinstance(st, fp8.Fp8State) and self.weight.dim() == 2:   # a move drops the padding of rows that are not whole 16 bytes: laid out again once, here
-                self.weight.data = fp8._rows16(self.weight.data.view(torch.float8_e4m3fn)).view(torch.uint8)
+            self._carry_quant(st.to(self.weight.device))
         if self.lora_A is not None:
             self.lora_A16 = None
             self.refresh_shadows()

@@ -606,3 +606,38 @@ def test_few_tokens_take_the_form_that_measured_best():
                          (0, [(48, 11264, 2048), (64, 28672, 4096), (65, 4096, 4096)])):
         for shape in shapes:
             assert _few(*shape) == form, shape
+
+
+# ------------------------------------------------------------------ copies of modules
+def _coded_linear(dev, K=200, quantize="fp8", seed=1):
+    from axolotl_b200.models.layers import FusedLinear
+
+    m = FusedLinear(K, [64, 24], ["a", "b"], bias=True, dtype=torch.bfloat16 if dev == "cuda" else torch.float32, device=dev)
+    with torch.no_grad():
+        m.weight.copy_(torch.randn(88, K, generator=torch.Generator().manual_seed(seed)))
+    m.quantize_fp8_() if quantize == "fp8" else m.quantize_nf4_()
+    return m
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("quantize,K", [("fp8", 200), ("fp8", 256), ("nf4", 256)])
+def test_a_copied_module_keeps_what_its_codes_stand_for(quantize, K, dev):
+    import copy
+    import io
+
+    m = _coded_linear(dev, K, quantize)
+    m.add_lora(8, 16, targets=["b"])
+    m.refresh_shadows()
+    x = torch.randn(5, K, generator=torch.Generator().manual_seed(2)).to(dev, m.bias.dtype)
+    want, buf = m(x), io.BytesIO()
+    torch.save(m, buf)
+    buf.seek(0)
+    box = torch.nn.Module()
+    box.a = box.b = m
+    twice = copy.deepcopy(box)
+    assert twice.a is twice.b
+    for c in (copy.deepcopy(m), twice.a, torch.load(buf, weights_only=False)):
+        assert torch.equal(c(x), want) and not c.weight.requires_grad and c.weight.data_ptr() != m.weight.data_ptr()
+        assert c.weight._axb_quant is not m.weight._axb_quant
+        if quantize == "fp8":
+            assert c.weight.stride(0) % 16 == 0 and c.weight._axb_quant.scale.data_ptr() != m.weight._axb_quant.scale.data_ptr()
