@@ -363,6 +363,34 @@ class FusedLinear(nn.Module):
             new._carry_quant(copy.deepcopy(st, memo))
         return new
 
+    def _save_to_state_dict(self, destination, prefix, keep_vars):
+        from ..ops import fp8
+
+        super()._save_to_state_dict(destination, prefix, keep_vars)
+        st = getattr(self.weight, "_axb_quant", None)
+        if isinstance(st, fp8.Fp8State):
+            destination[prefix + "weight_scale"] = st.scale
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
+        from ..ops import fp8
+
+        st = getattr(self.weight, "_axb_quant", None)
+        w, scale = state_dict.get(prefix + "weight"), state_dict.get(prefix + "weight_scale")
+        if w is not None and (isinstance(st, fp8.Fp8State) or st is None):
+            here = st is not None
+            if w.is_floating_point() == here or (scale is not None) != here or (here and scale.shape != st.scale.shape):
+                error_msgs.append(f"{prefix}weight: {'8-bit codes' if here else 'values'} here, {w.dtype} {tuple(w.shape)} with scales "
+                                  f"{None if scale is None else tuple(scale.shape)} there: codes go from a coded projection to a coded one, scales and all")
+                return
+            if here:
+                with torch.no_grad():
+                    st.scale.copy_(scale)
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
+        if isinstance(st, fp8.Fp8State):
+            self._carry_quant(st)                          # with assign=True the parameter is another one
+        if prefix + "weight_scale" in unexpected_keys:
+            unexpected_keys.remove(prefix + "weight_scale")
+
     def _apply(self, fn, *a, **kw):
         st = getattr(self.weight, "_axb_quant", None)
         super()._apply(fn, *a, **kw)

@@ -641,3 +641,34 @@ def test_a_copied_module_keeps_what_its_codes_stand_for(quantize, K, dev):
         assert c.weight._axb_quant is not m.weight._axb_quant
         if quantize == "fp8":
             assert c.weight.stride(0) % 16 == 0 and c.weight._axb_quant.scale.data_ptr() != m.weight._axb_quant.scale.data_ptr()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_state_dicts_hold_the_scales_of_the_codes(dev):
+    """Codes go from a coded module to a coded one with their scales; values and codes are not copied over one another."""
+    a, b = _coded_linear(dev, seed=1), _coded_linear(dev, seed=2)
+    x = torch.randn(5, 200, generator=torch.Generator().manual_seed(2)).to(dev, a.bias.dtype)
+    assert not torch.equal(a(x), b(x))
+    sd = a.state_dict()
+    assert set(sd) == {"weight", "weight_scale", "bias"} and sd["weight_scale"].shape == (1, 2)
+    res = b.load_state_dict(sd)
+    assert not res.missing_keys and not res.unexpected_keys and torch.equal(a(x), b(x)) and b.weight.stride(0) == 208
+    box = torch.nn.ModuleDict({"p": _coded_linear(dev, seed=3)})
+    box.load_state_dict({f"p.{k}": v for k, v in sd.items()})
+    assert torch.equal(box["p"](x), a(x))
+    c = _coded_linear(dev, seed=4)
+    c.load_state_dict({k: v.clone() for k, v in sd.items()}, assign=True)
+    assert torch.equal(c(x), a(x)) and c.weight.stride(0) == 208 and not c.weight.requires_grad
+    from axolotl_b200.models.layers import FusedLinear
+
+    dense = FusedLinear(200, [64, 24], ["a", "b"], bias=True, dtype=a.bias.dtype, device=dev)
+    with torch.no_grad():
+        dense.weight.zero_()
+    for target, source in ((dense, sd), (dense, {k: sd[k] for k in ("weight", "bias")}), (b, dense.state_dict()),
+                           (b, {k: sd[k] for k in ("weight", "bias")}), (b, {**sd, "weight_scale": sd["weight_scale"][:, :1]})):
+        before = target.weight.data.clone()
+        with pytest.raises(RuntimeError, match="codes"):
+            target.load_state_dict(source)
+        assert torch.equal(target.weight.data, before)
+    nf4 = _coded_linear(dev, 256, "nf4")
+    assert set(nf4.state_dict()) == {"weight", "bias"}
