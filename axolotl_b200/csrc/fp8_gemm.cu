@@ -16,8 +16,8 @@
 // Bound: the epilogue's turn of a block. TMEM reads (110 cycles) and multiply-adds (250, half a packed one a cycle and partition) follow
 // one another in a warp behind some 500 cycles of waits, arrivals and scale loads, against 512 of the tensor cores and as many of the
 // operands' 64 bytes a cycle and SM. A 4096 x 8192 by 4096 product takes 205 k cycles; 147 k with the epilogue left out, 160 k with its
-// reads or its arithmetic alone. 8192 x 4096 by 28672: 830 us, 2.3 PFLOP/s (985 back to back under the power cap); the input gradient of
-// 8192 x 14336 by 4096 449 us. No faster: 16 epilogue warps, scales through a ring of cp.async copies, two TMEM loads in flight, one
+// reads or its arithmetic alone. 8192 x 4096 by 28672: 850 us, 2.26 PFLOP/s (940 to 1000 back to back under the power cap); the input gradient of
+// 8192 x 14336 by 4096 440 us. No faster: 16 epilogue warps, scales through a ring of cp.async copies, two TMEM loads in flight, one
 // product of 256 columns a block.
 #include "axb_common.cuh"
 

@@ -1,6 +1,7 @@
 // A projection in 8-bit blocks with an adapter (ops/fp8.py) as one host call each way: a short training row spends less time on the device
-// than the interpreter needs to issue the launches one by one (960 x 4096 by 6144, rank 16, forward and backward: kernels 106 us; 253 us
-// with them issued from Python, 175 like this, 49 of it autograd's own).
+// than the interpreter needs to issue the launches one by one (960 x 4096 by 6144, rank 16, forward and backward: kernels 104 us, 98 replayed
+// from a graph; 253 us with them issued from Python, 166 like this, 49 of it autograd's own). Both ways, rank 48 in three blocks, fp32 masters,
+// gradients into flat buffers: 152 us (106 replayed), 8192 rows 494; rank 32 by 28672 313 and 2119.
 #include "axb_common.cuh"
 
 extern "C" int axb_gemm_skinny(const void* P, long long ldp, const void* S, long long lds, void* C, long long ldc, int R, int N,
@@ -62,7 +63,7 @@ AXB_DEVICE float4 join4(const float4* p, long long stride, int count, bool any) 
 }
 
 // t and the gradient of B from the parts of csrc/lora_fused.cu, four neighbouring values of a row for four lanes. Bound: the parts' bytes,
-// most of them still in the L2 (8192 x 14336, rank 16: 9 x 0.5 MB of t, 16 x 0.9 MB of B).
+// most of them still in the L2 (dy 8192 x 4096, rank 16: 9 x 0.5 MB of t, 16 x 0.3 MB of B, 5 us; 8192 x 6144, rank 48: 20 MB, 11 us).
 __global__ void __launch_bounds__(256) fp8_lora_join_kernel(const __grid_constant__ JoinParams p) {
   const int lane = threadIdx.x & 31, q = p.R >> 2;
   const long long n = (long long)p.T * q, n8 = (n + 7) & ~7ll, m = (long long)p.N * q;

@@ -17,6 +17,7 @@
 //                                       dB accumulators are double buffered per column block
 //   warps 2-5        : epilogue       - fp32 reductions into t32 / dB32 (several CTAs share every row), or (PARTS) stores: what a CTA
 //                                       has summed goes to a place of its own, and the caller adds the parts in a fixed order
+// dY 8192 x 4096, rank 16: 22 us in parts (32 with the reductions, whose order changes the last bits), 8192 x 6144, rank 48: 34 us.
 #include "axb_common.cuh"
 
 namespace {

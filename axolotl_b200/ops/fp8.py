@@ -8,7 +8,13 @@ finite value stays finite: where the nearest code would stand for 2^128, ``q`` i
 
 ``fp8_linear`` and ``fp8_lora_linear`` quantise their input once: the codes are the operand of the forward product and all that is
 kept of the input for the backward pass, half of what bf16 takes. The backward pass quantises the output gradient the same way and
-reads the same weight codes as the other operand order. The quantisers pass gradients straight through.
+reads the same weight codes as the other operand order. The quantisers pass gradients straight through; one gradient is not the derivative
+of what stands beside it: the low-rank product of an adapter reads the bf16 rows, ``y = x8 W8^T + s (x A^T) B^T``, and ``dA = (s dy B)^T x8``
+the coded ones, the only ones that are kept.
+
+``s x A^T`` and ``s dy B`` enter ``y`` and ``dx`` rounded to bf16, as in the bf16 layer (``ops.lora``), which leaves these within their own
+rounding. For ``dB`` and ``dA``, where it would add as much again, both are held as two bf16 numbers up to rank 64 (off by 2^-16). All sums
+of an adapter's gradients up to rank 64 are joined in a fixed order: the same bits every time.
 
 The reference keeps such weights in FP8 only under adapters (src/axolotl/integrations/kernels/libs/dsv4/lora_fp8.py:1-147: a library
 product in the forward pass, the weight expanded to bf16 in the backward pass) and expands them elsewhere
