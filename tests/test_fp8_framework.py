@@ -672,3 +672,31 @@ def test_state_dicts_hold_the_scales_of_the_codes(dev):
         assert torch.equal(target.weight.data, before)
     nf4 = _coded_linear(dev, 256, "nf4")
     assert set(nf4.state_dict()) == {"weight", "bias"}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("coded", [True, False])
+@pytest.mark.parametrize("T", [40, 600])
+def test_adapters_of_more_blocks_than_the_one_pass_kernel_takes(T, coded):
+    """Nine stacked adapters: the pass over dy for t and dB at once takes eight, so they go the way of large ranks. Small integers, so that
+    what the sums and the bf16 intermediates hold is exact and dB is compared bit for bit."""
+    from axolotl_b200.ops.fp8 import fp8_lora_linear, quantize_fp8_weight
+    from axolotl_b200.ops.lora import lora_linear
+
+    blocks = tuple((64 * i, 64, 8 * i, 8) for i in range(9))
+    K, N, R = 64, 576, 72
+    g = torch.Generator().manual_seed(T)
+    x, dy = (torch.randint(-1, 2, (T, n), generator=g).bfloat16() for n in (K, N))
+    A, B = torch.randint(-1, 2, (R, K), generator=g).float(), torch.zeros(N, R)
+    for r0, rows, c0, r in blocks:
+        B[r0:r0 + rows, c0:c0 + r] = torch.randint(-1, 2, (rows, r), generator=g).float()
+    Al, Bl = A.cuda().requires_grad_(True), B.cuda().requires_grad_(True)
+    args = (Al, Bl, A.bfloat16().cuda(), B.bfloat16().cuda(), 1.0, blocks)
+    w = torch.ones(N, K, device="cuda")
+    y = fp8_lora_linear(x.cuda(), *quantize_fp8_weight(w), *args) if coded else lora_linear(x.cuda(), w.bfloat16(), *args)
+    dA, dB = torch.autograd.grad(y, [Al, Bl], dy.cuda())
+    low = x.double() @ A.double().t()
+    for r0, rows, c0, r in blocks:
+        assert torch.equal(dB[r0:r0 + rows, c0:c0 + r].cpu().double(), dy[:, r0:r0 + rows].double().t() @ low[:, c0:c0 + r])
+    want = (dy.double() @ B.double()).bfloat16().double().t() @ x.double()
+    assert torch.equal(dA.cpu().double(), want)
