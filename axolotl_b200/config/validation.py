@@ -17,13 +17,14 @@ _PROJECTIONS = ([f"self_attn.{n}" for n in ("qkv_proj", "o_proj", "out_gate", "q
                 + ["per_layer_input_gate", "per_layer_projection"])
 
 
-def refuse_trained_codes(cfg: dict, names) -> None:
-    """``base_weights_fp8`` holds the weights of these names as codes, which take no gradient: refuses the keys that would train one."""
+def refuse_trained_codes(cfg: dict, names, known: bool = True) -> None:
+    """``base_weights_fp8`` holds the weights of these names as codes, which take no gradient: refuses the keys that would train one. Where the
+    names are not ``known`` to be the model's, one that a router's name (``mlp.gate``) explains as well is left to the model's own."""
     trained = [(k, re.compile(p)) for k, p in (("unfrozen_parameters", p) for p in cfg.get("unfrozen_parameters") or [])]
     trained += [("lora_modules_to_save", re.compile(re.escape(p))) for p in cfg.get("lora_modules_to_save") or []]
     for n in names if trained else ():
         for key, pattern in trained:
-            if pattern.search(n):
+            if pattern.search(n) and (known or not n.endswith("gate_up_proj.weight") or not pattern.search(n[:-len("_up_proj.weight")])):
                 raise ValueError(f"`{key}` {pattern.pattern!r} would train {n}, which `base_weights_fp8` holds as codes")
 
 
@@ -118,7 +119,7 @@ def validate(cfg: dict, capabilities: dict | None = None) -> list[str]:
             raise ValueError("8-bit base weights cannot be combined with tensor parallelism")
         if g("relora"):
             raise ValueError("`relora` folds its adapters into the base weights, which `base_weights_fp8` holds as codes")
-        refuse_trained_codes(cfg, (f"layers.{i}.{n}.weight" for i in range(256) for n in _PROJECTIONS))
+        refuse_trained_codes(cfg, (f"layers.{i}.{n}.weight" for i in range(256) for n in _PROJECTIONS), known=False)
     if ad == "llama-adapter":
         raise ValueError("`adapter: llama-adapter` is not supported")
     if g("lora_dropout") and (g("lora_mlp_kernel") or g("lora_qkv_kernel") or g("lora_o_kernel")):

@@ -700,3 +700,23 @@ def test_adapters_of_more_blocks_than_the_one_pass_kernel_takes(T, coded):
         assert torch.equal(dB[r0:r0 + rows, c0:c0 + r].cpu().double(), dy[:, r0:r0 + rows].double().t() @ low[:, c0:c0 + r])
     want = (dy.double() @ B.double()).bfloat16().double().t() @ x.double()
     assert torch.equal(dA.cpu().double(), want)
+
+
+@pytest.mark.parametrize("key,name", [("unfrozen_parameters", r"mlp\.gate"), ("lora_modules_to_save", "mlp.gate"),
+                                      ("unfrozen_parameters", r"layers\.\d+\.mlp\.gate")])
+def test_a_router_may_be_trained_beside_codes(key, name):
+    """`mlp.gate` is the router's name and the beginning of a dense layer's projection: the configuration does not know which the model has, the
+    set-up does."""
+    from axolotl_b200.config.load import load_cfg
+    from axolotl_b200.train.run import setup_adapter
+
+    cfg = load_cfg({**BASE, key: [name]})
+    with pytest.raises(ValueError, match=r"layers\.0\.mlp\.gate_up_proj\.weight"):
+        setup_adapter(cfg, _model())
+    from axolotl_b200.models.config import preset
+    from axolotl_b200.models.transformer import CausalLM
+
+    moe = CausalLM(preset("tiny-qwen3-moe", num_hidden_layers=2, vocab_size=512), dtype=torch.float32, device="cpu").init_weights(0)
+    setup_adapter(cfg, moe)
+    trained = [n for n, p in moe.named_parameters() if p.requires_grad and "lora" not in n]
+    assert trained and all(n.endswith("mlp.gate") for n in trained)
