@@ -138,7 +138,7 @@ static_assert(sizeof(AxbFp8Lora) == 17 * 8 + 8 * 8 + 12 * 4, "no gaps");
 
 extern "C" int axb_fp8_lora_fwd(const AxbFp8Lora* l, void* stream) {
   if (l->T <= 0) return 0;
-  const bool one = l->q && l->R <= 64 && axb_fp8_low_pays(l->T, l->K, l->R);         // xa and the 8-bit rows in one pass over x
+  const bool one = l->q && l->R <= 64 && axb_fp8_low_pays(l->T, l->K, l->R);   // xa and the 8-bit rows in one pass over x
   int rc;
   if (one) {
     const long long ldq = (l->K + 15ll) & ~15ll;
@@ -180,8 +180,8 @@ extern "C" int axb_fp8_lora_bwd(const AxbFp8Lora* l, void* stream) {
     p.chunks = (p.T + 511) / 512;
     const long long at = (long long)row * l->R;
     rc = axb_lora_bwd_dy_parts(static_cast<const char*>(l->x) + 2ll * row * l->ldx, l->ldx, l->B, l->ldb,
-                               static_cast<const char*>(l->xa) + 2 * at, static_cast<const char*>(l->xa) + 2 * (n + at), l->R, l->t_parts, l->dB_parts, p.T, l->N, l->R, l->blocks,
-                               l->n_blocks, l->splits, l->status, stream);
+                               static_cast<const char*>(l->xa) + 2 * at, static_cast<const char*>(l->xa) + 2 * (n + at), l->R, l->t_parts,
+                               l->dB_parts, p.T, l->N, l->R, l->blocks, l->n_blocks, l->splits, l->status, stream);
     if (rc) break;
     p.t = reinterpret_cast<uint2*>(static_cast<char*>(l->t) + 2 * at);
     p.t_lo = reinterpret_cast<uint2*>(static_cast<char*>(l->t) + 2 * (n + at));
@@ -198,7 +198,8 @@ extern "C" int axb_fp8_lora_bwd(const AxbFp8Lora* l, void* stream) {
   if (!rc && l->dA) {
     const long long ldq = (l->K + 15ll) & ~15ll, lds = (l->T + 3ll) & ~3ll;      // the layout of axb_fp8_linear
     rc = axb_fp8_adapter_grad(l->qx, ldq, reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(l->qx) + ldq * l->T), lds, l->t,
-                              static_cast<const char*>(l->t) + 2 * n, l->R, l->dA, l->ldda, l->T, l->K, l->R, l->dA_bf16 ? 2 : l->add_dA, l->status, stream);
+                              static_cast<const char*>(l->t) + 2 * n, l->R, l->dA, l->ldda, l->T, l->K, l->R,
+                              l->dA_bf16 ? 2 : l->add_dA, l->status, stream);
   }
   return rc;
 }
