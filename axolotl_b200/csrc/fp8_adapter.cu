@@ -261,8 +261,8 @@ __global__ void __launch_bounds__(FA_T, 2)
 }
 
 template <int NR, bool TWO>
-int launch_adapter_grad(const CUtensorMap& q, const CUtensorMap& sc, const CUtensorMap& g, const CUtensorMap& lo, const Fp8AdapterParams& p, int tiles, int chunks,
-                        int splits, cudaStream_t st) {
+int launch_adapter_grad(const CUtensorMap& q, const CUtensorMap& sc, const CUtensorMap& g, const CUtensorMap& lo, const Fp8AdapterParams& p,
+                        int tiles, int chunks, int splits, cudaStream_t st) {
   auto kern = fp8_adapter_grad_kernel<NR, TWO>;
   static std::atomic<unsigned long long> allowed{0};
   if (const int rc = axb_allow_smem((const void*)kern, FaCfg<TWO>::SMEM, allowed)) return rc;
@@ -274,7 +274,8 @@ int launch_adapter_grad(const CUtensorMap& q, const CUtensorMap& sc, const CUten
 }  // namespace
 
 // q: codes [T, K], rows of ldq bytes; s: fp32 [ceil(K / 128)][lds]; g: bf16 [T, R], row stride ldg; g_lo: the same, added to it (null: none);
-// out: [R, K], row stride ldo; kind 0: fp32, written, 1: fp32, added to, 2: bf16, written. q, s, g and g_lo start on 16 bytes and have row strides of whole 16 bytes.
+// out: [R, K], row stride ldo; kind 0: fp32, written, 1: fp32, added to, 2: bf16, written. q, s, g and g_lo start on 16 bytes and have row
+// strides of whole 16 bytes.
 extern "C" int axb_fp8_adapter_grad(const void* q, long long ldq, const float* s, long long lds, const void* g, const void* g_lo,
                                     long long ldg, void* out, long long ldo, int T, int K, int R, int kind, int* status, void* stream) {
   if (K <= 0 || R <= 0) return 0;

@@ -9,8 +9,8 @@ extern "C" int axb_gemm_skinny(const void* P, long long ldp, const void* S, long
                                const void* bias, int out_mode, int out_f32, int glu_kind, float glu_limit, int p_dep, int splits,
                                int pdl, int* status, void* stream);
 extern "C" int axb_lora_bwd_dy_parts(const void* dy, long long ld_dy, const void* B, long long ld_b, const void* xa, const void* xa_lo,
-                                     long long ld_xa, float* t_parts, float* dB_parts, int T, int N, int R, const int* blocks, int n_lora_blocks, int splits,
-                                     int* status, void* stream);
+                                     long long ld_xa, float* t_parts, float* dB_parts, int T, int N, int R, const int* blocks,
+                                     int n_lora_blocks, int splits, int* status, void* stream);
 extern "C" int axb_fp8_low_pays(int T, int K, int R);
 extern "C" int axb_fp8_quantize_low(const void* x, long long ldx, const void* A, long long lda, void* q, long long ldq, float* s, long long lds,
                                     void* xa, void* xa_lo, long long ldxa, int T, int K, int R, float scale, int* status, void* stream);

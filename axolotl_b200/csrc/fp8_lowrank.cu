@@ -5,7 +5,8 @@
 // operand of tcgen05.mma (A's block is the other one, N = 16 .. 64), and eight warps read the same tile back for the codes, a
 // conflict-free 16 bytes a lane. They hand the stage back as soon as the values are in registers. K is split over a cluster, whose partial
 // products meet in distributed shared memory in a fixed order. What it measures: 8192 x 14336, rank 16, 67 us: 5.9 TB/s and some 7 us of
-// start, join and end (rank 48, with a stage less, 73); 960 x 4096 12.3 us. No faster: eight quantising warps of eight passes, five stages for one CTA of an SM.
+// start, join and end (rank 48, with a stage less, 73); 960 x 4096 12.3 us. No faster: eight quantising warps of eight passes, five stages for
+// one CTA of an SM.
 #include "fp8_rows.cuh"
 
 namespace {
@@ -227,7 +228,9 @@ extern "C" int axb_fp8_quantize_low(const void* x, long long ldx, const void* A,
                                     void* xa, void* xa_lo, long long ldxa, int T, int K, int R, float scale, int* status, void* stream) {
   if (T <= 0 || K <= 0) return 0;
   auto bad = [](const void* a, long long bytes) { return (reinterpret_cast<uintptr_t>(a) & 15) != 0 || (bytes & 15) != 0; };
-  if (R <= 0 || R > 64 || (R & 7) || bad(x, 2 * ldx) || bad(A, 2 * lda) || bad(q, ldq) || bad(xa, 2 * ldxa) || bad(xa_lo, 0) || ldq < K || lds < T) return -2;
+  if (R <= 0 || R > 64 || (R & 7) || bad(x, 2 * ldx) || bad(A, 2 * lda) || bad(q, ldq) || bad(xa, 2 * ldxa) || bad(xa_lo, 0)
+      || ldq < K || lds < T)
+    return -2;
   const int NR = R <= 16 ? 16 : (R <= 32 ? 32 : 64);
   CUtensorMap tX, tA;
   int rc = axb_make_tmap_2d(&tX, x, T, K, ldx, 128, 64);

@@ -277,7 +277,8 @@ __global__ void __launch_bounds__(LF_THREADS, 1)
 
 template <bool PARTS>
 int launch_lora_bwd_dy(const void* dy, long long ld_dy, const void* B, long long ld_b, const void* xa, const void* xa_lo, long long ld_xa,
-                       float* t32, float* dB32, long long ldb32, int T, int N, int R, const int* blocks, int n_lora_blocks, int splits, int* status, void* stream) {
+                       float* t32, float* dB32, long long ldb32, int T, int N, int R, const int* blocks, int n_lora_blocks, int splits,
+                       int* status, void* stream) {
   if (R > 64 || n_lora_blocks < 1 || n_lora_blocks > 8) return -3;
   if ((ld_dy & 7) || (ld_b & 7) || (ld_xa & 7)) return -2;
   CUtensorMap tDY, tB, tXA, tXL;
@@ -322,12 +323,12 @@ extern "C" int axb_lora_bwd_dy(const void* dy, long long ld_dy, const void* B, l
                                    sms / ((T + LF_ROWS - 1) / LF_ROWS), status, stream);
 }
 
-// The same sums of an xa that is given as two bf16 numbers (xa + xa_lo), in parts, each written once by one CTA: t_parts fp32 [splits][T, R], dB_parts fp32 [ceil(T / 512)][N, R], of which only the
-// columns of the diagonal blocks are written; R a multiple of 8, both on 16 bytes, 1 <= splits <= ceil(N / 128). Added in a fixed order they
+// The same sums of an xa that is given as two bf16 numbers (xa + xa_lo), in parts, each written once by one CTA: t_parts fp32 [splits][T, R],
+// dB_parts fp32 [ceil(T / 512)][N, R], of which only the columns of the diagonal blocks are written; R a multiple of 8, both on 16 bytes, 1 <= splits <= ceil(N / 128). Added in a fixed order they
 // are the same bits every time.
 extern "C" int axb_lora_bwd_dy_parts(const void* dy, long long ld_dy, const void* B, long long ld_b, const void* xa, const void* xa_lo,
-                                     long long ld_xa, float* t_parts, float* dB_parts, int T, int N, int R, const int* blocks, int n_lora_blocks, int splits,
-                                     int* status, void* stream) {
+                                     long long ld_xa, float* t_parts, float* dB_parts, int T, int N, int R, const int* blocks,
+                                     int n_lora_blocks, int splits, int* status, void* stream) {
   if (T <= 0 || N <= 0 || R <= 0) return 0;
   if ((R & 7) || splits < 1 || splits > (N + 127) / 128) return -2;
   if ((reinterpret_cast<uintptr_t>(t_parts) | reinterpret_cast<uintptr_t>(dB_parts)) & 15) return -2;

@@ -380,7 +380,8 @@ class FusedLinear(nn.Module):
             here = st is not None
             if w.is_floating_point() == here or (scale is not None) != here or (here and scale.shape != st.scale.shape):
                 error_msgs.append(f"{prefix}weight: {'8-bit codes' if here else 'values'} here, {w.dtype} {tuple(w.shape)} with scales "
-                                  f"{None if scale is None else tuple(scale.shape)} there: codes go from a coded projection to a coded one, scales and all")
+                                  f"{None if scale is None else tuple(scale.shape)} there: codes go from a coded projection to a coded one, "
+                                  "scales and all")
                 return
             if here:
                 with torch.no_grad():
