@@ -324,8 +324,8 @@ extern "C" int axb_lora_bwd_dy(const void* dy, long long ld_dy, const void* B, l
 }
 
 // The same sums of an xa that is given as two bf16 numbers (xa + xa_lo), in parts, each written once by one CTA: t_parts fp32 [splits][T, R],
-// dB_parts fp32 [ceil(T / 512)][N, R], of which only the columns of the diagonal blocks are written; R a multiple of 8, both on 16 bytes, 1 <= splits <= ceil(N / 128). Added in a fixed order they
-// are the same bits every time.
+// dB_parts fp32 [ceil(T / 512)][N, R], of which only the columns of the diagonal blocks are written; R a multiple of 8, both on 16 bytes,
+// 1 <= splits <= ceil(N / 128). Added in a fixed order they are the same bits every time.
 extern "C" int axb_lora_bwd_dy_parts(const void* dy, long long ld_dy, const void* B, long long ld_b, const void* xa, const void* xa_lo,
                                      long long ld_xa, float* t_parts, float* dB_parts, int T, int N, int R, const int* blocks,
                                      int n_lora_blocks, int splits, int* status, void* stream) {
